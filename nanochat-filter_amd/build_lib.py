@@ -24,7 +24,7 @@ CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "nanochat_amd", "libnanochat_filter_amd.so")
 SOURCES = ["ltv_scan_fwd_bf16.hip", "ltv_scan_fwd_f32.hip", "ltv_scan_bwd_bf16.hip",
            "ltv_scan_bwd_f32.hip", "ltv_scan_abi.hip", "ltv_scan_lb.hip", "ltv_gemm.hip", "ltv_decode.hip",
-           "ltv_abi.cpp"]
+           "ltv_paged_cache.hip", "ltv_paged_attn.hip", "ltv_logprobs.hip", "ltv_abi.cpp"]
 ARCH = "gfx950"
 # roofline microbenchmarks for bench.py --workload peaks: a library of their own
 PEAKS_SOURCES = ["bench/ltv_peaks.hip"]
@@ -32,7 +32,7 @@ PEAKS_OUT = os.path.join(HERE, "nanochat_amd", "libltv_peaks.so")
 
 
 # host path for PyTorch over the C ABI (no device code)
-TORCH_SOURCES = ["torch/ltv_torch.cpp"]
+TORCH_SOURCES = ["torch/ltv_torch.cpp", "torch/ltv_serving.cpp"]
 TORCH_OUT = os.path.join(HERE, "nanochat_amd", "_ltv_torch.so")
 
 

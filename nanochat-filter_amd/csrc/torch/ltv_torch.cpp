@@ -23,6 +23,7 @@
 #include <utility>
 
 #include "../../../include/nanochat_filter_amd.h"
+#include "ltv_torch.hpp"
 
 namespace {
 
@@ -375,6 +376,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("qkv_filter", &qkv_filter);
   m.def("decode_rows", &decode_rows);
   m.def("drop_chain_workspaces", &drop_chain_workspaces);
+  bind_serving(m);
   // the workspace cache by itself, any tensors (its locking is tested without a device)
   m.def("_find_chain_workspace", [](int device, int64_t stream, size_t bytes) {
     return find_chain_workspace({device, reinterpret_cast<void*>(stream)}, bytes);
