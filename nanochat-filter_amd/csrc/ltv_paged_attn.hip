@@ -2,98 +2,621 @@
 //
 //   out[row] = sum_j p_j v_j,  p = softmax_{j <= pos(row)}(scale q[row] . k_j)
 //
-// One workgroup per (token, head): sixteen groups of sixteen lanes take the keys in
-// turn, a lane holding eight of the head's channels; each group keeps a running
-// maximum and sum, and the groups are joined at the end.
+// One pass over the keys with the running maximum m and sum l of each row's softmax:
+// for a tile of keys, s = scale log2(e) K q, m' = max(m, max s), p = 2^(s - m'),
+// l = l 2^(m - m') + sum p, o = o 2^(m - m') + V^T p, and out = o / l at the end.
+//
+// Rows.  A sequence's n tokens times the g = NH / NKVH query heads of one k/v head are
+// its rows, token-major: they share every key, so a decode step of a group of heads
+// reads its keys once.  A workgroup has 128 rows, 32 for each of four wavefronts.
+//
+// Layout of the products (32 x 32 MFMA blocks).  The scores are computed as S^T = K Q^T:
+// a lane then holds 16 keys of one row, so maximum and sum are taken in the lane and
+// once across the two half-wavefronts, and its values are, without any exchange, the
+// right-hand operand of O^T = V^T P^T: the order of the keys within a product is free
+// as long as V^T is read in the same one (ds_read_b64_tr_b16 transposes four keys of a
+// column at a time).  Both tiles are shared by the wavefronts through LDS, two buffers
+// deep: the next tile is on its way, straight into LDS, while this one is computed.
+//
+// Split.  Few rows and many keys leave compute units idle, so a sequence's keys are cut
+// into chunks that workgroups take side by side; a second kernel joins their (m, l, o).
 #include <algorithm>
+#include <type_traits>
 
+#include "ltv_gemm_dma.hpp"
 #include "ltv_paged.hpp"
 
 namespace ltv {
 namespace {
 
+constexpr int kAttnWaves = 4;
+constexpr int kAttnThreads = kAttnWaves * 64;
+constexpr int kAttnRows = kAttnWaves * 32;  // rows of a workgroup
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
 struct AttnArgs {
   PagedBatch batch;
-  const void* q;
-  const void* k;
-  const void* v;
-  void* out;
+  const char* q;
+  const char* k;
+  const char* v;
+  char* out;
   float* lse;
-  int64_t qs[3], ks[3], vs[3], os[3];  // elements
-  int NH, NKVH, D;
-  float scale;
+  float* part;                // partial o, then (m, l), of the split sequences
+  int64_t qs[3], os[3];       // bytes
+  int64_t kh, vh;             // bytes from head to head of the pages
+  uint32_t kp, ks, vp, vs;    // 16-byte units from page to page and row to row
+  int NH, NKVH, D, g;
+  int q_aligned;
+  float scale;                // with log2(e)
+  int tiles;                  // row tiles of the grid
+  int chunk, nsplit;          // keys of a split, splits of the grid
+  int rows_cap;               // sequences of more rows are not split
 };
 
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+// What differs by element type.  A chunk is 16 bytes of a row.
 template <typename T>
-__global__ void __launch_bounds__(256) attn_rows_kernel(const AttnArgs a) {
-  __shared__ float lds_ms[16][2];
-  __shared__ float lds_o[16][128];
-  const int h = blockIdx.y, b = blockIdx.z;
-  const int kvh = h / (a.NH / a.NKVH);
-  const PagedSeq s = paged_seq(a.batch, b);
+struct AttnType;
+
+template <>
+struct AttnType<bf16_t> {
+  static constexpr int kChunk = 8;  // elements
+  static constexpr int kKeys = 64;  // keys of a tile
+  // S^T += K Q^T over 16 channels: a lane's k and q chunk hold channels 8 (lane / 32) ..
+  static __device__ __forceinline__ f32x16 scores(uint4 k, uint4 q, f32x16 s) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, k),
+                                                   __builtin_bit_cast(bf16x8_t, q), s, 0, 0, 0);
+  }
+};
+
+template <>
+struct AttnType<float> {
+  static constexpr int kChunk = 4;
+  static constexpr int kKeys = 32;
+  static __device__ __forceinline__ f32x16 scores(uint4 k, uint4 q, f32x16 s) {
+    s = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(k.x), __uint_as_float(q.x), s, 0, 0, 0);
+    s = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(k.y), __uint_as_float(q.y), s, 0, 0, 0);
+    s = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(k.z), __uint_as_float(q.z), s, 0, 0, 0);
+    s = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(k.w), __uint_as_float(q.w), s, 0, 0, 0);
+    return s;
+  }
+};
+
+// Shape of a tile in LDS: rows of DP channels (D padded with zeros), unpadded; chunk c of
+// row r sits in a slot chosen so that the lanes of one read fall on different banks.
+//   K: 16 consecutive rows, one chunk each (ds_read_b128).
+//   V, bfloat16: four rows, 64 bytes each (ds_read_b64_tr_b16).
+//   V, float32: two rows four apart, 128 bytes each (ds_read_b32).
+template <typename T, int DP>
+struct AttnTile {
+  static constexpr int kKeys = AttnType<T>::kKeys;
+  static constexpr int kChunks = DP / AttnType<T>::kChunk;     // of a row
+  static constexpr int kPhase = kChunks < 16 ? 16 / kChunks : 1;  // rows of 256 bytes
+  static constexpr int kUnits = kKeys * kChunks;               // chunks of a tile
+  static constexpr int kLoads = kUnits / kAttnThreads;         // of a thread
+  static_assert(kUnits % kAttnThreads == 0, "a tile is loaded by all threads alike");
+  static __device__ __forceinline__ int k_swizzle(int r) {
+    return (r / kPhase) & 15 & (kChunks - 1);
+  }
+  static __device__ __forceinline__ int v_swizzle(int r) {
+    if constexpr (sizeof(T) == 4) return ((r >> 2) & 1) * 8;
+    return ((r / kPhase) & (4 / kPhase - 1)) * 4;
+  }
+  static __device__ __forceinline__ int k_slot(int r, int c) {
+    return r * kChunks + (c ^ k_swizzle(r));
+  }
+  static __device__ __forceinline__ int v_slot(int r, int c) {
+    return r * kChunks + (c ^ v_swizzle(r));
+  }
+};
+
+__device__ const uint4 kZeros = {0, 0, 0, 0};
+
+// One wavefront's 16 bytes per lane from `from` into LDS at `to` + 16 lane (`to` uniform).
+// Inline assembly, as in the projection's kernels: the compiler would wait for a builtin's
+// load before the next read of either buffer.  It has no output register; the wait is
+// wait_vmcnt and a barrier.  The nop covers the write of M0.
+__device__ __forceinline__ void load_lds16(uint4* to, const char* from) {
+  const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint4*)to;
+  asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(from), "{m0}"(base) : "memory");
+}
+
+__device__ __forceinline__ void barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// Whether any of a chunk's elements is infinite or NaN (all exponent bits set).
+__device__ __forceinline__ bool any_nonfinite(uint4 x, bf16_t) {
+  bool bad = false;
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    bad |= (w[i] & 0x7f80u) == 0x7f80u || (w[i] & 0x7f800000u) == 0x7f800000u;
+  return bad;
+}
+__device__ __forceinline__ bool any_nonfinite(uint4 x, float) {
+  bool bad = false;
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) bad |= (w[i] & 0x7f800000u) == 0x7f800000u;
+  return bad;
+}
+
+__device__ __forceinline__ float across_halves_max(float x) {
+  return fmaxf(x, __shfl_xor(x, 32));
+}
+
+// The splits of a sequence: 1, or how many chunks its keys make.
+__device__ __forceinline__ int splits_of(const AttnArgs& a, const PagedSeq& s) {
+  if ((int64_t)s.n * a.g > a.rows_cap) return 1;
+  return max(1, min(a.nsplit, (s.len + a.chunk - 1) / a.chunk));
+}
+
+// Partials of (sequence b, k/v head, split): rows_cap rows of D values, and of (m, l).
+__device__ __forceinline__ int64_t part_row(const AttnArgs& a, int bh, int split) {
+  return ((int64_t)bh * a.nsplit + split) * a.rows_cap;
+}
+
+// Rows row0 .. row_end - 1 of a workgroup over keys begin .. end - 1, each key that a row
+// does not see left alone altogether: the way of tiles with infinite or NaN values among
+// those that some rows do not see.  Sixteen groups of sixteen lanes take a row's keys in
+// turn, a lane holding eight channels.  at: the first row's place in the partials, or -1.
+template <typename T>
+__device__ __forceinline__ void rows_one_by_one(const AttnArgs& a, const PagedSeq& s, int b,
+                                                int kvh, int64_t row0, int64_t row_end, int begin,
+                                                int end, int64_t at, float* lds) {
+  float* lds_m = lds;
+  float* lds_l = lds + 16;
+  float* lds_o = lds + 32;  // 16 x 128
   const int c = threadIdx.x & 15, gi = threadIdx.x >> 4;
   const bool on = c * 8 < a.D;
-  for (int t = blockIdx.x; t < s.n; t += gridDim.x) {
-    const int pos = s.len - s.n + t;
-    const int64_t row = a.batch.starts != nullptr ? s.row0 + t : (int64_t)b * a.batch.T + t;
-    const int64_t qo = a.batch.starts != nullptr ? row * a.qs[1] : b * a.qs[0] + t * a.qs[1];
-    const int64_t oo = a.batch.starts != nullptr ? row * a.os[1] : b * a.os[0] + t * a.os[1];
-    const T* q = reinterpret_cast<const T*>(a.q) + qo + h * a.qs[2] + c * 8;
-    float qf[8], o[8];
+  for (int64_t row = row0; row < row_end; ++row) {
+    const int t = (int)(row / a.g), h = kvh * a.g + (int)(row - (int64_t)t * a.g);
+    const int last = min(end - 1, s.len - s.n + t);
+    const int64_t trow = a.batch.starts != nullptr ? s.row0 + t : (int64_t)b * a.batch.T + t;
+    const char* q = a.q + (a.batch.starts != nullptr ? trow * a.qs[1]
+                                                     : b * a.qs[0] + t * a.qs[1]) + h * a.qs[2];
+    float qf[8], o[8], m = -INFINITY, l = 0.0f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      qf[e] = on ? io_traits<T>::load(q + e) * a.scale : 0.0f;
+      qf[e] = on ? io_traits<T>::load(reinterpret_cast<const T*>(q) + c * 8 + e) : 0.0f;
       o[e] = 0.0f;
     }
-    float m = -INFINITY, l = 0.0f;
-    for (int j = gi; j <= pos; j += 16) {
-      const int col = a.batch.div.quot(j);
-      const int page = s.table[col];
+    for (int j = begin + gi; j <= last; j += 16) {
+      const int col = a.batch.div.quot(j), page = s.table[col];
       if (page < 0 || page >= a.batch.P) continue;
-      const int at = j - col * a.batch.div.size;
-      const T* k = reinterpret_cast<const T*>(a.k) + page * a.ks[0] + kvh * a.ks[1] +
-                   at * a.ks[2] + c * 8;
-      const T* v = reinterpret_cast<const T*>(a.v) + page * a.vs[0] + kvh * a.vs[1] +
-                   at * a.vs[2] + c * 8;
+      const uint32_t in = (uint32_t)(j - col * a.batch.div.size);
+      const T* k = reinterpret_cast<const T*>(
+          a.k + kvh * a.kh + (uint64_t)((uint32_t)page * a.kp + in * a.ks) * 16) + c * 8;
+      const T* v = reinterpret_cast<const T*>(
+          a.v + kvh * a.vh + (uint64_t)((uint32_t)page * a.vp + in * a.vs) * 16) + c * 8;
       float x = 0.0f;
       if (on)
-#pragma unroll
         for (int e = 0; e < 8; ++e) x = fmaf(qf[e], io_traits<T>::load(k + e), x);
-#pragma unroll
       for (int d = 1; d < 16; d <<= 1) x += __shfl_xor(x, d);
-      const float mn = fmaxf(m, x);
-      const float base = mn == -INFINITY ? 0.0f : mn;
-      const float was = __expf(m - base), p = __expf(x - base);
-      l = l * was + p;
+      x *= a.scale;
+      const float mn = fmaxf(m, x), base = mn == -INFINITY ? 0.0f : mn;
+      const float was = __builtin_amdgcn_exp2f(m - base), p = __builtin_amdgcn_exp2f(x - base);
+      l = fmaf(l, was, p);
       m = mn;
       if (on)
-#pragma unroll
         for (int e = 0; e < 8; ++e) o[e] = fmaf(p, io_traits<T>::load(v + e), o[e] * was);
     }
     __syncthreads();
     if (c == 0) {
-      lds_ms[gi][0] = m;
-      lds_ms[gi][1] = l;
+      lds_m[gi] = m;
+      lds_l[gi] = l;
     }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) lds_o[gi][c * 8 + e] = o[e];
+    for (int e = 0; e < 8; ++e) lds_o[gi * 128 + c * 8 + e] = o[e];
     __syncthreads();
     float mx = -INFINITY;
-    for (int i = 0; i < 16; ++i) mx = fmaxf(mx, lds_ms[i][0]);
+    for (int i = 0; i < 16; ++i) mx = fmaxf(mx, lds_m[i]);
     const float base = mx == -INFINITY ? 0.0f : mx;
     float sum = 0.0f, acc = 0.0f;
     const int d = threadIdx.x;
     for (int i = 0; i < 16; ++i) {
-      const float w = __expf(lds_ms[i][0] - base);
-      sum = fmaf(lds_ms[i][1], w, sum);
-      if (d < a.D) acc = fmaf(lds_o[i][d], w, acc);
+      // (a group without keys has weight 0)
+      const float w = lds_m[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(lds_m[i] - base);
+      sum = fmaf(lds_l[i], w, sum);
+      if (d < a.D) acc = fmaf(lds_o[i * 128 + d], w, acc);
     }
-    if (d < a.D)
-      io_traits<T>::store(reinterpret_cast<T*>(a.out) + oo + h * a.os[2] + d,
-                          sum == 0.0f ? 0.0f : acc / sum);
-    if (d == 0 && a.lse != nullptr)
-      a.lse[row * a.NH + h] = sum == 0.0f ? -INFINITY : base + __logf(sum);
+    if (at >= 0) {
+      if (d < a.D) a.part[(at + row) * a.D + d] = acc;
+      if (d == 0)
+        reinterpret_cast<float2*>(a.part + part_row(a, a.batch.B * a.NKVH, 0) * a.D)[at + row] =
+            make_float2(mx, sum);
+    } else {
+      char* out = a.out + (a.batch.starts != nullptr ? trow * a.os[1]
+                                                     : b * a.os[0] + t * a.os[1]) + h * a.os[2];
+      if (d < a.D)
+        io_traits<T>::store(reinterpret_cast<T*>(out) + d, sum == 0.0f ? 0.0f : acc / sum);
+      if (d == 0 && a.lse != nullptr)
+        a.lse[trow * a.NH + h] = sum == 0.0f ? -INFINITY
+                                             : (mx + __builtin_amdgcn_logf(sum)) * kLn2;
+    }
   }
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kAttnThreads, 2) attn_tile_kernel(const AttnArgs a) {
+  using Ty = AttnType<T>;
+  using Ti = AttnTile<T, DP>;
+  constexpr int KT = Ti::kKeys, KB = KT / 32;
+  constexpr int kSteps = Ti::kChunks / 2;  // score products' steps: two chunks each
+  constexpr int kDB = DP / 32;
+  __shared__ uint4 lds_k[2][Ti::kUnits];
+  __shared__ uint4 lds_v[2][Ti::kUnits];
+
+  const int nbh = a.batch.B * a.NKVH;
+  const int bh = blockIdx.x % nbh;
+  int rest = blockIdx.x / nbh;
+  const int split = rest % a.nsplit;
+  const int tile0 = a.tiles - 1 - rest / a.nsplit;  // the tiles with the most keys first
+  const int b = bh / a.NKVH, kvh = bh - b * a.NKVH;
+  const PagedSeq s = paged_seq(a.batch, b);
+  const int nsplit = splits_of(a, s);
+  if (split >= nsplit) return;
+  const int64_t rows = (int64_t)s.n * a.g;
+
+  const int lane = threadIdx.x & 63, ln = lane & 31, hf = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const char* kbase = a.k + (int64_t)kvh * a.kh;
+  const char* vbase = a.v + (int64_t)kvh * a.vh;
+  const int chunks = a.D / Ty::kChunk;
+
+  // (more rows than the grid was sized for: its tiles are walked again)
+  for (int64_t tile = tile0; tile * kAttnRows < rows; tile += a.tiles) {
+    const int64_t row = tile * kAttnRows + wave * 32 + ln;
+    const bool row_ok = row < rows;
+    const int t = row_ok ? (int)(row / a.g) : 0;
+    const int h = kvh * a.g + (row_ok ? (int)(row - (int64_t)t * a.g) : 0);
+    const int pos = row_ok ? s.len - s.n + t : -1;
+    const int64_t trow = a.batch.starts != nullptr ? s.row0 + t : (int64_t)b * a.batch.T + t;
+
+    // the last position that any row of the wavefront, and of the workgroup, sees
+    const bool wave_on = tile * kAttnRows + wave * 32 < rows;
+    const int64_t wlast = min(tile * kAttnRows + wave * 32 + 31, rows - 1);
+    const int wave_end = wave_on ? s.len - s.n + (int)(wlast / a.g) + 1 : 0;
+    const int wave_min = wave_on
+        ? s.len - s.n + (int)((tile * kAttnRows + wave * 32) / a.g) : 0;
+    const int64_t tlast = min(tile * kAttnRows + kAttnRows - 1, rows - 1);
+    int end = s.len - s.n + (int)(tlast / a.g) + 1;
+    const int begin = split * a.chunk;
+    if (split < nsplit - 1) end = min(end, begin + a.chunk);
+
+    // Q: chunk 2 step + half of the lane's row
+    uint4 qf[kSteps];
+    {
+      const char* q = a.q + (a.batch.starts != nullptr ? trow * a.qs[1]
+                                                       : b * a.qs[0] + t * a.qs[1]) + h * a.qs[2];
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+        const int c = 2 * i + hf;
+        qf[i] = make_uint4(0, 0, 0, 0);
+        if (row_ok && c < chunks) {
+          if (a.q_aligned) {
+            qf[i] = *reinterpret_cast<const uint4*>(q + c * 16);
+          } else {
+            T e[Ty::kChunk];
+#pragma unroll
+            for (int x = 0; x < Ty::kChunk; ++x)
+              e[x] = reinterpret_cast<const T*>(q)[c * Ty::kChunk + x];
+            __builtin_memcpy(&qf[i], e, 16);
+          }
+        }
+      }
+    }
+
+    f32x16 o[kDB];
+#pragma unroll
+    for (int d = 0; d < kDB; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
+    float m = -INFINITY, l = 0.0f;  // l: of this lane's keys
+
+    // The page of lane-th key of a tile, -1 where there is none.
+    auto page_of = [&](int kt) {
+      const int j = kt + (lane & (KT - 1));
+      if (j >= s.len || j >= end) return -1;
+      const int p = s.table[a.batch.div.quot(j)];
+      return p < a.batch.P ? p : -1;
+    };
+    uint64_t held = 0;
+    // Starts a tile's way into LDS: a thread's chunk u of the buffer is fetched from
+    // wherever the swizzle puts it; absent keys and channels past D are zeros.  Returns
+    // the keys that are there.
+    auto load = [&](int kt, int page, int buf) {
+      const int j = kt + (lane & (KT - 1));
+      const uint32_t at = (uint32_t)(j - a.batch.div.quot(j) * a.batch.div.size);
+      const uint32_t ku = (uint32_t)page * a.kp + at * a.ks;
+      const uint32_t vu = (uint32_t)page * a.vp + at * a.vs;
+      uint64_t there = __ballot(page >= 0);
+      if constexpr (KT == 32) there &= 0xffffffffull;
+#pragma unroll
+      for (int i = 0; i < Ti::kLoads; ++i) {
+        const int u = i * kAttnThreads + threadIdx.x;
+        const int r = u / Ti::kChunks, p = u % Ti::kChunks;
+        const uint32_t kq = __shfl(ku, r), vq = __shfl(vu, r);
+        const int kc = p ^ Ti::k_swizzle(r), vc = p ^ Ti::v_swizzle(r);
+        const bool ok = (there >> r) & 1;
+        const char* kf = ok && kc < chunks ? kbase + ((uint64_t)kq + kc) * 16
+                                           : reinterpret_cast<const char*>(&kZeros);
+        const char* vf = ok && vc < chunks ? vbase + ((uint64_t)vq + vc) * 16
+                                           : reinterpret_cast<const char*>(&kZeros);
+        load_lds16(&lds_k[buf][i * kAttnThreads + wave * 64], kf);
+        load_lds16(&lds_v[buf][i * kAttnThreads + wave * 64], vf);
+      }
+      return there;
+    };
+
+    int again = 0;
+    if (begin < end) {
+      int page = page_of(begin);
+      barrier();  // (the row tile before is read to its end)
+      uint64_t next = load(begin, page, 0);
+      page = page_of(begin + KT);
+      int buf = 0;
+      for (int kt = begin; kt < end; kt += KT, buf ^= 1) {
+        held = next;
+        // every wavefront's loads of this tile have landed, and the other buffer is read
+        wait_vmcnt<0>();
+        barrier();
+        if (kt + KT < end) {
+          next = load(kt + KT, page, buf ^ 1);
+          page = page_of(kt + 2 * KT);
+        }
+        if (kt < wave_end) {
+          f32x16 sc[KB];
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sc[kb][i] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i)
+              sc[kb] = Ty::scores(lds_k[buf][Ti::k_slot(kb * 32 + ln, 2 * i + hf)], qf[i], sc[kb]);
+          }
+          // keys that the lane's row sees, as bits from the lane half's first
+          constexpr uint64_t kAll = KT == 64 ? ~0ull : (1ull << (KT & 63)) - 1;
+          const bool masked = held != kAll || kt + KT - 1 > wave_min;
+          uint64_t seen = kAll;
+          if (masked) {
+            const int n = pos - kt + 1;  // keys up to the row's own
+            seen = n <= 0 ? 0 : held & (n >= 64 ? ~0ull : (1ull << n) - 1);
+            const uint64_t mine = seen >> (4 * hf);
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+                if (!((mine >> (kb * 32 + 8 * (i / 4) + i % 4)) & 1)) sc[kb][i] = -INFINITY;
+          }
+          float top = -INFINITY;
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, sc[kb][i]);
+          top = across_halves_max(top) * a.scale;
+          // the maximum in use stays until a score passes it by a factor of 2^8: the
+          // probabilities stay below 2^8, their sums far from overflow
+          if (__any(top > m + 8.0f)) {
+            const float mn = fmaxf(m, top);
+            const float was = m == mn ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            l *= was;
+#pragma unroll
+            for (int d = 0; d < kDB; ++d)
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[d][i] *= was;
+          }
+          const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float p = __builtin_amdgcn_exp2f(fmaf(sc[kb][i], a.scale, -base));
+              sc[kb][i] = p;
+              l += p;
+            }
+          // A value that some row of the tile may not see must not reach it, not even as
+          // 0 times infinity: rows of a masked tile that holds infinities or NaNs are
+          // computed again below.
+          if (masked) {
+            bool bad = false;
+#pragma unroll 1
+            for (int u = lane; u < Ti::kUnits; u += 64) bad |= any_nonfinite(lds_v[buf][u], T());
+            if (__any(bad)) again = 1;
+          }
+          // O^T += V^T P^T
+          if constexpr (sizeof(T) == 2) {
+            // A probability is rounded to bfloat16 for the product, 2^-8 of it at most.  Where
+            // one weighs more than about a 32nd of its row, the rest is multiplied too;
+            // below, the errors of a row's many terms average out far under the output's
+            // own rounding.
+            const bool fine = __any(__builtin_amdgcn_exp2f(top - base) * 16.0f > l);
+            auto product = [&](auto with_rest) {
+#pragma unroll
+              for (int e = 0; e < KB * 2; ++e) {
+                uint32_t w[4], rest[4];
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                  const float p0 = sc[e / 2][8 * (e % 2) + 2 * x];
+                  const float p1 = sc[e / 2][8 * (e % 2) + 2 * x + 1];
+                  w[x] = cvt_pk_bf16(p0, p1);
+                  if constexpr (decltype(with_rest)::value)
+                    rest[x] = cvt_pk_bf16(p0 - __uint_as_float(w[x] << 16),
+                                          p1 - __uint_as_float(w[x] & 0xffff0000u));
+                }
+                const bf16x8_t pf = __builtin_bit_cast(bf16x8_t, make_uint4(w[0], w[1], w[2], w[3]));
+#pragma unroll
+                for (int d = 0; d < kDB; ++d) {
+                  typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+                  union {
+                    s16x4 half[2];
+                    bf16x8_t v;
+                  } f;
+#pragma unroll
+                  for (int x = 0; x < 2; ++x) {
+                    const int r = 16 * e + 8 * x + 4 * hf + (lane & 15) / 4;
+                    const int ch = d * 32 + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+                    f.half[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                        (lds_s16x4*)(reinterpret_cast<bf16_t*>(&lds_v[buf][Ti::v_slot(r, ch / 8)]) +
+                                     ch % 8));
+                  }
+                  o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.v, pf, o[d], 0, 0, 0);
+                  if constexpr (decltype(with_rest)::value)
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                        f.v,
+                        __builtin_bit_cast(bf16x8_t, make_uint4(rest[0], rest[1], rest[2], rest[3])),
+                        o[d], 0, 0, 0);
+                }
+              }
+            };
+            if (fine)
+              product(std::true_type());
+            else
+              product(std::false_type());
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+#pragma unroll
+              for (int d = 0; d < kDB; ++d) {
+                const int r = 8 * (i / 4) + 4 * hf + i % 4, ch = d * 32 + ln;
+                const float v =
+                    reinterpret_cast<const float*>(&lds_v[buf][Ti::v_slot(r, ch / 4)])[ch % 4];
+                o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, sc[0][i], o[d], 0, 0, 0);
+              }
+          }
+        }
+      }
+    }
+
+    if (__syncthreads_or(again)) {
+      rows_one_by_one<T>(a, s, b, kvh, tile * kAttnRows, min(rows, (tile + 1) * kAttnRows), begin,
+                         end, nsplit > 1 ? part_row(a, bh, split) : -1,
+                         reinterpret_cast<float*>(lds_k));
+      continue;
+    }
+    l += __shfl_xor(l, 32);
+    if (row_ok) {
+      if (nsplit > 1) {
+        const int64_t at = part_row(a, bh, split) + row;
+        float* po = a.part + at * a.D;
+#pragma unroll
+        for (int d = 0; d < kDB; ++d)
+#pragma unroll
+          for (int i = 0; i < 16; i += 4) {
+            const int ch = d * 32 + 2 * i + 4 * hf;
+            if (ch < a.D)
+              *reinterpret_cast<float4*>(po + ch) =
+                  make_float4(o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]);
+          }
+        if (hf == 0)
+          reinterpret_cast<float2*>(a.part + part_row(a, nbh, 0) * a.D)[at] = make_float2(m, l);
+      } else {
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        char* out = a.out + (a.batch.starts != nullptr ? trow * a.os[1]
+                                                       : b * a.os[0] + t * a.os[1]) + h * a.os[2];
+#pragma unroll
+        for (int d = 0; d < kDB; ++d)
+#pragma unroll
+          for (int i = 0; i < 16; i += 4) {
+            const int ch = d * 32 + 2 * i + 4 * hf;
+            if (ch >= a.D) continue;
+            const float x[4] = {o[d][i] * inv, o[d][i + 1] * inv, o[d][i + 2] * inv,
+                                o[d][i + 3] * inv};
+            if constexpr (sizeof(T) == 2)
+              *reinterpret_cast<uint2*>(out + ch * 2) =
+                  make_uint2(cvt_pk_bf16(x[0], x[1]), cvt_pk_bf16(x[2], x[3]));
+            else
+              *reinterpret_cast<float4*>(out + ch * 4) = make_float4(x[0], x[1], x[2], x[3]);
+          }
+        if (hf == 0 && a.lse != nullptr)
+          a.lse[trow * a.NH + h] = l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
+      }
+    }
+  }
+}
+
+// Joins the splits of a row: one workgroup per row, its wavefronts taking the splits in
+// turn, a lane two channels.
+template <typename T>
+__global__ void __launch_bounds__(kAttnThreads) attn_join_kernel(const AttnArgs a) {
+  __shared__ float lds_o[kAttnWaves][128];
+  __shared__ float lds_l[kAttnWaves];
+  const int nbh = a.batch.B * a.NKVH;
+  const int bh = blockIdx.x % nbh, row = blockIdx.x / nbh;
+  const int b = bh / a.NKVH, kvh = bh - b * a.NKVH;
+  const PagedSeq s = paged_seq(a.batch, b);
+  const int nsplit = splits_of(a, s);
+  if (nsplit <= 1 || row >= (int64_t)s.n * a.g) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const float2* ml = reinterpret_cast<const float2*>(a.part + part_row(a, nbh, 0) * a.D);
+  float m = -INFINITY;
+  for (int i = lane; i < nsplit; i += 64) m = fmaxf(m, ml[part_row(a, bh, i) + row].x);
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
+  const float base = m == -INFINITY ? 0.0f : m;
+  const bool on = lane * 2 < a.D;
+  float ox = 0.0f, oy = 0.0f, l = 0.0f;
+  for (int i = wave; i < nsplit; i += kAttnWaves) {
+    const int64_t at = part_row(a, bh, i) + row;
+    const float2 p = ml[at];
+    const float w = __builtin_amdgcn_exp2f(p.x - base);
+    l = fmaf(p.y, w, l);
+    if (on) {
+      const float2 x = *reinterpret_cast<const float2*>(a.part + at * a.D + lane * 2);
+      // (a split without keys has weight 0; its o is 0 too)
+      ox = fmaf(x.x, w, ox);
+      oy = fmaf(x.y, w, oy);
+    }
+  }
+  if (on) {
+    lds_o[wave][lane * 2] = ox;
+    lds_o[wave][lane * 2 + 1] = oy;
+  }
+  if (lane == 0) lds_l[wave] = l;
+  __syncthreads();
+  const int d = threadIdx.x;
+  float sum = 0.0f, acc = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kAttnWaves; ++w) {
+    sum += lds_l[w];
+    if (d < a.D) acc += lds_o[w][d];
+  }
+  const int t = row / a.g, h = kvh * a.g + row - t * a.g;
+  const int64_t trow = a.batch.starts != nullptr ? s.row0 + t : (int64_t)b * a.batch.T + t;
+  char* out = a.out + (a.batch.starts != nullptr ? trow * a.os[1]
+                                                 : b * a.os[0] + t * a.os[1]) + h * a.os[2];
+  if (d < a.D)
+    io_traits<T>::store(reinterpret_cast<T*>(out) + d, sum == 0.0f ? 0.0f : acc / sum);
+  if (d == 0 && a.lse != nullptr)
+    a.lse[trow * a.NH + h] = sum == 0.0f ? -INFINITY
+                                         : (base + __builtin_amdgcn_logf(sum)) * kLn2;
+}
+
+// How a call is cut: row tiles of the grid, keys of a split, splits.
+struct AttnPlan {
+  int tiles, chunk, nsplit, rows_cap;
+};
+
+AttnPlan plan_attention(const ltv_paged_batch& b, int NH, int NKVH, int max_len) {
+  AttnPlan p;
+  const int64_t rows = (int64_t)std::max(b.T, 1) * (NH / NKVH);
+  p.tiles = (int)std::min<int64_t>((rows + kAttnRows - 1) / kAttnRows, 1 << 20);
+  const int64_t seqs = (int64_t)b.B * NKVH;
+  // With fewer workgroups than the card holds at a time (two per compute unit) every
+  // sequence is split, to twice that many; else those of a single row tile are, in
+  // chunks that keep a long one from outlasting the others.
+  const int64_t groups = seqs * p.tiles;
+  p.rows_cap = (int)(groups < 512 ? rows : std::min<int64_t>(rows, kAttnRows));
+  const int64_t want = (int64_t)std::max(max_len, 1) * (groups < 512 ? groups : seqs) / 1024;
+  p.chunk = (int)std::min<int64_t>(std::max<int64_t>((want + 127) / 128 * 128, 128), 1024);
+  p.nsplit = (std::max(max_len, 1) + p.chunk - 1) / p.chunk;
+  return p;
 }
 
 }  // namespace
@@ -101,9 +624,18 @@ __global__ void __launch_bounds__(256) attn_rows_kernel(const AttnArgs a) {
 
 using namespace ltv;
 
+namespace {
+size_t part_bytes(const AttnPlan& p, const ltv_paged_batch& b, int NKVH, int D) {
+  if (p.nsplit <= 1) return 0;
+  return (size_t)b.B * NKVH * p.nsplit * p.rows_cap * (D + 2) * sizeof(float);
+}
+}  // namespace
+
 extern "C" size_t ltv_paged_attention_workspace_size(int dtype, const ltv_paged_batch* batch,
                                                      int NH, int NKVH, int D, int max_len) {
-  return 0;
+  if (batch == nullptr || batch->B <= 0 || batch->T < 0 || NKVH <= 0 || NH < NKVH || D <= 0)
+    return 0;
+  return part_bytes(plan_attention(*batch, NH, NKVH, max_len), *batch, NKVH, D);
 }
 
 extern "C" int ltv_paged_attention(int dtype, const void* q, const int64_t q_strides[3],
@@ -122,26 +654,63 @@ extern "C" int ltv_paged_attention(int dtype, const void* q, const int64_t q_str
   LTV_REQUIRE(D % 8 == 0 && D <= 128, LTV_ERR_UNSUPPORTED,
               "head_dim must be a multiple of 8, at most 128 (D=%d)", D);
   if (batch->B == 0 || batch->total == 0 || NH == 0) return LTV_OK;
+  const bool pages = batch->num_pages > 0;
   LTV_REQUIRE(q && out && q_strides && out_strides && k_page_strides && v_page_strides &&
-                  ((k_pages && v_pages) || batch->num_pages == 0),
+                  (!pages || (k_pages && v_pages)),
               LTV_ERR_INVALID_ARG, "null pointer");
-  LTV_REQUIRE(scale > 0.0f && scale < INFINITY, LTV_ERR_INVALID_ARG,
-              "scale must be positive and finite (%g)", scale);
-  LTV_REQUIRE(batch->B <= 65535 && NH <= 65535, LTV_ERR_UNSUPPORTED,
-              "more than 65,535 sequences or heads");
-  AttnArgs a{PagedBatch(*batch), q, k_pages, v_pages, out, lse, {}, {}, {}, {}, NH, NKVH, D,
-             scale};
-  for (int i = 0; i < 3; ++i) {
-    a.qs[i] = q_strides[i];
-    a.ks[i] = k_page_strides[i];
-    a.vs[i] = v_page_strides[i];
-    a.os[i] = out_strides[i];
+  const int es = elem_size(dtype), chunk = 16 / es;
+  const AttnPlan p = plan_attention(*batch, NH, NKVH, max_len);
+  LTV_REQUIRE(workspace_bytes >= part_bytes(p, *batch, NKVH, D) && (p.nsplit <= 1 || workspace),
+              LTV_ERR_WORKSPACE, "workspace too small");
+  // pages are addressed in 16-byte units of 32 bits
+  bool fits = true, aligned = aligned16(k_pages) && aligned16(v_pages);
+  for (int i = 0; i < 3; ++i)
+    for (const int64_t st : {k_page_strides[i], v_page_strides[i]}) {
+      aligned = aligned && st % chunk == 0;
+      const int64_t n = i == 0 ? batch->num_pages : i == 1 ? 1 : batch->page_size;
+      fits = fits && st >= 0 && (st == 0 || n <= (int64_t(1) << 31) / std::max<int64_t>(1, st / chunk));
+    }
+  LTV_REQUIRE(!pages || aligned, LTV_ERR_UNSUPPORTED, "the pages' rows must be 16-byte aligned");
+  LTV_REQUIRE(!pages || fits, LTV_ERR_UNSUPPORTED,
+              "the pages of a layer must lie within 32 GiB, with strides that are not negative");
+  bool out_ok = aligned16(out), q_aligned = aligned16(q);
+  for (int i = batch->starts != nullptr ? 1 : 0; i < 3; ++i) {
+    out_ok = out_ok && out_strides[i] % chunk == 0;
+    q_aligned = q_aligned && q_strides[i] % chunk == 0;
   }
-  const dim3 grid(std::max(1, std::min(batch->T, 65535)), NH, batch->B);
-  if (dtype == LTV_DTYPE_F32)
-    hipLaunchKernelGGL(attn_rows_kernel<float>, grid, dim3(256), 0, (hipStream_t)stream, a);
-  else
-    hipLaunchKernelGGL(attn_rows_kernel<bf16_t>, grid, dim3(256), 0, (hipStream_t)stream, a);
+  LTV_REQUIRE(out_ok, LTV_ERR_UNSUPPORTED, "the output's rows must be 16-byte aligned");
+  AttnArgs a{PagedBatch(*batch), (const char*)q, (const char*)k_pages, (const char*)v_pages,
+             (char*)out, lse, (float*)workspace, {}, {}, k_page_strides[1] * es,
+             v_page_strides[1] * es, (uint32_t)(k_page_strides[0] / chunk),
+             (uint32_t)(k_page_strides[2] / chunk), (uint32_t)(v_page_strides[0] / chunk),
+             (uint32_t)(v_page_strides[2] / chunk), NH, NKVH, D, NH / NKVH, q_aligned ? 1 : 0,
+             scale * kLog2e, p.tiles, p.chunk, p.nsplit, p.rows_cap};
+  for (int i = 0; i < 3; ++i) {
+    a.qs[i] = q_strides[i] * es;
+    a.os[i] = out_strides[i] * es;
+  }
+  const int64_t seqs = (int64_t)batch->B * NKVH;
+  const int64_t grid = seqs * p.tiles * p.nsplit, joins = seqs * p.rows_cap;
+  LTV_REQUIRE(grid < (int64_t(1) << 31) && joins < (int64_t(1) << 31), LTV_ERR_UNSUPPORTED,
+              "too many workgroups");
+  const hipStream_t st = (hipStream_t)stream;
+  auto launch = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(kAttnThreads), 0, st, a);
+  };
+  if (dtype == LTV_DTYPE_F32) {
+    if (D <= 64) launch(attn_tile_kernel<float, 64>); else launch(attn_tile_kernel<float, 128>);
+  } else {
+    if (D <= 64) launch(attn_tile_kernel<bf16_t, 64>); else launch(attn_tile_kernel<bf16_t, 128>);
+  }
   LTV_LAUNCH_CHECK();
+  if (p.nsplit > 1) {
+    if (dtype == LTV_DTYPE_F32)
+      hipLaunchKernelGGL(attn_join_kernel<float>, dim3((unsigned)joins), dim3(kAttnThreads), 0, st,
+                         a);
+    else
+      hipLaunchKernelGGL(attn_join_kernel<bf16_t>, dim3((unsigned)joins), dim3(kAttnThreads), 0,
+                         st, a);
+    LTV_LAUNCH_CHECK();
+  }
   return LTV_OK;
 }
