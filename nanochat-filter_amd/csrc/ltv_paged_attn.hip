@@ -51,7 +51,9 @@ struct AttnArgs {
   float scale;                // with log2(e)
   int tiles;                  // row tiles of the grid
   int chunk, nsplit;          // keys of a split, splits of the grid
-  int rows_cap;               // sequences of more rows are not split
+  int64_t rows_cap;           // sequences of more rows are not split
+  int by_token;               // how the partials are laid out
+  int64_t part_rows;
 };
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -66,7 +68,7 @@ struct AttnType<bf16_t> {
   static constexpr int kChunk = 8;  // elements
   static constexpr int kKeys = 64;  // keys of a tile
   // S^T += K Q^T over 16 channels: a lane's k and q chunk hold channels 8 (lane / 32) ..
-  static __device__ __forceinline__ f32x16 scores(uint4 k, uint4 q, f32x16 s) {
+  static __device__ __forceinline__ f32x16 scores(u32x4_t k, uint4 q, f32x16 s) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, k),
                                                    __builtin_bit_cast(bf16x8_t, q), s, 0, 0, 0);
   }
@@ -76,7 +78,7 @@ template <>
 struct AttnType<float> {
   static constexpr int kChunk = 4;
   static constexpr int kKeys = 32;
-  static __device__ __forceinline__ f32x16 scores(uint4 k, uint4 q, f32x16 s) {
+  static __device__ __forceinline__ f32x16 scores(u32x4_t k, uint4 q, f32x16 s) {
     s = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(k.x), __uint_as_float(q.x), s, 0, 0, 0);
     s = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(k.y), __uint_as_float(q.y), s, 0, 0, 0);
     s = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(k.z), __uint_as_float(q.z), s, 0, 0, 0);
@@ -105,22 +107,24 @@ struct AttnTile {
     if constexpr (sizeof(T) == 4) return ((r >> 2) & 1) * 8;
     return ((r / kPhase) & (4 / kPhase - 1)) * 4;
   }
-  static __device__ __forceinline__ int k_slot(int r, int c) {
-    return r * kChunks + (c ^ k_swizzle(r));
-  }
-  static __device__ __forceinline__ int v_slot(int r, int c) {
-    return r * kChunks + (c ^ v_swizzle(r));
-  }
 };
 
 __device__ const uint4 kZeros = {0, 0, 0, 0};
+
+__device__ __forceinline__ uint32_t lds_address(uint4* p) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint4*)p;
+}
+template <typename V>
+__device__ __forceinline__ V lds_read(uint32_t at) {
+  return *(__attribute__((address_space(3))) const V*)(uintptr_t)at;
+}
 
 // One wavefront's 16 bytes per lane from `from` into LDS at `to` + 16 lane (`to` uniform).
 // Inline assembly, as in the projection's kernels: the compiler would wait for a builtin's
 // load before the next read of either buffer.  It has no output register; the wait is
 // wait_vmcnt and a barrier.  The nop covers the write of M0.
 __device__ __forceinline__ void load_lds16(uint4* to, const char* from) {
-  const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint4*)to;
+  const uint32_t base = lds_address(to);
   asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(from), "{m0}"(base) : "memory");
 }
 
@@ -157,19 +161,26 @@ __device__ __forceinline__ int splits_of(const AttnArgs& a, const PagedSeq& s) {
   return max(1, min(a.nsplit, (s.len + a.chunk - 1) / a.chunk));
 }
 
-// Partials of (sequence b, k/v head, split): rows_cap rows of D values, and of (m, l).
-__device__ __forceinline__ int64_t part_row(const AttnArgs& a, int bh, int split) {
-  return ((int64_t)bh * a.nsplit + split) * a.rows_cap;
+// A row's place among the partials (D values each; behind them all, its m and l): by its
+// token and head where any sequence may be split, else among the rows_cap of its sequence
+// and k/v head.
+__device__ __forceinline__ int64_t part_row(const AttnArgs& a, int bh, int split, int64_t row,
+                                            int64_t trow, int h) {
+  if (a.by_token) return ((int64_t)split * a.batch.total + trow) * a.NH + h;
+  return ((int64_t)bh * a.nsplit + split) * a.rows_cap + row;
+}
+__device__ __forceinline__ float2* part_ml(const AttnArgs& a) {
+  return reinterpret_cast<float2*>(a.part + a.part_rows * a.D);
 }
 
 // Rows row0 .. row_end - 1 of a workgroup over keys begin .. end - 1, each key that a row
 // does not see left alone altogether: the way of tiles with infinite or NaN values among
 // those that some rows do not see.  Sixteen groups of sixteen lanes take a row's keys in
-// turn, a lane holding eight channels.  at: the first row's place in the partials, or -1.
+// turn, a lane holding eight channels.  split: whose partials these are, or -1.
 template <typename T>
 __device__ __forceinline__ void rows_one_by_one(const AttnArgs& a, const PagedSeq& s, int b,
                                                 int kvh, int64_t row0, int64_t row_end, int begin,
-                                                int end, int64_t at, float* lds) {
+                                                int end, int split, float* lds) {
   float* lds_m = lds;
   float* lds_l = lds + 16;
   float* lds_o = lds + 32;  // 16 x 128
@@ -225,11 +236,10 @@ __device__ __forceinline__ void rows_one_by_one(const AttnArgs& a, const PagedSe
       sum = fmaf(lds_l[i], w, sum);
       if (d < a.D) acc = fmaf(lds_o[i * 128 + d], w, acc);
     }
-    if (at >= 0) {
-      if (d < a.D) a.part[(at + row) * a.D + d] = acc;
-      if (d == 0)
-        reinterpret_cast<float2*>(a.part + part_row(a, a.batch.B * a.NKVH, 0) * a.D)[at + row] =
-            make_float2(mx, sum);
+    if (split >= 0) {
+      const int64_t at = part_row(a, b * a.NKVH + kvh, split, row, trow, h);
+      if (d < a.D) a.part[at * a.D + d] = acc;
+      if (d == 0) part_ml(a)[at] = make_float2(mx, sum);
     } else {
       char* out = a.out + (a.batch.starts != nullptr ? trow * a.os[1]
                                                      : b * a.os[0] + t * a.os[1]) + h * a.os[2];
@@ -242,28 +252,32 @@ __device__ __forceinline__ void rows_one_by_one(const AttnArgs& a, const PagedSe
   }
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool PAD>
 __global__ void __launch_bounds__(kAttnThreads, 2) attn_tile_kernel(const AttnArgs a) {
   using Ty = AttnType<T>;
   using Ti = AttnTile<T, DP>;
   constexpr int KT = Ti::kKeys, KB = KT / 32;
   constexpr int kSteps = Ti::kChunks / 2;  // score products' steps: two chunks each
   constexpr int kDB = DP / 32;
-  __shared__ uint4 lds_k[2][Ti::kUnits];
-  __shared__ uint4 lds_v[2][Ti::kUnits];
+  constexpr int kRow = Ti::kChunks * 16, kTile = Ti::kUnits * 16;  // bytes
+  __shared__ uint4 lds[4 * Ti::kUnits];                            // K, V, and again
 
+  // Workgroup w runs on XCD w % 8.  Splits go around the XCDs from a start that differs
+  // by sequence, head and row tile, or those in use would land on few of them.  The row
+  // tiles with the most keys start first.
   const int nbh = a.batch.B * a.NKVH;
-  const int bh = blockIdx.x % nbh;
-  int rest = blockIdx.x / nbh;
-  const int split = rest % a.nsplit;
-  const int tile0 = a.tiles - 1 - rest / a.nsplit;  // the tiles with the most keys first
+  int rest = blockIdx.x;
+  int split = rest % a.nsplit;
+  rest /= a.nsplit;
+  const int bh = rest % nbh;
+  const int tile0 = a.tiles - 1 - rest / nbh;
+  split = (int)(((unsigned)split + (unsigned)bh + (unsigned)tile0) % (unsigned)a.nsplit);
   const int b = bh / a.NKVH, kvh = bh - b * a.NKVH;
   const PagedSeq s = paged_seq(a.batch, b);
   const int nsplit = splits_of(a, s);
   if (split >= nsplit) return;
   const int64_t rows = (int64_t)s.n * a.g;
 
-  const int lane = threadIdx.x & 63, ln = lane & 31, hf = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const char* kbase = a.k + (int64_t)kvh * a.kh;
   const char* vbase = a.v + (int64_t)kvh * a.vh;
@@ -271,6 +285,10 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_tile_kernel(const AttnAr
 
   // (more rows than the grid was sized for: its tiles are walked again)
   for (int64_t tile = tile0; tile * kAttnRows < rows; tile += a.tiles) {
+    // (opaque: what follows from the lane is not kept in registers around this loop)
+    int thread = threadIdx.x;
+    asm volatile("" : "+v"(thread));
+    const int lane = thread & 63, ln = lane & 31, hf = lane >> 5;
     const int64_t row = tile * kAttnRows + wave * 32 + ln;
     const bool row_ok = row < rows;
     const int t = row_ok ? (int)(row / a.g) : 0;
@@ -285,7 +303,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_tile_kernel(const AttnAr
     const int wave_min = wave_on
         ? s.len - s.n + (int)((tile * kAttnRows + wave * 32) / a.g) : 0;
     const int64_t tlast = min(tile * kAttnRows + kAttnRows - 1, rows - 1);
-    int end = s.len - s.n + (int)(tlast / a.g) + 1;
+    int end = a.batch.P > 0 ? s.len - s.n + (int)(tlast / a.g) + 1 : 0;
     const int begin = split * a.chunk;
     if (split < nsplit - 1) end = min(end, begin + a.chunk);
 
@@ -319,41 +337,56 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_tile_kernel(const AttnAr
       for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
     float m = -INFINITY, l = 0.0f;  // l: of this lane's keys
 
-    // The page of lane-th key of a tile, -1 where there is none.
+    // The page of the lane-th key of a tile (past the end: of the last key), -1: none.
     auto page_of = [&](int kt) {
-      const int j = kt + (lane & (KT - 1));
-      if (j >= s.len || j >= end) return -1;
-      const int p = s.table[a.batch.div.quot(j)];
+      const int p = s.table[a.batch.div.quot(min(kt + (lane & (KT - 1)), end - 1))];
       return p < a.batch.P ? p : -1;
     };
     uint64_t held = 0;
     // Starts a tile's way into LDS: a thread's chunk u of the buffer is fetched from
-    // wherever the swizzle puts it; absent keys and channels past D are zeros.  Returns
+    // wherever the swizzle puts it, channels past D are zeros.  For a key past the end the
+    // last one is fetched, for one of no page some row: their scores are masked.  Returns
     // the keys that are there.
     auto load = [&](int kt, int page, int buf) {
-      const int j = kt + (lane & (KT - 1));
-      const uint32_t at = (uint32_t)(j - a.batch.div.quot(j) * a.batch.div.size);
-      const uint32_t ku = (uint32_t)page * a.kp + at * a.ks;
-      const uint32_t vu = (uint32_t)page * a.vp + at * a.vs;
-      uint64_t there = __ballot(page >= 0);
+      const int j = kt + (lane & (KT - 1)), jj = min(j, end - 1);
+      const uint32_t at = (uint32_t)(jj - a.batch.div.quot(jj) * a.batch.div.size);
+      const uint32_t from = (uint32_t)max(page, 0);
+      const uint32_t ku = from * a.kp + at * a.ks;
+      const uint32_t vu = from * a.vp + at * a.vs;
+      uint64_t there = __ballot(page >= 0 && j < end);
       if constexpr (KT == 32) there &= 0xffffffffull;
 #pragma unroll
       for (int i = 0; i < Ti::kLoads; ++i) {
-        const int u = i * kAttnThreads + threadIdx.x;
+        const int u = i * kAttnThreads + thread;
         const int r = u / Ti::kChunks, p = u % Ti::kChunks;
         const uint32_t kq = __shfl(ku, r), vq = __shfl(vu, r);
         const int kc = p ^ Ti::k_swizzle(r), vc = p ^ Ti::v_swizzle(r);
-        const bool ok = (there >> r) & 1;
-        const char* kf = ok && kc < chunks ? kbase + ((uint64_t)kq + kc) * 16
-                                           : reinterpret_cast<const char*>(&kZeros);
-        const char* vf = ok && vc < chunks ? vbase + ((uint64_t)vq + vc) * 16
-                                           : reinterpret_cast<const char*>(&kZeros);
-        load_lds16(&lds_k[buf][i * kAttnThreads + wave * 64], kf);
-        load_lds16(&lds_v[buf][i * kAttnThreads + wave * 64], vf);
+        const char* kf = kbase + ((uint64_t)kq + kc) * 16;
+        const char* vf = vbase + ((uint64_t)vq + vc) * 16;
+        if constexpr (PAD) {
+          kf = kc < chunks ? kf : reinterpret_cast<const char*>(&kZeros);
+          vf = vc < chunks ? vf : reinterpret_cast<const char*>(&kZeros);
+        }
+        uint4* to = lds + buf * 2 * Ti::kUnits + i * kAttnThreads + wave * 64;
+        load_lds16(to, kf);
+        load_lds16(to + Ti::kUnits, vf);
       }
       return there;
     };
 
+    // Where the lane reads K's row ln, and V's four rows from 4 hf (bfloat16) or row 4 hf
+    // (float32), in the first buffer.  The swizzles exclusive-or a slot, so a later step's
+    // chunk is an exclusive or away; rows further on a constant.
+    const uint32_t lds0 = lds_address(lds);
+    const uint32_t kat = lds0 + ln * kRow + (hf ^ Ti::k_swizzle(ln)) * 16;
+    uint32_t vat = lds0 + kTile;
+    if constexpr (sizeof(T) == 2) {
+      const int r = 4 * hf + (lane & 15) / 4;
+      vat += r * kRow + ((((lane >> 4) & 1) * 2 + (lane & 3) / 2) ^ Ti::v_swizzle(r)) * 16 +
+             (lane & 1) * 8;
+    } else {
+      vat += 4 * hf * kRow + ((ln / 4) ^ Ti::v_swizzle(4 * hf)) * 16 + (ln % 4) * 4;
+    }
     int again = 0;
     if (begin < end) {
       int page = page_of(begin);
@@ -371,6 +404,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_tile_kernel(const AttnAr
           page = page_of(kt + 2 * KT);
         }
         if (kt < wave_end) {
+          const uint32_t ka = kat + buf * 2 * kTile, va = vat + buf * 2 * kTile;
           f32x16 sc[KB];
 #pragma unroll
           for (int kb = 0; kb < KB; ++kb) {
@@ -378,7 +412,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_tile_kernel(const AttnAr
             for (int i = 0; i < 16; ++i) sc[kb][i] = 0.0f;
 #pragma unroll
             for (int i = 0; i < kSteps; ++i)
-              sc[kb] = Ty::scores(lds_k[buf][Ti::k_slot(kb * 32 + ln, 2 * i + hf)], qf[i], sc[kb]);
+              sc[kb] = Ty::scores(lds_read<u32x4_t>((ka ^ (32 * i)) + kb * 32 * kRow), qf[i], sc[kb]);
           }
           // keys that the lane's row sees, as bits from the lane half's first
           constexpr uint64_t kAll = KT == 64 ? ~0ull : (1ull << (KT & 63)) - 1;
@@ -427,7 +461,8 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_tile_kernel(const AttnAr
           if (masked) {
             bool bad = false;
 #pragma unroll 1
-            for (int u = lane; u < Ti::kUnits; u += 64) bad |= any_nonfinite(lds_v[buf][u], T());
+            for (int u = lane; u < Ti::kUnits; u += 64) 
+              bad |= any_nonfinite(lds[(2 * buf + 1) * Ti::kUnits + u], T());
             if (__any(bad)) again = 1;
           }
           // O^T += V^T P^T
@@ -459,13 +494,9 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_tile_kernel(const AttnAr
                     bf16x8_t v;
                   } f;
 #pragma unroll
-                  for (int x = 0; x < 2; ++x) {
-                    const int r = 16 * e + 8 * x + 4 * hf + (lane & 15) / 4;
-                    const int ch = d * 32 + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+                  for (int x = 0; x < 2; ++x)
                     f.half[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                        (lds_s16x4*)(reinterpret_cast<bf16_t*>(&lds_v[buf][Ti::v_slot(r, ch / 8)]) +
-                                     ch % 8));
-                  }
+                        (lds_s16x4*)(uintptr_t)((va ^ (64 * d)) + (16 * e + 8 * x) * kRow));
                   o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.v, pf, o[d], 0, 0, 0);
                   if constexpr (decltype(with_rest)::value)
                     o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
@@ -484,9 +515,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_tile_kernel(const AttnAr
             for (int i = 0; i < 16; ++i)
 #pragma unroll
               for (int d = 0; d < kDB; ++d) {
-                const int r = 8 * (i / 4) + 4 * hf + i % 4, ch = d * 32 + ln;
-                const float v =
-                    reinterpret_cast<const float*>(&lds_v[buf][Ti::v_slot(r, ch / 4)])[ch % 4];
+                const float v = lds_read<float>((va ^ (128 * d)) + (8 * (i / 4) + i % 4) * kRow);
                 o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, sc[0][i], o[d], 0, 0, 0);
               }
           }
@@ -496,14 +525,13 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_tile_kernel(const AttnAr
 
     if (__syncthreads_or(again)) {
       rows_one_by_one<T>(a, s, b, kvh, tile * kAttnRows, min(rows, (tile + 1) * kAttnRows), begin,
-                         end, nsplit > 1 ? part_row(a, bh, split) : -1,
-                         reinterpret_cast<float*>(lds_k));
+                         end, nsplit > 1 ? split : -1, reinterpret_cast<float*>(lds));
       continue;
     }
     l += __shfl_xor(l, 32);
     if (row_ok) {
       if (nsplit > 1) {
-        const int64_t at = part_row(a, bh, split) + row;
+        const int64_t at = part_row(a, bh, split, row, trow, h);
         float* po = a.part + at * a.D;
 #pragma unroll
         for (int d = 0; d < kDB; ++d)
@@ -514,8 +542,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_tile_kernel(const AttnAr
               *reinterpret_cast<float4*>(po + ch) =
                   make_float4(o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]);
           }
-        if (hf == 0)
-          reinterpret_cast<float2*>(a.part + part_row(a, nbh, 0) * a.D)[at] = make_float2(m, l);
+        if (hf == 0) part_ml(a)[at] = make_float2(m, l);
       } else {
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         char* out = a.out + (a.batch.starts != nullptr ? trow * a.os[1]
@@ -541,82 +568,136 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_tile_kernel(const AttnAr
   }
 }
 
-// Joins the splits of a row: one workgroup per row, its wavefronts taking the splits in
-// turn, a lane two channels.
-template <typename T>
-__global__ void __launch_bounds__(kAttnThreads) attn_join_kernel(const AttnArgs a) {
-  __shared__ float lds_o[kAttnWaves][128];
-  __shared__ float lds_l[kAttnWaves];
-  const int nbh = a.batch.B * a.NKVH;
-  const int bh = blockIdx.x % nbh, row = blockIdx.x / nbh;
-  const int b = bh / a.NKVH, kvh = bh - b * a.NKVH;
-  const PagedSeq s = paged_seq(a.batch, b);
+// Joins the splits of a row: W wavefronts per row take them in turn, a lane two channels
+// (one wavefront, four rows to a workgroup, up to 16 splits; else 4 or 16).
+template <typename T, int W>
+__global__ void __launch_bounds__(W < 4 ? 256 : W * 64) attn_join_kernel(const AttnArgs a) {
+  __shared__ float lds_o[W][128];
+  __shared__ float lds_l[W];
+  const int lane = threadIdx.x & 63, wave = W == 1 ? 0 : threadIdx.x >> 6;
+  int64_t unit = blockIdx.x;
+  if (W == 1) unit = unit * 4 + (threadIdx.x >> 6);
+  int b, h;
+  int64_t row, trow;
+  PagedSeq s;
+  if (a.by_token) {
+    trow = unit / a.NH;
+    h = (int)(unit - trow * a.NH);
+    if (trow >= a.batch.total) return;
+    if (a.batch.starts != nullptr) {
+      // the last sequence that starts at the row or before it
+      int lo = 0, hi = a.batch.B - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (a.batch.starts[mid] <= trow) lo = mid; else hi = mid - 1;
+      }
+      b = lo;
+    } else {
+      b = (int)(trow / a.batch.T);
+    }
+    s = paged_seq(a.batch, b);
+    const int64_t t = a.batch.starts != nullptr ? trow - s.row0 : trow - (int64_t)b * a.batch.T;
+    if (t < 0 || t >= s.n) return;
+    row = t * a.g + h % a.g;
+  } else {
+    const int nbh = a.batch.B * a.NKVH;
+    row = unit / nbh;
+    const int bh = (int)(unit - row * nbh);
+    b = bh / a.NKVH;
+    s = paged_seq(a.batch, b);
+    if (row >= a.rows_cap || row >= (int64_t)s.n * a.g) return;
+    const int64_t t = row / a.g;
+    h = (bh - b * a.NKVH) * a.g + (int)(row - t * a.g);
+    trow = a.batch.starts != nullptr ? s.row0 + t : (int64_t)b * a.batch.T + t;
+  }
   const int nsplit = splits_of(a, s);
-  if (nsplit <= 1 || row >= (int64_t)s.n * a.g) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const float2* ml = reinterpret_cast<const float2*>(a.part + part_row(a, nbh, 0) * a.D);
+  if (nsplit <= 1) return;
+  const int bh = b * a.NKVH + h / a.g;
+  const int64_t first = part_row(a, bh, 0, row, trow, h);
+  const int64_t step = part_row(a, bh, 1, row, trow, h) - first;
+  const float2* ml = part_ml(a) + first;
+  const float* part = a.part + first * a.D;
   float m = -INFINITY;
-  for (int i = lane; i < nsplit; i += 64) m = fmaxf(m, ml[part_row(a, bh, i) + row].x);
+  for (int i = lane; i < nsplit; i += 64) m = fmaxf(m, ml[i * step].x);
 #pragma unroll
   for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
   const float base = m == -INFINITY ? 0.0f : m;
   const bool on = lane * 2 < a.D;
   float ox = 0.0f, oy = 0.0f, l = 0.0f;
-  for (int i = wave; i < nsplit; i += kAttnWaves) {
-    const int64_t at = part_row(a, bh, i) + row;
-    const float2 p = ml[at];
+#pragma unroll 4
+  for (int i = wave; i < nsplit; i += W) {
+    const float2 p = ml[i * step];
+    const float2 x = on ? *reinterpret_cast<const float2*>(part + i * step * a.D + lane * 2)
+                        : make_float2(0.0f, 0.0f);
+    // (a split without keys has weight 0; its sums are 0 too)
     const float w = __builtin_amdgcn_exp2f(p.x - base);
     l = fmaf(p.y, w, l);
+    ox = fmaf(x.x, w, ox);
+    oy = fmaf(x.y, w, oy);
+  }
+  if constexpr (W > 1) {
     if (on) {
-      const float2 x = *reinterpret_cast<const float2*>(a.part + at * a.D + lane * 2);
-      // (a split without keys has weight 0; its o is 0 too)
-      ox = fmaf(x.x, w, ox);
-      oy = fmaf(x.y, w, oy);
+      lds_o[wave][lane * 2] = ox;
+      lds_o[wave][lane * 2 + 1] = oy;
+    }
+    if (lane == 0) lds_l[wave] = l;
+    __syncthreads();
+    if (wave != 0) return;
+    ox = oy = l = 0.0f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      l += lds_l[w];
+      if (on) {
+        ox += lds_o[w][lane * 2];
+        oy += lds_o[w][lane * 2 + 1];
+      }
     }
   }
-  if (on) {
-    lds_o[wave][lane * 2] = ox;
-    lds_o[wave][lane * 2 + 1] = oy;
-  }
-  if (lane == 0) lds_l[wave] = l;
-  __syncthreads();
-  const int d = threadIdx.x;
-  float sum = 0.0f, acc = 0.0f;
-#pragma unroll
-  for (int w = 0; w < kAttnWaves; ++w) {
-    sum += lds_l[w];
-    if (d < a.D) acc += lds_o[w][d];
-  }
-  const int t = row / a.g, h = kvh * a.g + row - t * a.g;
-  const int64_t trow = a.batch.starts != nullptr ? s.row0 + t : (int64_t)b * a.batch.T + t;
+  const int64_t t = row / a.g;
   char* out = a.out + (a.batch.starts != nullptr ? trow * a.os[1]
                                                  : b * a.os[0] + t * a.os[1]) + h * a.os[2];
-  if (d < a.D)
-    io_traits<T>::store(reinterpret_cast<T*>(out) + d, sum == 0.0f ? 0.0f : acc / sum);
-  if (d == 0 && a.lse != nullptr)
-    a.lse[trow * a.NH + h] = sum == 0.0f ? -INFINITY
-                                         : (base + __builtin_amdgcn_logf(sum)) * kLn2;
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  if (on) {
+    if constexpr (sizeof(T) == 2)
+      reinterpret_cast<uint32_t*>(out)[lane] = cvt_pk_bf16(ox * inv, oy * inv);
+    else
+      reinterpret_cast<float2*>(out)[lane] = make_float2(ox * inv, oy * inv);
+  }
+  if (lane == 0 && a.lse != nullptr)
+    a.lse[trow * a.NH + h] = l == 0.0f ? -INFINITY : (base + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
-// How a call is cut: row tiles of the grid, keys of a split, splits.
+// How a call is cut: row tiles of the grid, keys of a split, splits, and where the
+// splits' partials go.
 struct AttnPlan {
-  int tiles, chunk, nsplit, rows_cap;
+  int tiles, chunk, nsplit, by_token;
+  int64_t rows_cap, joins, part_rows;
 };
 
 AttnPlan plan_attention(const ltv_paged_batch& b, int NH, int NKVH, int max_len) {
   AttnPlan p;
-  const int64_t rows = (int64_t)std::max(b.T, 1) * (NH / NKVH);
+  const int64_t g = NH / NKVH, rows = std::max(b.T, 1) * g, seqs = (int64_t)b.B * NKVH;
   p.tiles = (int)std::min<int64_t>((rows + kAttnRows - 1) / kAttnRows, 1 << 20);
-  const int64_t seqs = (int64_t)b.B * NKVH;
-  // With fewer workgroups than the card holds at a time (two per compute unit) every
-  // sequence is split, to twice that many; else those of a single row tile are, in
-  // chunks that keep a long one from outlasting the others.
-  const int64_t groups = seqs * p.tiles;
-  p.rows_cap = (int)(groups < 512 ? rows : std::min<int64_t>(rows, kAttnRows));
-  const int64_t want = (int64_t)std::max(max_len, 1) * (groups < 512 ? groups : seqs) / 1024;
-  p.chunk = (int)std::min<int64_t>(std::max<int64_t>((want + 127) / 128 * 128, 128), 1024);
-  p.nsplit = (std::max(max_len, 1) + p.chunk - 1) / p.chunk;
+  // The row tiles there are at most.  The card holds 512 workgroups at a time (two per
+  // compute unit).  With fewer row tiles than five times that, every sequence is split
+  // into about that many workgroups, or the last ones of few would run alone; else those
+  // of a single tile are.  Chunks of at most 1,024 keys for each tile of a sequence keep
+  // a long one from outlasting the others.
+  const int64_t tiles = std::min(seqs * p.tiles, (b.total * g / kAttnRows + b.B) * NKVH);
+  p.by_token = tiles < 2560;
+  p.rows_cap = p.by_token ? int64_t(1) << 40 : std::min<int64_t>(rows, kAttnRows);
+  const int64_t keys = std::max(max_len, 1);
+  const int64_t want = keys * (p.by_token ? tiles : seqs) / 2560;
+  p.chunk = (int)std::min<int64_t>(std::max<int64_t>((want + 127) / 128 * 128, 128),
+                                   p.by_token ? int64_t(1024) * p.tiles : 1024);
+  p.nsplit = (int)((keys + p.chunk - 1) / p.chunk);
+  p.joins = p.by_token ? b.total * NH : seqs * p.rows_cap;
+  p.part_rows = p.nsplit * (p.by_token ? b.total * NH : seqs * p.rows_cap);
   return p;
+}
+
+size_t part_bytes(const AttnPlan& p, int D) {
+  return p.nsplit <= 1 ? 0 : (size_t)p.part_rows * (D + 2) * sizeof(float);
 }
 
 }  // namespace
@@ -624,18 +705,11 @@ AttnPlan plan_attention(const ltv_paged_batch& b, int NH, int NKVH, int max_len)
 
 using namespace ltv;
 
-namespace {
-size_t part_bytes(const AttnPlan& p, const ltv_paged_batch& b, int NKVH, int D) {
-  if (p.nsplit <= 1) return 0;
-  return (size_t)b.B * NKVH * p.nsplit * p.rows_cap * (D + 2) * sizeof(float);
-}
-}  // namespace
-
 extern "C" size_t ltv_paged_attention_workspace_size(int dtype, const ltv_paged_batch* batch,
                                                      int NH, int NKVH, int D, int max_len) {
   if (batch == nullptr || batch->B <= 0 || batch->T < 0 || NKVH <= 0 || NH < NKVH || D <= 0)
     return 0;
-  return part_bytes(plan_attention(*batch, NH, NKVH, max_len), *batch, NKVH, D);
+  return part_bytes(plan_attention(*batch, NH, NKVH, max_len), D);
 }
 
 extern "C" int ltv_paged_attention(int dtype, const void* q, const int64_t q_strides[3],
@@ -660,7 +734,7 @@ extern "C" int ltv_paged_attention(int dtype, const void* q, const int64_t q_str
               LTV_ERR_INVALID_ARG, "null pointer");
   const int es = elem_size(dtype), chunk = 16 / es;
   const AttnPlan p = plan_attention(*batch, NH, NKVH, max_len);
-  LTV_REQUIRE(workspace_bytes >= part_bytes(p, *batch, NKVH, D) && (p.nsplit <= 1 || workspace),
+  LTV_REQUIRE(workspace_bytes >= part_bytes(p, D) && (p.nsplit <= 1 || workspace),
               LTV_ERR_WORKSPACE, "workspace too small");
   // pages are addressed in 16-byte units of 32 bits
   bool fits = true, aligned = aligned16(k_pages) && aligned16(v_pages);
@@ -684,32 +758,41 @@ extern "C" int ltv_paged_attention(int dtype, const void* q, const int64_t q_str
              v_page_strides[1] * es, (uint32_t)(k_page_strides[0] / chunk),
              (uint32_t)(k_page_strides[2] / chunk), (uint32_t)(v_page_strides[0] / chunk),
              (uint32_t)(v_page_strides[2] / chunk), NH, NKVH, D, NH / NKVH, q_aligned ? 1 : 0,
-             scale * kLog2e, p.tiles, p.chunk, p.nsplit, p.rows_cap};
+             scale * kLog2e, p.tiles, p.chunk, p.nsplit, p.rows_cap,
+             p.by_token, p.part_rows};
   for (int i = 0; i < 3; ++i) {
     a.qs[i] = q_strides[i] * es;
     a.os[i] = out_strides[i] * es;
   }
   const int64_t seqs = (int64_t)batch->B * NKVH;
-  const int64_t grid = seqs * p.tiles * p.nsplit, joins = seqs * p.rows_cap;
+  const int64_t grid = seqs * p.tiles * p.nsplit, joins = p.joins;
   LTV_REQUIRE(grid < (int64_t(1) << 31) && joins < (int64_t(1) << 31), LTV_ERR_UNSUPPORTED,
               "too many workgroups");
   const hipStream_t st = (hipStream_t)stream;
   auto launch = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(kAttnThreads), 0, st, a);
   };
-  if (dtype == LTV_DTYPE_F32) {
-    if (D <= 64) launch(attn_tile_kernel<float, 64>); else launch(attn_tile_kernel<float, 128>);
-  } else {
-    if (D <= 64) launch(attn_tile_kernel<bf16_t, 64>); else launch(attn_tile_kernel<bf16_t, 128>);
-  }
+  auto by_width = [&](auto type) {
+    using T = decltype(type);
+    if (D == 64) launch(attn_tile_kernel<T, 64, false>);
+    else if (D < 64) launch(attn_tile_kernel<T, 64, true>);
+    else if (D == 128) launch(attn_tile_kernel<T, 128, false>);
+    else launch(attn_tile_kernel<T, 128, true>);
+  };
+  if (dtype == LTV_DTYPE_F32) by_width(float()); else by_width(bf16_t());
   LTV_LAUNCH_CHECK();
   if (p.nsplit > 1) {
-    if (dtype == LTV_DTYPE_F32)
-      hipLaunchKernelGGL(attn_join_kernel<float>, dim3((unsigned)joins), dim3(kAttnThreads), 0, st,
-                         a);
-    else
-      hipLaunchKernelGGL(attn_join_kernel<bf16_t>, dim3((unsigned)joins), dim3(kAttnThreads), 0,
-                         st, a);
+    auto join = [&](auto type) {
+      using T = decltype(type);
+      if (p.nsplit <= 16)
+        hipLaunchKernelGGL((attn_join_kernel<T, 1>), dim3((unsigned)((joins + 3) / 4)), dim3(256),
+                           0, st, a);
+      else if (p.nsplit <= 64)
+        hipLaunchKernelGGL((attn_join_kernel<T, 4>), dim3((unsigned)joins), dim3(256), 0, st, a);
+      else
+        hipLaunchKernelGGL((attn_join_kernel<T, 16>), dim3((unsigned)joins), dim3(1024), 0, st, a);
+    };
+    if (dtype == LTV_DTYPE_F32) join(float()); else join(bf16_t());
     LTV_LAUNCH_CHECK();
   }
   return LTV_OK;
