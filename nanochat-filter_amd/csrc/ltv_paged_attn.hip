@@ -21,7 +21,6 @@
 // Split.  Few rows and many keys leave compute units idle, so a sequence's keys are cut
 // into chunks that workgroups take side by side; a second kernel joins their (m, l, o).
 #include <algorithm>
-#include <type_traits>
 
 #include "ltv_gemm_dma.hpp"
 #include "ltv_paged.hpp"
@@ -48,6 +47,7 @@ struct AttnArgs {
   uint32_t kp, ks, vp, vs;    // 16-byte units from page to page and row to row
   int NH, NKVH, D, g;
   int q_aligned;
+  int scalar_pages;           // page sizes and strides fit load_full
   float scale;                // with log2(e)
   int tiles;                  // row tiles of the grid
   int chunk, nsplit;          // keys of a split, splits of the grid
@@ -58,6 +58,11 @@ struct AttnArgs {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+// Nothing is moved across: the tile's loop is written in the order that it is to run in,
+// reads from LDS well ahead of the products that take them and exponentials between the
+// products.  (Left to itself the compiler puts each read right before its product.)
+__device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0); }
 
 // What differs by element type.  A chunk is 16 bytes of a row.
 template <typename T>
@@ -128,6 +133,13 @@ __device__ __forceinline__ void load_lds16(uint4* to, const char* from) {
   asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(from), "{m0}"(base) : "memory");
 }
 
+// The same from a uniform address and an offset of the lane.
+__device__ __forceinline__ void load_lds16(uint4* to, const char* from, uint32_t offset) {
+  const uint32_t base = lds_address(to);
+  asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(from),
+               "{m0}"(base) : "memory");
+}
+
 __device__ __forceinline__ void barrier() {
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   __builtin_amdgcn_s_barrier();
@@ -152,7 +164,9 @@ __device__ __forceinline__ bool any_nonfinite(uint4 x, float) {
 }
 
 __device__ __forceinline__ float across_halves_max(float x) {
-  return fmaxf(x, __shfl_xor(x, 32));
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false,
+                                                  false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
 // The splits of a sequence: 1, or how many chunks its keys make.
@@ -259,6 +273,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_tile_kernel(const AttnAr
   constexpr int KT = Ti::kKeys, KB = KT / 32;
   constexpr int kSteps = Ti::kChunks / 2;  // score products' steps: two chunks each
   constexpr int kDB = DP / 32;
+  constexpr uint64_t kAll = KT == 64 ? ~0ull : (1ull << (KT & 63)) - 1;  // a full tile's keys
   constexpr int kRow = Ti::kChunks * 16, kTile = Ti::kUnits * 16;  // bytes
   __shared__ uint4 lds[4 * Ti::kUnits];                            // K, V, and again
 
@@ -343,6 +358,30 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_tile_kernel(const AttnAr
       return p < a.batch.P ? p : -1;
     };
     uint64_t held = 0;
+    // A full tile of pages that all hold keys, and whose sizes are multiples of 16: the
+    // rows that a wavefront's load fetches are in one block of kBlock rows and so in one
+    // page, and the address is scalar but for an offset that does not change (float32 at
+    // 128 channels, whose loads are 8 rows: but for the swizzle of odd ones).
+    constexpr int kRows = kAttnThreads / Ti::kChunks, kBlock = kRows < 16 ? kRows : 16;
+    const int r0 = (thread / Ti::kChunks) % kBlock, p0 = thread % Ti::kChunks;
+    uint32_t koff[16 / kBlock];
+#pragma unroll
+    for (int x = 0; x < 16 / kBlock; ++x)
+      koff[x] = (r0 * a.ks + (p0 ^ Ti::k_swizzle(x * kBlock + r0))) * 16;
+    const uint32_t voff = (r0 * a.vs + (p0 ^ Ti::v_swizzle(r0))) * 16;
+    static_assert(sizeof(T) == 2 || Ti::kChunks < 32 || kBlock == 8, "V's swizzle repeats in 8 rows");
+    auto load_full = [&](int kt, int page, int buf) {
+#pragma unroll
+      for (int i = 0; i < Ti::kLoads; ++i) {
+        const int r = (i * kRows + wave * (64 / Ti::kChunks)) & ~(kBlock - 1);
+        const int j = kt + r;
+        const uint32_t at = (uint32_t)(j - a.batch.div.quot(j) * a.batch.div.size);
+        const uint32_t from = (uint32_t)__builtin_amdgcn_readlane(page, r);
+        uint4* to = lds + buf * 2 * Ti::kUnits + i * kAttnThreads + wave * 64;
+        load_lds16(to, kbase + (uint64_t)(from * a.kp + at * a.ks) * 16, koff[i % (16 / kBlock)]);
+        load_lds16(to + Ti::kUnits, vbase + (uint64_t)(from * a.vp + at * a.vs) * 16, voff);
+      }
+    };
     // Starts a tile's way into LDS: a thread's chunk u of the buffer is fetched from
     // wherever the swizzle puts it, channels past D are zeros.  For a key past the end the
     // last one is fetched, for one of no page some row: their scores are masked.  Returns
@@ -355,14 +394,25 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_tile_kernel(const AttnAr
       const uint32_t vu = from * a.vp + at * a.vs;
       uint64_t there = __ballot(page >= 0 && j < end);
       if constexpr (KT == 32) there &= 0xffffffffull;
+      if (!PAD && a.scalar_pages && there == kAll) {
+        load_full(kt, page, buf);
+        return there;
+      }
+      uint32_t kq[Ti::kLoads], vq[Ti::kLoads];
+#pragma unroll
+      for (int i = 0; i < Ti::kLoads; ++i) {
+        const int r = (i * kAttnThreads + thread) / Ti::kChunks;
+        kq[i] = __shfl(ku, r);
+        vq[i] = __shfl(vu, r);
+      }
+      in_order();
 #pragma unroll
       for (int i = 0; i < Ti::kLoads; ++i) {
         const int u = i * kAttnThreads + thread;
         const int r = u / Ti::kChunks, p = u % Ti::kChunks;
-        const uint32_t kq = __shfl(ku, r), vq = __shfl(vu, r);
         const int kc = p ^ Ti::k_swizzle(r), vc = p ^ Ti::v_swizzle(r);
-        const char* kf = kbase + ((uint64_t)kq + kc) * 16;
-        const char* vf = vbase + ((uint64_t)vq + vc) * 16;
+        const char* kf = kbase + ((uint64_t)kq[i] + kc) * 16;
+        const char* vf = vbase + ((uint64_t)vq[i] + vc) * 16;
         if constexpr (PAD) {
           kf = kc < chunks ? kf : reinterpret_cast<const char*>(&kZeros);
           vf = vc < chunks ? vf : reinterpret_cast<const char*>(&kZeros);
@@ -407,15 +457,26 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_tile_kernel(const AttnAr
           const uint32_t ka = kat + buf * 2 * kTile, va = vat + buf * 2 * kTile;
           f32x16 sc[KB];
 #pragma unroll
-          for (int kb = 0; kb < KB; ++kb) {
+          for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
             for (int i = 0; i < 16; ++i) sc[kb][i] = 0.0f;
+          {
+            constexpr int N = kSteps * KB, AHEAD = 6;
+            u32x4_t kf[AHEAD];
+            auto key = [&](int n) {
+              return lds_read<u32x4_t>((ka ^ (32 * (n / KB))) + n % KB * 32 * kRow);
+            };
 #pragma unroll
-            for (int i = 0; i < kSteps; ++i)
-              sc[kb] = Ty::scores(lds_read<u32x4_t>((ka ^ (32 * i)) + kb * 32 * kRow), qf[i], sc[kb]);
+            for (int n = 0; n < AHEAD; ++n) kf[n] = key(n);
+            in_order();
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+              sc[n % KB] = Ty::scores(kf[n % AHEAD], qf[n / KB], sc[n % KB]);
+              if (n + AHEAD < N) kf[n % AHEAD] = key(n + AHEAD);
+              in_order();
+            }
           }
           // keys that the lane's row sees, as bits from the lane half's first
-          constexpr uint64_t kAll = KT == 64 ? ~0ull : (1ull << (KT & 63)) - 1;
           const bool masked = held != kAll || kt + KT - 1 > wave_min;
           uint64_t seen = kAll;
           if (masked) {
@@ -447,14 +508,11 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_tile_kernel(const AttnAr
               for (int i = 0; i < 16; ++i) o[d][i] *= was;
           }
           const float base = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-          for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float p = __builtin_amdgcn_exp2f(fmaf(sc[kb][i], a.scale, -base));
-              sc[kb][i] = p;
-              l += p;
-            }
+          auto prob = [&](int kb, int i) {
+            const float p = __builtin_amdgcn_exp2f(fmaf(sc[kb][i], a.scale, -base));
+            sc[kb][i] = p;
+            l += p;
+          };
           // A value that some row of the tile may not see must not reach it, not even as
           // 0 times infinity: rows of a masked tile that holds infinities or NaNs are
           // computed again below.
@@ -467,50 +525,79 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_tile_kernel(const AttnAr
           }
           // O^T += V^T P^T
           if constexpr (sizeof(T) == 2) {
+            constexpr int N = KB * 2;  // steps of 16 keys
+            uint4 vf[2][kDB];
+            auto value = [&](int e, int d) {
+              typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+              union {
+                s16x4 half[2];
+                uint4 v;
+              } f;
+#pragma unroll
+              for (int x = 0; x < 2; ++x)
+                f.half[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (lds_s16x4*)(uintptr_t)((va ^ (64 * d)) + (16 * e + 8 * x) * kRow));
+              return f.v;
+            };
+            auto product = [&](int d, uint4 v, uint4 p) {
+              o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                  __builtin_bit_cast(bf16x8_t, v), __builtin_bit_cast(bf16x8_t, p), o[d], 0, 0, 0);
+            };
+            // probabilities 2 x, 2 x + 1 of step e
+            auto pair = [&](int e, int x) {
+              const int i = 8 * (e % 2) + 2 * x;
+              prob(e / 2, i);
+              prob(e / 2, i + 1);
+              return cvt_pk_bf16(sc[e / 2][i], sc[e / 2][i + 1]);
+            };
+            uint32_t w[4], next[4];
+#pragma unroll
+            for (int d = 0; d < kDB; ++d) vf[0][d] = value(0, d);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) w[x] = pair(0, x);
+            in_order();
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+#pragma unroll
+              for (int d = 0; d < kDB; ++d) {
+                product(d, vf[e & 1][d], make_uint4(w[0], w[1], w[2], w[3]));
+                if (e + 1 < N) {
+                  vf[(e + 1) & 1][d] = value(e + 1, d);
+#pragma unroll
+                  for (int x = d * 4 / kDB; x < (d + 1) * 4 / kDB; ++x) next[x] = pair(e + 1, x);
+                }
+                in_order();
+              }
+#pragma unroll
+              for (int x = 0; x < 4; ++x) w[x] = next[x];
+            }
             // A probability is rounded to bfloat16 for the product, 2^-8 of it at most.  Where
             // one weighs more than about a 32nd of its row, the rest is multiplied too;
             // below, the errors of a row's many terms average out far under the output's
             // own rounding.
             const bool fine = __any(__builtin_amdgcn_exp2f(top - base) * 16.0f > l);
-            auto product = [&](auto with_rest) {
+            if (fine) {
 #pragma unroll
-              for (int e = 0; e < KB * 2; ++e) {
-                uint32_t w[4], rest[4];
+              for (int e = 0; e < N; ++e) {
+#pragma unroll
+                for (int d = 0; d < kDB; ++d) vf[e & 1][d] = value(e, d);
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
                   const float p0 = sc[e / 2][8 * (e % 2) + 2 * x];
                   const float p1 = sc[e / 2][8 * (e % 2) + 2 * x + 1];
-                  w[x] = cvt_pk_bf16(p0, p1);
-                  if constexpr (decltype(with_rest)::value)
-                    rest[x] = cvt_pk_bf16(p0 - __uint_as_float(w[x] << 16),
-                                          p1 - __uint_as_float(w[x] & 0xffff0000u));
+                  const uint32_t r = cvt_pk_bf16(p0, p1);
+                  w[x] = cvt_pk_bf16(p0 - __uint_as_float(r << 16),
+                                     p1 - __uint_as_float(r & 0xffff0000u));
                 }
-                const bf16x8_t pf = __builtin_bit_cast(bf16x8_t, make_uint4(w[0], w[1], w[2], w[3]));
+                in_order();
 #pragma unroll
-                for (int d = 0; d < kDB; ++d) {
-                  typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-                  union {
-                    s16x4 half[2];
-                    bf16x8_t v;
-                  } f;
-#pragma unroll
-                  for (int x = 0; x < 2; ++x)
-                    f.half[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                        (lds_s16x4*)(uintptr_t)((va ^ (64 * d)) + (16 * e + 8 * x) * kRow));
-                  o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.v, pf, o[d], 0, 0, 0);
-                  if constexpr (decltype(with_rest)::value)
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                        f.v,
-                        __builtin_bit_cast(bf16x8_t, make_uint4(rest[0], rest[1], rest[2], rest[3])),
-                        o[d], 0, 0, 0);
-                }
+                for (int d = 0; d < kDB; ++d)
+                  product(d, vf[e & 1][d], make_uint4(w[0], w[1], w[2], w[3]));
               }
-            };
-            if (fine)
-              product(std::true_type());
-            else
-              product(std::false_type());
+            }
           } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) prob(0, i);
 #pragma unroll
             for (int i = 0; i < 16; ++i)
 #pragma unroll
@@ -744,6 +831,8 @@ extern "C" int ltv_paged_attention(int dtype, const void* q, const int64_t q_str
       const int64_t n = i == 0 ? batch->num_pages : i == 1 ? 1 : batch->page_size;
       fits = fits && st >= 0 && (st == 0 || n <= (int64_t(1) << 31) / std::max<int64_t>(1, st / chunk));
     }
+  // (16 rows' offsets in 32 bits)
+  const bool rows_fit = k_page_strides[2] < (1 << 20) && v_page_strides[2] < (1 << 20);
   LTV_REQUIRE(!pages || aligned, LTV_ERR_UNSUPPORTED, "the pages' rows must be 16-byte aligned");
   LTV_REQUIRE(!pages || fits, LTV_ERR_UNSUPPORTED,
               "the pages of a layer must lie within 32 GiB, with strides that are not negative");
@@ -758,7 +847,7 @@ extern "C" int ltv_paged_attention(int dtype, const void* q, const int64_t q_str
              v_page_strides[1] * es, (uint32_t)(k_page_strides[0] / chunk),
              (uint32_t)(k_page_strides[2] / chunk), (uint32_t)(v_page_strides[0] / chunk),
              (uint32_t)(v_page_strides[2] / chunk), NH, NKVH, D, NH / NKVH, q_aligned ? 1 : 0,
-             scale * kLog2e, p.tiles, p.chunk, p.nsplit, p.rows_cap,
+             batch->page_size % 16 == 0 && rows_fit ? 1 : 0, scale * kLog2e, p.tiles, p.chunk, p.nsplit, p.rows_cap,
              p.by_token, p.part_rows};
   for (int i = 0; i < 3; ++i) {
     a.qs[i] = q_strides[i] * es;
