@@ -4,8 +4,22 @@
 //   z = c tanh(x / c)  (or x),  m = max z,  S = sum e^{z - m},  A = sum (z - m) e^{z - m}
 //   lse = m + log S,   logprob = z_t - lse,   entropy = log S - A / S
 //
-// One workgroup per row.
+// With the cap, tanh(y) = 1 - 2 r with r = 1 / (1 + e^{2 y}): z - c = -2 c r lies in
+// [-2 c, 0], so c serves as the maximum, and its derivative is 4 r (1 - r).
+//
+// Forward.  One workgroup per row, one pass over it: each thread keeps m, S and A of its
+// elements and they are joined at the end.  The alternatives are found in the same pass.
+// The first elements (the lowest indices) are kept in registers; of the largest of each
+// of 64 groups of them the k-th is a bound that at least k elements reach, so from there
+// on only larger elements can be among the top k (an equal one has a higher index), a few
+// k of them on usual rows.  They are collected and ranked at the end.  A row that has more
+// (one that rises along its indices) is read again with the k-th of those collected as
+// the bound, which at least halves them, until they fit.
+//
+// Backward.  Elementwise given lse; a workgroup takes a piece of a row and sets the
+// elements of the target and the alternatives again, with their own terms.
 #include <algorithm>
+#include <type_traits>
 
 #include "../../include/nanochat_serving_amd.h"
 #include "ltv_abi_internal.hpp"
@@ -14,8 +28,8 @@
 namespace ltv {
 namespace {
 
-constexpr int kRowThreads = 256;
-constexpr int kRowWaves = kRowThreads / 64;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
 
 struct LogpArgs {
   const void* x;
@@ -30,8 +44,13 @@ struct LogpArgs {
   float cap;
 };
 
+// r of the cap's tanh; cap_scale = 2 log2(e) / c
+__device__ __forceinline__ float cap_r(float x, float cap_scale) {
+  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * cap_scale));
+}
+
 __device__ __forceinline__ float capped(float x, float cap) {
-  return cap > 0.0f ? cap * tanhf(x / cap) : x;
+  return cap > 0.0f ? fmaf(-2.0f * cap, cap_r(x, 2.0f * kLog2e / cap), cap) : x;
 }
 
 // A total order of the logits with their indices: larger value first (NaN above all,
@@ -42,69 +61,244 @@ __device__ __forceinline__ uint64_t order_key(float x, int i) {
   if (x != x) k = 0xffffffffu;
   return ((uint64_t)k << 32) | (uint32_t)(0x7fffffff - i);
 }
-
-template <typename F>
-__device__ __forceinline__ float block_reduce(float v, float* lds, F f) {
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) v = f(v, __shfl_xor(v, d));
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
-  __syncthreads();
-  float r = lds[0];
-  for (int w = 1; w < kRowWaves; ++w) r = f(r, lds[w]);
-  return r;
+__device__ __forceinline__ float key_value(uint64_t key) {
+  const uint32_t k = (uint32_t)(key >> 32);
+  return __uint_as_float((k & 0x80000000u) ? k & 0x7fffffffu : ~k);
+}
+__device__ __forceinline__ int key_index(uint64_t key) {
+  return 0x7fffffff - (int)(uint32_t)key;
 }
 
-__device__ __forceinline__ float f_add(float a, float b) { return a + b; }
-// (NaN wins)
-__device__ __forceinline__ float f_max(float a, float b) {
-  return a != a ? a : b != b ? b : fmaxf(a, b);
-}
-
+// 16 bytes at any alignment of the element.
 template <typename T>
-__global__ void __launch_bounds__(kRowThreads) logprobs_forward_kernel(const LogpArgs a) {
-  __shared__ float lds[kRowWaves];
-  __shared__ unsigned long long best;
-  const int64_t n = blockIdx.x;
-  const T* x = reinterpret_cast<const T*>(a.x) + n * a.xs;
-  const int tid = threadIdx.x;
-  float m = -INFINITY;
-  for (int j = tid; j < a.V; j += kRowThreads)
-    m = f_max(m, capped(io_traits<T>::load(x + j), a.cap));
-  m = block_reduce(m, lds, f_max);
-  float s = 0.0f, t = 0.0f;
-  for (int j = tid; j < a.V; j += kRowThreads) {
-    const float d = capped(io_traits<T>::load(x + j), a.cap) - m, e = expf(d);
-    s += e;
-    if (!(e == 0.0f)) t = fmaf(d, e, t);
+__device__ __forceinline__ uint4 load_vec(const T* p) {
+  uint4 v;
+  __builtin_memcpy(&v, p, 16);
+  return v;
+}
+
+// m, S and A of some elements: S = sum 2^d, A = sum d 2^d with d = (x - m) log2(e) (the
+// difference first: the logits may be of any size).  With the cap m stays c, and A counts
+// r instead of d = -2 c log2(e) r.
+template <bool CAP>
+struct Sums {
+  float m = -INFINITY, s = 0.0f, a = 0.0f;
+
+  // S and A from another maximum w above the old, or from far below it (w 2^w -> 0)
+  static __device__ __forceinline__ float moved_a(float d, float s, float a, float w) {
+    return w == 0.0f ? s * 0.0f : fmaf(d, s, a) * w;  // (a NaN stays)
   }
-  s = block_reduce(s, lds, f_add);
-  t = block_reduce(t, lds, f_add);
-  const float lse = m + logf(s);
-  if (tid == 0) {
-    const int64_t id = a.targets[n];
-    a.logprobs[n] = id >= 0 && id < a.V
-                        ? capped(io_traits<T>::load(x + id), a.cap) - lse : 0.0f;
-    if (a.entropy != nullptr) a.entropy[n] = logf(s) - t / s;
-    if (a.lse != nullptr) a.lse[n] = lse;
-  }
-  unsigned long long last = ~0ull;
-  for (int i = 0; i < a.top_k; ++i) {
-    unsigned long long mine = 0;
-    for (int j = tid; j < a.V; j += kRowThreads) {
-      const unsigned long long k = order_key(io_traits<T>::load(x + j), j);
-      if (k < last && k > mine) mine = k;
+  template <int N>
+  __device__ __forceinline__ void add(const float (&x)[N], float cap_scale, float cap_exp) {
+    if constexpr (CAP) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float r = cap_r(x[i], cap_scale);
+        const float e = __builtin_amdgcn_exp2f(r * cap_exp);
+        s += e;
+        a = fmaf(r, e, a);
+      }
+    } else {
+      float top = x[0];
+#pragma unroll
+      for (int i = 1; i < N; ++i) top = fmaxf(top, x[i]);
+      if (top > m) {
+        if (m != -INFINITY) {
+          const float d = (m - top) * kLog2e, was = __builtin_amdgcn_exp2f(d);
+          a = moved_a(d, s, a, was);
+          s *= was;
+        }
+        m = top;
+      }
+      const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float d = (x[i] - base) * kLog2e;
+        const float e = __builtin_amdgcn_exp2f(d);
+        s += e;
+        a = fmaf(fmaxf(d, -1000.0f), e, a);  // (-inf adds nothing; NaN comes by e)
+      }
     }
+  }
+  __device__ __forceinline__ void join(float m2, float s2, float a2) {
+    if constexpr (CAP) {
+      s += s2;
+      a += a2;
+    } else {
+      const float mn = fmaxf(m, m2);
+      if (mn == -INFINITY) {
+        s += s2;  // 0, or a NaN
+        return;
+      }
+      const float d1 = (m - mn) * kLog2e, d2 = (m2 - mn) * kLog2e;
+      const float w1 = __builtin_amdgcn_exp2f(d1), w2 = __builtin_amdgcn_exp2f(d2);
+      a = moved_a(d1, s, a, w1) + moved_a(d2, s2, a2, w2);
+      s = s * w1 + s2 * w2;
+      m = mn;
+    }
+  }
+};
+
+constexpr int kGroups = 64;    // of the first elements: as many as top_k may be
+constexpr int kCands = 1024;   // collected elements
+
+// The k-th largest of the 64 lanes' keys, 0 if fewer are not 0 (every lane gets it).
+__device__ __forceinline__ uint64_t kth_of_lanes(uint64_t mine, int k) {
+  int above = 0;
+#pragma unroll 8
+  for (int i = 0; i < 64; ++i) above += __shfl(mine, i) > mine;
+  const uint64_t at = __ballot(above == k - 1 && mine != 0);
+  return at == 0 ? 0 : __shfl(mine, __builtin_ctzll(at));
+}
+
+template <typename T, int THREADS, bool CAP, bool TOP>
+__global__ void __launch_bounds__(THREADS) logprobs_forward_kernel(const LogpArgs p) {
+  constexpr int N = io_traits<T>::kVec, kWaves = THREADS / 64;
+  constexpr int kFirst = 8192 / (THREADS * N);  // vectors of a thread kept for the bound
+  constexpr int kAhead = 4;                     // loads in flight
+  __shared__ float lds_sums[kWaves][3];
+  __shared__ unsigned long long groups[TOP ? kGroups : 1];
+  __shared__ unsigned long long cands[TOP ? kCands : 1];
+  __shared__ unsigned long long bound_lds;
+  __shared__ int count;
+  const int64_t n = blockIdx.x;
+  const T* row = reinterpret_cast<const T*>(p.x) + n * p.xs;
+  const int tid = threadIdx.x, lane = tid & 63, V = p.V;
+  const float cap_scale = CAP ? 2.0f * kLog2e / p.cap : 0.0f;
+  const float cap_exp = CAP ? -2.0f * p.cap * kLog2e : 0.0f;
+  const int whole = V / N;  // vectors that the row fills; the rest are single elements
+  Sums<CAP> sums;
+  float bound = INFINITY;
+
+  auto collect = [&](float x, int i) {
+    const int at = atomicAdd(&count, 1);
+    if (at < kCands) cands[at] = order_key(x, i);
+  };
+  auto take = [&](const uint4& q, int v) {
+    float x[N];
+    unpack16(q, x, T());
+    sums.add(x, cap_scale, cap_exp);
+    if constexpr (TOP) {
+      bool any = false;
+#pragma unroll
+      for (int i = 0; i < N; ++i) any |= !(x[i] <= bound);
+      if (any)
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          if (!(x[i] <= bound)) collect(x[i], v * N + i);
+    }
+  };
+
+  int v = tid;
+  if constexpr (TOP) {
+    if (tid < kGroups) groups[tid] = 0;
+    if (tid == 0) count = 0;
     __syncthreads();
-    if (tid == 0) best = 0;
+    uint4 q[kFirst];
+#pragma unroll
+    for (int j = 0; j < kFirst; ++j)
+      if (v + j * THREADS < whole) q[j] = load_vec(row + (int64_t)(v + j * THREADS) * N);
+    uint64_t best = 0;
+#pragma unroll
+    for (int j = 0; j < kFirst; ++j)
+      if (v + j * THREADS < whole) {
+        float x[N];
+        unpack16(q[j], x, T());
+        sums.add(x, cap_scale, cap_exp);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const uint64_t key = order_key(x[i], (v + j * THREADS) * N + i);
+          best = key > best ? key : best;
+        }
+      }
+    if (best != 0) atomicMax(&groups[lane], (unsigned long long)best);
     __syncthreads();
-    atomicMax(&best, mine);
-    __syncthreads();
-    last = best;
-    const int j = 0x7fffffff - (int)(last & 0xffffffffu);
-    if (tid == 0) {
-      a.top_ids[n * a.top_k + i] = j;
-      a.top_lp[n * a.top_k + i] = capped(io_traits<T>::load(x + j), a.cap) - lse;
+    const uint64_t key = kth_of_lanes(groups[lane], p.top_k);
+#pragma unroll
+    for (int j = 0; j < kFirst; ++j)
+      if (v + j * THREADS < whole) {
+        float x[N];
+        unpack16(q[j], x, T());
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const int at = (v + j * THREADS) * N + i;
+          if (order_key(x[i], at) >= key) collect(x[i], at);
+        }
+      }
+    // (fewer than top_k groups: the row is not much longer, and all of it is collected)
+    bound = key == 0 ? -INFINITY : key_value(key);
+    if (key == 0 && whole <= kFirst * THREADS) bound = NAN;
+    v += kFirst * THREADS;
+  }
+  for (; v < whole; v += kAhead * THREADS) {
+    uint4 q[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+      if (v + j * THREADS < whole) q[j] = load_vec(row + (int64_t)(v + j * THREADS) * N);
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+      if (v + j * THREADS < whole) take(q[j], v + j * THREADS);
+  }
+  if (whole * N + tid < V) {
+    const float x[1] = {io_traits<T>::load(row + whole * N + tid)};
+    sums.add(x, cap_scale, cap_exp);
+    if (TOP && !(x[0] <= bound)) collect(x[0], whole * N + tid);
+  }
+
+  // join the threads' sums
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1)
+    sums.join(__shfl_xor(sums.m, d), __shfl_xor(sums.s, d), __shfl_xor(sums.a, d));
+  if (lane == 0) {
+    lds_sums[tid >> 6][0] = sums.m;
+    lds_sums[tid >> 6][1] = sums.s;
+    lds_sums[tid >> 6][2] = sums.a;
+  }
+  __syncthreads();
+  sums = Sums<CAP>();
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) sums.join(lds_sums[w][0], lds_sums[w][1], lds_sums[w][2]);
+  const float log_s = __builtin_amdgcn_logf(sums.s);
+  const float lse = CAP ? fmaf(log_s, kLn2, p.cap) : fmaf(log_s, kLn2, sums.m);
+  if (tid == 0) {
+    const int64_t id = p.targets[n];
+    p.logprobs[n] =
+        id >= 0 && id < V ? capped(io_traits<T>::load(row + id), CAP ? p.cap : 0.0f) - lse : 0.0f;
+    const float a = sums.a / sums.s;
+    if (p.entropy != nullptr)
+      p.entropy[n] = CAP ? fmaf(log_s, kLn2, 2.0f * p.cap * a) : (log_s - a) * kLn2;
+    if (p.lse != nullptr) p.lse[n] = lse;
+  }
+
+  if constexpr (TOP) {
+    int have = count;
+    while (have > kCands) {
+      // the k-th of those collected is the new bound
+      for (int e = tid; e < kCands; e += THREADS) {
+        const uint64_t mine = cands[e];
+        int above = 0;
+        for (int j = 0; j < kCands; ++j) above += cands[j] > mine;
+        if (above == p.top_k - 1) bound_lds = mine;
+      }
+      __syncthreads();
+      const uint64_t key = bound_lds;
+      if (tid == 0) count = 0;
+      __syncthreads();
+      for (int j = tid; j < V; j += THREADS) {
+        const float x = io_traits<T>::load(row + j);
+        if (order_key(x, j) >= key) collect(x, j);
+      }
+      __syncthreads();
+      have = count;
+    }
+    for (int e = tid; e < have; e += THREADS) {
+      const uint64_t mine = cands[e];
+      int above = 0;
+      for (int j = 0; j < have; ++j) above += cands[j] > mine;
+      if (above < p.top_k) {
+        p.top_ids[n * p.top_k + above] = key_index(mine);
+        p.top_lp[n * p.top_k + above] = capped(key_value(mine), CAP ? p.cap : 0.0f) - lse;
+      }
     }
   }
 }
@@ -123,32 +317,87 @@ struct LogpGradArgs {
   int64_t gs;
   int V, top_k;
   float cap;
+  int piece;  // elements of a workgroup
 };
 
-template <typename T>
-__global__ void __launch_bounds__(kRowThreads) logprobs_backward_kernel(const LogpGradArgs a) {
-  const int64_t n = blockIdx.x;
-  const T* x = reinterpret_cast<const T*>(a.x) + n * a.xs;
-  T* gx = reinterpret_cast<T*>(a.gx) + n * a.gs;
-  const int64_t target = a.targets[n];
-  const bool given = target >= 0 && target < a.V;
-  const float g = given && a.g_lp != nullptr ? a.g_lp[n] : 0.0f;
-  const float ge = a.g_ent != nullptr ? a.g_ent[n] : 0.0f;
-  const float ent = a.g_ent != nullptr ? a.entropy[n] : 0.0f;
-  const int k = a.g_top != nullptr ? a.top_k : 0;
-  float total = g;
-  for (int i = 0; i < k; ++i) total += a.g_top[n * a.top_k + i];
-  const float lse = a.lse[n];
-  for (int j = threadIdx.x; j < a.V; j += kRowThreads) {
-    const float z = capped(io_traits<T>::load(x + j), a.cap);
-    const float lp = z - lse, p = expf(lp);
-    float d = -p * total;
-    if (!(p == 0.0f)) d -= ge * p * (lp + ent);
-    if (j == target) d += g;
-    for (int i = 0; i < k; ++i)
-      if (a.top_ids[n * a.top_k + i] == j) d += a.g_top[n * a.top_k + i];
-    if (a.cap > 0.0f) d *= 1.0f - (z / a.cap) * (z / a.cap);
-    io_traits<T>::store(gx + j, d);
+constexpr int kGradThreads = 256;
+
+// dx of an element, without the terms of a target or an alternative (extra).
+template <bool CAP>
+struct Grad {
+  float lse, total, ge, ent, cap, cap_scale;
+  __device__ __forceinline__ float operator()(float x, float extra) const {
+    float z = x, slope = 1.0f;
+    if constexpr (CAP) {
+      const float r = cap_r(x, cap_scale);
+      z = fmaf(-2.0f * cap, r, cap);
+      slope = 4.0f * r * (1.0f - r);
+    }
+    const float lp = z - lse, e = __builtin_amdgcn_exp2f(lp * kLog2e);
+    // (an entry without probability has none, however low its log)
+    const float d = -e * fmaf(ge, fmaxf(lp, -1e30f) + ent, total);
+    return (d + extra) * slope;
+  }
+};
+
+template <typename T, bool CAP>
+__global__ void __launch_bounds__(kGradThreads) logprobs_backward_kernel(const LogpGradArgs p) {
+  constexpr int N = io_traits<T>::kVec, kAhead = 2;
+  const int64_t n = blockIdx.y;
+  const int begin = blockIdx.x * p.piece, end = min(p.V - begin, p.piece) + begin;
+  const T* x = reinterpret_cast<const T*>(p.x) + n * p.xs;
+  T* gx = reinterpret_cast<T*>(p.gx) + n * p.gs;
+  const int tid = threadIdx.x;
+  const int64_t target = p.targets[n];
+  const bool given = target >= 0 && target < p.V;
+  const float g = given && p.g_lp != nullptr ? p.g_lp[n] : 0.0f;
+  const int k = p.g_top != nullptr ? p.top_k : 0;
+  Grad<CAP> grad;
+  grad.lse = p.lse[n];
+  grad.ge = p.g_ent != nullptr ? p.g_ent[n] : 0.0f;
+  grad.ent = p.g_ent != nullptr ? p.entropy[n] : 0.0f;
+  grad.cap = p.cap;
+  grad.cap_scale = CAP ? 2.0f * kLog2e / p.cap : 0.0f;
+  grad.total = g;
+  for (int i = 0; i < k; ++i) grad.total += p.g_top[n * p.top_k + i];
+
+  const int whole = (end - begin) / N;
+  for (int v = tid; v < whole; v += kAhead * kGradThreads) {
+    uint4 q[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+      if (v + j * kGradThreads < whole)
+        q[j] = load_vec(x + begin + (int64_t)(v + j * kGradThreads) * N);
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+      if (v + j * kGradThreads < whole) {
+        float f[N];
+        unpack16(q[j], f, T());
+#pragma unroll
+        for (int i = 0; i < N; ++i) f[i] = grad(f[i], 0.0f);
+        uint4 o;
+        if constexpr (sizeof(T) == 2)
+          o = make_uint4(cvt_pk_bf16(f[0], f[1]), cvt_pk_bf16(f[2], f[3]), cvt_pk_bf16(f[4], f[5]),
+                         cvt_pk_bf16(f[6], f[7]));
+        else
+          o = pack16(f, T());
+        __builtin_memcpy(gx + begin + (int64_t)(v + j * kGradThreads) * N, &o, 16);
+      }
+  }
+  if (begin + whole * N + tid < end) {
+    const int j = begin + whole * N + tid;
+    io_traits<T>::store(gx + j, grad(io_traits<T>::load(x + j), 0.0f));
+  }
+  __syncthreads();
+  // the target's and the alternatives' elements again (thread k: a target that is none)
+  if (tid <= k) {
+    int64_t j = tid < k ? p.top_ids[n * p.top_k + tid] : given ? target : -1;
+    float extra = tid < k ? p.g_top[n * p.top_k + tid] + (j == target ? g : 0.0f) : g;
+    if (tid == k)
+      for (int i = 0; i < k; ++i)
+        if (p.top_ids[n * p.top_k + i] == j) j = -1;
+    if (j >= begin && j < end)
+      io_traits<T>::store(gx + j, grad(io_traits<T>::load(x + j), extra));
   }
 }
 
@@ -183,12 +432,24 @@ extern "C" int ltv_token_logprobs_forward(int dtype, const void* logits, int64_t
               "null output");
   const LogpArgs a{logits, row_stride, targets, logprobs, entropy, lse, top_logprobs, top_ids,
                    V, top_k, softcap};
-  if (dtype == LTV_DTYPE_F32)
-    hipLaunchKernelGGL(logprobs_forward_kernel<float>, dim3((unsigned)N), dim3(kRowThreads), 0,
-                       (hipStream_t)stream, a);
-  else
-    hipLaunchKernelGGL(logprobs_forward_kernel<bf16_t>, dim3((unsigned)N), dim3(kRowThreads), 0,
-                       (hipStream_t)stream, a);
+  const hipStream_t st = (hipStream_t)stream;
+  const dim3 grid((unsigned)N);
+  // Few rows: all of a compute unit's wavefronts to a row; many: more rows at a time.
+  auto launch = [&](auto type, auto cap, auto top) {
+    using T = decltype(type);
+    constexpr bool C = decltype(cap)::value, K = decltype(top)::value;
+    if (N < 512)
+      hipLaunchKernelGGL((logprobs_forward_kernel<T, 1024, C, K>), grid, dim3(1024), 0, st, a);
+    else
+      hipLaunchKernelGGL((logprobs_forward_kernel<T, 256, C, K>), grid, dim3(256), 0, st, a);
+  };
+  auto by_top = [&](auto type, auto cap) {
+    if (top_k > 0) launch(type, cap, std::true_type()); else launch(type, cap, std::false_type());
+  };
+  auto by_cap = [&](auto type) {
+    if (softcap > 0.0f) by_top(type, std::true_type()); else by_top(type, std::false_type());
+  };
+  if (dtype == LTV_DTYPE_F32) by_cap(float()); else by_cap(bf16_t());
   LTV_LAUNCH_CHECK();
   return LTV_OK;
 }
@@ -205,14 +466,35 @@ extern "C" int ltv_token_logprobs_backward(int dtype, const void* logits, int64_
   if (N == 0) return LTV_OK;
   LTV_REQUIRE(lse && grad_logits && (!g_entropy || entropy) && (!g_top || top_k == 0 || top_ids),
               LTV_ERR_INVALID_ARG, "null pointer");
-  const LogpGradArgs a{logits, row_stride, targets, lse, entropy, top_ids, g_logprobs, g_entropy,
-                       g_top, grad_logits, grad_row_stride, V, top_k, softcap};
-  if (dtype == LTV_DTYPE_F32)
-    hipLaunchKernelGGL(logprobs_backward_kernel<float>, dim3((unsigned)N), dim3(kRowThreads), 0,
-                       (hipStream_t)stream, a);
-  else
-    hipLaunchKernelGGL(logprobs_backward_kernel<bf16_t>, dim3((unsigned)N), dim3(kRowThreads), 0,
-                       (hipStream_t)stream, a);
-  LTV_LAUNCH_CHECK();
+  // rows are cut into pieces, of 4,096 elements at least, until there are 4,096 of them
+  const int64_t want = std::max<int64_t>(1, (4096 + N - 1) / N);
+  const int piece = (int)std::max<int64_t>(4096, ((V + want - 1) / want + 4095) / 4096 * 4096);
+  LogpGradArgs a{logits, row_stride, targets, lse, entropy, top_ids, g_logprobs, g_entropy,
+                 g_top, grad_logits, grad_row_stride, V, top_k, softcap, piece};
+  const hipStream_t st = (hipStream_t)stream;
+  // (the grid's second axis ends at 65,535)
+  for (int64_t n0 = 0; n0 < N; n0 += 65535) {
+    const dim3 grid((unsigned)((V + piece - 1) / piece), (unsigned)std::min<int64_t>(65535, N - n0));
+    auto launch = [&](auto type) {
+      using T = decltype(type);
+      if (softcap > 0.0f)
+        hipLaunchKernelGGL((logprobs_backward_kernel<T, true>), grid, dim3(kGradThreads), 0, st, a);
+      else
+        hipLaunchKernelGGL((logprobs_backward_kernel<T, false>), grid, dim3(kGradThreads), 0, st, a);
+    };
+    if (dtype == LTV_DTYPE_F32) launch(float()); else launch(bf16_t());
+    LTV_LAUNCH_CHECK();
+    const int64_t m = grid.y;
+    const int es = dtype == LTV_DTYPE_F32 ? 4 : 2;
+    a.x = (const char*)a.x + m * row_stride * es;
+    a.gx = (char*)a.gx + m * grad_row_stride * es;
+    a.targets += m;
+    a.lse += m;
+    a.entropy = a.entropy ? a.entropy + m : nullptr;
+    a.g_lp = a.g_lp ? a.g_lp + m : nullptr;
+    a.g_ent = a.g_ent ? a.g_ent + m : nullptr;
+    a.top_ids = a.top_ids ? a.top_ids + m * top_k : nullptr;
+    a.g_top = a.g_top ? a.g_top + m * top_k : nullptr;
+  }
   return LTV_OK;
 }

@@ -195,6 +195,7 @@ template <typename T>
 __device__ __forceinline__ void rows_one_by_one(const AttnArgs& a, const PagedSeq& s, int b,
                                                 int kvh, int64_t row0, int64_t row_end, int begin,
                                                 int end, int split, float* lds) {
+#pragma clang fp contract(off)  // (x - base below must not be a fused form of the product)
   float* lds_m = lds;
   float* lds_l = lds + 16;
   float* lds_o = lds + 32;  // 16 x 128
@@ -499,6 +500,9 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_tile_kernel(const AttnAr
           // probabilities stay below 2^8, their sums far from overflow
           if (__any(top > m + 8.0f)) {
             const float mn = fmaxf(m, top);
+            // (from here on the argument of an exponential, a fused multiply and subtract of
+            // a rounded product, is off by 2^-6 and more: one by one it never exceeds 0)
+            if (__any(fabsf(mn) > 0x1p18f && mn != -INFINITY)) again = 1;
             const float was = m == mn ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
             m = mn;
             l *= was;

@@ -214,6 +214,21 @@ def test_large_scores(dtype):
     _check(got, attention64(q, cache, [0, 1], [2, 40], 0.125), dtype, 64, [300, 60])
 
 
+@pytest.mark.parametrize("T", [1, 40])
+@pytest.mark.parametrize("size", [1e6, 1e20])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_enormous_scores(dtype, size, T):
+    """Scores of any finite size: the largest takes all, nothing overflows."""
+    cache = Cache([T + 150], 1, 64, 16, dtype, 21)
+    cache.k.mul_(size)
+    q = [cache.rand(T, 2, 64, dtype=dtype)]
+    want = attention64(q, cache, [0], [T], 0.125)
+    # (a second key within 2^-10 of the largest would share: none does here)
+    out = _run(cache, q, [T], False)[0][0]
+    assert float((out.double() - want[0][0]).abs().max()) <= (2.0 ** -8 if dtype == BF else 1e-6) * float(
+        cache.v.abs().max())
+
+
 def test_scores_falling_and_rising_along_the_keys():
     """The running maximum changes in every tile, or never again after the first."""
     for sign in (1.0, -1.0):
