@@ -159,13 +159,16 @@ int ltv_paged_cache_compact(const ltv_page_state* state, const ltv_page_blocks* 
  *                  logits in descending order of x (NaN above all), equal ones in
  *                  ascending order of index
  *   lse[n]       : kept for the backward                (may be NULL)
- * All outputs contiguous; sums in fp32.  Replaces what nanochat's sampling and
+ * All outputs contiguous; sums in fp32.  workspace: ltv_token_logprobs_workspace_size
+ * bytes (0 where a row is not cut into pieces), 16-byte aligned.  Replaces what nanochat's sampling and
  * scoring do with log_softmax, gather and topk on the logits.
  * ---------------------------------------------------------------------- */
+size_t ltv_token_logprobs_workspace_size(int64_t N, int V, int top_k);
 int ltv_token_logprobs_forward(int dtype, const void* logits, int64_t row_stride,
                                const int64_t* targets, float* logprobs, float* entropy,
-                               float* lse, float* top_logprobs, int64_t* top_ids, int64_t N,
-                               int V, int top_k, float softcap, void* stream);
+                               float* lse, float* top_logprobs, int64_t* top_ids,
+                               void* workspace, size_t workspace_bytes, int64_t N, int V,
+                               int top_k, float softcap, void* stream);
 
 /* Gradient of the above for the logits, (N, V) in their dtype:
  *   dz_j = g_logp (1[j = target] - p_j) - g_entropy p_j (log p_j + entropy)

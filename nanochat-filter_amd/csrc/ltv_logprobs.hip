@@ -7,8 +7,9 @@
 // With the cap, tanh(y) = 1 - 2 r with r = 1 / (1 + e^{2 y}): z - c = -2 c r lies in
 // [-2 c, 0], so c serves as the maximum, and its derivative is 4 r (1 - r).
 //
-// Forward.  One workgroup per row, one pass over it: each thread keeps m, S and A of its
-// elements and they are joined at the end.  The alternatives are found in the same pass.
+// Forward.  One pass over the logits: each thread keeps m, S and A of its elements and they
+// are joined at the end.  A workgroup takes a row, or, where there are few rows, a piece of
+// one; a second kernel then joins the pieces.  The alternatives are found in the same pass.
 // The first elements (the lowest indices) are kept in registers; of the largest of each
 // of 64 groups of them the k-th is a bound that at least k elements reach, so from there
 // on only larger elements can be among the top k (an equal one has a higher index), a few
@@ -42,6 +43,9 @@ struct LogpArgs {
   int64_t* top_ids;
   int V, top_k;
   float cap;
+  int piece, pieces;         // elements of a workgroup, workgroups of a row
+  float* part_sums;          // (N, pieces, 3), pieces > 1
+  uint64_t* part_keys;       // (N, pieces, top_k)
 };
 
 // r of the cap's tanh; cap_scale = 2 log2(e) / c
@@ -142,37 +146,78 @@ struct Sums {
 constexpr int kGroups = 64;    // of the first elements: as many as top_k may be
 constexpr int kCands = 1024;   // collected elements
 
+__device__ __forceinline__ uint64_t of_lane(uint64_t x, int i) {  // (i uniform)
+  return ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), i) << 32) |
+         (uint32_t)__builtin_amdgcn_readlane((int)x, i);
+}
+
 // The k-th largest of the 64 lanes' keys, 0 if fewer are not 0 (every lane gets it).
 __device__ __forceinline__ uint64_t kth_of_lanes(uint64_t mine, int k) {
   int above = 0;
-#pragma unroll 8
-  for (int i = 0; i < 64; ++i) above += __shfl(mine, i) > mine;
+#pragma unroll
+  for (int i = 0; i < 64; ++i) above += of_lane(mine, i) > mine;
   const uint64_t at = __ballot(above == k - 1 && mine != 0);
-  return at == 0 ? 0 : __shfl(mine, __builtin_ctzll(at));
+  return at == 0 ? 0 : of_lane(mine, __builtin_ctzll(at));
 }
 
-template <typename T, int THREADS, bool CAP, bool TOP>
-__global__ void __launch_bounds__(THREADS) logprobs_forward_kernel(const LogpArgs p) {
-  constexpr int N = io_traits<T>::kVec, kWaves = THREADS / 64;
-  constexpr int kFirst = 8192 / (THREADS * N);  // vectors of a thread kept for the bound
-  constexpr int kAhead = 4;                     // loads in flight
+constexpr int kThreads = 256, kWaves = kThreads / 64;
+
+// What a row's sums make: log(sum of exponentials) and entropy.
+template <bool CAP>
+__device__ __forceinline__ void row_results(const Sums<CAP>& sums, float cap, float& lse,
+                                            float& entropy) {
+  const float log_s = __builtin_amdgcn_logf(sums.s), a = sums.a / sums.s;
+  lse = fmaf(log_s, kLn2, CAP ? cap : sums.m);
+  entropy = CAP ? fmaf(log_s, kLn2, 2.0f * cap * a) : (log_s - a) * kLn2;
+}
+
+// The target's logit (one thread reads it ahead), and the row's results that are not
+// alternatives.
+struct Target {
+  bool given = false;
+  float x = 0.0f;
+};
+template <typename T>
+__device__ __forceinline__ Target target_of(const LogpArgs& p, int64_t n, const T* row) {
+  Target t;
+  const int64_t id = p.targets[n];
+  t.given = id >= 0 && id < p.V;
+  if (t.given) t.x = io_traits<T>::load(row + id);
+  return t;
+}
+__device__ __forceinline__ void store_row(const LogpArgs& p, int64_t n, const Target& t, float cap,
+                                          float lse, float entropy) {
+  p.logprobs[n] = t.given ? capped(t.x, cap) - lse : 0.0f;
+  if (p.entropy != nullptr) p.entropy[n] = entropy;
+  if (p.lse != nullptr) p.lse[n] = lse;
+}
+
+template <typename T, bool CAP, bool TOP>
+__global__ void __launch_bounds__(kThreads) logprobs_forward_kernel(const LogpArgs p) {
+  constexpr int N = io_traits<T>::kVec;
+  constexpr int kFirst = 8192 / (kThreads * N);  // vectors of a thread kept for the bound
+  constexpr int kAhead = 4;                      // loads in flight
   __shared__ float lds_sums[kWaves][3];
   __shared__ unsigned long long groups[TOP ? kGroups : 1];
   __shared__ unsigned long long cands[TOP ? kCands : 1];
   __shared__ unsigned long long bound_lds;
   __shared__ int count;
   const int64_t n = blockIdx.x;
-  const T* row = reinterpret_cast<const T*>(p.x) + n * p.xs;
-  const int tid = threadIdx.x, lane = tid & 63, V = p.V;
+  const int begin = blockIdx.y * p.piece;
+  const T* whole_row = reinterpret_cast<const T*>(p.x) + n * p.xs;
+  const T* row = whole_row + begin;
+  const int tid = threadIdx.x, lane = tid & 63, V = min(p.V - begin, p.piece);
   const float cap_scale = CAP ? 2.0f * kLog2e / p.cap : 0.0f;
   const float cap_exp = CAP ? -2.0f * p.cap * kLog2e : 0.0f;
-  const int whole = V / N;  // vectors that the row fills; the rest are single elements
+  const int whole = V / N;  // vectors that the piece fills; the rest are single elements
   Sums<CAP> sums;
   float bound = INFINITY;
+  Target target;
+  if (tid == 0 && p.pieces == 1) target = target_of(p, n, whole_row);
 
   auto collect = [&](float x, int i) {
     const int at = atomicAdd(&count, 1);
-    if (at < kCands) cands[at] = order_key(x, i);
+    if (at < kCands) cands[at] = order_key(x, begin + i);
   };
   auto take = [&](const uint4& q, int v) {
     float x[N];
@@ -197,17 +242,17 @@ __global__ void __launch_bounds__(THREADS) logprobs_forward_kernel(const LogpArg
     uint4 q[kFirst];
 #pragma unroll
     for (int j = 0; j < kFirst; ++j)
-      if (v + j * THREADS < whole) q[j] = load_vec(row + (int64_t)(v + j * THREADS) * N);
+      if (v + j * kThreads < whole) q[j] = load_vec(row + (int64_t)(v + j * kThreads) * N);
     uint64_t best = 0;
 #pragma unroll
     for (int j = 0; j < kFirst; ++j)
-      if (v + j * THREADS < whole) {
+      if (v + j * kThreads < whole) {
         float x[N];
         unpack16(q[j], x, T());
         sums.add(x, cap_scale, cap_exp);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-          const uint64_t key = order_key(x[i], (v + j * THREADS) * N + i);
+          const uint64_t key = order_key(x[i], begin + (v + j * kThreads) * N + i);
           best = key > best ? key : best;
         }
       }
@@ -216,28 +261,27 @@ __global__ void __launch_bounds__(THREADS) logprobs_forward_kernel(const LogpArg
     const uint64_t key = kth_of_lanes(groups[lane], p.top_k);
 #pragma unroll
     for (int j = 0; j < kFirst; ++j)
-      if (v + j * THREADS < whole) {
+      if (v + j * kThreads < whole) {
         float x[N];
         unpack16(q[j], x, T());
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-          const int at = (v + j * THREADS) * N + i;
-          if (order_key(x[i], at) >= key) collect(x[i], at);
+          const int at = (v + j * kThreads) * N + i;
+          if (order_key(x[i], begin + at) >= key) collect(x[i], at);
         }
       }
-    // (fewer than top_k groups: the row is not much longer, and all of it is collected)
-    bound = key == 0 ? -INFINITY : key_value(key);
-    if (key == 0 && whole <= kFirst * THREADS) bound = NAN;
-    v += kFirst * THREADS;
+    // (fewer than top_k groups: the piece has few elements, and all are collected)
+    bound = key == 0 ? NAN : key_value(key);
+    v += kFirst * kThreads;
   }
-  for (; v < whole; v += kAhead * THREADS) {
+  for (; v < whole; v += kAhead * kThreads) {
     uint4 q[kAhead];
 #pragma unroll
     for (int j = 0; j < kAhead; ++j)
-      if (v + j * THREADS < whole) q[j] = load_vec(row + (int64_t)(v + j * THREADS) * N);
+      if (v + j * kThreads < whole) q[j] = load_vec(row + (int64_t)(v + j * kThreads) * N);
 #pragma unroll
     for (int j = 0; j < kAhead; ++j)
-      if (v + j * THREADS < whole) take(q[j], v + j * THREADS);
+      if (v + j * kThreads < whole) take(q[j], v + j * kThreads);
   }
   if (whole * N + tid < V) {
     const float x[1] = {io_traits<T>::load(row + whole * N + tid)};
@@ -258,23 +302,20 @@ __global__ void __launch_bounds__(THREADS) logprobs_forward_kernel(const LogpArg
   sums = Sums<CAP>();
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) sums.join(lds_sums[w][0], lds_sums[w][1], lds_sums[w][2]);
-  const float log_s = __builtin_amdgcn_logf(sums.s);
-  const float lse = CAP ? fmaf(log_s, kLn2, p.cap) : fmaf(log_s, kLn2, sums.m);
-  if (tid == 0) {
-    const int64_t id = p.targets[n];
-    p.logprobs[n] =
-        id >= 0 && id < V ? capped(io_traits<T>::load(row + id), CAP ? p.cap : 0.0f) - lse : 0.0f;
-    const float a = sums.a / sums.s;
-    if (p.entropy != nullptr)
-      p.entropy[n] = CAP ? fmaf(log_s, kLn2, 2.0f * p.cap * a) : (log_s - a) * kLn2;
-    if (p.lse != nullptr) p.lse[n] = lse;
+  const int64_t part = n * p.pieces + blockIdx.y;
+  float lse = 0.0f, entropy;
+  if (p.pieces > 1) {
+    if (tid < 3) p.part_sums[part * 3 + tid] = tid == 0 ? sums.m : tid == 1 ? sums.s : sums.a;
+  } else {
+    row_results(sums, p.cap, lse, entropy);
+    if (tid == 0) store_row(p, n, target, CAP ? p.cap : 0.0f, lse, entropy);
   }
 
   if constexpr (TOP) {
     int have = count;
     while (have > kCands) {
       // the k-th of those collected is the new bound
-      for (int e = tid; e < kCands; e += THREADS) {
+      for (int e = tid; e < kCands; e += kThreads) {
         const uint64_t mine = cands[e];
         int above = 0;
         for (int j = 0; j < kCands; ++j) above += cands[j] > mine;
@@ -284,23 +325,92 @@ __global__ void __launch_bounds__(THREADS) logprobs_forward_kernel(const LogpArg
       const uint64_t key = bound_lds;
       if (tid == 0) count = 0;
       __syncthreads();
-      for (int j = tid; j < V; j += THREADS) {
+      for (int j = tid; j < V; j += kThreads) {
         const float x = io_traits<T>::load(row + j);
-        if (order_key(x, j) >= key) collect(x, j);
+        if (order_key(x, begin + j) >= key) collect(x, j);
       }
       __syncthreads();
       have = count;
     }
-    for (int e = tid; e < have; e += THREADS) {
+    for (int e = tid; e < have; e += kThreads) {
       const uint64_t mine = cands[e];
       int above = 0;
       for (int j = 0; j < have; ++j) above += cands[j] > mine;
-      if (above < p.top_k) {
+      if (above >= p.top_k) continue;
+      if (p.pieces > 1) {
+        p.part_keys[part * p.top_k + above] = mine;
+      } else {
         p.top_ids[n * p.top_k + above] = key_index(mine);
         p.top_lp[n * p.top_k + above] = capped(key_value(mine), CAP ? p.cap : 0.0f) - lse;
       }
     }
+    // (a last piece of fewer elements than alternatives)
+    if (p.pieces > 1)
+      for (int e = have + tid; e < p.top_k; e += kThreads) p.part_keys[part * p.top_k + e] = 0;
   }
+}
+
+constexpr int kPieces = 16;  // of a row, at most
+
+constexpr int kJoinThreads = kPieces * kGroups;
+
+// Joins a row's pieces: one workgroup, every piece's sums, and the best of the pieces'
+// alternatives, each ranked by as many threads as there are for it.  (A search in each
+// piece's ordered list per alternative, fewer comparisons but one after the other, took
+// 7.3 us instead of 6.0 for 16 rows of 16 pieces with 20 alternatives.)
+template <typename T, bool CAP>
+__global__ void __launch_bounds__(kJoinThreads) logprobs_join_kernel(const LogpArgs p) {
+  __shared__ unsigned long long keys[kJoinThreads];
+  __shared__ int rank[kJoinThreads];
+  __shared__ float lse_lds;
+  const int64_t n = blockIdx.x;
+  const int tid = threadIdx.x, all = p.pieces * p.top_k;
+  if (tid < all) {
+    keys[tid] = p.part_keys[n * all + tid];
+    rank[tid] = 0;
+  }
+  Target target;
+  if (tid == 0) target = target_of(p, n, reinterpret_cast<const T*>(p.x) + n * p.xs);
+  // (lanes past the pieces hold nothing)
+  Sums<CAP> sums;
+  const float* part = p.part_sums + (n * p.pieces + (tid & 63)) * 3;
+  if ((tid & 63) < p.pieces) {
+    sums.m = part[0];
+    sums.s = part[1];
+    sums.a = part[2];
+  }
+#pragma unroll
+  for (int d = 1; d < kPieces; d <<= 1)
+    sums.join(__shfl_xor(sums.m, d), __shfl_xor(sums.s, d), __shfl_xor(sums.a, d));
+  if (tid == 0) {
+    float lse, entropy;
+    row_results(sums, p.cap, lse, entropy);
+    store_row(p, n, target, CAP ? p.cap : 0.0f, lse, entropy);
+    lse_lds = lse;
+  }
+  if (all == 0) return;
+  __syncthreads();
+  const int e = tid % all, share = kJoinThreads / all;
+  if (tid / all < share) {
+    const uint64_t mine = keys[e];
+    int above = 0;
+#pragma unroll 8
+    for (int j = tid / all; j < all; j += share) above += keys[j] > mine;
+    atomicAdd(&rank[e], above);
+  }
+  __syncthreads();
+  if (tid < all && keys[tid] != 0 && rank[tid] < p.top_k) {
+    p.top_ids[n * p.top_k + rank[tid]] = key_index(keys[tid]);
+    p.top_lp[n * p.top_k + rank[tid]] =
+        capped(key_value(keys[tid]), CAP ? p.cap : 0.0f) - lse_lds;
+  }
+}
+
+// Pieces that a row is cut into: one for 512 rows and more, which fill the card; else up to
+// 16, of 4,096 elements at least, towards 1,024 workgroups.
+int row_pieces(int64_t N, int V) {
+  if (N >= 512 || N <= 0) return 1;
+  return (int)std::max<int64_t>(1, std::min<int64_t>({kPieces, (1024 + N - 1) / N, V / 4096}));
 }
 
 struct LogpGradArgs {
@@ -420,38 +530,52 @@ int check_rows(int dtype, const void* x, int64_t row_stride, const int64_t* targ
 
 using namespace ltv;
 
+extern "C" size_t ltv_token_logprobs_workspace_size(int64_t N, int V, int top_k) {
+  if (N <= 0 || V <= 0 || top_k < 0 || row_pieces(N, V) == 1) return 0;
+  return (size_t)N * row_pieces(N, V) * (top_k * sizeof(uint64_t) + 3 * sizeof(float));
+}
+
 extern "C" int ltv_token_logprobs_forward(int dtype, const void* logits, int64_t row_stride,
                                           const int64_t* targets, float* logprobs, float* entropy,
                                           float* lse, float* top_logprobs, int64_t* top_ids,
-                                          int64_t N, int V, int top_k, float softcap,
-                                          void* stream) {
+                                          void* workspace, size_t workspace_bytes, int64_t N,
+                                          int V, int top_k, float softcap, void* stream) {
   const int bad = check_rows(dtype, logits, row_stride, targets, N, V, top_k, softcap);
   if (bad != LTV_OK) return bad;
   if (N == 0) return LTV_OK;
   LTV_REQUIRE(logprobs && (top_k == 0 || (top_logprobs && top_ids)), LTV_ERR_INVALID_ARG,
               "null output");
+  const int pieces = row_pieces(N, V);
+  LTV_REQUIRE(workspace_bytes >= ltv_token_logprobs_workspace_size(N, V, top_k) &&
+                  (pieces == 1 || (workspace && aligned16(workspace))),
+              LTV_ERR_WORKSPACE, "workspace too small");
+  uint64_t* keys = reinterpret_cast<uint64_t*>(workspace);
+  // (a multiple of 64 elements: pieces of an aligned row are aligned)
+  const int piece = ((V + pieces - 1) / pieces + 63) / 64 * 64;
   const LogpArgs a{logits, row_stride, targets, logprobs, entropy, lse, top_logprobs, top_ids,
-                   V, top_k, softcap};
+                   V, top_k, softcap, piece, (V + piece - 1) / piece,
+                   reinterpret_cast<float*>(keys + N * pieces * top_k), keys};
   const hipStream_t st = (hipStream_t)stream;
-  const dim3 grid((unsigned)N);
-  // Few rows: all of a compute unit's wavefronts to a row; many: more rows at a time.
-  auto launch = [&](auto type, auto cap, auto top) {
+  const dim3 grid((unsigned)N, a.pieces);
+  auto launch = [&](auto type, auto cap) -> int {
     using T = decltype(type);
-    constexpr bool C = decltype(cap)::value, K = decltype(top)::value;
-    if (N < 512)
-      hipLaunchKernelGGL((logprobs_forward_kernel<T, 1024, C, K>), grid, dim3(1024), 0, st, a);
+    constexpr bool C = decltype(cap)::value;
+    if (top_k > 0)
+      hipLaunchKernelGGL((logprobs_forward_kernel<T, C, true>), grid, dim3(kThreads), 0, st, a);
     else
-      hipLaunchKernelGGL((logprobs_forward_kernel<T, 256, C, K>), grid, dim3(256), 0, st, a);
-  };
-  auto by_top = [&](auto type, auto cap) {
-    if (top_k > 0) launch(type, cap, std::true_type()); else launch(type, cap, std::false_type());
+      hipLaunchKernelGGL((logprobs_forward_kernel<T, C, false>), grid, dim3(kThreads), 0, st, a);
+    LTV_LAUNCH_CHECK();
+    if (a.pieces > 1) {
+      hipLaunchKernelGGL((logprobs_join_kernel<T, C>), dim3((unsigned)N), dim3(kJoinThreads),
+                         0, st, a);
+      LTV_LAUNCH_CHECK();
+    }
+    return LTV_OK;
   };
   auto by_cap = [&](auto type) {
-    if (softcap > 0.0f) by_top(type, std::true_type()); else by_top(type, std::false_type());
+    return softcap > 0.0f ? launch(type, std::true_type()) : launch(type, std::false_type());
   };
-  if (dtype == LTV_DTYPE_F32) by_cap(float()); else by_cap(bf16_t());
-  LTV_LAUNCH_CHECK();
-  return LTV_OK;
+  return dtype == LTV_DTYPE_F32 ? by_cap(float()) : by_cap(bf16_t());
 }
 
 extern "C" int ltv_token_logprobs_backward(int dtype, const void* logits, int64_t row_stride,

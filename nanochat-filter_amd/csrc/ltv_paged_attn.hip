@@ -169,6 +169,9 @@ __device__ __forceinline__ float across_halves_max(float x) {
   return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
+// (row numbers stay below 2^30: divisions of 64 bits would take longer than small calls)
+__device__ __forceinline__ int over(int a, int b) { return (int)((unsigned)a / (unsigned)b); }
+
 // The splits of a sequence: 1, or how many chunks its keys make.
 __device__ __forceinline__ int splits_of(const AttnArgs& a, const PagedSeq& s) {
   if ((int64_t)s.n * a.g > a.rows_cap) return 1;
@@ -193,16 +196,16 @@ __device__ __forceinline__ float2* part_ml(const AttnArgs& a) {
 // turn, a lane holding eight channels.  split: whose partials these are, or -1.
 template <typename T>
 __device__ __forceinline__ void rows_one_by_one(const AttnArgs& a, const PagedSeq& s, int b,
-                                                int kvh, int64_t row0, int64_t row_end, int begin,
-                                                int end, int split, float* lds) {
+                                                int kvh, int row0, int row_end, int begin, int end,
+                                                int split, float* lds) {
 #pragma clang fp contract(off)  // (x - base below must not be a fused form of the product)
   float* lds_m = lds;
   float* lds_l = lds + 16;
   float* lds_o = lds + 32;  // 16 x 128
   const int c = threadIdx.x & 15, gi = threadIdx.x >> 4;
   const bool on = c * 8 < a.D;
-  for (int64_t row = row0; row < row_end; ++row) {
-    const int t = (int)(row / a.g), h = kvh * a.g + (int)(row - (int64_t)t * a.g);
+  for (int row = row0; row < row_end; ++row) {
+    const int t = over(row, a.g), h = kvh * a.g + row - t * a.g;
     const int last = min(end - 1, s.len - s.n + t);
     const int64_t trow = a.batch.starts != nullptr ? s.row0 + t : (int64_t)b * a.batch.T + t;
     const char* q = a.q + (a.batch.starts != nullptr ? trow * a.qs[1]
@@ -283,16 +286,17 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_tile_kernel(const AttnAr
   // tiles with the most keys start first.
   const int nbh = a.batch.B * a.NKVH;
   int rest = blockIdx.x;
-  int split = rest % a.nsplit;
-  rest /= a.nsplit;
-  const int bh = rest % nbh;
-  const int tile0 = a.tiles - 1 - rest / nbh;
+  const int split_rest = over(rest, a.nsplit);
+  int split = rest - split_rest * a.nsplit;
+  rest = split_rest;
+  const int tile_bh = over(rest, nbh), bh = rest - tile_bh * nbh;
+  const int tile0 = a.tiles - 1 - tile_bh;
   split = (int)(((unsigned)split + (unsigned)bh + (unsigned)tile0) % (unsigned)a.nsplit);
-  const int b = bh / a.NKVH, kvh = bh - b * a.NKVH;
+  const int b = over(bh, a.NKVH), kvh = bh - b * a.NKVH;
   const PagedSeq s = paged_seq(a.batch, b);
   const int nsplit = splits_of(a, s);
   if (split >= nsplit) return;
-  const int64_t rows = (int64_t)s.n * a.g;
+  const int rows = s.n * a.g;
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const char* kbase = a.k + (int64_t)kvh * a.kh;
@@ -300,26 +304,25 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_tile_kernel(const AttnAr
   const int chunks = a.D / Ty::kChunk;
 
   // (more rows than the grid was sized for: its tiles are walked again)
-  for (int64_t tile = tile0; tile * kAttnRows < rows; tile += a.tiles) {
+  for (int tile = tile0; tile * kAttnRows < rows; tile += a.tiles) {
     // (opaque: what follows from the lane is not kept in registers around this loop)
     int thread = threadIdx.x;
     asm volatile("" : "+v"(thread));
     const int lane = thread & 63, ln = lane & 31, hf = lane >> 5;
-    const int64_t row = tile * kAttnRows + wave * 32 + ln;
+    const int row = tile * kAttnRows + wave * 32 + ln;
     const bool row_ok = row < rows;
-    const int t = row_ok ? (int)(row / a.g) : 0;
-    const int h = kvh * a.g + (row_ok ? (int)(row - (int64_t)t * a.g) : 0);
+    const int t = row_ok ? over(row, a.g) : 0;
+    const int h = kvh * a.g + (row_ok ? row - t * a.g : 0);
     const int pos = row_ok ? s.len - s.n + t : -1;
     const int64_t trow = a.batch.starts != nullptr ? s.row0 + t : (int64_t)b * a.batch.T + t;
 
     // the last position that any row of the wavefront, and of the workgroup, sees
     const bool wave_on = tile * kAttnRows + wave * 32 < rows;
-    const int64_t wlast = min(tile * kAttnRows + wave * 32 + 31, rows - 1);
-    const int wave_end = wave_on ? s.len - s.n + (int)(wlast / a.g) + 1 : 0;
-    const int wave_min = wave_on
-        ? s.len - s.n + (int)((tile * kAttnRows + wave * 32) / a.g) : 0;
-    const int64_t tlast = min(tile * kAttnRows + kAttnRows - 1, rows - 1);
-    int end = a.batch.P > 0 ? s.len - s.n + (int)(tlast / a.g) + 1 : 0;
+    const int wfirst = tile * kAttnRows + wave * 32, last = rows - 1;
+    const int wave_end = wave_on ? s.len - s.n + over(min(wfirst + 31, last), a.g) + 1 : 0;
+    const int wave_min = wave_on ? s.len - s.n + over(wfirst, a.g) : 0;
+    const int tlast = over(min(tile * kAttnRows + kAttnRows - 1, last), a.g);
+    int end = a.batch.P > 0 ? s.len - s.n + tlast + 1 : 0;
     const int begin = split * a.chunk;
     if (split < nsplit - 1) end = min(end, begin + a.chunk);
 
@@ -666,14 +669,15 @@ __global__ void __launch_bounds__(W < 4 ? 256 : W * 64) attn_join_kernel(const A
   __shared__ float lds_o[W][128];
   __shared__ float lds_l[W];
   const int lane = threadIdx.x & 63, wave = W == 1 ? 0 : threadIdx.x >> 6;
-  int64_t unit = blockIdx.x;
+  int unit = blockIdx.x;
   if (W == 1) unit = unit * 4 + (threadIdx.x >> 6);
-  int b, h;
-  int64_t row, trow;
+  int b, h, row, t;
+  int64_t trow;
   PagedSeq s;
   if (a.by_token) {
-    trow = unit / a.NH;
-    h = (int)(unit - trow * a.NH);
+    const int token = over(unit, a.NH);
+    trow = token;
+    h = unit - token * a.NH;
     if (trow >= a.batch.total) return;
     if (a.batch.starts != nullptr) {
       // the last sequence that starts at the row or before it
@@ -684,26 +688,26 @@ __global__ void __launch_bounds__(W < 4 ? 256 : W * 64) attn_join_kernel(const A
       }
       b = lo;
     } else {
-      b = (int)(trow / a.batch.T);
+      b = over(token, a.batch.T);
     }
     s = paged_seq(a.batch, b);
-    const int64_t t = a.batch.starts != nullptr ? trow - s.row0 : trow - (int64_t)b * a.batch.T;
+    t = (int)(a.batch.starts != nullptr ? trow - s.row0 : trow - (int64_t)b * a.batch.T);
     if (t < 0 || t >= s.n) return;
     row = t * a.g + h % a.g;
   } else {
     const int nbh = a.batch.B * a.NKVH;
-    row = unit / nbh;
-    const int bh = (int)(unit - row * nbh);
-    b = bh / a.NKVH;
+    row = over(unit, nbh);
+    const int bh = unit - row * nbh;
+    b = over(bh, a.NKVH);
     s = paged_seq(a.batch, b);
-    if (row >= a.rows_cap || row >= (int64_t)s.n * a.g) return;
-    const int64_t t = row / a.g;
-    h = (bh - b * a.NKVH) * a.g + (int)(row - t * a.g);
+    if (row >= a.rows_cap || row >= s.n * a.g) return;
+    t = over(row, a.g);
+    h = (bh - b * a.NKVH) * a.g + row - t * a.g;
     trow = a.batch.starts != nullptr ? s.row0 + t : (int64_t)b * a.batch.T + t;
   }
   const int nsplit = splits_of(a, s);
   if (nsplit <= 1) return;
-  const int bh = b * a.NKVH + h / a.g;
+  const int bh = b * a.NKVH + over(h, a.g);
   const int64_t first = part_row(a, bh, 0, row, trow, h);
   const int64_t step = part_row(a, bh, 1, row, trow, h) - first;
   const float2* ml = part_ml(a) + first;
@@ -744,7 +748,6 @@ __global__ void __launch_bounds__(W < 4 ? 256 : W * 64) attn_join_kernel(const A
       }
     }
   }
-  const int64_t t = row / a.g;
   char* out = a.out + (a.batch.starts != nullptr ? trow * a.os[1]
                                                  : b * a.os[0] + t * a.os[1]) + h * a.os[2];
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -779,7 +782,7 @@ AttnPlan plan_attention(const ltv_paged_batch& b, int NH, int NKVH, int max_len)
   p.rows_cap = p.by_token ? int64_t(1) << 40 : std::min<int64_t>(rows, kAttnRows);
   const int64_t keys = std::max(max_len, 1);
   const int64_t want = keys * (p.by_token ? tiles : seqs) / 2560;
-  p.chunk = (int)std::min<int64_t>(std::max<int64_t>((want + 127) / 128 * 128, 128),
+  p.chunk = (int)std::min<int64_t>(std::max<int64_t>((want + 63) / 64 * 64, 64),
                                    p.by_token ? int64_t(1024) * p.tiles : 1024);
   p.nsplit = (int)((keys + p.chunk - 1) / p.chunk);
   p.joins = p.by_token ? b.total * NH : seqs * p.rows_cap;
@@ -818,7 +821,11 @@ extern "C" int ltv_paged_attention(int dtype, const void* q, const int64_t q_str
               LTV_ERR_INVALID_ARG, "bad heads (NH=%d NKVH=%d D=%d)", NH, NKVH, D);
   LTV_REQUIRE(D % 8 == 0 && D <= 128, LTV_ERR_UNSUPPORTED,
               "head_dim must be a multiple of 8, at most 128 (D=%d)", D);
+  LTV_REQUIRE(scale > 0.0f && scale < INFINITY, LTV_ERR_INVALID_ARG,
+              "scale must be positive and finite (%g)", scale);
   if (batch->B == 0 || batch->total == 0 || NH == 0) return LTV_OK;
+  LTV_REQUIRE(batch->total * NH < (int64_t(1) << 30), LTV_ERR_UNSUPPORTED,
+              "too many new tokens in a call");
   const bool pages = batch->num_pages > 0;
   LTV_REQUIRE(q && out && q_strides && out_strides && k_page_strides && v_page_strides &&
                   (!pages || (k_pages && v_pages)),
@@ -859,7 +866,7 @@ extern "C" int ltv_paged_attention(int dtype, const void* q, const int64_t q_str
   }
   const int64_t seqs = (int64_t)batch->B * NKVH;
   const int64_t grid = seqs * p.tiles * p.nsplit, joins = p.joins;
-  LTV_REQUIRE(grid < (int64_t(1) << 31) && joins < (int64_t(1) << 31), LTV_ERR_UNSUPPORTED,
+  LTV_REQUIRE(grid < (int64_t(1) << 31) && joins < (int64_t(1) << 30), LTV_ERR_UNSUPPORTED,
               "too many workgroups");
   const hipStream_t st = (hipStream_t)stream;
   auto launch = [&](auto kernel) {

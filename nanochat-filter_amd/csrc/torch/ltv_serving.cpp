@@ -433,13 +433,16 @@ LogpOut logprobs_forward(const Tensor& logits, const Tensor& targets, int64_t to
   LogpOut o{at::empty(shape, f32), at::empty(shape, f32), at::empty(top_shape, f32),
             at::empty(top_shape, f32.dtype(at::kLong)), at::empty(shape, f32)};
   if (N == 0) return o;
+  const size_t bytes = ltv_token_logprobs_workspace_size(N, to_int(V, "the vocabulary"), (int)top_k);
+  Tensor ws;
+  if (bytes > 0) ws = at::empty({(int64_t)bytes}, f32.dtype(at::kByte));
   check_rc(ltv_token_logprobs_forward(
                dtype_of(r.x, "logits"), r.x.data_ptr(), r.x.stride(0),
                r.targets.data_ptr<int64_t>(), o.logprobs.data_ptr<float>(),
                o.entropy.data_ptr<float>(), o.lse.data_ptr<float>(),
                top_k > 0 ? o.top.data_ptr<float>() : nullptr,
-               top_k > 0 ? o.ids.data_ptr<int64_t>() : nullptr, N, to_int(V, "the vocabulary"),
-               (int)top_k, (float)cap, stream_of(r.x)),
+               top_k > 0 ? o.ids.data_ptr<int64_t>() : nullptr, bytes > 0 ? ws.data_ptr() : nullptr,
+               bytes, N, (int)V, (int)top_k, (float)cap, stream_of(r.x)),
            "ltv_token_logprobs_forward");
   return o;
 }
