@@ -21,6 +21,7 @@
 // Split.  Few rows and many keys leave compute units idle, so a sequence's keys are cut
 // into chunks that workgroups take side by side; a second kernel joins their (m, l, o).
 #include <algorithm>
+#include <type_traits>
 
 #include "ltv_gemm_dma.hpp"
 #include "ltv_paged.hpp"
@@ -47,9 +48,9 @@ struct AttnArgs {
   uint32_t kp, ks, vp, vs;    // 16-byte units from page to page and row to row
   int NH, NKVH, D, g;
   int q_aligned;
-  int scalar_pages;           // page sizes and strides fit load_full
+  int scalar_pages;           // load_full: 1 pages are multiples of 16 rows, 2 of 64
   float scale;                // with log2(e)
-  int tiles;                  // row tiles of the grid
+  int tiles, group;           // row tiles of the grid, and how many follow each other
   int chunk, nsplit;          // keys of a split, splits of the grid
   int64_t rows_cap;           // sequences of more rows are not split
   int by_token;               // how the partials are laid out
@@ -130,13 +131,13 @@ __device__ __forceinline__ V lds_read(uint32_t at) {
 // wait_vmcnt and a barrier.  The nop covers the write of M0.
 __device__ __forceinline__ void load_lds16(uint4* to, const char* from) {
   const uint32_t base = lds_address(to);
-  asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(from), "{m0}"(base) : "memory");
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(from), "{m0}"(base) : "memory");
 }
 
 // The same from a uniform address and an offset of the lane.
 __device__ __forceinline__ void load_lds16(uint4* to, const char* from, uint32_t offset) {
   const uint32_t base = lds_address(to);
-  asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(from),
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(from),
                "{m0}"(base) : "memory");
 }
 
@@ -281,19 +282,28 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_tile_kernel(const AttnAr
   constexpr int kRow = Ti::kChunks * 16, kTile = Ti::kUnits * 16;  // bytes
   __shared__ uint4 lds[4 * Ti::kUnits];                            // K, V, and again
 
-  // Workgroup w runs on XCD w % 8.  Splits go around the XCDs from a start that differs
-  // by sequence, head and row tile, or those in use would land on few of them.  The row
-  // tiles with the most keys start first.
-  const int nbh = a.batch.B * a.NKVH;
-  int rest = blockIdx.x;
-  const int split_rest = over(rest, a.nsplit);
-  int split = rest - split_rest * a.nsplit;
-  rest = split_rest;
-  const int tile_bh = over(rest, nbh), bh = rest - tile_bh * nbh;
-  const int tile0 = a.tiles - 1 - tile_bh;
-  split = (int)(((unsigned)split + (unsigned)bh + (unsigned)tile0) % (unsigned)a.nsplit);
+  // Workgroup w runs on XCD w % 8.  Up to four row tiles that read the same keys -- those of
+  // one sequence, k/v head and split -- follow each other on one XCD, whose L2 then holds
+  // the keys for all but the first of them; such groups go around the XCDs, those of the
+  // last rows, with the most keys, first.  A sequence's splits start at an XCD that differs
+  // by sequence and head, or those in use of short sequences would land on few of them.
+  const int xcd = blockIdx.x & 7, place = blockIdx.x >> 3;
+  const int round = over(place, a.group), unit = round * 8 + xcd;
+  const int pairs = a.batch.B * a.NKVH * a.nsplit, rank = over(unit, pairs);
+  const int pair = unit - rank * pairs, bh = over(pair, a.nsplit);
+  const int tile0 = a.tiles - 1 - rank * a.group - (place - round * a.group);
+  if (tile0 < 0) return;
+  const int split = (int)((unsigned)(pair - bh * a.nsplit + bh) % (unsigned)a.nsplit);
   const int b = over(bh, a.NKVH), kvh = bh - b * a.NKVH;
   const PagedSeq s = paged_seq(a.batch, b);
+  // The page of the lane-th key of a tile, -1: none.  (Read without waiting for the
+  // sequence's length; what is past the end is sorted out where it is used.)
+  auto page_of = [&](int kt) {
+    const int col = a.batch.div.quot(kt + ((int)threadIdx.x & (KT - 1)));
+    const int p = a.batch.W > 0 ? s.table[min(col, a.batch.W - 1)] : -1;
+    return p < a.batch.P ? p : -1;
+  };
+  const int begin = split * a.chunk, first_page = page_of(begin);
   const int nsplit = splits_of(a, s);
   if (split >= nsplit) return;
   const int rows = s.n * a.g;
@@ -323,7 +333,6 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_tile_kernel(const AttnAr
     const int wave_min = wave_on ? s.len - s.n + over(wfirst, a.g) : 0;
     const int tlast = over(min(tile * kAttnRows + kAttnRows - 1, last), a.g);
     int end = a.batch.P > 0 ? s.len - s.n + tlast + 1 : 0;
-    const int begin = split * a.chunk;
     if (split < nsplit - 1) end = min(end, begin + a.chunk);
 
     // Q: chunk 2 step + half of the lane's row
@@ -356,11 +365,6 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_tile_kernel(const AttnAr
       for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
     float m = -INFINITY, l = 0.0f;  // l: of this lane's keys
 
-    // The page of the lane-th key of a tile (past the end: of the last key), -1: none.
-    auto page_of = [&](int kt) {
-      const int p = s.table[a.batch.div.quot(min(kt + (lane & (KT - 1)), end - 1))];
-      return p < a.batch.P ? p : -1;
-    };
     uint64_t held = 0;
     // A full tile of pages that all hold keys, and whose sizes are multiples of 16: the
     // rows that a wavefront's load fetches are in one block of kBlock rows and so in one
@@ -374,34 +378,41 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_tile_kernel(const AttnAr
       koff[x] = (r0 * a.ks + (p0 ^ Ti::k_swizzle(x * kBlock + r0))) * 16;
     const uint32_t voff = (r0 * a.vs + (p0 ^ Ti::v_swizzle(r0))) * 16;
     static_assert(sizeof(T) == 2 || Ti::kChunks < 32 || kBlock == 8, "V's swizzle repeats in 8 rows");
-    auto load_full = [&](int kt, int page, int buf) {
-#pragma unroll
-      for (int i = 0; i < Ti::kLoads; ++i) {
-        const int r = (i * kRows + wave * (64 / Ti::kChunks)) & ~(kBlock - 1);
-        const int j = kt + r;
-        const uint32_t at = (uint32_t)(j - a.batch.div.quot(j) * a.batch.div.size);
-        const uint32_t from = (uint32_t)__builtin_amdgcn_readlane(page, r);
-        uint4* to = lds + buf * 2 * Ti::kUnits + i * kAttnThreads + wave * 64;
-        load_lds16(to, kbase + (uint64_t)(from * a.kp + at * a.ks) * 16, koff[i % (16 / kBlock)]);
+    // Load x of such a tile: K's and V's alternate.  They are issued between the products of
+    // the tile before, as fast as the memory pipe takes them: all at once, each wavefront
+    // stands until the others' are through.
+    auto load_full = [&](int x, int kt, int page, int buf) {
+      const int i = x / 2;
+      const bool of_v = x & 1;
+      const int r = (i * kRows + wave * (64 / Ti::kChunks)) & ~(kBlock - 1);
+      // (pages of whole tiles: one page and row, and constant steps from it)
+      const int j = a.scalar_pages == 2 ? kt : kt + r;
+      uint32_t at = (uint32_t)(j - a.batch.div.quot(j) * a.batch.div.size);
+      const uint32_t from = (uint32_t)__builtin_amdgcn_readlane(page, a.scalar_pages == 2 ? 0 : r);
+      if (a.scalar_pages == 2) at += r;
+      uint4* to = lds + buf * 2 * Ti::kUnits + i * kAttnThreads + wave * 64;
+      if (of_v)
         load_lds16(to + Ti::kUnits, vbase + (uint64_t)(from * a.vp + at * a.vs) * 16, voff);
-      }
+      else
+        load_lds16(to, kbase + (uint64_t)(from * a.kp + at * a.ks) * 16, koff[i % (16 / kBlock)]);
     };
-    // Starts a tile's way into LDS: a thread's chunk u of the buffer is fetched from
+    constexpr int kFullLoads = 2 * Ti::kLoads;
+    // Whether a tile is one for load_full, and the keys that are there.
+    auto is_full = [&](int kt, int page, uint64_t& there) {
+      there = __ballot(page >= 0 && kt + (lane & (KT - 1)) < end);
+      if constexpr (KT == 32) there &= 0xffffffffull;
+      return !PAD && a.scalar_pages && there == kAll;
+    };
+    // Starts any tile's way into LDS: a thread's chunk u of the buffer is fetched from
     // wherever the swizzle puts it, channels past D are zeros.  For a key past the end the
-    // last one is fetched, for one of no page some row: their scores are masked.  Returns
-    // the keys that are there.
+    // last one is fetched, for one of no page some row: their scores are masked.
     auto load = [&](int kt, int page, int buf) {
       const int j = kt + (lane & (KT - 1)), jj = min(j, end - 1);
       const uint32_t at = (uint32_t)(jj - a.batch.div.quot(jj) * a.batch.div.size);
-      const uint32_t from = (uint32_t)max(page, 0);
+      const int own = max(page, 0), of_last = __shfl(own, min(lane & (KT - 1), end - 1 - kt));
+      const uint32_t from = (uint32_t)(j < end ? own : of_last);
       const uint32_t ku = from * a.kp + at * a.ks;
       const uint32_t vu = from * a.vp + at * a.vs;
-      uint64_t there = __ballot(page >= 0 && j < end);
-      if constexpr (KT == 32) there &= 0xffffffffull;
-      if (!PAD && a.scalar_pages && there == kAll) {
-        load_full(kt, page, buf);
-        return there;
-      }
       uint32_t kq[Ti::kLoads], vq[Ti::kLoads];
 #pragma unroll
       for (int i = 0; i < Ti::kLoads; ++i) {
@@ -425,7 +436,6 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_tile_kernel(const AttnAr
         load_lds16(to, kf);
         load_lds16(to + Ti::kUnits, vf);
       }
-      return there;
     };
 
     // Where the lane reads K's row ln, and V's four rows from 4 hf (bfloat16) or row 4 hf
@@ -443,9 +453,11 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_tile_kernel(const AttnAr
     }
     int again = 0;
     if (begin < end) {
-      int page = page_of(begin);
+      int page = first_page;
       barrier();  // (the row tile before is read to its end)
-      uint64_t next = load(begin, page, 0);
+      uint64_t next;
+      is_full(begin, page, next);
+      load(begin, page, 0);
       page = page_of(begin + KT);
       int buf = 0;
       for (int kt = begin; kt < end; kt += KT, buf ^= 1) {
@@ -453,9 +465,16 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_tile_kernel(const AttnAr
         // every wavefront's loads of this tile have landed, and the other buffer is read
         wait_vmcnt<0>();
         barrier();
+        bool full = false;
+        const int page_next = page;
         if (kt + KT < end) {
-          next = load(kt + KT, page, buf ^ 1);
+          full = is_full(kt + KT, page, next);
+          if (!full) load(kt + KT, page, buf ^ 1);
           page = page_of(kt + 2 * KT);
+        }
+        if (full && kt >= wave_end) {
+#pragma unroll
+          for (int x = 0; x < kFullLoads; ++x) load_full(x, kt + KT, page_next, buf ^ 1);
         }
         if (kt < wave_end) {
           const uint32_t ka = kat + buf * 2 * kTile, va = vat + buf * 2 * kTile;
@@ -464,8 +483,9 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_tile_kernel(const AttnAr
           for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
             for (int i = 0; i < 16; ++i) sc[kb][i] = 0.0f;
-          {
+          auto scores = [&](auto with_loads) {
             constexpr int N = kSteps * KB, AHEAD = 6;
+            static_assert(N == 2 * kFullLoads, "a load to two products");
             u32x4_t kf[AHEAD];
             auto key = [&](int n) {
               return lds_read<u32x4_t>((ka ^ (32 * (n / KB))) + n % KB * 32 * kRow);
@@ -477,9 +497,12 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_tile_kernel(const AttnAr
             for (int n = 0; n < N; ++n) {
               sc[n % KB] = Ty::scores(kf[n % AHEAD], qf[n / KB], sc[n % KB]);
               if (n + AHEAD < N) kf[n % AHEAD] = key(n + AHEAD);
+              if (decltype(with_loads)::value && (n & 1))
+                load_full(n / 2, kt + KT, page_next, buf ^ 1);
               in_order();
             }
-          }
+          };
+          if (full) scores(std::true_type()); else scores(std::false_type());
           // keys that the lane's row sees, as bits from the lane half's first
           const bool masked = held != kAll || kt + KT - 1 > wave_min;
           uint64_t seen = kAll;
@@ -493,11 +516,14 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_tile_kernel(const AttnAr
               for (int i = 0; i < 16; ++i)
                 if (!((mine >> (kb * 32 + 8 * (i / 4) + i % 4)) & 1)) sc[kb][i] = -INFINITY;
           }
-          float top = -INFINITY;
+          float part_top[KB * 2], top = -INFINITY;  // of the lane's keys of each 16
 #pragma unroll
-          for (int kb = 0; kb < KB; ++kb)
+          for (int e = 0; e < KB * 2; ++e) {
+            part_top[e] = sc[e / 2][8 * (e % 2)];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) top = fmaxf(top, sc[kb][i]);
+            for (int i = 1; i < 8; ++i) part_top[e] = fmaxf(part_top[e], sc[e / 2][8 * (e % 2) + i]);
+            top = fmaxf(top, part_top[e]);
+          }
           top = across_halves_max(top) * a.scale;
           // the maximum in use stays until a score passes it by a factor of 2^8: the
           // probabilities stay below 2^8, their sums far from overflow
@@ -525,7 +551,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_tile_kernel(const AttnAr
           // computed again below.
           if (masked) {
             bool bad = false;
-#pragma unroll 1
+#pragma unroll 4
             for (int u = lane; u < Ti::kUnits; u += 64) 
               bad |= any_nonfinite(lds[(2 * buf + 1) * Ti::kUnits + u], T());
             if (__any(bad)) again = 1;
@@ -557,6 +583,17 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_tile_kernel(const AttnAr
               prob(e / 2, i + 1);
               return cvt_pk_bf16(sc[e / 2][i], sc[e / 2][i + 1]);
             };
+            // A probability is rounded to bfloat16 for the product, by 2^-8 of it at most.  Of
+            // 16 keys with one that weighs more than about a 32nd of its row so far, the rest
+            // is multiplied too; below that, the errors of a row's many terms average out far
+            // under the output's own rounding.
+            uint32_t fine = 0;
+            if (__any(__builtin_amdgcn_exp2f(top - base) * 16.0f > l)) {
+#pragma unroll
+              for (int e = 0; e < N; ++e)
+                if (__any(__builtin_amdgcn_exp2f(fmaf(part_top[e], a.scale, -base)) * 16.0f > l))
+                  fine |= 1u << e;
+            }
             uint32_t w[4], next[4];
 #pragma unroll
             for (int d = 0; d < kDB; ++d) vf[0][d] = value(0, d);
@@ -575,43 +612,41 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_tile_kernel(const AttnAr
                 }
                 in_order();
               }
+              if (fine & (1u << e)) {
+                uint32_t rest[4];
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                  const int i = 8 * (e % 2) + 2 * x;
+                  rest[x] = cvt_pk_bf16(sc[e / 2][i] - __uint_as_float(w[x] << 16),
+                                        sc[e / 2][i + 1] - __uint_as_float(w[x] & 0xffff0000u));
+                }
+#pragma unroll
+                for (int d = 0; d < kDB; ++d)
+                  product(d, vf[e & 1][d], make_uint4(rest[0], rest[1], rest[2], rest[3]));
+              }
 #pragma unroll
               for (int x = 0; x < 4; ++x) w[x] = next[x];
             }
-            // A probability is rounded to bfloat16 for the product, 2^-8 of it at most.  Where
-            // one weighs more than about a 32nd of its row, the rest is multiplied too;
-            // below, the errors of a row's many terms average out far under the output's
-            // own rounding.
-            const bool fine = __any(__builtin_amdgcn_exp2f(top - base) * 16.0f > l);
-            if (fine) {
-#pragma unroll
-              for (int e = 0; e < N; ++e) {
-#pragma unroll
-                for (int d = 0; d < kDB; ++d) vf[e & 1][d] = value(e, d);
-#pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                  const float p0 = sc[e / 2][8 * (e % 2) + 2 * x];
-                  const float p1 = sc[e / 2][8 * (e % 2) + 2 * x + 1];
-                  const uint32_t r = cvt_pk_bf16(p0, p1);
-                  w[x] = cvt_pk_bf16(p0 - __uint_as_float(r << 16),
-                                     p1 - __uint_as_float(r & 0xffff0000u));
-                }
-                in_order();
-#pragma unroll
-                for (int d = 0; d < kDB; ++d)
-                  product(d, vf[e & 1][d], make_uint4(w[0], w[1], w[2], w[3]));
-              }
-            }
           } else {
+            constexpr int N = 16 * kDB, AHEAD = 8;
+            float vf[AHEAD];
+            auto value = [&](int n) {
+              const int i = n / kDB;
+              return lds_read<float>((va ^ (128 * (n % kDB))) + (8 * (i / 4) + i % 4) * kRow);
+            };
 #pragma unroll
-            for (int i = 0; i < 16; ++i) prob(0, i);
+            for (int n = 0; n < AHEAD; ++n) vf[n] = value(n);
+            prob(0, 0);
+            prob(0, 1);
+            in_order();
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-#pragma unroll
-              for (int d = 0; d < kDB; ++d) {
-                const float v = lds_read<float>((va ^ (128 * d)) + (8 * (i / 4) + i % 4) * kRow);
-                o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, sc[0][i], o[d], 0, 0, 0);
-              }
+            for (int n = 0; n < N; ++n) {
+              o[n % kDB] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf[n % AHEAD], sc[0][n / kDB],
+                                                                o[n % kDB], 0, 0, 0);
+              if (n + AHEAD < N) vf[n % AHEAD] = value(n + AHEAD);
+              if (n % kDB == 0 && n / kDB + 2 < 16) prob(0, n / kDB + 2);
+              in_order();
+            }
           }
         }
       }
@@ -764,7 +799,7 @@ __global__ void __launch_bounds__(W < 4 ? 256 : W * 64) attn_join_kernel(const A
 // How a call is cut: row tiles of the grid, keys of a split, splits, and where the
 // splits' partials go.
 struct AttnPlan {
-  int tiles, chunk, nsplit, by_token;
+  int tiles, group, chunk, nsplit, by_token;
   int64_t rows_cap, joins, part_rows;
 };
 
@@ -772,6 +807,8 @@ AttnPlan plan_attention(const ltv_paged_batch& b, int NH, int NKVH, int max_len)
   AttnPlan p;
   const int64_t g = NH / NKVH, rows = std::max(b.T, 1) * g, seqs = (int64_t)b.B * NKVH;
   p.tiles = (int)std::min<int64_t>((rows + kAttnRows - 1) / kAttnRows, 1 << 20);
+  const int groups = (p.tiles + 3) / 4;
+  p.group = (p.tiles + groups - 1) / groups;
   // The row tiles there are at most.  The card holds 512 workgroups at a time (two per
   // compute unit).  With fewer row tiles than five times that, every sequence is split
   // into about that many workgroups, or the last ones of few would run alone; else those
@@ -782,7 +819,8 @@ AttnPlan plan_attention(const ltv_paged_batch& b, int NH, int NKVH, int max_len)
   p.rows_cap = p.by_token ? int64_t(1) << 40 : std::min<int64_t>(rows, kAttnRows);
   const int64_t keys = std::max(max_len, 1);
   const int64_t want = keys * (p.by_token ? tiles : seqs) / 2560;
-  p.chunk = (int)std::min<int64_t>(std::max<int64_t>((want + 63) / 64 * 64, 64),
+  const int64_t least = rows <= 32 ? 64 : 128;  // (of few rows: all their latency is a tile's)
+  p.chunk = (int)std::min<int64_t>(std::max<int64_t>((want + 63) / 64 * 64, least),
                                    p.by_token ? int64_t(1024) * p.tiles : 1024);
   p.nsplit = (int)((keys + p.chunk - 1) / p.chunk);
   p.joins = p.by_token ? b.total * NH : seqs * p.rows_cap;
@@ -858,14 +896,15 @@ extern "C" int ltv_paged_attention(int dtype, const void* q, const int64_t q_str
              v_page_strides[1] * es, (uint32_t)(k_page_strides[0] / chunk),
              (uint32_t)(k_page_strides[2] / chunk), (uint32_t)(v_page_strides[0] / chunk),
              (uint32_t)(v_page_strides[2] / chunk), NH, NKVH, D, NH / NKVH, q_aligned ? 1 : 0,
-             batch->page_size % 16 == 0 && rows_fit ? 1 : 0, scale * kLog2e, p.tiles, p.chunk, p.nsplit, p.rows_cap,
+             !rows_fit || batch->page_size % 16 != 0 ? 0 : batch->page_size % 64 == 0 ? 2 : 1, scale * kLog2e, p.tiles, p.group, p.chunk, p.nsplit, p.rows_cap,
              p.by_token, p.part_rows};
   for (int i = 0; i < 3; ++i) {
     a.qs[i] = q_strides[i] * es;
     a.os[i] = out_strides[i] * es;
   }
   const int64_t seqs = (int64_t)batch->B * NKVH;
-  const int64_t grid = seqs * p.tiles * p.nsplit, joins = p.joins;
+  const int64_t units = seqs * p.nsplit * ((p.tiles + p.group - 1) / p.group);
+  const int64_t grid = (units + 7) / 8 * 8 * p.group, joins = p.joins;
   LTV_REQUIRE(grid < (int64_t(1) << 31) && joins < (int64_t(1) << 30), LTV_ERR_UNSUPPORTED,
               "too many workgroups");
   const hipStream_t st = (hipStream_t)stream;
