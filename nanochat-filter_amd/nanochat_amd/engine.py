@@ -1,0 +1,122 @@
+"""Generation and scoring with the GPT harness over the paged cache: a prompt in
+chunks, several samples from it (``generate``), and the log probabilities of given
+texts (``score``).
+
+The reference's ``nanochat/engine.py`` prefills a prompt once and copies the cache to
+every sample; here the samples share the prompt's pages, a finished sample's pages are
+free for the others, and log probabilities, entropy and alternatives come from one
+pass over the logits.
+"""
+
+from __future__ import annotations
+
+from typing import NamedTuple, Optional, Sequence
+
+import torch
+
+from nanochat_amd.gpt import GPT
+from nanochat_amd.ops.token_logprobs import TokenLogprobs, token_logprobs
+from nanochat_amd.paged_kv_cache import PagedKVCache
+
+
+class Sample(NamedTuple):
+    tokens: list      # the continuation, a stop token included
+    logprobs: list    # of each of its tokens
+
+
+def make_cache(model: GPT, num_pages: int, max_seqs: int, page_size: int = 64) -> PagedKVCache:
+    c = model.config
+    return PagedKVCache(c.n_layer, c.n_head, c.n_kv_head, c.n_embd // c.n_head,
+                        num_pages=num_pages, max_seqs=max_seqs, max_len=c.sequence_len,
+                        page_size=page_size, device=model.wte.weight.device)
+
+
+def _autocast():
+    return torch.autocast(device_type="cuda", dtype=torch.bfloat16)
+
+
+@torch.no_grad()
+def prefill(model: GPT, cache: PagedKVCache, slot: int, tokens: Sequence[int],
+            chunk: int = 2048) -> torch.Tensor:
+    """Feeds the prompt into an empty slot, ``chunk`` tokens at a time; the logits after
+    its last token, (1, vocabulary), before the cap."""
+    if not len(tokens):
+        raise ValueError("an empty prompt")
+    idx = torch.tensor(tokens, device=cache.page_table.device)[None]
+    with _autocast():
+        for x in idx.split(chunk, dim=1):
+            hidden = model.cached_features(x, cache.step([slot], x.size(1)))
+        return model.raw_logits(hidden[:, -1])
+
+
+@torch.no_grad()
+def generate(model: GPT, prompt: Sequence[int], num_samples: int, max_tokens: int, *,
+             top_k: int = 20, temperature: float = 1.0, stop: Optional[int] = None,
+             seed: int = 0, cache: Optional[PagedKVCache] = None,
+             chunk: int = 2048) -> list[Sample]:
+    """``num_samples`` continuations of the prompt, sampled among the ``top_k`` most
+    probable tokens (``temperature`` 0: the most probable).  The log probabilities are
+    the model's own, of the whole vocabulary."""
+    if num_samples <= 0 or max_tokens <= 0 or temperature < 0:
+        raise ValueError("at least one sample of one token, and no negative temperature")
+    n = num_samples
+    if cache is None:
+        page = 64
+        shared, own = -(-len(prompt) // page), -(-max_tokens // page) + 1
+        cache = make_cache(model, shared + n * own, n, page)
+    device = cache.page_table.device
+    g = torch.Generator(device=device).manual_seed(seed)
+    logits = prefill(model, cache, 0, prompt, chunk).expand(n, -1)
+    if n > 1:
+        cache.fork([0] * (n - 1), list(range(1, n)))
+    out = [Sample([], []) for _ in range(n)]
+    live = list(range(n))
+    none = torch.full((n,), -1, device=device)
+    for _ in range(max_tokens):
+        lp = token_logprobs(logits, none[:len(live)], top_k=top_k, softcap=GPT.SOFTCAP)
+        if temperature > 0:
+            p = torch.softmax(lp.top_logprobs / temperature, dim=-1)
+            pick = torch.multinomial(p, 1, generator=g)
+        else:
+            pick = torch.zeros(len(live), 1, dtype=torch.int64, device=device)
+        tokens = lp.top_ids.gather(1, pick)
+        probs = lp.top_logprobs.gather(1, pick)
+        going = []
+        for i, (s, t, p) in enumerate(zip(live, tokens[:, 0].tolist(), probs[:, 0].tolist())):
+            out[s].tokens.append(t)
+            out[s].logprobs.append(p)
+            if t != stop and len(out[s].tokens) < max_tokens:
+                going.append(i)
+        ended = [s for i, s in enumerate(live) if i not in set(going)]
+        if ended:
+            cache.free(ended)
+        live = [live[i] for i in going]
+        if not live:
+            break
+        with _autocast():
+            hidden = model.cached_features(tokens[torch.tensor(going, device=device)],
+                                           cache.step(live, 1))
+            logits = model.raw_logits(hidden[:, -1])
+    cache.compact()
+    return out
+
+
+@torch.no_grad()
+def score(model: GPT, tokens: Sequence[int], *, top_k: int = 0,
+          cache: Optional[PagedKVCache] = None, slot: int = 0,
+          chunk: int = 2048) -> TokenLogprobs:
+    """Log probability, entropy and alternatives at each of ``tokens[1:]`` given what is
+    before it, fed through an empty slot of the cache ``chunk`` tokens at a time."""
+    if len(tokens) < 2:
+        raise ValueError("at least two tokens")
+    if cache is None:
+        cache = make_cache(model, -(-len(tokens) // 64), slot + 1)
+    idx = torch.tensor(tokens, device=cache.page_table.device)
+    parts = []
+    with _autocast():
+        for x, y in zip(idx[:-1].split(chunk), idx[1:].split(chunk)):
+            hidden = model.cached_features(x[None], cache.step([slot], len(x)))
+            parts.append(token_logprobs(model.raw_logits(hidden[0]), y, top_k=top_k,
+                                        softcap=GPT.SOFTCAP))
+    cache.free([slot])
+    return TokenLogprobs(*(None if p[0] is None else torch.cat(p) for p in zip(*parts)))

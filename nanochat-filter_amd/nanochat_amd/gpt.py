@@ -17,8 +17,9 @@ plugs into; only what a training step computes:
   * init as ``gpt.py:396-440``: wte ~ N(0, 1), lm_head ~ N(0, 0.001), c_fc and
     the filter U(-s, s) with s = sqrt(3/C), output projections zero (the
     harness can randomise them so gradients reach the filter at step 0).
-KV-cache inference, generation, optimizers and checkpoint loading are not
-part of the harness.
+Inference over the paged cache is ``cached_features`` and ``raw_logits``
+(``nanochat_amd.engine`` generates and scores with them).  Optimizers and
+checkpoint loading are not part of the harness.
 """
 
 from __future__ import annotations
@@ -72,6 +73,7 @@ class CausalSelfAttention(nn.Module):
     def __init__(self, config: GPTConfig, layer_idx: int):
         super().__init__()
         self.n_head, self.n_kv_head = config.n_head, config.n_kv_head
+        self.layer_idx = layer_idx
         self.head_dim = config.n_embd // config.n_head
         self.qkv_computer = LtvCombinedQkvComputerModule(
             layer_idx,
@@ -95,6 +97,16 @@ class CausalSelfAttention(nn.Module):
             scale=self.scale, enable_gqa=self.n_head != self.n_kv_head)
         return self.c_proj(y.transpose(1, 2).reshape(B, T, C))
 
+    def forward_cached(self, x, cos_sin, step):
+        """The new tokens x (B, T, C) of a step of the paged cache; cos_sin at their
+        positions, (B, T, 1, head_dim / 2)."""
+        B, T, C = x.size()
+        q, k, v = self.qkv_computer(x, step)
+        cos, sin = cos_sin
+        q, k = norm(apply_rotary_emb(q, cos, sin)), norm(apply_rotary_emb(k, cos, sin))
+        y = step.attend(self.layer_idx, q, k, v, scale=self.scale)
+        return self.c_proj(y.reshape(B, T, C))
+
 
 class MLP(nn.Module):
     def __init__(self, config: GPTConfig):
@@ -116,8 +128,14 @@ class Block(nn.Module):
         x = x + self.attn(norm(x), cos_sin)
         return x + self.mlp(norm(x))
 
+    def forward_cached(self, x, cos_sin, step):
+        x = x + self.attn.forward_cached(norm(x), cos_sin, step)
+        return x + self.mlp(norm(x))
+
 
 class GPT(nn.Module):
+    SOFTCAP = 15.0  # of the logits
+
     def __init__(self, config: GPTConfig, pad_vocab_to: int = 64):
         super().__init__()
         self.config = config
@@ -151,6 +169,22 @@ class GPT(nn.Module):
     def filters(self):
         return [blk.attn.qkv_computer.ltv_filter for blk in self.h]
 
+    def cached_features(self, idx: torch.Tensor, step) -> torch.Tensor:
+        """The final hidden states (B, T, C) of a step's new tokens idx (B, T)
+        (``PagedKVCache.step``), given what the cache holds of their sequences."""
+        T = idx.size(1)
+        at = torch.tensor(step.positions, device=idx.device)[:, None] + torch.arange(
+            T, device=idx.device)
+        cos_sin = self.cos[0][at], self.sin[0][at]
+        x = norm(self.wte(idx))
+        for blk in self.h:
+            x = blk.forward_cached(x, cos_sin, step)
+        return norm(x)
+
+    def raw_logits(self, hidden: torch.Tensor) -> torch.Tensor:
+        """Logits (..., vocab_size) before the cap, which ``token_logprobs`` applies."""
+        return self.lm_head(hidden)[..., : self.config.vocab_size]
+
     def forward(self, idx: torch.Tensor, targets: torch.Tensor | None = None):
         B, T = idx.shape
         cos_sin = (self.cos[:, :T], self.sin[:, :T])
@@ -158,7 +192,7 @@ class GPT(nn.Module):
         for blk in self.h:
             x = blk(x, cos_sin)
         logits = self.lm_head(norm(x))[..., : self.config.vocab_size].float()
-        logits = 15.0 * torch.tanh(logits / 15.0)
+        logits = self.SOFTCAP * torch.tanh(logits / self.SOFTCAP)
         if targets is None:
             return logits
         return F.cross_entropy(logits.view(-1, logits.size(-1)), targets.view(-1), ignore_index=-1)
