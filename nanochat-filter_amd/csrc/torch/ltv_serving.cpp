@@ -9,6 +9,8 @@
 #include <c10/hip/HIPCachingAllocator.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/extension.h>
 
 #include <cmath>
@@ -408,7 +410,8 @@ Rows rows_of(const Tensor& logits, const Tensor& targets) {
   TORCH_CHECK(logits.is_cuda(), "LTV HIP kernels need GPU tensors, got logits on ",
               logits.device());
   on_device(targets, "targets", logits);
-  TORCH_CHECK_VALUE(logits.dim() >= 1 && targets.sizes() == logits.sizes().slice(0, logits.dim() - 1),
+  TORCH_CHECK_VALUE(logits.dim() >= 1 &&
+                        targets.sizes() == logits.sizes().slice(0, logits.dim() - 1),
                     "logits must be (..., vocabulary) and targets (...), got ", logits.sizes(),
                     " and ", targets.sizes());
   TORCH_CHECK_TYPE(targets.scalar_type() == at::kLong || targets.scalar_type() == at::kInt,
@@ -494,8 +497,15 @@ class TokenLogprobs : public torch::autograd::Function<TokenLogprobs> {
   static variable_list backward(AutogradContext* ctx, const variable_list& g) {
     const variable_list s = ctx->get_saved_variables();
     if (!g[0].defined() && !g[1].defined() && !g[2].defined()) return {{}, {}, {}, {}};
-    return {logprobs_backward(s[0], s[1], s[2], s[3], s[4], g[0], g[1], g[2],
-                              ctx->saved_data["cap"].toDouble()), {}, {}, {}};
+    Tensor gx = logprobs_backward(s[0], s[1], s[2], s[3], s[4], g[0], g[1], g[2],
+                                  ctx->saved_data["cap"].toDouble());
+    // (with create_graph: a second derivative is refused, not taken as zero)
+    if (at::GradMode::is_enabled())
+      torch::autograd::set_history(
+          gx, std::make_shared<torch::autograd::Error>(
+                  "token_logprobs is differentiable once only",
+                  torch::autograd::collect_next_edges(s[0], g[0], g[1], g[2])));
+    return {gx, {}, {}, {}};
   }
 };
 

@@ -33,7 +33,7 @@ def token_logprobs(logits: Tensor, targets: Tensor, *, top_k: int = 0,
     A target outside [0, V) (-1, the ignored index of the training loss) has log
     probability 0 and no gradient.  The alternatives are the ``top_k`` <= 64 largest
     logits in descending order, equal ones by ascending index, NaN above all.  Sums are
-    in float32.  Differentiable: logprobs, entropy and top_logprobs."""
+    in float32.  Differentiable once: logprobs, entropy and top_logprobs."""
     cap = 0.0 if softcap is None else float(softcap)
     if softcap is not None and not cap > 0.0:
         raise ValueError(f"softcap must be positive and finite, got {softcap}")

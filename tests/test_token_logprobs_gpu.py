@@ -263,6 +263,16 @@ def test_gradient_of_some_outputs():
     assert not out.top_ids.requires_grad
 
 
+def test_second_gradient_is_refused():
+    x, t = _randn(3, 40, seed=11).requires_grad_(True), _targets(3, 40)
+    lp = _ops().token_logprobs(x, t).logprobs.sum()
+    (want,) = torch.autograd.grad(lp, [x], retain_graph=True)
+    (got,) = torch.autograd.grad(lp, [x], create_graph=True)
+    assert torch.equal(got.detach(), want)
+    with pytest.raises(RuntimeError, match="once"):
+        torch.autograd.grad(got.square().sum(), [x])
+
+
 def test_gradient_with_masked_entries():
     """-inf and lowest entries have probability 0 and gradient 0, not NaN."""
     for dtype in (BF, F32):
