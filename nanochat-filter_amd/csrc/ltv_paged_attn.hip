@@ -18,8 +18,11 @@
 // column at a time).  Both tiles are shared by the wavefronts through LDS, two buffers
 // deep: the next tile is on its way, straight into LDS, while this one is computed.
 //
-// Split.  Few rows and many keys leave compute units idle, so a sequence's keys are cut
-// into chunks that workgroups take side by side; a second kernel joins their (m, l, o).
+// Work.  All row tiles of a call, each as long as its keys, are laid on a line, and the
+// line is cut into equal ranges, one for each workgroup that the card holds at a time: no
+// workgroup is empty or ends late, whatever mixture of lengths a call has.  The line is made
+// on the device, which knows the lengths.  A range begins and ends within a row tile as it
+// comes; a second kernel joins the (m, l, o) of the tiles that were cut.
 #include <algorithm>
 #include <type_traits>
 
@@ -42,7 +45,7 @@ struct AttnArgs {
   const char* v;
   char* out;
   float* lse;
-  float* part;                // partial o, then (m, l), of the split sequences
+  float* part;                // partial o, then (m, l), of the tiles that are cut
   int64_t qs[3], os[3];       // bytes
   int64_t kh, vh;             // bytes from head to head of the pages
   uint32_t kp, ks, vp, vs;    // 16-byte units from page to page and row to row
@@ -50,11 +53,15 @@ struct AttnArgs {
   int q_aligned;
   int scalar_pages;           // load_full: 1 pages are multiples of 16 rows, 2 of 64
   float scale;                // with log2(e)
-  int tiles, group;           // row tiles of the grid, and how many follow each other
-  int chunk, nsplit;          // keys of a split, splits of the grid
-  int64_t rows_cap;           // sequences of more rows are not split
-  int by_token;               // how the partials are laid out
+  int log_group, ranges;      // log2 of the workgroups side by side, and how many such groups
+  int least;                  // shortest range
+  int unit;                   // log2 of the blocks of keys in a unit of length
+  int group_tokens, slope;    // tokens of a group's row tiles; units that each is longer by
+  int part_tile;              // rows of a partial tile
+  PageDiv by_g, by_ranges;    // divisions by g and by the number of ranges
   int64_t part_rows;
+  int* head;                  // how many ranges the call came to
+  struct Cut* cuts;
 };
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -170,22 +177,78 @@ __device__ __forceinline__ float across_halves_max(float x) {
   return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
+// The sum of x over the lanes up to each: within rows of 16 by shifts, then the rows' last.
+__device__ __forceinline__ uint32_t wave_sum_up_to(uint32_t x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast 15, 31
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
+  return x;
+}
+
 // (row numbers stay below 2^30: divisions of 64 bits would take longer than small calls)
 __device__ __forceinline__ int over(int a, int b) { return (int)((unsigned)a / (unsigned)b); }
 
-// The splits of a sequence: 1, or how many chunks its keys make.
-__device__ __forceinline__ int splits_of(const AttnArgs& a, const PagedSeq& s) {
-  if ((int64_t)s.n * a.g > a.rows_cap) return 1;
-  return max(1, min(a.nsplit, (s.len + a.chunk - 1) / a.chunk));
+// The line.  A sequence's row tiles are taken in groups of 2^a.log_group that workgroups of
+// one XCD work on side by side, so that its L2 holds what they read for all but the first:
+// tiles of one k/v head, which read the same keys, or where it has fewer, of several heads.
+// A group is as long as the blocks of keys (of one tile in LDS) of its longest row tile, in
+// units of 2^a.unit blocks, about: c0, and slope more for each group of the head.
+struct Line {
+  int tiles, heads;  // row tiles, heads of a group
+  int groups;        // of a head
+  int rounds;        // times that many heads, all together
+  uint32_t c0, head, all;
+
+  __device__ __forceinline__ uint32_t before(const AttnArgs& a, int j) const {
+    const uint32_t k = j;  // (the product's half modulo 2^32, whatever k is)
+    return k * c0 + a.slope * (k % 2 ? (k - 1) / 2 * k : k / 2 * (k - 1));
+  }
+  template <int KT>
+  static __device__ __forceinline__ Line of(const AttnArgs& a, int n, int len) {
+    Line u{0, 1, 0, 0, 0, 0, 0};
+    if (n <= 0) return u;
+    u.tiles = (n * a.g + kAttnRows - 1) / kAttnRows;
+    const int several = u.tiles == 1 ? a.log_group : u.tiles == 2 && a.log_group == 2 ? 1 : 0;
+    u.heads = 1 << several;
+    u.groups = (u.tiles + (1 << a.log_group) - 1) >> a.log_group;
+    u.rounds = (a.NKVH + u.heads - 1) >> several;
+    const int past = max(len - n, 0);
+    u.c0 = max(1, (min(len, past + min(n, a.group_tokens)) + KT - 1) / KT >> a.unit);
+    u.head = u.before(a, u.groups);
+    u.all = u.rounds * u.head;
+    return u;
+  }
+};
+
+// Keys that the last row of a row tile sees, and the block of keys at which a cut at f of
+// the tile's c units is.
+__device__ __forceinline__ int keys_of(const AttnArgs& a, const PagedSeq& s, int tile) {
+  const int last = a.by_g.quot(min((tile + 1) * kAttnRows, s.n * a.g) - 1);
+  return a.batch.P > 0 && a.batch.W > 0 ? max(s.len - s.n + last + 1, 0) : 0;
+}
+__device__ __forceinline__ int cut_at(uint32_t f, uint32_t c, int blocks) {
+  if (f >= c) return blocks;
+  return min(blocks, (int)fmaf((float)f, (float)blocks * __builtin_amdgcn_rcpf((float)c), 0.5f));
 }
 
-// A row's place among the partials (D values each; behind them all, its m and l): by its
-// token and head where any sequence may be split, else among the rows_cap of its sequence
-// and k/v head.
-__device__ __forceinline__ int64_t part_row(const AttnArgs& a, int bh, int split, int64_t row,
-                                            int64_t trow, int h) {
-  if (a.by_token) return ((int64_t)split * a.batch.total + trow) * a.NH + h;
-  return ((int64_t)bh * a.nsplit + split) * a.rows_cap + row;
+// A row tile whose first cut is a workgroup's begin, for the joining kernel.
+struct Cut {
+  int rows;           // 0: none
+  int b, kvh, token;  // token: of the sequence's first, in packed rows
+  int tile, last;     // last: range with a piece of it
+  uint32_t at, c;     // where its group is on the line, and how long
+  int blocks;         // of keys
+  uint32_t length;    // of a range
+  int pad[2];
+};
+
+// Rows of partials (D values each; behind them all, each row's m and l): two row tiles for
+// each workgroup, of the piece that continues a tile and of the one that begins the last.
+__device__ __forceinline__ int64_t part_at(const AttnArgs& a, int range, int member, bool begins) {
+  return ((int64_t)((range << a.log_group) + member) * 2 + begins) * a.part_tile;
 }
 __device__ __forceinline__ float2* part_ml(const AttnArgs& a) {
   return reinterpret_cast<float2*>(a.part + a.part_rows * a.D);
@@ -194,11 +257,11 @@ __device__ __forceinline__ float2* part_ml(const AttnArgs& a) {
 // Rows row0 .. row_end - 1 of a workgroup over keys begin .. end - 1, each key that a row
 // does not see left alone altogether: the way of tiles with infinite or NaN values among
 // those that some rows do not see.  Sixteen groups of sixteen lanes take a row's keys in
-// turn, a lane holding eight channels.  split: whose partials these are, or -1.
+// turn, a lane holding eight channels.  part0: the partials of row0, or -1.
 template <typename T>
 __device__ __forceinline__ void rows_one_by_one(const AttnArgs& a, const PagedSeq& s, int b,
                                                 int kvh, int row0, int row_end, int begin, int end,
-                                                int split, float* lds) {
+                                                int64_t part0, float* lds) {
 #pragma clang fp contract(off)  // (x - base below must not be a fused form of the product)
   float* lds_m = lds;
   float* lds_l = lds + 16;
@@ -206,7 +269,7 @@ __device__ __forceinline__ void rows_one_by_one(const AttnArgs& a, const PagedSe
   const int c = threadIdx.x & 15, gi = threadIdx.x >> 4;
   const bool on = c * 8 < a.D;
   for (int row = row0; row < row_end; ++row) {
-    const int t = over(row, a.g), h = kvh * a.g + row - t * a.g;
+    const int t = a.by_g.quot(row), h = kvh * a.g + row - t * a.g;
     const int last = min(end - 1, s.len - s.n + t);
     const int64_t trow = a.batch.starts != nullptr ? s.row0 + t : (int64_t)b * a.batch.T + t;
     const char* q = a.q + (a.batch.starts != nullptr ? trow * a.qs[1]
@@ -255,8 +318,8 @@ __device__ __forceinline__ void rows_one_by_one(const AttnArgs& a, const PagedSe
       sum = fmaf(lds_l[i], w, sum);
       if (d < a.D) acc = fmaf(lds_o[i * 128 + d], w, acc);
     }
-    if (split >= 0) {
-      const int64_t at = part_row(a, b * a.NKVH + kvh, split, row, trow, h);
+    if (part0 >= 0) {
+      const int64_t at = part0 + row - row0;
       if (d < a.D) a.part[at * a.D + d] = acc;
       if (d == 0) part_ml(a)[at] = make_float2(mx, sum);
     } else {
@@ -282,89 +345,99 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_tile_kernel(const AttnAr
   constexpr int kRow = Ti::kChunks * 16, kTile = Ti::kUnits * 16;  // bytes
   __shared__ uint4 lds[4 * Ti::kUnits];                            // K, V, and again
 
-  // Workgroup w runs on XCD w % 8.  Up to four row tiles that read the same keys -- those of
-  // one sequence, k/v head and split -- follow each other on one XCD, whose L2 then holds
-  // the keys for all but the first of them; such groups go around the XCDs, those of the
-  // last rows, with the most keys, first.  A sequence's splits start at an XCD that differs
-  // by sequence and head, or those in use of short sequences would land on few of them.
-  const int xcd = blockIdx.x & 7, place = blockIdx.x >> 3;
-  const int round = over(place, a.group), unit = round * 8 + xcd;
-  const int pairs = a.batch.B * a.NKVH * a.nsplit, rank = over(unit, pairs);
-  const int pair = unit - rank * pairs, bh = over(pair, a.nsplit);
-  const int tile0 = a.tiles - 1 - rank * a.group - (place - round * a.group);
-  if (tile0 < 0) return;
-  const int split = (int)((unsigned)(pair - bh * a.nsplit + bh) % (unsigned)a.nsplit);
-  const int b = over(bh, a.NKVH), kvh = bh - b * a.NKVH;
-  const PagedSeq s = paged_seq(a.batch, b);
-  // The page of the lane-th key of a tile, -1: none.  (Read without waiting for the
-  // sequence's length; what is past the end is sorted out where it is used.)
-  auto page_of = [&](int kt) {
-    const int col = a.batch.div.quot(kt + ((int)threadIdx.x & (KT - 1)));
-    const int p = a.batch.W > 0 ? s.table[min(col, a.batch.W - 1)] : -1;
-    return p < a.batch.P ? p : -1;
-  };
-  const int begin = split * a.chunk, first_page = page_of(begin);
-  const int nsplit = splits_of(a, s);
-  if (split >= nsplit) return;
-  const int rows = s.n * a.g;
-
+  // The lengths of all sequences, a run of them to each thread, and their sum.
+  __shared__ uint32_t sums[kAttnWaves];
+  __shared__ struct { PagedSeq s; int b; uint32_t at; } found;  // the sequence of a range's begin
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const char* kbase = a.k + (int64_t)kvh * a.kh;
-  const char* vbase = a.v + (int64_t)kvh * a.vh;
+  const int per = (a.batch.B + kAttnThreads - 1) / kAttnThreads;
+  const int b0 = min((int)threadIdx.x * per, a.batch.B), b1 = min(b0 + per, a.batch.B);
+  uint32_t mine = 0;
+  PagedSeq q{a.batch.table, 0, 0, 0};
+  for (int i = b0; i < b1; ++i) {
+    q = paged_seq(a.batch, i);
+    mine += Line::of<KT>(a, q.n, q.len).all;
+  }
+  uint32_t upto = wave_sum_up_to(mine);
+  if ((threadIdx.x & 63) == 63) sums[wave] = upto;
+  if (threadIdx.x == 0) {
+    found.s = q;
+    found.b = 0;
+    found.at = 0;
+  }
+  __syncthreads();
+  uint32_t all = 0;
+#pragma unroll
+  for (int w = 0; w < kAttnWaves; ++w) {
+    if (w < wave) upto += sums[w];
+    all += sums[w];
+  }
+  all = __builtin_amdgcn_readfirstlane(all);
+  const uint32_t length = max(a.least, a.by_ranges.quot(all + a.ranges - 1));
+  const int ranges = min(over(all + length - 1, length), a.ranges);
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    *a.head = ranges;
+  }
+  // Workgroup w runs on XCD w % 8: consecutive ranges stay on one.
+  const int per_xcd = (ranges + 7) / 8, local = blockIdx.x >> 3 >> a.log_group;
+  const int range = (blockIdx.x & 7) * per_xcd + local;
+  const int member = (blockIdx.x >> 3) & ((1 << a.log_group) - 1);
+  if (local >= per_xcd || range >= ranges) return;
+  const uint32_t x0 = range * length, x1 = min(x0 + length, all);
+  if (threadIdx.x == 0) a.cuts[(range << a.log_group) + member].rows = 0;  // (until it has one)
+  if (x0 >= upto - mine && x0 < upto) {
+    uint32_t at = upto - mine;
+    int i = b0;
+    if (per > 1)
+      for (;; ++i) {
+        q = paged_seq(a.batch, i);
+        const uint32_t here = Line::of<KT>(a, q.n, q.len).all;
+        if (x0 - at < here || i == b1 - 1) break;
+        at += here;
+      }
+    found.s = q;
+    found.b = i;
+    found.at = at;
+  }
+  __syncthreads();
+  auto uniform = [](auto x) {  // (from LDS, into scalar registers)
+    static_assert(sizeof(x) % 4 == 0, "whole words");
+    int w[sizeof(x) / 4];
+    __builtin_memcpy(w, &x, sizeof(x));
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(x) / 4; ++i) w[i] = __builtin_amdgcn_readfirstlane(w[i]);
+    __builtin_memcpy(&x, w, sizeof(x));
+    return x;
+  };
+  int b = uniform(found.b);
+  uint32_t at = uniform(found.at);  // of the group on the line
+  PagedSeq s{uniform(found.s.table), uniform(found.s.len), uniform(found.s.n),
+             uniform(found.s.row0)};
+  Line u = Line::of<KT>(a, s.n, s.len);
+  if (u.all == 0) return;  // (starts that do not ascend)
+  int round = over(x0 - at, u.head), group = 0;
+  at += round * u.head;
+  for (int hi = u.groups - 1; group < hi;) {
+    const int mid = (group + hi + 1) >> 1;
+    if (u.before(a, mid) <= x0 - at) group = mid; else hi = mid - 1;
+  }
+  at += u.before(a, group);
   const int chunks = a.D / Ty::kChunk;
 
-  // (more rows than the grid was sized for: its tiles are walked again)
-  for (int tile = tile0; tile * kAttnRows < rows; tile += a.tiles) {
-    // (opaque: what follows from the lane is not kept in registers around this loop)
+  // Keys begin .. end of a row tile, into its rows of the output or the partials from part0
+  // on (-1: none).
+  auto piece = [&](int kvh, int tile, int begin, int end, int64_t part0) {
+    const char* kbase = a.k + (int64_t)kvh * a.kh;
+    const char* vbase = a.v + (int64_t)kvh * a.vh;
+    // The page of the lane-th key of a tile, -1: none.
+    auto page_of = [&](int kt) {
+      const int col = a.batch.div.quot(kt + ((int)threadIdx.x & (KT - 1)));
+      const int p = s.table[min(col, a.batch.W - 1)];
+      return p < a.batch.P ? p : -1;
+    };
+    // (opaque: what follows from the lane is not kept in registers around the pieces)
     int thread = threadIdx.x;
     asm volatile("" : "+v"(thread));
     const int lane = thread & 63, ln = lane & 31, hf = lane >> 5;
-    const int row = tile * kAttnRows + wave * 32 + ln;
-    const bool row_ok = row < rows;
-    const int t = row_ok ? over(row, a.g) : 0;
-    const int h = kvh * a.g + (row_ok ? row - t * a.g : 0);
-    const int pos = row_ok ? s.len - s.n + t : -1;
-    const int64_t trow = a.batch.starts != nullptr ? s.row0 + t : (int64_t)b * a.batch.T + t;
-
-    // the last position that any row of the wavefront, and of the workgroup, sees
-    const bool wave_on = tile * kAttnRows + wave * 32 < rows;
-    const int wfirst = tile * kAttnRows + wave * 32, last = rows - 1;
-    const int wave_end = wave_on ? s.len - s.n + over(min(wfirst + 31, last), a.g) + 1 : 0;
-    const int wave_min = wave_on ? s.len - s.n + over(wfirst, a.g) : 0;
-    const int tlast = over(min(tile * kAttnRows + kAttnRows - 1, last), a.g);
-    int end = a.batch.P > 0 ? s.len - s.n + tlast + 1 : 0;
-    if (split < nsplit - 1) end = min(end, begin + a.chunk);
-
-    // Q: chunk 2 step + half of the lane's row
-    uint4 qf[kSteps];
-    {
-      const char* q = a.q + (a.batch.starts != nullptr ? trow * a.qs[1]
-                                                       : b * a.qs[0] + t * a.qs[1]) + h * a.qs[2];
-#pragma unroll
-      for (int i = 0; i < kSteps; ++i) {
-        const int c = 2 * i + hf;
-        qf[i] = make_uint4(0, 0, 0, 0);
-        if (row_ok && c < chunks) {
-          if (a.q_aligned) {
-            qf[i] = *reinterpret_cast<const uint4*>(q + c * 16);
-          } else {
-            T e[Ty::kChunk];
-#pragma unroll
-            for (int x = 0; x < Ty::kChunk; ++x)
-              e[x] = reinterpret_cast<const T*>(q)[c * Ty::kChunk + x];
-            __builtin_memcpy(&qf[i], e, 16);
-          }
-        }
-      }
-    }
-
-    f32x16 o[kDB];
-#pragma unroll
-    for (int d = 0; d < kDB; ++d)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
-    float m = -INFINITY, l = 0.0f;  // l: of this lane's keys
-
     uint64_t held = 0;
     // A full tile of pages that all hold keys, and whose sizes are multiples of 16: the
     // rows that a wavefront's load fetches are in one block of kBlock rows and so in one
@@ -451,14 +524,65 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_tile_kernel(const AttnAr
     } else {
       vat += 4 * hf * kRow + ((ln / 4) ^ Ti::v_swizzle(4 * hf)) * 16 + (ln % 4) * 4;
     }
-    int again = 0;
+    // the first tile on its way before all else
+    uint64_t next = 0;
+    int page = -1;
     if (begin < end) {
-      int page = first_page;
+      page = page_of(begin);
       barrier();  // (the row tile before is read to its end)
-      uint64_t next;
       is_full(begin, page, next);
       load(begin, page, 0);
       page = page_of(begin + KT);
+    }
+
+    const int rows = s.n * a.g, row = tile * kAttnRows + wave * 32 + ln;
+    const bool row_ok = row < rows;
+    const int t = row_ok ? a.by_g.quot(row) : 0;
+    const int h = kvh * a.g + (row_ok ? row - t * a.g : 0);
+    const int pos = row_ok ? s.len - s.n + t : -1;
+    const int64_t trow = a.batch.starts != nullptr ? s.row0 + t : (int64_t)b * a.batch.T + t;
+
+    // the last position that any row of the wavefront, and of the workgroup, sees
+    const bool wave_on = tile * kAttnRows + wave * 32 < rows;
+    const int wfirst = tile * kAttnRows + wave * 32, last = rows - 1;
+    const int wave_end = wave_on ? s.len - s.n + a.by_g.quot(min(wfirst + 31, last)) + 1 : 0;
+    const int wave_min = wave_on ? s.len - s.n + a.by_g.quot(wfirst) : 0;
+
+    // Q: chunk 2 step + half of the lane's row
+    uint4 qf[kSteps];
+    {
+      const char* q = a.q + (a.batch.starts != nullptr ? trow * a.qs[1]
+                                                       : b * a.qs[0] + t * a.qs[1]) + h * a.qs[2];
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) qf[i] = make_uint4(0, 0, 0, 0);
+      if (row_ok && a.q_aligned) {
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i)
+          if (!PAD || 2 * i + hf < chunks)
+            qf[i] = *reinterpret_cast<const uint4*>(q + (2 * i + hf) * 16);
+      } else if (row_ok) {
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+          const int c = 2 * i + hf;
+          if (c >= chunks) continue;
+          T e[Ty::kChunk];
+#pragma unroll
+          for (int x = 0; x < Ty::kChunk; ++x)
+            e[x] = reinterpret_cast<const T*>(q)[c * Ty::kChunk + x];
+          __builtin_memcpy(&qf[i], e, 16);
+        }
+      }
+    }
+
+    f32x16 o[kDB];
+#pragma unroll
+    for (int d = 0; d < kDB; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
+    float m = -INFINITY, l = 0.0f;  // l: of this lane's keys
+
+    int again = 0;
+    if (begin < end) {
       int buf = 0;
       for (int kt = begin; kt < end; kt += KT, buf ^= 1) {
         held = next;
@@ -654,13 +778,13 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_tile_kernel(const AttnAr
 
     if (__syncthreads_or(again)) {
       rows_one_by_one<T>(a, s, b, kvh, tile * kAttnRows, min(rows, (tile + 1) * kAttnRows), begin,
-                         end, nsplit > 1 ? split : -1, reinterpret_cast<float*>(lds));
-      continue;
+                         end, part0, reinterpret_cast<float*>(lds));
+      return;
     }
     l += __shfl_xor(l, 32);
     if (row_ok) {
-      if (nsplit > 1) {
-        const int64_t at = part_row(a, bh, split, row, trow, h);
+      if (part0 >= 0) {
+        const int64_t at = part0 + wave * 32 + ln;
         float* po = a.part + at * a.D;
 #pragma unroll
         for (int d = 0; d < kDB; ++d)
@@ -694,142 +818,182 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_tile_kernel(const AttnAr
           a.lse[trow * a.NH + h] = l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
       }
     }
+  };
+
+  for (uint32_t x = x0; x < x1;) {
+    // units from .. to of a group's c
+    const uint32_t c = u.c0 + a.slope * group;
+    const uint32_t from = x - at, to = min(x1 - at, c);
+    // (several heads: one or two tiles of each)
+    const int k = u.heads == 1 ? 0 : member >> (u.tiles - 1);
+    const int kvh = round * u.heads + k;
+    const int tile = u.heads == 1 ? (group << a.log_group) + member : member & (u.tiles - 1);
+    const bool on = k < u.heads && kvh < a.NKVH && tile < u.tiles;
+    // (a sequence of more rows than the call was sized for is not cut)
+    const int rows = s.n * a.g;
+    const bool cuts = min(rows, kAttnRows) <= a.part_tile;
+    if (on && (cuts || from == 0)) {
+      const bool whole = !cuts || (from == 0 && to == c);
+      const int keys = keys_of(a, s, tile), blocks = (keys + KT - 1) / KT;
+      const int begin = whole ? 0 : cut_at(from, c, blocks) * KT;
+      const int end = whole || to == c ? keys : min(keys, cut_at(to, c, blocks) * KT);
+      if (whole || begin < end)
+        piece(kvh, tile, begin, end, whole ? -1 : part_at(a, range, member, from == 0));
+      if (x == x0 && from > 0 && from <= length && threadIdx.x == 0)
+        a.cuts[(range << a.log_group) + member] =
+            Cut{min(rows - tile * kAttnRows, kAttnRows), b, kvh, (int)s.row0, tile,
+                min(over(at + c - 1, length), ranges - 1), at, c, blocks, length, {}};
+    }
+    x = at + to;
+    at += c;
+    if (++group == u.groups) {
+      group = 0;
+      ++round;
+    }
+    while (round >= u.rounds && x < x1) {
+      if (++b >= a.batch.B) return;
+      s = paged_seq(a.batch, b);
+      u = Line::of<KT>(a, s.n, s.len);
+      round = 0;
+    }
   }
 }
 
-// Joins the splits of a row: W wavefronts per row take them in turn, a lane two channels
-// (one wavefront, four rows to a workgroup, up to 16 splits; else 4 or 16).
-template <typename T, int W>
-__global__ void __launch_bounds__(W < 4 ? 256 : W * 64) attn_join_kernel(const AttnArgs a) {
-  __shared__ float lds_o[W][128];
-  __shared__ float lds_l[W];
-  const int lane = threadIdx.x & 63, wave = W == 1 ? 0 : threadIdx.x >> 6;
-  int unit = blockIdx.x;
-  if (W == 1) unit = unit * 4 + (threadIdx.x >> 6);
-  int b, h, row, t;
-  int64_t trow;
-  PagedSeq s;
-  if (a.by_token) {
-    const int token = over(unit, a.NH);
-    trow = token;
-    h = unit - token * a.NH;
-    if (trow >= a.batch.total) return;
-    if (a.batch.starts != nullptr) {
-      // the last sequence that starts at the row or before it
-      int lo = 0, hi = a.batch.B - 1;
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (a.batch.starts[mid] <= trow) lo = mid; else hi = mid - 1;
-      }
-      b = lo;
-    } else {
-      b = over(token, a.batch.T);
-    }
-    s = paged_seq(a.batch, b);
-    t = (int)(a.batch.starts != nullptr ? trow - s.row0 : trow - (int64_t)b * a.batch.T);
-    if (t < 0 || t >= s.n) return;
-    row = t * a.g + h % a.g;
-  } else {
-    const int nbh = a.batch.B * a.NKVH;
-    row = over(unit, nbh);
-    const int bh = unit - row * nbh;
-    b = over(bh, a.NKVH);
-    s = paged_seq(a.batch, b);
-    if (row >= a.rows_cap || row >= s.n * a.g) return;
-    t = over(row, a.g);
-    h = (bh - b * a.NKVH) * a.g + row - t * a.g;
-    trow = a.batch.starts != nullptr ? s.row0 + t : (int64_t)b * a.batch.T + t;
-  }
-  const int nsplit = splits_of(a, s);
-  if (nsplit <= 1) return;
-  const int bh = b * a.NKVH + over(h, a.g);
-  const int64_t first = part_row(a, bh, 0, row, trow, h);
-  const int64_t step = part_row(a, bh, 1, row, trow, h) - first;
-  const float2* ml = part_ml(a) + first;
-  const float* part = a.part + first * a.D;
-  float m = -INFINITY;
-  for (int i = lane; i < nsplit; i += 64) m = fmaxf(m, ml[i * step].x);
+// Joins the pieces of the row tiles that were cut, 32 lanes to a row and four channels to a
+// lane.  Of few pieces 32 lanes take all of a row, of many the eight groups of a workgroup
+// share a row's.  It is all latency: the record of the cut, then the partials of four pieces
+// at a time.
+template <typename T>
+__global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a, int rows_each) {
+  constexpr int G = 8;  // groups
+  __shared__ float lds_o[G][128];
+  __shared__ float2 lds_ml[G];
+  const int range = blockIdx.x >> a.log_group, member = blockIdx.x & ((1 << a.log_group) - 1);
+  const Cut cut = a.cuts[blockIdx.x];
+  if (range >= *a.head) return;
+  const int first = range - 1, pieces = cut.last - first + 1;
+  const int row0 = blockIdx.y * rows_each, row_end = min(cut.rows, row0 + rows_each);
+  if (row0 >= row_end) return;
+  const bool share = pieces > (rows_each == 1 ? 4 : 16);
+  const int lane = threadIdx.x & 31, gi = threadIdx.x >> 5;
+  const bool on = lane * 4 < a.D;
+  for (int row = row0 + (share ? 0 : gi); row < row_end; row += share ? 1 : G) {
+    float m = -INFINITY, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int p0 = first + (share ? gi : 0); p0 <= cut.last; p0 += 4 * (share ? G : 1)) {
+      float2 ml[4];
+      float4 v[4];
 #pragma unroll
-  for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
-  const float base = m == -INFINITY ? 0.0f : m;
-  const bool on = lane * 2 < a.D;
-  float ox = 0.0f, oy = 0.0f, l = 0.0f;
-#pragma unroll 4
-  for (int i = wave; i < nsplit; i += W) {
-    const float2 p = ml[i * step];
-    const float2 x = on ? *reinterpret_cast<const float2*>(part + i * step * a.D + lane * 2)
-                        : make_float2(0.0f, 0.0f);
-    // (a split without keys has weight 0; its sums are 0 too)
-    const float w = __builtin_amdgcn_exp2f(p.x - base);
-    l = fmaf(p.y, w, l);
-    ox = fmaf(x.x, w, ox);
-    oy = fmaf(x.y, w, oy);
-  }
-  if constexpr (W > 1) {
+      for (int i = 0; i < 4; ++i) {
+        const int p = p0 + i * (share ? G : 1), pp = min(p, cut.last);
+        const uint32_t x = pp * cut.length;
+        const uint32_t from = x > cut.at ? x - cut.at : 0, to = x + cut.length - cut.at;
+        const int64_t at = part_at(a, pp, member, x <= cut.at) + row;
+        ml[i] = part_ml(a)[at];
+        v[i] = on ? *reinterpret_cast<const float4*>(a.part + at * a.D + lane * 4)
+                  : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        // (a piece of no keys was not written)
+        if (p > cut.last || cut_at(from, cut.c, cut.blocks) == cut_at(to, cut.c, cut.blocks)) {
+          ml[i] = make_float2(-INFINITY, 0.0f);
+          v[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+      }
+      float mn = m;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mn = fmaxf(mn, ml[i].x);
+      const float base = mn == -INFINITY ? 0.0f : mn;
+      const float was = __builtin_amdgcn_exp2f(m - base);
+      m = mn;
+      l *= was;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] *= was;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        // (a piece without keys for the row has weight 0; its sums are 0 too)
+        const float w = __builtin_amdgcn_exp2f(ml[i].x - base);
+        l = fmaf(ml[i].y, w, l);
+        o[0] = fmaf(v[i].x, w, o[0]);
+        o[1] = fmaf(v[i].y, w, o[1]);
+        o[2] = fmaf(v[i].z, w, o[2]);
+        o[3] = fmaf(v[i].w, w, o[3]);
+      }
+    }
+    if (share) {
+      __syncthreads();  // (the row before is read)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) lds_o[gi][lane * 4 + e] = o[e];
+      if (lane == 0) lds_ml[gi] = make_float2(m, l);
+      __syncthreads();
+      if (gi != 0) continue;
+#pragma unroll
+      for (int i = 0; i < G; ++i) m = fmaxf(m, lds_ml[i].x);
+      const float base = m == -INFINITY ? 0.0f : m;
+      l = o[0] = o[1] = o[2] = o[3] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < G; ++i) {
+        const float w = __builtin_amdgcn_exp2f(lds_ml[i].x - base);
+        l = fmaf(lds_ml[i].y, w, l);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = fmaf(lds_o[i][lane * 4 + e], w, o[e]);
+      }
+    }
+    const int r = cut.tile * kAttnRows + row, t = a.by_g.quot(r), h = cut.kvh * a.g + r - t * a.g;
+    const int64_t trow = (a.batch.starts != nullptr ? cut.token : (int64_t)cut.b * a.batch.T) + t;
+    char* out = a.out + (a.batch.starts != nullptr ? trow * a.os[1]
+                                                   : cut.b * a.os[0] + t * a.os[1]) + h * a.os[2];
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     if (on) {
-      lds_o[wave][lane * 2] = ox;
-      lds_o[wave][lane * 2 + 1] = oy;
+      if constexpr (sizeof(T) == 2)
+        reinterpret_cast<uint2*>(out)[lane] =
+            make_uint2(cvt_pk_bf16(o[0] * inv, o[1] * inv), cvt_pk_bf16(o[2] * inv, o[3] * inv));
+      else
+        reinterpret_cast<float4*>(out)[lane] =
+            make_float4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
     }
-    if (lane == 0) lds_l[wave] = l;
-    __syncthreads();
-    if (wave != 0) return;
-    ox = oy = l = 0.0f;
-#pragma unroll
-    for (int w = 0; w < W; ++w) {
-      l += lds_l[w];
-      if (on) {
-        ox += lds_o[w][lane * 2];
-        oy += lds_o[w][lane * 2 + 1];
-      }
-    }
+    if (lane == 0 && a.lse != nullptr)
+      a.lse[trow * a.NH + h] =
+          l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
   }
-  char* out = a.out + (a.batch.starts != nullptr ? trow * a.os[1]
-                                                 : b * a.os[0] + t * a.os[1]) + h * a.os[2];
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  if (on) {
-    if constexpr (sizeof(T) == 2)
-      reinterpret_cast<uint32_t*>(out)[lane] = cvt_pk_bf16(ox * inv, oy * inv);
-    else
-      reinterpret_cast<float2*>(out)[lane] = make_float2(ox * inv, oy * inv);
-  }
-  if (lane == 0 && a.lse != nullptr)
-    a.lse[trow * a.NH + h] = l == 0.0f ? -INFINITY : (base + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
-// How a call is cut: row tiles of the grid, keys of a split, splits, and where the
-// splits' partials go.
+// How a call is cut.
 struct AttnPlan {
-  int tiles, group, chunk, nsplit, by_token;
-  int64_t rows_cap, joins, part_rows;
+  int group, ranges, least, unit, group_tokens, slope, part_tile;
+  bool joins;
+  int64_t part_rows;
+  size_t bytes, cuts_at;
 };
 
-AttnPlan plan_attention(const ltv_paged_batch& b, int NH, int NKVH, int max_len) {
+AttnPlan plan_attention(const ltv_paged_batch& b, int NH, int NKVH, int D, int max_len, int KT) {
   AttnPlan p;
-  const int64_t g = NH / NKVH, rows = std::max(b.T, 1) * g, seqs = (int64_t)b.B * NKVH;
-  p.tiles = (int)std::min<int64_t>((rows + kAttnRows - 1) / kAttnRows, 1 << 20);
-  const int groups = (p.tiles + 3) / 4;
-  p.group = (p.tiles + groups - 1) / groups;
-  // The row tiles there are at most.  The card holds 512 workgroups at a time (two per
-  // compute unit).  With fewer row tiles than five times that, every sequence is split
-  // into about that many workgroups, or the last ones of few would run alone; else those
-  // of a single tile are.  Chunks of at most 1,024 keys for each tile of a sequence keep
-  // a long one from outlasting the others.
-  const int64_t tiles = std::min(seqs * p.tiles, (b.total * g / kAttnRows + b.B) * NKVH);
-  p.by_token = tiles < 2560;
-  p.rows_cap = p.by_token ? int64_t(1) << 40 : std::min<int64_t>(rows, kAttnRows);
-  const int64_t keys = std::max(max_len, 1);
-  const int64_t want = keys * (p.by_token ? tiles : seqs) / 2560;
-  const int64_t least = rows <= 32 ? 64 : 128;  // (of few rows: all their latency is a tile's)
-  p.chunk = (int)std::min<int64_t>(std::max<int64_t>((want + 63) / 64 * 64, least),
-                                   p.by_token ? int64_t(1024) * p.tiles : 1024);
-  p.nsplit = (int)((keys + p.chunk - 1) / p.chunk);
-  p.joins = p.by_token ? b.total * NH : seqs * p.rows_cap;
-  p.part_rows = p.nsplit * (p.by_token ? b.total * NH : seqs * p.rows_cap);
+  const int64_t g = NH / NKVH, rows = std::max(b.T, 1) * g;
+  const int64_t tiles = (rows + kAttnRows - 1) / kAttnRows;
+  p.group = KT == 32 ? 1 : tiles >= 3 ? 4 : (int)tiles;
+  p.group_tokens = (int)((p.group * kAttnRows + g - 1) / g);
+  p.part_tile = (int)std::min<int64_t>(rows, kAttnRows);
+  // (of few rows all their latency is a tile's: there no range is too short)
+  p.least = (rows <= 32 ? 64 : 128) / KT;
+  // The card holds 512 workgroups at a time, two to a compute unit.  Fewer, if the call has
+  // no more tiles than that.
+  const int64_t groups =
+      NKVH * std::min((tiles + p.group - 1) / p.group * b.B,
+                      b.total * g / (p.group * kAttnRows) + b.B);
+  const int64_t most = groups * ((std::max(max_len, 1) + KT - 1) / KT);
+  p.ranges = (int)std::min<int64_t>(512 / p.group, (most + p.least - 1) / p.least);
+  p.ranges = std::max(8, (p.ranges + 7) / 8 * 8);
+  // Positions on the line have 32 bits: units of more blocks where it could be longer than
+  // 2^30, whatever the lengths are.
+  const int64_t keys = (int64_t)b.table_width * b.page_size;
+  const double bound = (double)NKVH * ((double)b.total * g / (p.group * kAttnRows) + b.B) *
+                       ((double)(keys + b.total) / KT + 64);
+  p.unit = 0;
+  while (bound / (double)(int64_t(1) << p.unit) > (double)(1 << 30)) ++p.unit;
+  p.slope = (int)(p.group * kAttnRows / g / KT) >> p.unit;
+  p.joins = keys > KT;
+  const int64_t n = (int64_t)p.ranges * p.group;
+  p.part_rows = p.joins ? n * 2 * p.part_tile : 0;
+  p.cuts_at = (size_t)p.part_rows * (D + 2) * sizeof(float);
+  p.bytes = p.cuts_at + n * sizeof(Cut) + 16;
   return p;
-}
-
-size_t part_bytes(const AttnPlan& p, int D) {
-  return p.nsplit <= 1 ? 0 : (size_t)p.part_rows * (D + 2) * sizeof(float);
 }
 
 }  // namespace
@@ -841,7 +1005,7 @@ extern "C" size_t ltv_paged_attention_workspace_size(int dtype, const ltv_paged_
                                                      int NH, int NKVH, int D, int max_len) {
   if (batch == nullptr || batch->B <= 0 || batch->T < 0 || NKVH <= 0 || NH < NKVH || D <= 0)
     return 0;
-  return part_bytes(plan_attention(*batch, NH, NKVH, max_len), D);
+  return plan_attention(*batch, NH, NKVH, D, max_len, dtype == LTV_DTYPE_F32 ? 32 : 64).bytes;
 }
 
 extern "C" int ltv_paged_attention(int dtype, const void* q, const int64_t q_strides[3],
@@ -869,9 +1033,8 @@ extern "C" int ltv_paged_attention(int dtype, const void* q, const int64_t q_str
                   (!pages || (k_pages && v_pages)),
               LTV_ERR_INVALID_ARG, "null pointer");
   const int es = elem_size(dtype), chunk = 16 / es;
-  const AttnPlan p = plan_attention(*batch, NH, NKVH, max_len);
-  LTV_REQUIRE(workspace_bytes >= part_bytes(p, D) && (p.nsplit <= 1 || workspace),
-              LTV_ERR_WORKSPACE, "workspace too small");
+  const AttnPlan p = plan_attention(*batch, NH, NKVH, D, max_len, dtype == LTV_DTYPE_F32 ? 32 : 64);
+  LTV_REQUIRE(workspace && workspace_bytes >= p.bytes, LTV_ERR_WORKSPACE, "workspace too small");
   // pages are addressed in 16-byte units of 32 bits
   bool fits = true, aligned = aligned16(k_pages) && aligned16(v_pages);
   for (int i = 0; i < 3; ++i)
@@ -896,20 +1059,19 @@ extern "C" int ltv_paged_attention(int dtype, const void* q, const int64_t q_str
              v_page_strides[1] * es, (uint32_t)(k_page_strides[0] / chunk),
              (uint32_t)(k_page_strides[2] / chunk), (uint32_t)(v_page_strides[0] / chunk),
              (uint32_t)(v_page_strides[2] / chunk), NH, NKVH, D, NH / NKVH, q_aligned ? 1 : 0,
-             !rows_fit || batch->page_size % 16 != 0 ? 0 : batch->page_size % 64 == 0 ? 2 : 1, scale * kLog2e, p.tiles, p.group, p.chunk, p.nsplit, p.rows_cap,
-             p.by_token, p.part_rows};
+             !rows_fit || batch->page_size % 16 != 0 ? 0 : batch->page_size % 64 == 0 ? 2 : 1,
+             scale * kLog2e, p.group == 4 ? 2 : p.group - 1, p.ranges, p.least, p.unit, p.group_tokens, p.slope,
+             p.part_tile, PageDiv(NH / NKVH), PageDiv(p.ranges), p.part_rows, nullptr, nullptr};
+  a.cuts = (Cut*)((char*)workspace + p.cuts_at);
+  a.head = (int*)(a.cuts + (size_t)p.ranges * p.group);
   for (int i = 0; i < 3; ++i) {
     a.qs[i] = q_strides[i] * es;
     a.os[i] = out_strides[i] * es;
   }
-  const int64_t seqs = (int64_t)batch->B * NKVH;
-  const int64_t units = seqs * p.nsplit * ((p.tiles + p.group - 1) / p.group);
-  const int64_t grid = (units + 7) / 8 * 8 * p.group, joins = p.joins;
-  LTV_REQUIRE(grid < (int64_t(1) << 31) && joins < (int64_t(1) << 30), LTV_ERR_UNSUPPORTED,
-              "too many workgroups");
+  const unsigned grid = p.ranges * p.group;
   const hipStream_t st = (hipStream_t)stream;
   auto launch = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(kAttnThreads), 0, st, a);
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(kAttnThreads), 0, st, a);
   };
   auto by_width = [&](auto type) {
     using T = decltype(type);
@@ -920,16 +1082,12 @@ extern "C" int ltv_paged_attention(int dtype, const void* q, const int64_t q_str
   };
   if (dtype == LTV_DTYPE_F32) by_width(float()); else by_width(bf16_t());
   LTV_LAUNCH_CHECK();
-  if (p.nsplit > 1) {
+  if (p.joins) {
     auto join = [&](auto type) {
       using T = decltype(type);
-      if (p.nsplit <= 16)
-        hipLaunchKernelGGL((attn_join_kernel<T, 1>), dim3((unsigned)((joins + 3) / 4)), dim3(256),
-                           0, st, a);
-      else if (p.nsplit <= 64)
-        hipLaunchKernelGGL((attn_join_kernel<T, 4>), dim3((unsigned)joins), dim3(256), 0, st, a);
-      else
-        hipLaunchKernelGGL((attn_join_kernel<T, 16>), dim3((unsigned)joins), dim3(1024), 0, st, a);
+      const int each = p.part_tile <= 16 ? 1 : 8;
+      hipLaunchKernelGGL(attn_join_kernel<T>, dim3(grid, (p.part_tile + each - 1) / each),
+                         dim3(256), 0, st, a, each);
     };
     if (dtype == LTV_DTYPE_F32) join(float()); else join(bf16_t());
     LTV_LAUNCH_CHECK();
