@@ -24,7 +24,10 @@ struct PageDiv {
     }
   }
   __device__ __forceinline__ int quot(int n) const {
-    return size == 1 ? n : (int)(__umulhi((uint32_t)n, mul) >> shift);
+    return size == 1 ? n : quot_of_many(n);
+  }
+  __device__ __forceinline__ int quot_of_many(int n) const {  // (size > 1)
+    return (int)(__umulhi((uint32_t)n, mul) >> shift);
   }
 };
 

@@ -51,12 +51,14 @@ struct AttnArgs {
   uint32_t kp, ks, vp, vs;    // 16-byte units from page to page and row to row
   int NH, NKVH, D, g;
   int q_aligned;
-  int scalar_pages;           // load_full: 1 pages are multiples of 16 rows, 2 of 64
+  int scalar_pages;           // load_full: pages are multiples of 16 rows ..
+  int row_mask;               // .. 0: of 64, else -1
   float scale;                // with log2(e)
   int log_group, ranges;      // log2 of the workgroups side by side, and how many such groups
   int least;                  // shortest range
   int unit;                   // log2 of the blocks of keys in a unit of length
   int group_tokens, slope;    // tokens of a group's row tiles; units that each is longer by
+  int extra;                  // units that a group's begin counts for
   int part_tile;              // rows of a partial tile
   PageDiv by_g, by_ranges;    // divisions by g and by the number of ranges
   int64_t part_rows;
@@ -216,7 +218,7 @@ struct Line {
     u.groups = (u.tiles + (1 << a.log_group) - 1) >> a.log_group;
     u.rounds = (a.NKVH + u.heads - 1) >> several;
     const int past = max(len - n, 0);
-    u.c0 = max(1, (min(len, past + min(n, a.group_tokens)) + KT - 1) / KT >> a.unit);
+    u.c0 = max(1, (min(len, past + min(n, a.group_tokens)) + KT - 1) / KT >> a.unit) + a.extra;
     u.head = u.before(a, u.groups);
     u.all = u.rounds * u.head;
     return u;
@@ -224,14 +226,16 @@ struct Line {
 };
 
 // Keys that the last row of a row tile sees, and the block of keys at which a cut at f of
-// the tile's c units is.
+// the tile's c units is, the first `extra` of which stand for no keys.
 __device__ __forceinline__ int keys_of(const AttnArgs& a, const PagedSeq& s, int tile) {
   const int last = a.by_g.quot(min((tile + 1) * kAttnRows, s.n * a.g) - 1);
   return a.batch.P > 0 && a.batch.W > 0 ? max(s.len - s.n + last + 1, 0) : 0;
 }
-__device__ __forceinline__ int cut_at(uint32_t f, uint32_t c, int blocks) {
+__device__ __forceinline__ int cut_at(uint32_t f, uint32_t c, int blocks, uint32_t extra) {
   if (f >= c) return blocks;
-  return min(blocks, (int)fmaf((float)f, (float)blocks * __builtin_amdgcn_rcpf((float)c), 0.5f));
+  if (f <= extra) return 0;
+  return min(blocks, (int)fmaf((float)(f - extra),
+                               (float)blocks * __builtin_amdgcn_rcpf((float)(c - extra)), 0.5f));
 }
 
 // A row tile whose first cut is a workgroup's begin, for the joining kernel.
@@ -459,10 +463,10 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_tile_kernel(const AttnAr
       const bool of_v = x & 1;
       const int r = (i * kRows + wave * (64 / Ti::kChunks)) & ~(kBlock - 1);
       // (pages of whole tiles: one page and row, and constant steps from it)
-      const int j = a.scalar_pages == 2 ? kt : kt + r;
-      uint32_t at = (uint32_t)(j - a.batch.div.quot(j) * a.batch.div.size);
-      const uint32_t from = (uint32_t)__builtin_amdgcn_readlane(page, a.scalar_pages == 2 ? 0 : r);
-      if (a.scalar_pages == 2) at += r;
+      const int j = kt + (r & a.row_mask);
+      const uint32_t from = (uint32_t)__builtin_amdgcn_readlane(page, r & a.row_mask);
+      const uint32_t at = (uint32_t)(j - a.batch.div.quot_of_many(j) * a.batch.div.size) +
+                          (r & ~a.row_mask);
       uint4* to = lds + buf * 2 * Ti::kUnits + i * kAttnThreads + wave * 64;
       if (of_v)
         load_lds16(to + Ti::kUnits, vbase + (uint64_t)(from * a.vp + at * a.vs) * 16, voff);
@@ -820,7 +824,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_tile_kernel(const AttnAr
     }
   };
 
-  for (uint32_t x = x0; x < x1;) {
+  for (uint32_t x = x0;;) {
     // units from .. to of a group's c
     const uint32_t c = u.c0 + a.slope * group;
     const uint32_t from = x - at, to = min(x1 - at, c);
@@ -835,22 +839,27 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_tile_kernel(const AttnAr
     if (on && (cuts || from == 0)) {
       const bool whole = !cuts || (from == 0 && to == c);
       const int keys = keys_of(a, s, tile), blocks = (keys + KT - 1) / KT;
-      const int begin = whole ? 0 : cut_at(from, c, blocks) * KT;
-      const int end = whole || to == c ? keys : min(keys, cut_at(to, c, blocks) * KT);
-      if (whole || begin < end)
-        piece(kvh, tile, begin, end, whole ? -1 : part_at(a, range, member, from == 0));
+      const int begin = whole ? 0 : cut_at(from, c, blocks, a.extra) * KT;
+      const int end = whole || to == c ? keys : min(keys, cut_at(to, c, blocks, a.extra) * KT);
       if (x == x0 && from > 0 && from <= length && threadIdx.x == 0)
         a.cuts[(range << a.log_group) + member] =
             Cut{min(rows - tile * kAttnRows, kAttnRows), b, kvh, (int)s.row0, tile,
                 min(over(at + c - 1, length), ranges - 1), at, c, blocks, length, {}};
+      if (whole || begin < end)
+        piece(kvh, tile, begin, end, whole ? -1 : part_at(a, range, member, from == 0));
     }
     x = at + to;
+    if (x >= x1) return;
     at += c;
-    if (++group == u.groups) {
+    ++group;
+    // (taken anew, so that it is not kept in registers through a piece)
+    s = paged_seq(a.batch, b);
+    u = Line::of<KT>(a, s.n, s.len);
+    if (group == u.groups) {
       group = 0;
       ++round;
     }
-    while (round >= u.rounds && x < x1) {
+    while (round >= u.rounds) {
       if (++b >= a.batch.B) return;
       s = paged_seq(a.batch, b);
       u = Line::of<KT>(a, s.n, s.len);
@@ -892,7 +901,8 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a, int ro
         v[i] = on ? *reinterpret_cast<const float4*>(a.part + at * a.D + lane * 4)
                   : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         // (a piece of no keys was not written)
-        if (p > cut.last || cut_at(from, cut.c, cut.blocks) == cut_at(to, cut.c, cut.blocks)) {
+        if (p > cut.last || cut_at(from, cut.c, cut.blocks, a.extra) ==
+                                cut_at(to, cut.c, cut.blocks, a.extra)) {
           ml[i] = make_float2(-INFINITY, 0.0f);
           v[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         }
@@ -957,7 +967,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a, int ro
 
 // How a call is cut.
 struct AttnPlan {
-  int group, ranges, least, unit, group_tokens, slope, part_tile;
+  int group, ranges, least, unit, group_tokens, slope, extra, part_tile;
   bool joins;
   int64_t part_rows;
   size_t bytes, cuts_at;
@@ -988,6 +998,12 @@ AttnPlan plan_attention(const ltv_paged_batch& b, int NH, int NKVH, int D, int m
   p.unit = 0;
   while (bound / (double)(int64_t(1) << p.unit) > (double)(1 << 30)) ++p.unit;
   p.slope = (int)(p.group * kAttnRows / g / KT) >> p.unit;
+  // What a piece costs beside its keys -- its rows, the first tile's way, the remainders that
+  // the first tiles take, its partials -- counted in blocks: four of many rows, one of few;
+  // none where there is a range for every few blocks.  (Chunks mixed with decoding 110 us
+  // without, 98 with it, float32 chunks 50 and 48, a ragged decode step 282 and 274, a small
+  // one 17.6 and 18.4.)
+  p.extra = (rows > 32 ? 4 : most > 4096 ? 1 : 0) >> p.unit;
   p.joins = keys > KT;
   const int64_t n = (int64_t)p.ranges * p.group;
   p.part_rows = p.joins ? n * 2 * p.part_tile : 0;
@@ -1059,8 +1075,8 @@ extern "C" int ltv_paged_attention(int dtype, const void* q, const int64_t q_str
              v_page_strides[1] * es, (uint32_t)(k_page_strides[0] / chunk),
              (uint32_t)(k_page_strides[2] / chunk), (uint32_t)(v_page_strides[0] / chunk),
              (uint32_t)(v_page_strides[2] / chunk), NH, NKVH, D, NH / NKVH, q_aligned ? 1 : 0,
-             !rows_fit || batch->page_size % 16 != 0 ? 0 : batch->page_size % 64 == 0 ? 2 : 1,
-             scale * kLog2e, p.group == 4 ? 2 : p.group - 1, p.ranges, p.least, p.unit, p.group_tokens, p.slope,
+             rows_fit && batch->page_size % 16 == 0, batch->page_size % 64 == 0 ? 0 : -1,
+             scale * kLog2e, p.group == 4 ? 2 : p.group - 1, p.ranges, p.least, p.unit, p.group_tokens, p.slope, p.extra,
              p.part_tile, PageDiv(NH / NKVH), PageDiv(p.ranges), p.part_rows, nullptr, nullptr};
   a.cuts = (Cut*)((char*)workspace + p.cuts_at);
   a.head = (int*)(a.cuts + (size_t)p.ranges * p.group);
