@@ -59,7 +59,7 @@ struct AttnArgs {
   int unit;                   // log2 of the blocks of keys in a unit of length
   int group_tokens, slope;    // tokens of a group's row tiles; units that each is longer by
   int extra;                  // units that a group's begin counts for
-  int part_tile;              // rows of a partial tile
+  int part_tile;              // rows of a partial tile, 0: none is cut
   PageDiv by_g, by_ranges;    // divisions by g and by the number of ranges
   int64_t part_rows;
   int* head;                  // how many ranges the call came to
@@ -833,7 +833,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_tile_kernel(const AttnAr
     const int kvh = round * u.heads + k;
     const int tile = u.heads == 1 ? (group << a.log_group) + member : member & (u.tiles - 1);
     const bool on = k < u.heads && kvh < a.NKVH && tile < u.tiles;
-    // (a sequence of more rows than the call was sized for is not cut)
+    // (a sequence of more rows than there is room for is not cut)
     const int rows = s.n * a.g;
     const bool cuts = min(rows, kAttnRows) <= a.part_tile;
     if (on && (cuts || from == 0)) {
@@ -979,7 +979,10 @@ AttnPlan plan_attention(const ltv_paged_batch& b, int NH, int NKVH, int D, int m
   const int64_t tiles = (rows + kAttnRows - 1) / kAttnRows;
   p.group = KT == 32 ? 1 : tiles >= 3 ? 4 : (int)tiles;
   p.group_tokens = (int)((p.group * kAttnRows + g - 1) / g);
-  p.part_tile = (int)std::min<int64_t>(rows, kAttnRows);
+  // (where no sequence can have more than a block of keys none is cut)
+  const int64_t keys = (int64_t)b.table_width * b.page_size;
+  p.joins = keys > KT;
+  p.part_tile = p.joins ? (int)std::min<int64_t>(rows, kAttnRows) : 0;
   // (of few rows all their latency is a tile's: there no range is too short)
   p.least = (rows <= 32 ? 64 : 128) / KT;
   // The card holds 512 workgroups at a time, two to a compute unit.  Fewer, if the call has
@@ -992,7 +995,6 @@ AttnPlan plan_attention(const ltv_paged_batch& b, int NH, int NKVH, int D, int m
   p.ranges = std::max(8, (p.ranges + 7) / 8 * 8);
   // Positions on the line have 32 bits: units of more blocks where it could be longer than
   // 2^30, whatever the lengths are.
-  const int64_t keys = (int64_t)b.table_width * b.page_size;
   const double bound = (double)NKVH * ((double)b.total * g / (p.group * kAttnRows) + b.B) *
                        ((double)(keys + b.total) / KT + 64);
   p.unit = 0;
@@ -1004,9 +1006,8 @@ AttnPlan plan_attention(const ltv_paged_batch& b, int NH, int NKVH, int D, int m
   // without, 98 with it, float32 chunks 50 and 48, a ragged decode step 282 and 274, a small
   // one 17.6 and 18.4.)
   p.extra = (rows > 32 ? 4 : most > 4096 ? 1 : 0) >> p.unit;
-  p.joins = keys > KT;
   const int64_t n = (int64_t)p.ranges * p.group;
-  p.part_rows = p.joins ? n * 2 * p.part_tile : 0;
+  p.part_rows = n * 2 * p.part_tile;
   p.cuts_at = (size_t)p.part_rows * (D + 2) * sizeof(float);
   p.bytes = p.cuts_at + n * sizeof(Cut) + 16;
   return p;

@@ -103,6 +103,44 @@ def test_long_context_split_over_many(dtype):
     _case(dtype, 4, 1, 64, 64, [1, 1, 2], [40000, 10, 9000], packed=True, seed=3, qscale=2.0)
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("B", [257, 700])
+def test_many_sequences(B, dtype):
+    """More sequences than a workgroup has threads, most of them short, some in chunks."""
+    new = [1 + (i % 97 == 5) * (i % 150) for i in range(B)]
+    new[B // 2] = 0
+    _case(dtype, 4, 2, 64, 16, new, [(i * 37) % 230 for i in range(B)], packed=True, seed=23)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("NH,NKVH,D", [(8, 4, 128), (6, 6, 64), (3, 1, 128)])
+def test_long_chunk_among_short_ones(NH, NKVH, D, dtype):
+    """One sequence has nearly all the work: its row tiles are cut many times."""
+    _case(dtype, NH, NKVH, D, 16, [1] * 9 + [200, 3, 70, 1], [5, 300] * 4 + [0, 5000, 9, 40, 2500],
+          packed=True, seed=24, qscale=2.0)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("page", [16, 32, 64])
+def test_many_rows_of_few_keys(page, dtype):
+    """More new tokens than the table has room for: the first ones see nothing."""
+    _case(dtype, 4, 2, 64, page, [700, 300, 40], [-690, -270, -8], packed=True, seed=25)
+    _case(dtype, 4, 4, 64, page, [300, 300], [-287, -299], packed=False, seed=26)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_wide_table(dtype):
+    """A table with room for 2^30 tokens of each sequence, hardly any of it used."""
+    new, lens = [600, 1, 40], [700, 300, 41]
+    cache = Cache(lens, 32, 8, 128, dtype, 27)
+    wide = torch.full((3, 1 << 23), -1, dtype=torch.int32, device=DEV)
+    wide[:, :cache.table.shape[1]] = cache.table
+    cache.table = wide
+    q = [cache.rand(n, 32, 8, dtype=dtype) for n in new]
+    got = _run(cache, q, new, True)
+    _check(got, attention64(q, cache, [0, 1, 2], new, 8 ** -0.5), dtype, 8, lens)
+
+
 @pytest.mark.parametrize("layout", ["token", "gaps"])
 @pytest.mark.parametrize("dtype", [BF, F32])
 def test_page_layouts(layout, dtype):
