@@ -335,6 +335,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_forward_kernel(const LogpAr
     for (int e = tid; e < have; e += kThreads) {
       const uint64_t mine = cands[e];
       int above = 0;
+#pragma unroll 8
       for (int j = 0; j < have; ++j) above += cands[j] > mine;
       if (above >= p.top_k) continue;
       if (p.pieces > 1) {
@@ -355,19 +356,28 @@ constexpr int kPieces = 16;  // of a row, at most
 constexpr int kJoinThreads = kPieces * kGroups;
 
 // Joins a row's pieces: one workgroup, every piece's sums, and the best of the pieces'
-// alternatives, each ranked by as many threads as there are for it.  (A search in each
-// piece's ordered list per alternative, fewer comparisons but one after the other, took
-// 7.3 us instead of 6.0 for 16 rows of 16 pieces with 20 alternatives.)
+// alternatives.  The k-th largest of the first few of every piece bounds the k-th largest of
+// all from below; what is not under it, hardly more than k, is collected and ranked.
+// (Ranking all against all is four times the work: 3.1 us instead of 5.7 for 16 rows of 16
+// pieces with 20 alternatives.)
 template <typename T, bool CAP>
 __global__ void __launch_bounds__(kJoinThreads) logprobs_join_kernel(const LogpArgs p) {
-  __shared__ unsigned long long keys[kJoinThreads];
-  __shared__ int rank[kJoinThreads];
+  __shared__ unsigned long long cands[kJoinThreads];
+  __shared__ unsigned long long bound;
+  __shared__ int count;
   __shared__ float lse_lds;
   const int64_t n = blockIdx.x;
   const int tid = threadIdx.x, all = p.pieces * p.top_k;
-  if (tid < all) {
-    keys[tid] = p.part_keys[n * all + tid];
-    rank[tid] = 0;
+  const uint64_t mine = tid < all ? p.part_keys[n * all + tid] : 0;
+  if (tid < 64 && all > 0) {
+    const int each = min(64 / p.pieces, p.top_k), piece = tid / each;
+    const uint64_t key = piece < p.pieces
+                             ? p.part_keys[n * all + piece * p.top_k + tid - piece * each] : 0;
+    const uint64_t kth = kth_of_lanes(key, p.top_k);
+    if (tid == 0) {
+      bound = kth;
+      count = 0;
+    }
   }
   Target target;
   if (tid == 0) target = target_of(p, n, reinterpret_cast<const T*>(p.x) + n * p.xs);
@@ -390,19 +400,18 @@ __global__ void __launch_bounds__(kJoinThreads) logprobs_join_kernel(const LogpA
   }
   if (all == 0) return;
   __syncthreads();
-  const int e = tid % all, share = kJoinThreads / all;
-  if (tid / all < share) {
-    const uint64_t mine = keys[e];
-    int above = 0;
-#pragma unroll 8
-    for (int j = tid / all; j < all; j += share) above += keys[j] > mine;
-    atomicAdd(&rank[e], above);
-  }
+  // (0: no entry)
+  if (mine != 0 && mine >= bound) cands[atomicAdd(&count, 1)] = mine;
   __syncthreads();
-  if (tid < all && keys[tid] != 0 && rank[tid] < p.top_k) {
-    p.top_ids[n * p.top_k + rank[tid]] = key_index(keys[tid]);
-    p.top_lp[n * p.top_k + rank[tid]] =
-        capped(key_value(keys[tid]), CAP ? p.cap : 0.0f) - lse_lds;
+  const int have = count;
+  if (tid >= have) return;
+  const uint64_t key = cands[tid];
+  int rank = 0;
+#pragma unroll 8
+  for (int j = 0; j < have; ++j) rank += cands[j] > key;
+  if (rank < p.top_k) {
+    p.top_ids[n * p.top_k + rank] = key_index(key);
+    p.top_lp[n * p.top_k + rank] = capped(key_value(key), CAP ? p.cap : 0.0f) - lse_lds;
   }
 }
 
