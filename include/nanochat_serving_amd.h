@@ -43,6 +43,9 @@ int ltv_serving_abi_version(void);
  * Token t is at position seq_lens[slot] - n_i + t; at a negative position it is
  * no token (appended nowhere, attends to nothing).  A slot outside [0, num_slots)
  * is an empty sequence.
+ *
+ * Limits (LTV_ERR_UNSUPPORTED past them): page_size <= 2^20, table_width * page_size
+ * and total < 2^31.
  * ---------------------------------------------------------------------- */
 typedef struct ltv_paged_batch {
   const int32_t* page_table;
@@ -56,8 +59,9 @@ typedef struct ltv_paged_batch {
 
 /* Writes the new tokens' keys and values into their pages.
  * k, v: token rows (NKVH, D), strides (sequence, token, head); the sequence stride
- * is not used with starts.  Any alignment.  No reference counterpart (its cache is
- * contiguous: nanochat/kv_cache.py insert_kv). */
+ * is not used with starts.  Any alignment.  B <= 65,535, and total * NKVH * D < 2^31
+ * elements where rows are not 16-byte aligned, else units of 16 bytes.  No reference
+ * counterpart (its cache is contiguous: nanochat/kv_cache.py insert_kv). */
 int ltv_paged_cache_append(int dtype, const void* k, const int64_t k_strides[3], const void* v,
                            const int64_t v_strides[3], void* k_pages,
                            const int64_t k_page_strides[3], void* v_pages,
@@ -77,7 +81,8 @@ int ltv_paged_cache_append(int dtype, const void* k, const int64_t k_strides[3],
  * q: strides (sequence, token, head), last stride 1, any alignment.  out: strides
  * likewise, 16-byte aligned rows.  lse: one float per (row, head), contiguous.
  * scale > 0.  D a multiple of 8, at most 128.  max_len: the longest sequence expected (a hint:
- * it chooses how the keys are split, not which are read).
+ * it chooses how many workgroups there are, not which keys are read).  The pages of a layer
+ * lie within 32 GiB, with strides that are not negative; total * NH < 2^30.
  * workspace: ltv_paged_attention_workspace_size bytes, 16-byte aligned.
  * ---------------------------------------------------------------------- */
 size_t ltv_paged_attention_workspace_size(int dtype, const ltv_paged_batch* batch, int NH,
@@ -93,7 +98,8 @@ int ltv_paged_attention(int dtype, const void* q, const int64_t q_strides[3],
 /* ------------------------------------------------------------------------
  * The pages of all layers, for the calls that move pages: `layers` pairs of a k
  * and a v page array whose pages are dense blocks of block_bytes bytes (a multiple
- * of 16), page_bytes apart, the layers layer_bytes apart; 16-byte aligned.
+ * of 16, less than 2^31), page_bytes apart, the layers layer_bytes apart; 16-byte
+ * aligned.  A call copies less than 2^31 pieces of 8 KiB.
  * ---------------------------------------------------------------------- */
 typedef struct ltv_page_blocks {
   void* k;
@@ -160,8 +166,8 @@ int ltv_paged_cache_compact(const ltv_page_state* state, const ltv_page_blocks* 
  *                  ascending order of index
  *   lse[n]       : kept for the backward                (may be NULL)
  * All outputs contiguous; sums in fp32.  workspace: ltv_token_logprobs_workspace_size
- * bytes (0 where a row is not cut into pieces), 16-byte aligned.  Replaces what nanochat's sampling and
- * scoring do with log_softmax, gather and topk on the logits.
+ * bytes (0 where a row is not cut into pieces), 16-byte aligned.  N < 2^31.  Replaces
+ * what nanochat's sampling and scoring do with log_softmax, gather and topk on the logits.
  * ---------------------------------------------------------------------- */
 size_t ltv_token_logprobs_workspace_size(int64_t N, int V, int top_k);
 int ltv_token_logprobs_forward(int dtype, const void* logits, int64_t row_stride,

