@@ -198,6 +198,23 @@ def test_missing_pages(T, dtype):
            [200, 150, 90])
 
 
+@pytest.mark.parametrize("cached", [20, 4000])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_nan_query(dtype, cached):
+    """A query that is NaN gives NaN, in one piece or many, and leaves the others alone."""
+    cache = Cache([cached + 3, 50], 2, 64, 16, dtype, 28)
+    q = [cache.rand(3, 4, 64, dtype=dtype), cache.rand(3, 4, 64, dtype=dtype)]
+    want = attention64(q, cache, [0, 1], [3, 3], 64 ** -0.5)
+    q[0][1, 2] = math.nan
+    got = _run(cache, q, [3, 3], True)
+    assert bool(got[0][0][1, 2].isnan().all()) and bool(got[0][1][1, 2].isnan())
+    for (out, lse), (o64, l64, *_) in zip(got, want):
+        out[out.isnan()] = o64[out.isnan()].to(dtype)
+        lse[lse.isnan()] = l64[lse.isnan()].float()
+    assert bool(got[0][0].isfinite().all())
+    _check(got, want, dtype, 64, [cached + 3, 50])
+
+
 @pytest.mark.parametrize("poison", [math.nan, math.inf, -math.inf, "lowest"])
 @pytest.mark.parametrize("T", [1, 6, 48, 150])
 @pytest.mark.parametrize("dtype", [BF, F32])
