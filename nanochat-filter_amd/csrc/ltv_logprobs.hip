@@ -21,7 +21,7 @@
 //
 // Backward.  Elementwise given lse; a workgroup takes a piece of a row and sets the
 // elements of the target and the alternatives again, with their own terms.  4,096 rows of
-// 50,257 bfloat16 logits 155 us, 5.3 TB/s read and written.
+// 50,257 bfloat16 logits 153 us, 5.4 TB/s read and written.
 #include <algorithm>
 #include <type_traits>
 
@@ -441,8 +441,6 @@ struct LogpGradArgs {
   int piece;  // elements of a workgroup
 };
 
-constexpr int kGradThreads = 256;
-
 // dx of an element, without the terms of a target or an alternative (extra).
 template <bool CAP>
 struct Grad {
@@ -461,7 +459,11 @@ struct Grad {
   }
 };
 
-template <typename T, bool CAP>
+// kGradThreads: 1,024 for pieces of 64 KiB and more, so that fewer are read and written side by
+// side (4,096 rows of 50,257 bfloat16 logits 171 us with 256, 153 with 1,024; 2,000 of float32
+// 171 and 145), else 256 (2,000 rows of bfloat16, pieces of 40 KiB, 86 and 89; 4,096 of 1,000
+// logits 7 and 13).
+template <typename T, bool CAP, int kGradThreads>
 __global__ void __launch_bounds__(kGradThreads) logprobs_backward_kernel(const LogpGradArgs p) {
   constexpr int N = io_traits<T>::kVec, kAhead = 2;
   const int64_t n = blockIdx.y;
@@ -610,14 +612,18 @@ extern "C" int ltv_token_logprobs_backward(int dtype, const void* logits, int64_
   // (the grid's second axis ends at 65,535)
   for (int64_t n0 = 0; n0 < N; n0 += 65535) {
     const dim3 grid((unsigned)((V + piece - 1) / piece), (unsigned)std::min<int64_t>(65535, N - n0));
-    auto launch = [&](auto type) {
+    auto launch = [&](auto type, auto cap) {
       using T = decltype(type);
-      if (softcap > 0.0f)
-        hipLaunchKernelGGL((logprobs_backward_kernel<T, true>), grid, dim3(kGradThreads), 0, st, a);
+      constexpr bool C = decltype(cap)::value;
+      if ((int64_t)std::min(piece, V) * (int)sizeof(T) >= 65536)
+        hipLaunchKernelGGL((logprobs_backward_kernel<T, C, 1024>), grid, dim3(1024), 0, st, a);
       else
-        hipLaunchKernelGGL((logprobs_backward_kernel<T, false>), grid, dim3(kGradThreads), 0, st, a);
+        hipLaunchKernelGGL((logprobs_backward_kernel<T, C, 256>), grid, dim3(256), 0, st, a);
     };
-    if (dtype == LTV_DTYPE_F32) launch(float()); else launch(bf16_t());
+    auto by_cap = [&](auto type) {
+      if (softcap > 0.0f) launch(type, std::true_type()); else launch(type, std::false_type());
+    };
+    if (dtype == LTV_DTYPE_F32) by_cap(float()); else by_cap(bf16_t());
     LTV_LAUNCH_CHECK();
     const int64_t m = grid.y;
     const int es = dtype == LTV_DTYPE_F32 ? 4 : 2;

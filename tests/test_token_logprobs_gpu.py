@@ -227,6 +227,12 @@ def test_gradient(N, V, pad, k, cap, dtype):
         assert bool((err <= bound).all()), float((err / bound).max())
 
 
+@pytest.mark.parametrize("cap,dtype", [(15.0, BF), (None, F32)])
+def test_gradient_of_many_long_rows(cap, dtype):
+    """Rows of more than 64 KiB that are not cut into pieces."""
+    test_gradient(4097, 33001, 33024, 2, cap, dtype)
+
+
 def test_gradient_against_differences():
     """Directional derivatives by central differences of the float32 forward; their own
     error is eps^2 of a third derivative of order one, and 10 roundings over eps."""
