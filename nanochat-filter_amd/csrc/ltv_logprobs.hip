@@ -21,7 +21,7 @@
 //
 // Backward.  Elementwise given lse; a workgroup takes a piece of a row and sets the
 // elements of the target and the alternatives again, with their own terms.  4,096 rows of
-// 50,257 bfloat16 logits 153 us, 5.4 TB/s read and written.
+// 50,257 bfloat16 logits about 150 us, 5.5 TB/s read and written.
 #include <algorithm>
 #include <type_traits>
 
@@ -460,9 +460,9 @@ struct Grad {
 };
 
 // kGradThreads: 1,024 for pieces of 64 KiB and more, so that fewer are read and written side by
-// side (4,096 rows of 50,257 bfloat16 logits 171 us with 256, 153 with 1,024; 2,000 of float32
-// 171 and 145), else 256 (2,000 rows of bfloat16, pieces of 40 KiB, 86 and 89; 4,096 of 1,000
-// logits 7 and 13).
+// side (4,096 rows of 50,257 bfloat16 logits, forward and gradient, 275 us with 256, 265 with
+// 512, 257 with 1,024; the gradient of 2,000 rows of float32 171 and 145), else 256 (2,000 rows
+// of bfloat16, pieces of 40 KiB, 86 and 89; 4,096 of 1,000 logits 7 and 13).
 template <typename T, bool CAP, int kGradThreads>
 __global__ void __launch_bounds__(kGradThreads) logprobs_backward_kernel(const LogpGradArgs p) {
   constexpr int N = io_traits<T>::kVec, kAhead = 2;
