@@ -8,7 +8,8 @@
 //
 // Rows.  A sequence's n tokens times the g = NH / NKVH query heads of one k/v head are
 // its rows, token-major: they share every key, so a decode step of a group of heads
-// reads its keys once.  A workgroup has 128 rows, 32 for each of four wavefronts.
+// reads its keys once.  A workgroup has 128 rows, 32 for each of four wavefronts (or one
+// wavefront, where many sequences have few rows each).
 //
 // Layout of the products (32 x 32 MFMA blocks).  The scores are computed as S^T = K Q^T:
 // a lane then holds 16 keys of one row, so maximum and sum are taken in the lane and
@@ -42,10 +43,14 @@
 namespace ltv {
 namespace {
 
-constexpr int kAttnWaves = 4;
-constexpr int kAttnThreads = kAttnWaves * 64;
-constexpr int kAttnRows = kAttnWaves * 32;  // rows of a workgroup
-constexpr int kAttnGrid = 512;              // workgroups that the card holds, two to a unit
+// A workgroup: four wavefronts and tiles of 64 keys (float32: 32), two to a compute unit; of
+// few rows, which one wavefront holds, that one and tiles of 32 keys, four to a unit.
+template <typename T, bool FEW>
+struct AttnShape {
+  static constexpr int kWaves = FEW ? 1 : 4, kThreads = kWaves * 64, kRows = kWaves * 32;
+  static constexpr int kGrid = FEW ? 1024 : 512;  // workgroups that the card holds
+  static constexpr int kKeys = FEW || sizeof(T) == 4 ? 32 : 64;  // of a tile
+};
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -69,6 +74,7 @@ struct AttnArgs {
   int unit;                   // log2 of the blocks of keys in a unit of length
   int group_tokens, slope;    // tokens of a group's row tiles; units that each is longer by
   int extra;                  // units that a group's begin counts for
+  int log_rows;               // of a row tile
   int part_tile;              // rows of a partial tile, 0: none is cut
   PageDiv by_g, by_ranges;    // divisions by g and by the number of ranges
   int64_t part_rows;
@@ -91,7 +97,6 @@ struct AttnType;
 template <>
 struct AttnType<bf16_t> {
   static constexpr int kChunk = 8;  // elements
-  static constexpr int kKeys = 64;  // keys of a tile
   // S^T += K Q^T over 16 channels: a lane's k and q chunk hold channels 8 (lane / 32) ..
   static __device__ __forceinline__ f32x16 scores(u32x4_t k, uint4 q, f32x16 s) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, k),
@@ -102,7 +107,6 @@ struct AttnType<bf16_t> {
 template <>
 struct AttnType<float> {
   static constexpr int kChunk = 4;
-  static constexpr int kKeys = 32;
   static __device__ __forceinline__ f32x16 scores(u32x4_t k, uint4 q, f32x16 s) {
     s = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(k.x), __uint_as_float(q.x), s, 0, 0, 0);
     s = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(k.y), __uint_as_float(q.y), s, 0, 0, 0);
@@ -117,9 +121,9 @@ struct AttnType<float> {
 //   K: 16 consecutive rows, one chunk each (ds_read_b128).
 //   V, bfloat16: four rows, 64 bytes each (ds_read_b64_tr_b16).
 //   V, float32: two rows four apart, 128 bytes each (ds_read_b32).
-template <typename T, int DP>
+template <typename T, int DP, bool FEW>
 struct AttnTile {
-  static constexpr int kKeys = AttnType<T>::kKeys;
+  static constexpr int kKeys = AttnShape<T, FEW>::kKeys, kAttnThreads = AttnShape<T, FEW>::kThreads;
   static constexpr int kChunks = DP / AttnType<T>::kChunk;     // of a row
   static constexpr int kPhase = kChunks < 16 ? 16 / kChunks : 1;  // rows of 256 bytes
   static constexpr int kUnits = kKeys * kChunks;               // chunks of a tile
@@ -222,7 +226,7 @@ struct Line {
   static __device__ __forceinline__ Line of(const AttnArgs& a, int n, int len) {
     Line u{0, 1, 0, 0, 0, 0, 0};
     if (n <= 0) return u;
-    u.tiles = (n * a.g + kAttnRows - 1) / kAttnRows;
+    u.tiles = (n * a.g + (1 << a.log_rows) - 1) >> a.log_rows;
     const int several = u.tiles == 1 ? a.log_group : u.tiles == 2 && a.log_group == 2 ? 1 : 0;
     u.heads = 1 << several;
     u.groups = (u.tiles + (1 << a.log_group) - 1) >> a.log_group;
@@ -238,7 +242,7 @@ struct Line {
 // Keys that the last row of a row tile sees, and the block of keys at which a cut at f of
 // the tile's c units is, the first `extra` of which stand for no keys.
 __device__ __forceinline__ int keys_of(const AttnArgs& a, const PagedSeq& s, int tile) {
-  const int last = a.by_g.quot(min((tile + 1) * kAttnRows, s.n * a.g) - 1);
+  const int last = a.by_g.quot(min((tile + 1) << a.log_rows, s.n * a.g) - 1);
   return a.batch.P > 0 && a.batch.W > 0 ? max(s.len - s.n + last + 1, 0) : 0;
 }
 __device__ __forceinline__ int cut_at(uint32_t f, uint32_t c, int blocks, uint32_t extra) {
@@ -280,16 +284,16 @@ __device__ __forceinline__ float2* part_ml(const AttnArgs& a) {
 
 // Rows row0 .. row_end - 1 of a workgroup over keys begin .. end - 1, each key that a row
 // does not see left alone altogether: the way of tiles with infinite or NaN values among
-// those that some rows do not see.  Sixteen groups of sixteen lanes take a row's keys in
-// turn, a lane holding eight channels.  part0: the partials of row0, or -1.
-template <typename T>
+// those that some rows do not see.  Groups of sixteen lanes take a row's keys in turn, a lane holding eight channels.  part0: the partials of row0, or -1.
+template <typename T, int THREADS>
 __device__ __forceinline__ void rows_one_by_one(const AttnArgs& a, const PagedSeq& s, int b,
                                                 int kvh, int row0, int row_end, int begin, int end,
                                                 int64_t part0, float* lds) {
 #pragma clang fp contract(off)  // (x - base below must not be a fused form of the product)
   float* lds_m = lds;
-  float* lds_l = lds + 16;
-  float* lds_o = lds + 32;  // 16 x 128
+  constexpr int G = THREADS / 16;
+  float* lds_l = lds + G;
+  float* lds_o = lds + 2 * G;  // G x 128
   const int c = threadIdx.x & 15, gi = threadIdx.x >> 4;
   const bool on = c * 8 < a.D;
   for (int row = row0; row < row_end; ++row) {
@@ -304,7 +308,7 @@ __device__ __forceinline__ void rows_one_by_one(const AttnArgs& a, const PagedSe
       qf[e] = on ? io_traits<T>::load(reinterpret_cast<const T*>(q) + c * 8 + e) : 0.0f;
       o[e] = 0.0f;
     }
-    for (int j = begin + gi; j <= last; j += 16) {
+    for (int j = begin + gi; j <= last; j += G) {
       const int col = a.batch.div.quot(j), page = s.table[col];
       if (page < 0 || page >= a.batch.P) continue;
       const uint32_t in = (uint32_t)(j - col * a.batch.div.size);
@@ -332,36 +336,45 @@ __device__ __forceinline__ void rows_one_by_one(const AttnArgs& a, const PagedSe
     for (int e = 0; e < 8; ++e) lds_o[gi * 128 + c * 8 + e] = o[e];
     __syncthreads();
     float mx = -INFINITY;
-    for (int i = 0; i < 16; ++i) mx = fmaxf(mx, lds_m[i]);
+    for (int i = 0; i < G; ++i) mx = fmaxf(mx, lds_m[i]);
     const float base = mx == -INFINITY ? 0.0f : mx;
-    float sum = 0.0f, acc = 0.0f;
-    const int d = threadIdx.x;
-    for (int i = 0; i < 16; ++i) {
+    float sum = 0.0f, acc[128 / THREADS + 1] = {};
+    const int d0 = threadIdx.x;
+    for (int i = 0; i < G; ++i) {
       // (a group without keys has weight 0)
       const float w = lds_m[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(lds_m[i] - base);
       sum = fmaf(lds_l[i], w, sum);
-      if (d < a.D) acc = fmaf(lds_o[i * 128 + d], w, acc);
+#pragma unroll
+      for (int e = 0, d = d0; d < 128; ++e, d += THREADS) acc[e] = fmaf(lds_o[i * 128 + d], w, acc[e]);
     }
     if (part0 >= 0) {
       const int64_t at = part0 + row - row0;
-      if (d < a.D) a.part[at * a.D + d] = acc;
-      if (d == 0) part_ml(a)[at] = make_float2(mx, sum);
+#pragma unroll
+      for (int e = 0, d = d0; d < 128; ++e, d += THREADS)
+        if (d < a.D) a.part[at * a.D + d] = acc[e];
+      if (d0 == 0) part_ml(a)[at] = make_float2(mx, sum);
     } else {
       char* out = a.out + (a.batch.starts != nullptr ? trow * a.os[1]
                                                      : b * a.os[0] + t * a.os[1]) + h * a.os[2];
-      if (d < a.D)
-        io_traits<T>::store(reinterpret_cast<T*>(out) + d, sum == 0.0f ? 0.0f : acc / sum);
-      if (d == 0 && a.lse != nullptr)
+#pragma unroll
+      for (int e = 0, d = d0; d < 128; ++e, d += THREADS)
+        if (d < a.D)
+          io_traits<T>::store(reinterpret_cast<T*>(out) + d, sum == 0.0f ? 0.0f : acc[e] / sum);
+      if (d0 == 0 && a.lse != nullptr)
         a.lse[trow * a.NH + h] = sum == 0.0f ? -INFINITY
                                              : (mx + __builtin_amdgcn_logf(sum)) * kLn2;
     }
   }
 }
 
-template <typename T, int DP, bool PAD>
-__global__ void __launch_bounds__(kAttnThreads, 2) attn_tile_kernel(const AttnArgs a) {
+template <typename T, int DP, bool PAD, bool FEW>
+__global__ void __launch_bounds__((AttnShape<T, FEW>::kThreads), FEW ? 1 : 2)
+    attn_tile_kernel(const AttnArgs a) {
   using Ty = AttnType<T>;
-  using Ti = AttnTile<T, DP>;
+  using Ti = AttnTile<T, DP, FEW>;
+  using Shape = AttnShape<T, FEW>;
+  constexpr int kAttnWaves = Shape::kWaves, kAttnThreads = Shape::kThreads,
+                kAttnRows = Shape::kRows;
   constexpr int KT = Ti::kKeys, KB = KT / 32;
   constexpr int kSteps = Ti::kChunks / 2;  // score products' steps: two chunks each
   constexpr int kDB = DP / 32;
@@ -402,7 +415,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_tile_kernel(const AttnAr
   // Of the two workgroups of a compute unit the older is served first where the products
   // bound them, and had ended with a fifth of the other's work left: it gets more of it
   // (a long prompt 1,225 us with equal ranges, 1,187 with these).
-  const bool full = a.log_group > 0 && line.count << a.log_group == kAttnGrid;
+  const bool full = a.log_group > 0 && line.count << a.log_group == Shape::kGrid;
   line.lead = full ? line.length / 8 : 0;
   if (blockIdx.x == 0 && threadIdx.x == 0) *a.head = line.count;
   // Workgroup w runs on XCD w % 8: consecutive ranges stay on one.
@@ -565,9 +578,10 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_tile_kernel(const AttnAr
     }
 
     // (Of few rows one wavefront has all products: not on the same SIMD in both workgroups of a
-    // compute unit.  2,048 sequences of 30 to 100 tokens 271 us, so and with all wavefronts
-    // looking for infinities 254.)
-    const int wrow = tile * kAttnRows + ((wave + blockIdx.x / (kAttnGrid / 2) * 2) & 3) * 32;
+    // compute unit.  512 sequences of 100 to 300 tokens 113 us, so and with all wavefronts
+    // looking for infinities 109.)
+    const int wrow = tile * kAttnRows +
+                     (FEW ? 0 : (wave + blockIdx.x / (Shape::kGrid / 2) * 2) & 3) * 32;
     const int rows = s.n * a.g, row = wrow + ln;
     const bool row_ok = row < rows;
     const int t = row_ok ? a.by_g.quot(row) : 0;
@@ -653,7 +667,6 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_tile_kernel(const AttnAr
             for (int i = 0; i < 16; ++i) sc[kb][i] = 0.0f;
           auto scores = [&](auto with_loads) {
             constexpr int N = kSteps * KB, AHEAD = 6;
-            static_assert(N == 2 * kFullLoads, "a load to two products");
             u32x4_t kf[AHEAD];
             auto key = [&](int n) {
               return lds_read<u32x4_t>((ka ^ (32 * (n / KB))) + n % KB * 32 * kRow);
@@ -665,8 +678,10 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_tile_kernel(const AttnAr
             for (int n = 0; n < N; ++n) {
               sc[n % KB] = Ty::scores(kf[n % AHEAD], qf[n / KB], sc[n % KB]);
               if (n + AHEAD < N) kf[n % AHEAD] = key(n + AHEAD);
-              if (decltype(with_loads)::value && (n & 1))
-                load_full(n / 2, kt + KT, page_next, buf ^ 1);
+              if constexpr (decltype(with_loads)::value)
+#pragma unroll
+                for (int x = n * kFullLoads / N; x < (n + 1) * kFullLoads / N; ++x)
+                  load_full(x, kt + KT, page_next, buf ^ 1);
               in_order();
             }
           };
@@ -811,7 +826,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_tile_kernel(const AttnAr
     }
 
     if (__syncthreads_or(again)) {
-      rows_one_by_one<T>(a, s, b, kvh, tile * kAttnRows, min(rows, (tile + 1) * kAttnRows), begin,
+      rows_one_by_one<T, kAttnThreads>(a, s, b, kvh, tile * kAttnRows, min(rows, (tile + 1) * kAttnRows), begin,
                          end, part0, reinterpret_cast<float*>(lds));
       return;
     }
@@ -977,7 +992,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a, int ro
         for (int e = 0; e < 4; ++e) o[e] = fmaf(lds_o[i][lane * 4 + e], w, o[e]);
       }
     }
-    const int r = cut.tile * kAttnRows + row, t = a.by_g.quot(r), h = cut.kvh * a.g + r - t * a.g;
+    const int r = (cut.tile << a.log_rows) + row, t = a.by_g.quot(r), h = cut.kvh * a.g + r - t * a.g;
     const int64_t trow = (a.batch.starts != nullptr ? cut.token : (int64_t)cut.b * a.batch.T) + t;
     char* out = a.out + (a.batch.starts != nullptr ? trow * a.os[1]
                                                    : cut.b * a.os[0] + t * a.os[1]) + h * a.os[2];
@@ -998,20 +1013,26 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a, int ro
 
 // How a call is cut.
 struct AttnPlan {
-  int group, ranges, least, unit, group_tokens, slope, extra, part_tile;
+  bool few;
+  int log_rows, group, ranges, least, unit, group_tokens, slope, extra, part_tile;
   bool joins;
   int64_t part_rows;
   size_t bytes, cuts_at;
 };
 
-AttnPlan plan_attention(const ltv_paged_batch& b, int NH, int NKVH, int D, int max_len, int KT) {
+template <typename T, bool FEW>
+AttnPlan plan_shape(const ltv_paged_batch& b, int NH, int NKVH, int D, int max_len) {
+  using Shape = AttnShape<T, FEW>;
+  constexpr int KT = Shape::kKeys, kAttnRows = Shape::kRows;
   AttnPlan p;
+  p.few = FEW;
+  p.log_rows = FEW ? 5 : 7;
   const int64_t g = NH / NKVH, rows = std::max(b.T, 1) * g;
   const int64_t tiles = (rows + kAttnRows - 1) / kAttnRows;
   // Groups of four (one, two and four: 132, 126 and 112 us of chunks among decoding sequences,
   // 1,270, 1,246 and 1,239 of the long prompt); float32, whose products take eight times as
   // long as its reads, is better off with each tile by itself (one and four: 49.6 and 52.2).
-  p.group = KT == 32 ? 1 : tiles >= 3 ? 4 : (int)tiles;
+  p.group = FEW || sizeof(T) == 4 ? 1 : tiles >= 3 ? 4 : (int)tiles;
   p.group_tokens = (int)((p.group * kAttnRows + g - 1) / g);
   // (where no sequence can have more than a block of keys none is cut)
   const int64_t keys = (int64_t)b.table_width * b.page_size;
@@ -1025,7 +1046,7 @@ AttnPlan plan_attention(const ltv_paged_batch& b, int NH, int NKVH, int D, int m
       NKVH * std::min((tiles + p.group - 1) / p.group * b.B,
                       b.total * g / (p.group * kAttnRows) + b.B);
   const int64_t most = groups * ((std::max(max_len, 1) + KT - 1) / KT);
-  p.ranges = (int)std::min<int64_t>(kAttnGrid / p.group, (most + p.least - 1) / p.least);
+  p.ranges = (int)std::min<int64_t>(Shape::kGrid / p.group, (most + p.least - 1) / p.least);
   p.ranges = std::max(8, (p.ranges + 7) / 8 * 8);
   // Positions on the line have 32 bits: units of more blocks where it could be longer than
   // 2^30, whatever the lengths are.
@@ -1039,12 +1060,27 @@ AttnPlan plan_attention(const ltv_paged_batch& b, int NH, int NKVH, int D, int m
   // none where there is a range for every few blocks.  (Chunks mixed with decoding 110 us
   // without, 98 with it, float32 chunks 50 and 48, a ragged decode step 282 and 274, a small
   // one 17.6 and 18.4.)
-  p.extra = (rows > 32 ? 4 : most > 4096 ? 1 : 0) >> p.unit;
+  p.extra = (rows > 32 ? 4 : most > 8 * Shape::kGrid ? 1 : 0) >> p.unit;
   const int64_t n = (int64_t)p.ranges * p.group;
   p.part_rows = n * 2 * p.part_tile;
   p.cuts_at = (size_t)p.part_rows * (D + 2) * sizeof(float);
   p.bytes = p.cuts_at + n * sizeof(Cut) + 16;
   return p;
+}
+
+// Which shape.  One wavefront in four workgroups of a unit where each sequence and head has few
+// rows and there are as many of them as ranges of the other shape: 2,048 sequences of 30 to 100
+// tokens (6 heads) 253 and 185 us, 128 of up to 2,000 (8 heads) 142 and 132.  Of fewer and
+// longer ones the pieces are more to join, and their first tiles sooner there when four
+// wavefronts load them together: 64 of up to 2,000 (4 heads) 37.7 and 40.6, one very long among
+// 15 others 272 and 275, four short ones 17.9 and 23.0; so with more rows (32: 46.5 and 49.2).
+// float32 has its products to wait for.
+AttnPlan plan_attention(const ltv_paged_batch& b, int dtype, int NH, int NKVH, int D, int max_len) {
+  if (dtype == LTV_DTYPE_F32) return plan_shape<float, false>(b, NH, NKVH, D, max_len);
+  const int64_t rows = (int64_t)std::max(b.T, 1) * (NH / NKVH);
+  if (rows <= 16 && (int64_t)b.B * NKVH >= AttnShape<bf16_t, false>::kGrid)
+    return plan_shape<bf16_t, true>(b, NH, NKVH, D, max_len);
+  return plan_shape<bf16_t, false>(b, NH, NKVH, D, max_len);
 }
 
 }  // namespace
@@ -1056,7 +1092,7 @@ extern "C" size_t ltv_paged_attention_workspace_size(int dtype, const ltv_paged_
                                                      int NH, int NKVH, int D, int max_len) {
   if (batch == nullptr || batch->B <= 0 || batch->T < 0 || NKVH <= 0 || NH < NKVH || D <= 0)
     return 0;
-  return plan_attention(*batch, NH, NKVH, D, max_len, dtype == LTV_DTYPE_F32 ? 32 : 64).bytes;
+  return plan_attention(*batch, dtype, NH, NKVH, D, max_len).bytes;
 }
 
 extern "C" int ltv_paged_attention(int dtype, const void* q, const int64_t q_strides[3],
@@ -1084,7 +1120,7 @@ extern "C" int ltv_paged_attention(int dtype, const void* q, const int64_t q_str
                   (!pages || (k_pages && v_pages)),
               LTV_ERR_INVALID_ARG, "null pointer");
   const int es = elem_size(dtype), chunk = 16 / es;
-  const AttnPlan p = plan_attention(*batch, NH, NKVH, D, max_len, dtype == LTV_DTYPE_F32 ? 32 : 64);
+  const AttnPlan p = plan_attention(*batch, dtype, NH, NKVH, D, max_len);
   LTV_REQUIRE(workspace && workspace_bytes >= p.bytes, LTV_ERR_WORKSPACE, "workspace too small");
   // pages are addressed in 16-byte units of 32 bits
   bool fits = true, aligned = aligned16(k_pages) && aligned16(v_pages);
@@ -1112,8 +1148,8 @@ extern "C" int ltv_paged_attention(int dtype, const void* q, const int64_t q_str
              (uint32_t)(v_page_strides[2] / chunk), NH, NKVH, D, NH / NKVH, q_aligned ? 1 : 0,
              rows_fit && batch->page_size % 16 == 0,
              scale * kLog2e, p.group == 4 ? 2 : p.group - 1, p.ranges, p.least, p.unit,
-             p.group_tokens, p.slope, p.extra,
-             p.part_tile, PageDiv(NH / NKVH), PageDiv(p.ranges), p.part_rows, nullptr, nullptr};
+             p.group_tokens, p.slope, p.extra, p.log_rows, p.part_tile, PageDiv(NH / NKVH),
+             PageDiv(p.ranges), p.part_rows, nullptr, nullptr};
   a.cuts = (Cut*)((char*)workspace + p.cuts_at);
   a.head = (int*)(a.cuts + (size_t)p.ranges * p.group);
   for (int i = 0; i < 3; ++i) {
@@ -1122,17 +1158,21 @@ extern "C" int ltv_paged_attention(int dtype, const void* q, const int64_t q_str
   }
   const unsigned grid = p.ranges * p.group;
   const hipStream_t st = (hipStream_t)stream;
-  auto launch = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(grid), dim3(kAttnThreads), 0, st, a);
+  auto launch = [&](auto kernel, int threads) {
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(threads), 0, st, a);
   };
-  auto by_width = [&](auto type) {
+  auto by_width = [&](auto type, auto few) {
     using T = decltype(type);
-    if (D == 64) launch(attn_tile_kernel<T, 64, false>);
-    else if (D < 64) launch(attn_tile_kernel<T, 64, true>);
-    else if (D == 128) launch(attn_tile_kernel<T, 128, false>);
-    else launch(attn_tile_kernel<T, 128, true>);
+    constexpr bool F = decltype(few)::value;
+    constexpr int threads = AttnShape<T, F>::kThreads;
+    if (D == 64) launch(attn_tile_kernel<T, 64, false, F>, threads);
+    else if (D < 64) launch(attn_tile_kernel<T, 64, true, F>, threads);
+    else if (D == 128) launch(attn_tile_kernel<T, 128, false, F>, threads);
+    else launch(attn_tile_kernel<T, 128, true, F>, threads);
   };
-  if (dtype == LTV_DTYPE_F32) by_width(float()); else by_width(bf16_t());
+  if (dtype == LTV_DTYPE_F32) by_width(float(), std::false_type());
+  else if (p.few) by_width(bf16_t(), std::true_type());
+  else by_width(bf16_t(), std::false_type());
   LTV_LAUNCH_CHECK();
   if (p.joins) {
     auto join = [&](auto type) {

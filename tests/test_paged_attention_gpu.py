@@ -112,6 +112,40 @@ def test_many_sequences(B, dtype):
     _case(dtype, 4, 2, 64, 16, new, [(i * 37) % 230 for i in range(B)], packed=True, seed=23)
 
 
+@pytest.mark.parametrize("B,NH,NKVH,D,page", [(130, 12, 4, 128, 16), (90, 6, 6, 64, 7),
+                                              (600, 2, 1, 96, 48), (70, 64, 8, 128, 64)])
+@pytest.mark.parametrize("T", [1, 2])
+def test_many_short_sequences(T, B, NH, NKVH, D, page):
+    """Enough sequences and heads for the shape of one wavefront; a long one among them."""
+    cached = [(i * 53) % 140 for i in range(B)]
+    cached[B // 3], cached[7], cached[8] = 3000, 0, -T  # (no token in the cache at all)
+    _case(BF, NH, NKVH, D, page, [T] * B, cached, packed=False, seed=29)
+
+
+def test_many_short_sequences_and_wrong_hints():
+    """Hints that are too small for some of them: more rows, and keys, than were expected."""
+    B = 140
+    new = [1 + 49 * (i % 60 == 3) for i in range(B)]
+    _case(BF, 8, 4, 128, 16, new, [(i * 29) % 300 for i in range(B)], packed=True, seed=31,
+          max_new=1, max_len=16)
+
+
+@pytest.mark.parametrize("poison", [math.nan, math.inf])
+def test_many_short_sequences_with_poison(poison):
+    """The same where masked places hold infinities and NaN, in keys and values."""
+    B, lens = 140, [2 + (i * 31) % 90 for i in range(140)]
+    cache = Cache(lens, 4, 64, 16, BF, 30, spare=4)
+    used = torch.zeros(cache.P, 16, dtype=torch.bool, device=DEV)
+    for i, n in enumerate(lens):
+        pos = torch.arange(n, device=DEV)
+        used[cache.table[i, pos // 16].long(), pos % 16] = True
+    for x in (cache.k, cache.v):
+        x.transpose(1, 2)[~used] = poison
+    q = [cache.rand(1, 8, 64, dtype=BF) for _ in range(B)]
+    _check(_run(cache, q, [1] * B, False), attention64(q, cache, list(range(B)), [1] * B, 64 ** -0.5),
+           BF, 64, lens)
+
+
 @pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("NH,NKVH,D", [(8, 4, 128), (6, 6, 64), (3, 1, 128)])
 def test_long_chunk_among_short_ones(NH, NKVH, D, dtype):
