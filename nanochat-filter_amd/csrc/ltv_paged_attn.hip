@@ -430,7 +430,7 @@ __global__ void __launch_bounds__((AttnShape<T, FEW>::kThreads), FEW ? 1 : 2)
   if (x0 >= upto - mine && x0 < upto) {
     uint32_t at = upto - mine;
     int i = b0;
-    if (per > 1)
+    if (!FEW && per > 1)
       for (;; ++i) {
         q = paged_seq(a.batch, i);
         const uint32_t here = Line::of<KT>(a, q.n, q.len).all;
@@ -453,6 +453,33 @@ __global__ void __launch_bounds__((AttnShape<T, FEW>::kThreads), FEW ? 1 : 2)
   };
   int b = uniform(found.b);
   uint32_t at = uniform(found.at);  // of the group on the line
+  if (FEW && per > 1) {
+    // Which of the thread's sequences, one to a lane.  (2,048 of them 184 us searched by the
+    // thread, 176 so; in the other shape, with a fourth of them to a thread, it only adds
+    // instructions to every start: chunks among decoding sequences 103 and 104.)
+    const int end = min(b + per, a.batch.B), lane = threadIdx.x;
+    __syncthreads();  // (found is read)
+    for (;; b += 64) {
+      PagedSeq mine{a.batch.table, 0, 0, 0};
+      if (b + lane < end) mine = paged_seq(a.batch, b + lane);
+      const uint32_t here = Line::of<KT>(a, mine.n, mine.len).all, to = wave_sum_up_to(here);
+      const uint64_t past = __ballot(x0 - at < to);
+      if (past == 0 && b + 64 < end) {
+        at += __builtin_amdgcn_readlane(to, 63);
+        continue;
+      }
+      const int l = past == 0 ? 0 : __builtin_ctzll(past);
+      if (lane == l) {
+        found.s = mine;
+        found.b = b + l;
+        found.at = at + to - here;
+      }
+      break;
+    }
+    __syncthreads();
+    b = uniform(found.b);
+    at = uniform(found.at);
+  }
   PagedSeq s{uniform(found.s.table), uniform(found.s.len), uniform(found.s.n),
              uniform(found.s.row0)};
   Line u = Line::of<KT>(a, s.n, s.len);
@@ -1121,7 +1148,8 @@ extern "C" int ltv_paged_attention(int dtype, const void* q, const int64_t q_str
               LTV_ERR_INVALID_ARG, "null pointer");
   const int es = elem_size(dtype), chunk = 16 / es;
   const AttnPlan p = plan_attention(*batch, dtype, NH, NKVH, D, max_len);
-  LTV_REQUIRE(workspace && workspace_bytes >= p.bytes, LTV_ERR_WORKSPACE, "workspace too small");
+  LTV_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= p.bytes, LTV_ERR_WORKSPACE,
+              "workspace too small");
   // pages are addressed in 16-byte units of 32 bits
   bool fits = true, aligned = aligned16(k_pages) && aligned16(v_pages);
   for (int i = 0; i < 3; ++i)

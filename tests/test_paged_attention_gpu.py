@@ -113,7 +113,8 @@ def test_many_sequences(B, dtype):
 
 
 @pytest.mark.parametrize("B,NH,NKVH,D,page", [(130, 12, 4, 128, 16), (90, 6, 6, 64, 7),
-                                              (600, 2, 1, 96, 48), (70, 64, 8, 128, 64)])
+                                              (600, 2, 1, 96, 48), (70, 64, 8, 128, 64),
+                                              (4500, 1, 1, 64, 16)])
 @pytest.mark.parametrize("T", [1, 2])
 def test_many_short_sequences(T, B, NH, NKVH, D, page):
     """Enough sequences and heads for the shape of one wavefront; a long one among them."""
