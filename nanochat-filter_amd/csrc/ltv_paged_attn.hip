@@ -31,9 +31,8 @@
 // What bounds it.  One new token of each sequence: memory, 64 sequences of 8,000 tokens at 5.8
 // TB/s (a copy reaches 5.0, half of it writes).  Long chunks: the matrix unit and the clock
 // that it leaves, 12,289 tokens over 32,289 at 826 TFLOP/s where a plain product of two 8,192
-// x 8,192 matrices reaches 1,121.  Little work: latency, 2 us
-// until a workgroup has found its range, 4 until its first tile has landed, 2 to write, 3 to
-// join.
+// x 8,192 matrices reaches 1,121.  Little work: latency, 2 us until a workgroup has found its
+// range, 4 until its first tile has landed, 2 to write, 3 to join.
 #include <algorithm>
 #include <type_traits>
 
@@ -284,7 +283,8 @@ __device__ __forceinline__ float2* part_ml(const AttnArgs& a) {
 
 // Rows row0 .. row_end - 1 of a workgroup over keys begin .. end - 1, each key that a row
 // does not see left alone altogether: the way of tiles with infinite or NaN values among
-// those that some rows do not see.  Groups of sixteen lanes take a row's keys in turn, a lane holding eight channels.  part0: the partials of row0, or -1.
+// those that some rows do not see.  Groups of sixteen lanes take a row's keys in turn, a lane
+// holding eight channels.  part0: the partials of row0, or -1.
 template <typename T, int THREADS>
 __device__ __forceinline__ void rows_one_by_one(const AttnArgs& a, const PagedSeq& s, int b,
                                                 int kvh, int row0, int row_end, int begin, int end,
@@ -1097,7 +1097,7 @@ AttnPlan plan_shape(const ltv_paged_batch& b, int NH, int NKVH, int D, int max_l
 
 // Which shape.  One wavefront in four workgroups of a unit where each sequence and head has few
 // rows and there are as many of them as ranges of the other shape: 2,048 sequences of 30 to 100
-// tokens (6 heads) 253 and 185 us, 128 of up to 2,000 (8 heads) 142 and 132.  Of fewer and
+// tokens (6 heads) 253 and 177 us, 128 of up to 2,000 (8 heads) 142 and 132.  Of fewer and
 // longer ones the pieces are more to join, and their first tiles sooner there when four
 // wavefronts load them together: 64 of up to 2,000 (4 heads) 37.7 and 40.6, one very long among
 // 15 others 272 and 275, four short ones 17.9 and 23.0; so with more rows (32: 46.5 and 49.2).
