@@ -904,7 +904,7 @@ __global__ void __launch_bounds__((AttnShape<T, FEW>::kThreads), FEW ? 1 : 2)
     const int k = u.heads == 1 ? 0 : member >> (u.tiles - 1);
     const int kvh = round * u.heads + k;
     const int tile = u.heads == 1 ? (group << a.log_group) + member : member & (u.tiles - 1);
-    const bool on = k < u.heads && kvh < a.NKVH && tile < u.tiles;
+    const bool on = k < u.heads && (unsigned)kvh < (unsigned)a.NKVH && tile < u.tiles;
     // (a sequence of more rows than there is room for is not cut)
     const int rows = s.n * a.g;
     const bool cuts = min(rows, kAttnRows) <= a.part_tile;

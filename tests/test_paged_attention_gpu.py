@@ -368,6 +368,18 @@ def test_repeats_are_bitwise_equal(T):
                            first)
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_starts_out_of_order_stay_in_range(dtype):
+    """Starts that fall, overlap or lie outside: the rows of one sequence only are its own."""
+    cache = Cache([200, 30, 40, 500, 20], 4, 64, 16, dtype, 32)
+    q = cache.rand(7, 8, 64, dtype=dtype)
+    starts = torch.tensor([0, 3, 2, -5, 40, 7], dtype=torch.int32, device=DEV)
+    out, lse = _ops().paged_attention(q, cache.k, cache.v, cache.table, cache.lens, starts=starts,
+                                      return_lse=True)
+    want = attention64([q], cache, [3], [7], 64 ** -0.5)  # (from -5 to 40: all seven rows)
+    _check([(out[3:], lse[3:])], [(*(x[3:] for x in want[0][:3]), want[0][3])], dtype, 64, [500])
+
+
 def test_no_tokens_and_no_sequences():
     cache = Cache([10], 2, 64, 16, BF, 16)
     ops = _ops()
