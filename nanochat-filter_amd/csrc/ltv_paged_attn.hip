@@ -1083,11 +1083,11 @@ AttnPlan plan_shape(const ltv_paged_batch& b, int NH, int NKVH, int D, int max_l
   while (bound / (double)(int64_t(1) << p.unit) > (double)(1 << 30)) ++p.unit;
   p.slope = (int)(p.group * kAttnRows / g / KT) >> p.unit;
   // What a piece costs beside its keys -- its rows, the first tile's way, the remainders that
-  // the first tiles take, its partials -- counted in blocks: four of many rows, one of few;
-  // none where there is a range for every few blocks.  (Chunks mixed with decoding 110 us
-  // without, 98 with it, float32 chunks 50 and 48, a ragged decode step 282 and 274, a small
-  // one 17.6 and 18.4.)
-  p.extra = (rows > 32 ? 4 : most > 8 * Shape::kGrid ? 1 : 0) >> p.unit;
+  // the first tiles take, its partials -- counted in blocks: four, or none where few rows have
+  // a range for every few blocks.  (Without and with it: chunks mixed with decoding 110 and 98
+  // us, float32 chunks 50 and 48, a ragged decode step 282 and 261; a small one 17.6 and, with
+  // one block, 18.4.  Two, four and eight for 256 sequences of up to 2,000 tokens 222, 219, 224.)
+  p.extra = (FEW || rows > 32 || most > 8 * Shape::kGrid ? 4 : 0) >> p.unit;
   const int64_t n = (int64_t)p.ranges * p.group;
   p.part_rows = n * 2 * p.part_tile;
   p.cuts_at = (size_t)p.part_rows * (D + 2) * sizeof(float);
