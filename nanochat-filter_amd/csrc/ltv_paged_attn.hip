@@ -24,13 +24,13 @@
 // workgroup is empty or ends late, whatever mixture of lengths a call has.  The line is made
 // on the device, which knows the lengths.  A range begins and ends within a row tile as it
 // comes; a second kernel joins the (m, l, o) of the tiles that were cut.  (Every sequence cut
-// into the same number of chunks instead, in the same calls: 322 us and 274 now for a decode
+// into the same number of chunks instead, in the same calls: 322 us and 260 now for a decode
 // step with one very long context, 144 and 98 for chunks among decoding sequences, 1,500 and
 // 1,195 for the last chunk of a long prompt.)
 //
 // What bounds it.  One new token of each sequence: memory, 64 sequences of 8,000 tokens at 5.8
 // TB/s (a copy reaches 5.0, half of it writes).  Long chunks: the matrix unit and the clock
-// that it leaves, 12,289 tokens over 32,289 at 826 TFLOP/s where a plain product of two 8,192
+// that it leaves, 12,289 tokens over 32,289 at 803 to 826 TFLOP/s where a plain product of two 8,192
 // x 8,192 matrices reaches 1,121.  Little work: latency, 2 us until a workgroup has found its
 // range, 4 until its first tile has landed, 2 to write, 3 to join.
 #include <algorithm>
@@ -1097,7 +1097,7 @@ AttnPlan plan_shape(const ltv_paged_batch& b, int NH, int NKVH, int D, int max_l
 
 // Which shape.  One wavefront in four workgroups of a unit where each sequence and head has few
 // rows and there are as many of them as ranges of the other shape: 2,048 sequences of 30 to 100
-// tokens (6 heads) 253 and 177 us, 128 of up to 2,000 (8 heads) 142 and 132.  Of fewer and
+// tokens (6 heads) 253 and 167 us, 128 of up to 2,000 (8 heads) 142 and 123.  Of fewer and
 // longer ones the pieces are more to join, and their first tiles sooner there when four
 // wavefronts load them together: 64 of up to 2,000 (4 heads) 37.7 and 40.6, one very long among
 // 15 others 272 and 275, four short ones 17.9 and 23.0; so with more rows (32: 46.5 and 49.2).
