@@ -1095,17 +1095,21 @@ AttnPlan plan_shape(const ltv_paged_batch& b, int NH, int NKVH, int D, int max_l
   return p;
 }
 
-// Which shape.  One wavefront in four workgroups of a unit where each sequence and head has few
-// rows and there are as many of them as ranges of the other shape: 2,048 sequences of 30 to 100
-// tokens (6 heads) 253 and 167 us, 128 of up to 2,000 (8 heads) 142 and 123.  Of fewer and
-// longer ones the pieces are more to join, and their first tiles sooner there when four
-// wavefronts load them together: 64 of up to 2,000 (4 heads) 37.7 and 40.6, one very long among
-// 15 others 272 and 275, four short ones 17.9 and 23.0; so with more rows (32: 46.5 and 49.2).
-// float32 has its products to wait for.
+// Which shape.  One wavefront in four workgroups of a unit where there are many sequences of few
+// rows that are not long: a step of 2,048 sequences of 30 to 100 tokens (6 heads) 246 us with
+// four wavefronts and 167 with one, 512 of 100 to 300 99 and 82, 32 of 300 to 700 26.4 and 21.9,
+// 40 of 200 to 1,000 (8 heads) 29.3 and 29.1.  Of long ones the pieces are more to join and the
+// tiles half as large: 128 of up to 2,000 (8 heads) 119 and 123, 64 of 8,000 (4 heads) 183 and
+// 187.  Where there are very many the longest says little about the others, and one wavefront
+// has less to lose: 256 of up to 2,000 (8 heads) 213 and 219.  With little work what counts is
+// how soon a tile is there, which four wavefronts load together (four sequences 17.9 and 23.0);
+// of more rows, too, the pieces weigh more (32 rows 46.5 and 49.2).  float32 has its products
+// to wait for.
 AttnPlan plan_attention(const ltv_paged_batch& b, int dtype, int NH, int NKVH, int D, int max_len) {
   if (dtype == LTV_DTYPE_F32) return plan_shape<float, false>(b, NH, NKVH, D, max_len);
-  const int64_t rows = (int64_t)std::max(b.T, 1) * (NH / NKVH);
-  if (rows <= 16 && (int64_t)b.B * NKVH >= AttnShape<bf16_t, false>::kGrid)
+  const int64_t rows = (int64_t)std::max(b.T, 1) * (NH / NKVH), units = (int64_t)b.B * NKVH;
+  const int64_t blocks = units * ((std::max(max_len, 1) + 63) / 64);
+  if (rows <= 16 && blocks >= 1024 && (max_len <= 1024 || units >= 2048))
     return plan_shape<bf16_t, true>(b, NH, NKVH, D, max_len);
   return plan_shape<bf16_t, false>(b, NH, NKVH, D, max_len);
 }

@@ -115,17 +115,19 @@ def test_many_sequences(B, dtype):
 @pytest.mark.parametrize("B,NH,NKVH,D,page", [(130, 12, 4, 128, 16), (90, 6, 6, 64, 7),
                                               (600, 2, 1, 96, 48), (70, 64, 8, 128, 64),
                                               (4500, 1, 1, 64, 16)])
+@pytest.mark.parametrize("max_len", [None, 512])
 @pytest.mark.parametrize("T", [1, 2])
-def test_many_short_sequences(T, B, NH, NKVH, D, page):
-    """Enough sequences and heads for the shape of one wavefront; a long one among them."""
+def test_many_short_sequences(T, max_len, B, NH, NKVH, D, page):
+    """Enough sequences and heads for the shape of one wavefront, where they are said to be
+    short; a long one among them all the same."""
     cached = [(i * 53) % 140 for i in range(B)]
     cached[B // 3], cached[7], cached[8] = 3000, 0, -T  # (no token in the cache at all)
-    _case(BF, NH, NKVH, D, page, [T] * B, cached, packed=False, seed=29)
+    _case(BF, NH, NKVH, D, page, [T] * B, cached, packed=False, seed=29, max_len=max_len)
 
 
-def test_many_short_sequences_and_wrong_hints():
+@pytest.mark.parametrize("B", [140, 300])
+def test_many_short_sequences_and_wrong_hints(B):
     """Hints that are too small for some of them: more rows, and keys, than were expected."""
-    B = 140
     new = [1 + 49 * (i % 60 == 3) for i in range(B)]
     _case(BF, 8, 4, 128, 16, new, [(i * 29) % 300 for i in range(B)], packed=True, seed=31,
           max_new=1, max_len=16)
