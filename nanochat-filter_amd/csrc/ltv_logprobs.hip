@@ -4,8 +4,13 @@
 //   z = c tanh(x / c)  (or x),  m = max z,  S = sum e^{z - m},  A = sum (z - m) e^{z - m}
 //   lse = m + log S,   logprob = z_t - lse,   entropy = log S - A / S
 //
-// With the cap, tanh(y) = 1 - 2 r with r = 1 / (1 + e^{2 y}): z - c = -2 c r lies in
-// [-2 c, 0], so c serves as the maximum, and its derivative is 4 r (1 - r).
+// With a cap up to 64, tanh(y) = 1 - 2 r with r = 1 / (1 + e^{2 y}): z = c - 2 c r lies in
+// [-c, c], where e^z and the sum of 2^31 of them neither overflow nor vanish in float32, so 0
+// serves as the maximum; z's derivative is 4 r (1 - r).  Its error is some roundings of c (of
+// 15: 2e-6 at most), not of z, for half the instructions of a tanh.  With a larger cap z is
+// c tanh(x / c) to its own last bits, and m is the row's maximum: 4,096 rows of 65,536
+// bfloat16 logits with five alternatives take 224 us with a cap of 100 and 120 with one of
+// 50, 4,096 of 50,257 with their gradient 388 and 256.
 //
 // Forward.  One pass over the logits: each thread keeps m, S and A of its elements and they
 // are joined at the end.  A workgroup takes a row, or, where there are few rows, a piece of
@@ -52,13 +57,28 @@ struct LogpArgs {
   uint64_t* part_keys;       // (N, pieces, top_k)
 };
 
-// r of the cap's tanh; cap_scale = 2 log2(e) / c
+// How z follows from x: none, by r, by tanh.
+enum Cap { kNoCap, kCap, kWideCap };
+constexpr float kMostCap = 64.0f;  // by r
+
+// r of the cap's tanh; cap_scale = 2 log2(e) / c (finite for the smallest c, too)
+__device__ __forceinline__ float cap_scale_of(float cap) {
+  return fminf(2.0f * kLog2e / cap, 3.0e38f);
+}
 __device__ __forceinline__ float cap_r(float x, float cap_scale) {
   return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * cap_scale));
 }
 
+// (below 2^-13 of the cap x (1 - (x / c)^2 / 3 + ..) rounds to x)
+__device__ __forceinline__ float wide_capped(float x, float cap) {
+  return fabsf(x) <= cap * 0x1p-13f ? x : cap * tanhf(x / cap);
+}
+
+template <Cap CAP>
 __device__ __forceinline__ float capped(float x, float cap) {
-  return cap > 0.0f ? fmaf(-2.0f * cap, cap_r(x, 2.0f * kLog2e / cap), cap) : x;
+  if constexpr (CAP == kNoCap) return x;
+  if constexpr (CAP == kWideCap) return wide_capped(x, cap);
+  return fmaf(-2.0f * cap, cap_r(x, cap_scale_of(cap)), cap);
 }
 
 // A total order of the logits with their indices: larger value first (NaN above all,
@@ -86,9 +106,9 @@ __device__ __forceinline__ uint4 load_vec(const T* p) {
 }
 
 // m, S and A of some elements: S = sum 2^d, A = sum d 2^d with d = (x - m) log2(e) (the
-// difference first: the logits may be of any size).  With the cap m stays c, and A counts
-// r instead of d = -2 c log2(e) r.
-template <bool CAP>
+// difference first: the logits may be of any size).  By r there is no m: S = sum e^z, and A
+// counts r instead of d.
+template <Cap CAP>
 struct Sums {
   float m = -INFINITY, s = 0.0f, a = 0.0f;
 
@@ -97,16 +117,20 @@ struct Sums {
     return w == 0.0f ? s * 0.0f : fmaf(d, s, a) * w;  // (a NaN stays)
   }
   template <int N>
-  __device__ __forceinline__ void add(const float (&x)[N], float cap_scale, float cap_exp) {
-    if constexpr (CAP) {
+  __device__ __forceinline__ void add(const float (&logits)[N], float cap) {
+    if constexpr (CAP == kCap) {
+      const float cap_scale = cap_scale_of(cap), at0 = cap * kLog2e, slope = -2.0f * at0;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const float r = cap_r(x[i], cap_scale);
-        const float e = __builtin_amdgcn_exp2f(r * cap_exp);
+        const float r = cap_r(logits[i], cap_scale);
+        const float e = __builtin_amdgcn_exp2f(fmaf(r, slope, at0));
         s += e;
         a = fmaf(r, e, a);
       }
     } else {
+      float x[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[i] = capped<CAP>(logits[i], cap);
       float top = x[0];
 #pragma unroll
       for (int i = 1; i < N; ++i) top = fmaxf(top, x[i]);
@@ -129,7 +153,7 @@ struct Sums {
     }
   }
   __device__ __forceinline__ void join(float m2, float s2, float a2) {
-    if constexpr (CAP) {
+    if constexpr (CAP == kCap) {
       s += s2;
       a += a2;
     } else {
@@ -167,12 +191,13 @@ __device__ __forceinline__ uint64_t kth_of_lanes(uint64_t mine, int k) {
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 
 // What a row's sums make: log(sum of exponentials) and entropy.
-template <bool CAP>
+template <Cap CAP>
 __device__ __forceinline__ void row_results(const Sums<CAP>& sums, float cap, float& lse,
                                             float& entropy) {
   const float log_s = __builtin_amdgcn_logf(sums.s), a = sums.a / sums.s;
-  lse = fmaf(log_s, kLn2, CAP ? cap : sums.m);
-  entropy = CAP ? fmaf(log_s, kLn2, 2.0f * cap * a) : (log_s - a) * kLn2;
+  lse = fmaf(log_s, kLn2, CAP == kCap ? 0.0f : sums.m);
+  // (by r: the mean of z is c - 2 c a)
+  entropy = CAP == kCap ? fmaf(log_s, kLn2, cap * fmaf(2.0f, a, -1.0f)) : (log_s - a) * kLn2;
 }
 
 // The target's logit (one thread reads it ahead), and the row's results that are not
@@ -189,14 +214,15 @@ __device__ __forceinline__ Target target_of(const LogpArgs& p, int64_t n, const 
   if (t.given) t.x = io_traits<T>::load(row + id);
   return t;
 }
-__device__ __forceinline__ void store_row(const LogpArgs& p, int64_t n, const Target& t, float cap,
+template <Cap CAP>
+__device__ __forceinline__ void store_row(const LogpArgs& p, int64_t n, const Target& t,
                                           float lse, float entropy) {
-  p.logprobs[n] = t.given ? capped(t.x, cap) - lse : 0.0f;
+  p.logprobs[n] = t.given ? capped<CAP>(t.x, p.cap) - lse : 0.0f;
   if (p.entropy != nullptr) p.entropy[n] = entropy;
   if (p.lse != nullptr) p.lse[n] = lse;
 }
 
-template <typename T, bool CAP, bool TOP>
+template <typename T, Cap CAP, bool TOP>
 __global__ void __launch_bounds__(kThreads) logprobs_forward_kernel(const LogpArgs p) {
   constexpr int N = io_traits<T>::kVec;
   constexpr int kFirst = 8192 / (kThreads * N);  // vectors of a thread kept for the bound
@@ -211,8 +237,6 @@ __global__ void __launch_bounds__(kThreads) logprobs_forward_kernel(const LogpAr
   const T* whole_row = reinterpret_cast<const T*>(p.x) + n * p.xs;
   const T* row = whole_row + begin;
   const int tid = threadIdx.x, lane = tid & 63, V = min(p.V - begin, p.piece);
-  const float cap_scale = CAP ? 2.0f * kLog2e / p.cap : 0.0f;
-  const float cap_exp = CAP ? -2.0f * p.cap * kLog2e : 0.0f;
   const int whole = V / N;  // vectors that the piece fills; the rest are single elements
   Sums<CAP> sums;
   float bound = INFINITY;
@@ -226,7 +250,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_forward_kernel(const LogpAr
   auto take = [&](const uint4& q, int v) {
     float x[N];
     unpack16(q, x, T());
-    sums.add(x, cap_scale, cap_exp);
+    sums.add(x, p.cap);
     if constexpr (TOP) {
       bool any = false;
 #pragma unroll
@@ -253,7 +277,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_forward_kernel(const LogpAr
       if (v + j * kThreads < whole) {
         float x[N];
         unpack16(q[j], x, T());
-        sums.add(x, cap_scale, cap_exp);
+        sums.add(x, p.cap);
         top[j] = x[0];
 #pragma unroll
         for (int i = 1; i < N; ++i) top[j] = __builtin_elementwise_maximum(top[j], x[i]);
@@ -299,7 +323,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_forward_kernel(const LogpAr
   }
   if (whole * N + tid < V) {
     const float x[1] = {io_traits<T>::load(row + whole * N + tid)};
-    sums.add(x, cap_scale, cap_exp);
+    sums.add(x, p.cap);
     if (TOP && !(x[0] <= bound)) collect(x[0], whole * N + tid);
   }
 
@@ -322,7 +346,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_forward_kernel(const LogpAr
     if (tid < 3) p.part_sums[part * 3 + tid] = tid == 0 ? sums.m : tid == 1 ? sums.s : sums.a;
   } else {
     row_results(sums, p.cap, lse, entropy);
-    if (tid == 0) store_row(p, n, target, CAP ? p.cap : 0.0f, lse, entropy);
+    if (tid == 0) store_row<CAP>(p, n, target, lse, entropy);
   }
 
   if constexpr (TOP) {
@@ -356,7 +380,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_forward_kernel(const LogpAr
         p.part_keys[part * p.top_k + above] = mine;
       } else {
         p.top_ids[n * p.top_k + above] = key_index(mine);
-        p.top_lp[n * p.top_k + above] = capped(key_value(mine), CAP ? p.cap : 0.0f) - lse;
+        p.top_lp[n * p.top_k + above] = capped<CAP>(key_value(mine), p.cap) - lse;
       }
     }
     // (a last piece of fewer elements than alternatives)
@@ -373,7 +397,7 @@ constexpr int kJoinThreads = kPieces * kGroups;
 // alternatives.  The k-th largest of the first few of every piece bounds the k-th largest of
 // all from below; what is not under it, hardly more than k, is collected and ranked.
 // (16 rows of 16 pieces with 20 alternatives: 3.1 us, with all ranked against all 5.7.)
-template <typename T, bool CAP>
+template <typename T, Cap CAP>
 __global__ void __launch_bounds__(kJoinThreads) logprobs_join_kernel(const LogpArgs p) {
   __shared__ unsigned long long cands[kJoinThreads];
   __shared__ unsigned long long bound;
@@ -408,7 +432,7 @@ __global__ void __launch_bounds__(kJoinThreads) logprobs_join_kernel(const LogpA
   if (tid == 0) {
     float lse, entropy;
     row_results(sums, p.cap, lse, entropy);
-    store_row(p, n, target, CAP ? p.cap : 0.0f, lse, entropy);
+    store_row<CAP>(p, n, target, lse, entropy);
     lse_lds = lse;
   }
   if (all == 0) return;
@@ -424,7 +448,7 @@ __global__ void __launch_bounds__(kJoinThreads) logprobs_join_kernel(const LogpA
   for (int j = 0; j < have; ++j) rank += cands[j] > key;
   if (rank < p.top_k) {
     p.top_ids[n * p.top_k + rank] = key_index(key);
-    p.top_lp[n * p.top_k + rank] = capped(key_value(key), CAP ? p.cap : 0.0f) - lse_lds;
+    p.top_lp[n * p.top_k + rank] = capped<CAP>(key_value(key), p.cap) - lse_lds;
   }
 }
 
@@ -453,15 +477,19 @@ struct LogpGradArgs {
 };
 
 // dx of an element, without the terms of a target or an alternative (extra).
-template <bool CAP>
+template <Cap CAP>
 struct Grad {
   float lse, total, ge, ent, cap, cap_scale;
   __device__ __forceinline__ float operator()(float x, float extra) const {
     float z = x, slope = 1.0f;
-    if constexpr (CAP) {
+    if constexpr (CAP == kCap) {
       const float r = cap_r(x, cap_scale);
       z = fmaf(-2.0f * cap, r, cap);
       slope = 4.0f * r * (1.0f - r);
+    } else if constexpr (CAP == kWideCap) {
+      z = wide_capped(x, cap);
+      const float t = z / cap;
+      slope = fmaf(-t, t, 1.0f);
     }
     const float lp = z - lse, e = __builtin_amdgcn_exp2f(lp * kLog2e);
     // (an entry without probability has none, however low its log)
@@ -474,7 +502,7 @@ struct Grad {
 // side (4,096 rows of 50,257 bfloat16 logits, forward and gradient, 275 us with 256, 265 with
 // 512, 257 with 1,024; the gradient of 2,000 rows of float32 171 and 145), else 256 (2,000 rows
 // of bfloat16, pieces of 40 KiB, 86 and 89; 4,096 of 1,000 logits 7 and 13).
-template <typename T, bool CAP, int kGradThreads>
+template <typename T, Cap CAP, int kGradThreads>
 __global__ void __launch_bounds__(kGradThreads) logprobs_backward_kernel(const LogpGradArgs p) {
   constexpr int N = io_traits<T>::kVec, kAhead = 2;
   const int64_t n = blockIdx.y;
@@ -491,7 +519,7 @@ __global__ void __launch_bounds__(kGradThreads) logprobs_backward_kernel(const L
   grad.ge = p.g_ent != nullptr ? p.g_ent[n] : 0.0f;
   grad.ent = p.g_ent != nullptr ? p.entropy[n] : 0.0f;
   grad.cap = p.cap;
-  grad.cap_scale = CAP ? 2.0f * kLog2e / p.cap : 0.0f;
+  grad.cap_scale = CAP == kCap ? cap_scale_of(p.cap) : 0.0f;
   grad.total = g;
   for (int i = 0; i < k; ++i) grad.total += p.g_top[n * p.top_k + i];
 
@@ -534,6 +562,9 @@ __global__ void __launch_bounds__(kGradThreads) logprobs_backward_kernel(const L
       io_traits<T>::store(gx + j, grad(io_traits<T>::load(x + j), extra));
   }
 }
+
+template <Cap CAP>
+using cap_type = std::integral_constant<Cap, CAP>;
 
 int check_rows(int dtype, const void* x, int64_t row_stride, const int64_t* targets, int64_t N,
                int V, int top_k, float softcap) {
@@ -583,7 +614,7 @@ extern "C" int ltv_token_logprobs_forward(int dtype, const void* logits, int64_t
   const dim3 grid((unsigned)N, a.pieces);
   auto launch = [&](auto type, auto cap) -> int {
     using T = decltype(type);
-    constexpr bool C = decltype(cap)::value;
+    constexpr Cap C = decltype(cap)::value;
     if (top_k > 0)
       hipLaunchKernelGGL((logprobs_forward_kernel<T, C, true>), grid, dim3(kThreads), 0, st, a);
     else
@@ -597,7 +628,8 @@ extern "C" int ltv_token_logprobs_forward(int dtype, const void* logits, int64_t
     return LTV_OK;
   };
   auto by_cap = [&](auto type) {
-    return softcap > 0.0f ? launch(type, std::true_type()) : launch(type, std::false_type());
+    if (softcap > kMostCap) return launch(type, cap_type<kWideCap>());
+    return softcap > 0.0f ? launch(type, cap_type<kCap>()) : launch(type, cap_type<kNoCap>());
   };
   return dtype == LTV_DTYPE_F32 ? by_cap(float()) : by_cap(bf16_t());
 }
@@ -625,14 +657,16 @@ extern "C" int ltv_token_logprobs_backward(int dtype, const void* logits, int64_
     const dim3 grid((unsigned)((V + piece - 1) / piece), (unsigned)std::min<int64_t>(65535, N - n0));
     auto launch = [&](auto type, auto cap) {
       using T = decltype(type);
-      constexpr bool C = decltype(cap)::value;
+      constexpr Cap C = decltype(cap)::value;
       if ((int64_t)std::min(piece, V) * (int)sizeof(T) >= 65536)
         hipLaunchKernelGGL((logprobs_backward_kernel<T, C, 1024>), grid, dim3(1024), 0, st, a);
       else
         hipLaunchKernelGGL((logprobs_backward_kernel<T, C, 256>), grid, dim3(256), 0, st, a);
     };
     auto by_cap = [&](auto type) {
-      if (softcap > 0.0f) launch(type, std::true_type()); else launch(type, std::false_type());
+      if (softcap > kMostCap) launch(type, cap_type<kWideCap>());
+      else if (softcap > 0.0f) launch(type, cap_type<kCap>());
+      else launch(type, cap_type<kNoCap>());
     };
     if (dtype == LTV_DTYPE_F32) by_cap(float()); else by_cap(bf16_t());
     LTV_LAUNCH_CHECK();
