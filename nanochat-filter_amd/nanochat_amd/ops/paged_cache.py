@@ -85,7 +85,9 @@ def paged_cache_reserve(page_table: Tensor, seq_lens: Tensor, ref_counts: Tensor
 
     Returns an int32 tensor of one element: 0; or, with nothing changed, how many pages
     are missing; or -1 for a slot or count out of range or a sequence longer than its
-    table row."""
+    table row.  Where it is not 0 there are no new tokens: appending some would overwrite
+    the last ones there are.  A caller that does not wait for it passes on
+    ``torch.where(status == 0, slots, -1)`` as the slots, which are no sequences then."""
     if torch.compiler.is_compiling():
         return _reserve_op(page_table, seq_lens, ref_counts, slots, counts, k_pages, v_pages)
     return N.torch_ext().paged_cache_reserve(page_table, seq_lens, ref_counts, slots, counts,

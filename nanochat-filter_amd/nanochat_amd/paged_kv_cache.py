@@ -60,6 +60,9 @@ class PagedKVCache:
         self.rows = tuple(torch.zeros(n_layer, max_seqs, n, head_dim, dtype=dtype, device=device)
                           for n in (n_head, n_kv_head, n_kv_head))
         self.lens = [0] * max_seqs  # what seq_lens holds, known on the host
+        # on the device: 0, or the status of the first of the steps not yet looked at that
+        # found no room; None where there are no such steps
+        self._status = None
 
     def _slots(self, slots: Sequence[int]) -> torch.Tensor:
         if len(set(slots)) != len(slots):
@@ -70,9 +73,14 @@ class PagedKVCache:
 
     def step(self, slots: Sequence[int], n_new: int, check: bool = True) -> "PagedStep":
         """Room for ``n_new`` more tokens in each of the slots, and the view of them that
-        a model's layers take.  Raises if the pages run out, with nothing changed; with
-        ``check`` off it does not wait for the device to say so, and the caller looks at
-        the step's ``status`` (0, or how many pages were missing and nothing reserved)."""
+        a model's layers take.  Raises if the pages run out, with nothing changed.
+
+        With ``check`` off it does not wait for the device to say so.  If they ran out, this
+        step and those that follow it change nothing in the cache (their attention is 0),
+        until ``check_steps`` or a step with ``check`` on has raised; ``status`` of a step is
+        0, or how many pages were missing at the first of them."""
+        if check:
+            self.check_steps()
         index = self._slots(slots)
         if n_new <= 0:
             raise ValueError(f"a step has new tokens, got {n_new}")
@@ -82,15 +90,39 @@ class PagedKVCache:
         fresh = [self.lens[s] == 0 for s in slots]
         if any(fresh) and not all(fresh):
             raise ValueError("a step's sequences are all new or all continued")
-        status = paged_cache_reserve(
-            self.page_table, self.seq_lens, self.ref_counts, index,
-            torch.full_like(index, n_new), self.k_pages, self.v_pages)
-        if check and int(status):
-            raise RuntimeError(f"the paged cache is full: {int(status)} pages are missing")
+        counts = torch.full_like(index, n_new)
+        if not check and self._status is not None:
+            counts = torch.where(self._status == 0, counts, 0)
+        status = paged_cache_reserve(self.page_table, self.seq_lens, self.ref_counts, index,
+                                     counts, self.k_pages, self.v_pages)
+        room = None
+        if check:
+            self._raise_for(int(status))
+        else:
+            if self._status is not None:
+                status = torch.where(self._status == 0, status, self._status)
+            self._status, room = status, status == 0
         positions = [self.lens[s] for s in slots]
         for s in slots:
             self.lens[s] += n_new
-        return PagedStep(self, index, positions, n_new, status)
+        return PagedStep(self, index, positions, n_new, status, room)
+
+    def check_steps(self) -> None:
+        """Wait for the steps that were made with ``check`` off, and raise if one of them
+        found no room: it and the steps after it are undone, ``lens`` is what it was."""
+        if self._status is None:
+            return
+        status, self._status = int(self._status), None
+        if status:
+            self.lens[:] = self.seq_lens.tolist()
+        self._raise_for(status)
+
+    @staticmethod
+    def _raise_for(status: int) -> None:
+        if status < 0:
+            raise RuntimeError("the cache's lengths are not those of its steps")
+        if status:
+            raise RuntimeError(f"the paged cache is full: {status} pages are missing")
 
     def fork(self, src: Sequence[int], dst: Sequence[int]) -> None:
         """Slots dst continue from slots src (one src may be named several times)."""
@@ -137,9 +169,13 @@ class PagedStep:
     (``has_last_qkv``, ``last_qkv``, ``update_last_qkv``), and attention."""
 
     def __init__(self, cache: PagedKVCache, slots: torch.Tensor, positions: list, n_new: int,
-                 status: torch.Tensor):
-        self.cache, self.slots, self.positions, self.n_new = cache, slots, positions, n_new
+                 status: torch.Tensor, room: Optional[torch.Tensor] = None):
+        self.cache, self.positions, self.n_new = cache, positions, n_new
         self.status = status
+        # whether there was room (None: there was), known on the device; without it the
+        # step is one of no slots, or the tokens would go where the last ones before are
+        self._room = room
+        self.slots = slots if room is None else torch.where(room, slots, -1)
         self._index = slots.long()
         self.q, self.k, self.v = (_Rows(r, self._index) for r in cache.rows)
 
@@ -153,7 +189,10 @@ class PagedStep:
     def update_last_qkv(self, layer_idx: int, q: torch.Tensor, k: torch.Tensor,
                         v: torch.Tensor) -> None:
         for rows, t in zip(self.cache.rows, (q, k, v)):
-            rows[layer_idx].index_copy_(0, self._index, t.to(rows.dtype))
+            t = t.to(rows.dtype)
+            if self._room is not None:
+                t = torch.where(self._room, t, rows[layer_idx].index_select(0, self._index))
+            rows[layer_idx].index_copy_(0, self._index, t)
 
     def attend(self, layer_idx: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                scale: Optional[float] = None) -> torch.Tensor:
