@@ -5,12 +5,18 @@
 // What is read on the device (lengths, page ids, slots, starts, counts) is checked
 // there; what can be seen on the host is checked here: ValueError for shapes and
 // numbers, TypeError for dtypes, RuntimeError for tensors on the wrong device.
+//
+// Tensors that are not of the ordinary kind, and calls that a tracer, mode or transform
+// looks at, are left to the library ops, which those can see: None comes back.
+#include <ATen/TensorSubclassLikeUtils.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPCachingAllocator.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <cmath>
@@ -51,6 +57,24 @@ struct Workspace {
   }
   void* ptr() const { return bytes > 0 ? mem.get() : nullptr; }
 };
+
+bool ordinary(const Tensor& t) {
+  return !at::isTensorSubclassLike(t) && !t.is_neg() && !t._is_zerotensor();
+}
+bool ordinary(const OptTensor& t) { return !t.has_value() || ordinary(*t); }
+
+// (a mode is seen by each tensor's check)
+template <typename... Ts>
+bool ordinary_call(const Ts&... ts) {
+  return !torch::jit::tracer::isTracing() && (ordinary(ts) && ...);
+}
+
+// (asked before a call goes to a library op: there a transform's tangents are just dropped)
+void no_tangent(const Tensor& t, const char* name) {
+  TORCH_CHECK(!(c10::AutogradState::get_tls_state().get_fw_grad_mode() &&
+                t._fw_grad(/*level=*/0).defined()),
+              name, " has a tangent, but there is no forward-mode derivative");
+}
 
 void on_device(const Tensor& t, const char* name, const Tensor& like) {
   TORCH_CHECK(t.is_cuda(), "LTV HIP kernels need GPU tensors, got ", name, " on ", t.device());
@@ -183,9 +207,12 @@ void no_grad_needed(const Tensor& t, const char* name) {
 // ---------------------------------------------------------------------------
 // the cache
 // ---------------------------------------------------------------------------
-void append(const Tensor& k_in, const Tensor& v_in, const Tensor& k_pages, const Tensor& v_pages,
+bool append(const Tensor& k_in, const Tensor& v_in, const Tensor& k_pages, const Tensor& v_pages,
             const Tensor& table, const Tensor& lens, const OptTensor& slots,
             const OptTensor& starts, const OptInt& max_new) {
+  no_tangent(k_in, "k");
+  no_tangent(v_in, "v");
+  if (!ordinary_call(k_in, v_in, k_pages, v_pages, table, lens, slots, starts)) return false;
   const int dt = dtype_of(k_in, "k");
   TORCH_CHECK(k_in.is_cuda(), "LTV HIP kernels need GPU tensors, got k on ", k_in.device());
   on_device(v_in, "v", k_in);
@@ -207,6 +234,7 @@ void append(const Tensor& k_in, const Tensor& v_in, const Tensor& k_pages, const
                                   kp.s, v_pages.data_ptr(), vp.s, &b.b, (int)heads, (int)D,
                                   stream_of(k)),
            "ltv_paged_cache_append");
+  return true;
 }
 
 // (compact needs no lengths)
@@ -275,8 +303,10 @@ ltv_page_blocks make_blocks(const Tensor& k, const Tensor& v) {
   return b;
 }
 
-Tensor reserve(const Tensor& table, const Tensor& lens, const Tensor& refs, const Tensor& slots_in,
-               const Tensor& counts_in, const Tensor& k_pages, const Tensor& v_pages) {
+OptTensor reserve(const Tensor& table, const Tensor& lens, const Tensor& refs,
+                  const Tensor& slots_in, const Tensor& counts_in, const Tensor& k_pages,
+                  const Tensor& v_pages) {
+  if (!ordinary_call(table, lens, refs, slots_in, counts_in, k_pages, v_pages)) return {};
   const ltv_page_blocks blocks = make_blocks(k_pages, v_pages);
   on_device(table, "page_table", k_pages);
   const int page = to_int(k_pages.size(-2), "the page size");
@@ -300,45 +330,52 @@ Tensor reserve(const Tensor& table, const Tensor& lens, const Tensor& refs, cons
   return status;
 }
 
-void fork_slots(const Tensor& table, const Tensor& lens, const Tensor& refs, const Tensor& src_in,
+bool fork_slots(const Tensor& table, const Tensor& lens, const Tensor& refs, const Tensor& src_in,
                 const Tensor& dst_in) {
+  if (!ordinary_call(table, lens, refs, src_in, dst_in)) return false;
   const ltv_page_state state = make_state(table, lens, refs, 1);
   const Tensor src = int_vector(src_in, "src", table), dst = int_vector(dst_in, "dst", table);
   TORCH_CHECK_VALUE(src.numel() == dst.numel(), src.numel(), " src slots, but ", dst.numel(),
                     " dst slots");
   c10::OptionalDeviceGuard guard(table.device());
-  if (src.numel() == 0) return;
+  if (src.numel() == 0) return true;
   check_rc(ltv_paged_cache_fork(&state, src.data_ptr<int32_t>(), dst.data_ptr<int32_t>(),
                                 to_int(src.numel(), "the number of slots"), stream_of(table)),
            "ltv_paged_cache_fork");
+  return true;
 }
 
-void free_slots(const Tensor& table, const Tensor& lens, const Tensor& refs,
+bool free_slots(const Tensor& table, const Tensor& lens, const Tensor& refs,
                 const Tensor& slots_in) {
+  if (!ordinary_call(table, lens, refs, slots_in)) return false;
   const ltv_page_state state = make_state(table, lens, refs, 1);
   const Tensor slots = int_vector(slots_in, "slots", table);
   c10::OptionalDeviceGuard guard(table.device());
-  if (slots.numel() == 0) return;
+  if (slots.numel() == 0) return true;
   check_rc(ltv_paged_cache_free(&state, slots.data_ptr<int32_t>(),
                                 to_int(slots.numel(), "the number of slots"), stream_of(table)),
            "ltv_paged_cache_free");
+  return true;
 }
 
-void copy_pages(const Tensor& k_pages, const Tensor& v_pages, const Tensor& src_in,
+bool copy_pages(const Tensor& k_pages, const Tensor& v_pages, const Tensor& src_in,
                 const Tensor& dst_in) {
+  if (!ordinary_call(k_pages, v_pages, src_in, dst_in)) return false;
   const ltv_page_blocks blocks = make_blocks(k_pages, v_pages);
   const Tensor src = int_vector(src_in, "src", k_pages), dst = int_vector(dst_in, "dst", k_pages);
   TORCH_CHECK_VALUE(src.numel() == dst.numel(), src.numel(), " src pages, but ", dst.numel(),
                     " dst pages");
   c10::OptionalDeviceGuard guard(k_pages.device());
-  if (src.numel() == 0) return;
+  if (src.numel() == 0) return true;
   check_rc(ltv_paged_cache_copy(&blocks, src.data_ptr<int32_t>(), dst.data_ptr<int32_t>(),
                                 to_int(src.numel(), "the number of pages"), stream_of(k_pages)),
            "ltv_paged_cache_copy");
+  return true;
 }
 
-Tensor compact(const Tensor& table, const Tensor& refs, const Tensor& k_pages,
-               const Tensor& v_pages) {
+OptTensor compact(const Tensor& table, const Tensor& refs, const Tensor& k_pages,
+                  const Tensor& v_pages) {
+  if (!ordinary_call(table, refs, k_pages, v_pages)) return {};
   const ltv_page_blocks blocks = make_blocks(k_pages, v_pages);
   on_device(table, "page_table", k_pages);
   ltv_page_state state = make_state(table, std::nullopt, refs, 1);
@@ -357,12 +394,14 @@ Tensor compact(const Tensor& table, const Tensor& refs, const Tensor& k_pages,
 // attention
 // ---------------------------------------------------------------------------
 // (out, lse or None)
-std::tuple<Tensor, OptTensor> attention(const Tensor& q_in, const Tensor& k_pages,
-                                        const Tensor& v_pages, const Tensor& table,
-                                        const Tensor& lens, const OptTensor& slots,
-                                        const OptTensor& starts, const OptInt& max_new,
-                                        const OptInt& max_len, std::optional<double> scale,
-                                        bool return_lse) {
+std::optional<std::tuple<Tensor, OptTensor>> attention(
+    const Tensor& q_in, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table,
+    const Tensor& lens, const OptTensor& slots, const OptTensor& starts, const OptInt& max_new,
+    const OptInt& max_len, std::optional<double> scale, bool return_lse) {
+  no_tangent(q_in, "q");
+  no_tangent(k_pages, "k_pages");
+  no_tangent(v_pages, "v_pages");
+  if (!ordinary_call(q_in, k_pages, v_pages, table, lens, slots, starts)) return {};
   const int dt = dtype_of(q_in, "q");
   TORCH_CHECK(q_in.is_cuda(), "LTV HIP kernels need GPU tensors, got q on ", q_in.device());
   no_grad_needed(q_in, "q");
@@ -384,7 +423,7 @@ std::tuple<Tensor, OptTensor> attention(const Tensor& q_in, const Tensor& k_page
   Tensor out = at::empty(q.sizes(), q.options().requires_grad(false));
   OptTensor lse;
   if (return_lse) lse = at::empty(q.sizes().slice(0, q.dim() - 1), out.options().dtype(at::kFloat));
-  if (out.numel() == 0) return {out, lse};
+  if (out.numel() == 0) return std::make_tuple(out, lse);
   const Workspace ws(
       ltv_paged_attention_workspace_size(dt, &b.b, (int)NH, (int)NKVH, (int)D, most));
   const Strides3 qs = Strides3::tokens(q), os = Strides3::tokens(out),
@@ -395,7 +434,7 @@ std::tuple<Tensor, OptTensor> attention(const Tensor& q_in, const Tensor& k_page
                                ws.ptr(), ws.bytes, (int)NH, (int)NKVH,
                                (int)D, most, (float)sc, stream_of(q)),
            "ltv_paged_attention");
-  return {out, lse};
+  return std::make_tuple(out, lse);
 }
 
 // ---------------------------------------------------------------------------
@@ -459,16 +498,19 @@ LogpOut logprobs_forward(const Tensor& logits, const Tensor& targets, int64_t to
   return o;
 }
 
-Tensor logprobs_backward(const Tensor& logits, const Tensor& targets, const Tensor& lse,
-                         const Tensor& entropy, const Tensor& ids, const OptTensor& g_lp,
-                         const OptTensor& g_ent, const OptTensor& g_top, double cap) {
+Tensor backward_of(const Tensor& logits, const Tensor& targets, const Tensor& lse,
+                   const Tensor& entropy, const Tensor& ids, const OptTensor& g_lp,
+                   const OptTensor& g_ent, const OptTensor& g_top, double cap) {
+  no_tangent(logits, "logits");
   const Rows r = rows_of(logits, targets);
   c10::OptionalDeviceGuard guard(r.x.device());
   Tensor gx = at::empty(logits.sizes(), logits.options().requires_grad(false).memory_format(
                                             at::MemoryFormat::Contiguous));
   if (gx.numel() == 0) return gx;
   auto grad = [](const OptTensor& g) {
-    return g.has_value() && g->defined() ? g->to(at::kFloat).contiguous() : Tensor();
+    if (!g.has_value() || !g->defined()) return Tensor();
+    no_tangent(*g, "the gradient");
+    return g->to(at::kFloat).contiguous();
   };
   auto ptr = [](const Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; };
   const Tensor a = grad(g_lp), b = grad(g_ent), c = grad(g_top);
@@ -497,8 +539,8 @@ class TokenLogprobs : public torch::autograd::Function<TokenLogprobs> {
   static variable_list backward(AutogradContext* ctx, const variable_list& g) {
     const variable_list s = ctx->get_saved_variables();
     if (!g[0].defined() && !g[1].defined() && !g[2].defined()) return {{}, {}, {}, {}};
-    Tensor gx = logprobs_backward(s[0], s[1], s[2], s[3], s[4], g[0], g[1], g[2],
-                                  ctx->saved_data["cap"].toDouble());
+    Tensor gx = backward_of(s[0], s[1], s[2], s[3], s[4], g[0], g[1], g[2],
+                            ctx->saved_data["cap"].toDouble());
     // (with create_graph: a second derivative is refused, not taken as zero)
     if (at::GradMode::is_enabled())
       torch::autograd::set_history(
@@ -510,24 +552,34 @@ class TokenLogprobs : public torch::autograd::Function<TokenLogprobs> {
 };
 
 // (logprobs, entropy, top_logprobs, top_ids)
-std::tuple<Tensor, Tensor, Tensor, Tensor> token_logprobs(const Tensor& logits,
-                                                          const Tensor& targets, int64_t top_k,
-                                                          double cap) {
+std::optional<std::tuple<Tensor, Tensor, Tensor, Tensor>> token_logprobs(const Tensor& logits,
+                                                                         const Tensor& targets,
+                                                                         int64_t top_k,
+                                                                         double cap) {
+  no_tangent(logits, "logits");
+  if (!ordinary_call(logits, targets)) return {};
   if (at::GradMode::is_enabled() && logits.requires_grad()) {
     const variable_list o = TokenLogprobs::apply(logits, targets, top_k, cap);
-    return {o[0], o[1], o[2], o[3]};
+    return std::make_tuple(o[0], o[1], o[2], o[3]);
   }
   LogpOut o = logprobs_forward(logits, targets, top_k, cap, false);
-  return {o.logprobs, o.entropy, o.top, o.ids};
+  return std::make_tuple(o.logprobs, o.entropy, o.top, o.ids);
 }
 
 // (with the row sums that the backward reads)
-std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> token_logprobs_forward(const Tensor& logits,
-                                                                          const Tensor& targets,
-                                                                          int64_t top_k,
-                                                                          double cap) {
+std::optional<std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor>> token_logprobs_forward(
+    const Tensor& logits, const Tensor& targets, int64_t top_k, double cap) {
+  no_tangent(logits, "logits");
+  if (!ordinary_call(logits, targets)) return {};
   LogpOut o = logprobs_forward(logits, targets, top_k, cap, true);
-  return {o.logprobs, o.entropy, o.top, o.ids, o.lse};
+  return std::make_tuple(o.logprobs, o.entropy, o.top, o.ids, o.lse);
+}
+
+OptTensor token_logprobs_backward(const Tensor& logits, const Tensor& targets, const Tensor& lse,
+                                  const Tensor& entropy, const Tensor& ids, const OptTensor& g_lp,
+                                  const OptTensor& g_ent, const OptTensor& g_top, double cap) {
+  if (!ordinary_call(logits, targets, lse, entropy, ids, g_lp, g_ent, g_top)) return {};
+  return backward_of(logits, targets, lse, entropy, ids, g_lp, g_ent, g_top, cap);
 }
 
 }  // namespace
@@ -543,5 +595,5 @@ void bind_serving(pybind11::module_& m) {
   m.def("paged_attention", &attention, nogil());
   m.def("token_logprobs", &token_logprobs, nogil());
   m.def("token_logprobs_forward", &token_logprobs_forward, nogil());
-  m.def("token_logprobs_backward", &logprobs_backward, nogil());
+  m.def("token_logprobs_backward", &token_logprobs_backward, nogil());
 }

@@ -248,6 +248,13 @@ def torch_ext():
     return _ext
 
 
+def done(result):
+    """What the native host path gave inside a library op, where it leaves nothing to others."""
+    if result is None or result is False:
+        raise RuntimeError("LTV HIP kernels need tensors of the ordinary kind")
+    return result
+
+
 def last_error() -> str:
     return lib().ltv_last_error().decode("utf-8", "replace")
 

@@ -30,7 +30,8 @@ The reference's cache is contiguous (``nanochat/kv_cache.py`` ``insert_kv``) and
 copied whole to start several samples from one prompt (``prefill``).
 
 In eager mode the functions go straight to the native host path; under
-``torch.compile`` to the ``nanochat_amd`` library ops of the same names.
+``torch.compile``, and for what that path leaves (tensor subclasses, tracing, modes,
+transforms), to the ``nanochat_amd`` library ops of the same names.
 """
 
 from __future__ import annotations
@@ -49,10 +50,9 @@ def paged_cache_append(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, p
     """Write the new tokens' keys and values, the last n tokens of each sequence's
     ``seq_lens``, into their pages.  Tokens at negative positions or of pages that the
     table does not hold are dropped."""
-    if torch.compiler.is_compiling():
-        return _append_op(k, v, k_pages, v_pages, page_table, seq_lens, slots, starts, max_new)
-    N.torch_ext().paged_cache_append(k, v, k_pages, v_pages, page_table, seq_lens, slots, starts,
-                                     max_new)
+    args = (k, v, k_pages, v_pages, page_table, seq_lens, slots, starts, max_new)
+    if torch.compiler.is_compiling() or not N.torch_ext().paged_cache_append(*args):
+        _append_op(*args)
 
 
 def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tensor,
@@ -67,12 +67,10 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Ten
     shape without head_dim; -inf where there is nothing), which joins attention over
     several caches.  float32 or bfloat16, head_dim a multiple of 8 up to 128; inference
     only."""
-    if torch.compiler.is_compiling():
-        out, lse = _attention_op(q, k_pages, v_pages, page_table, seq_lens, slots, starts, max_new,
-                                 max_len, scale)
-    else:
-        out, lse = N.torch_ext().paged_attention(q, k_pages, v_pages, page_table, seq_lens, slots,
-                                                 starts, max_new, max_len, scale, return_lse)
+    args = (q, k_pages, v_pages, page_table, seq_lens, slots, starts, max_new, max_len, scale)
+    got = None if torch.compiler.is_compiling() else N.torch_ext().paged_attention(*args,
+                                                                                   return_lse)
+    out, lse = _attention_op(*args) if got is None else got
     return (out, lse) if return_lse else out
 
 
@@ -88,35 +86,34 @@ def paged_cache_reserve(page_table: Tensor, seq_lens: Tensor, ref_counts: Tensor
     table row.  Where it is not 0 there are no new tokens: appending some would overwrite
     the last ones there are.  A caller that does not wait for it passes on
     ``torch.where(status == 0, slots, -1)`` as the slots, which are no sequences then."""
-    if torch.compiler.is_compiling():
-        return _reserve_op(page_table, seq_lens, ref_counts, slots, counts, k_pages, v_pages)
-    return N.torch_ext().paged_cache_reserve(page_table, seq_lens, ref_counts, slots, counts,
-                                             k_pages, v_pages)
+    args = (page_table, seq_lens, ref_counts, slots, counts, k_pages, v_pages)
+    got = None if torch.compiler.is_compiling() else N.torch_ext().paged_cache_reserve(*args)
+    return _reserve_op(*args) if got is None else got
 
 
 def paged_cache_fork(page_table: Tensor, seq_lens: Tensor, ref_counts: Tensor, src: Tensor,
                      dst: Tensor) -> None:
     """Slot dst[i] becomes slot src[i], sharing its pages; what dst held is let go.  No
     dst is another dst or a src (src[i] == dst[i] does nothing)."""
-    if torch.compiler.is_compiling():
-        return _fork_op(page_table, seq_lens, ref_counts, src, dst)
-    N.torch_ext().paged_cache_fork(page_table, seq_lens, ref_counts, src, dst)
+    args = (page_table, seq_lens, ref_counts, src, dst)
+    if torch.compiler.is_compiling() or not N.torch_ext().paged_cache_fork(*args):
+        _fork_op(*args)
 
 
 def paged_cache_free(page_table: Tensor, seq_lens: Tensor, ref_counts: Tensor,
                      slots: Tensor) -> None:
     """Empty the slots; pages that no other slot holds become free."""
-    if torch.compiler.is_compiling():
-        return _free_op(page_table, seq_lens, ref_counts, slots)
-    N.torch_ext().paged_cache_free(page_table, seq_lens, ref_counts, slots)
+    args = (page_table, seq_lens, ref_counts, slots)
+    if torch.compiler.is_compiling() or not N.torch_ext().paged_cache_free(*args):
+        _free_op(*args)
 
 
 def paged_cache_copy(k_pages: Tensor, v_pages: Tensor, src: Tensor, dst: Tensor) -> None:
     """Copy page src[i] to page dst[i], in every layer; entries with an id outside
     [0, P) are skipped.  No dst is another dst or a src."""
-    if torch.compiler.is_compiling():
-        return _copy_op(k_pages, v_pages, src, dst)
-    N.torch_ext().paged_cache_copy(k_pages, v_pages, src, dst)
+    args = (k_pages, v_pages, src, dst)
+    if torch.compiler.is_compiling() or not N.torch_ext().paged_cache_copy(*args):
+        _copy_op(*args)
 
 
 def paged_cache_compact(page_table: Tensor, ref_counts: Tensor, k_pages: Tensor,
@@ -124,20 +121,20 @@ def paged_cache_compact(page_table: Tensor, ref_counts: Tensor, k_pages: Tensor,
     """Move the pages in use to the lowest ids (those past their number, in order, into
     the holes below it); the table and counts follow.  Returns their number, an int32
     tensor of one element."""
-    if torch.compiler.is_compiling():
-        return _compact_op(page_table, ref_counts, k_pages, v_pages)
-    return N.torch_ext().paged_cache_compact(page_table, ref_counts, k_pages, v_pages)
+    args = (page_table, ref_counts, k_pages, v_pages)
+    got = None if torch.compiler.is_compiling() else N.torch_ext().paged_cache_compact(*args)
+    return _compact_op(*args) if got is None else got
 
 
 # ---------------------------------------------------------------------------
-# library ops (torch.compile)
+# library ops (torch.compile, tracing, modes, transforms)
 # ---------------------------------------------------------------------------
 @torch.library.custom_op("nanochat_amd::paged_cache_append", mutates_args=("k_pages", "v_pages"))
 def _append_op(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tensor,
                seq_lens: Tensor, slots: Optional[Tensor], starts: Optional[Tensor],
                max_new: Optional[int]) -> None:
-    N.torch_ext().paged_cache_append(k, v, k_pages, v_pages, page_table, seq_lens, slots, starts,
-                                     max_new)
+    N.done(N.torch_ext().paged_cache_append(k, v, k_pages, v_pages, page_table, seq_lens, slots,
+                                            starts, max_new))
 
 
 @_append_op.register_fake
@@ -150,8 +147,8 @@ def _attention_op(q: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tenso
                   seq_lens: Tensor, slots: Optional[Tensor], starts: Optional[Tensor],
                   max_new: Optional[int], max_len: Optional[int],
                   scale: Optional[float]) -> Tuple[Tensor, Tensor]:
-    out, lse = N.torch_ext().paged_attention(q, k_pages, v_pages, page_table, seq_lens, slots,
-                                             starts, max_new, max_len, scale, True)
+    out, lse = N.done(N.torch_ext().paged_attention(q, k_pages, v_pages, page_table, seq_lens,
+                                                    slots, starts, max_new, max_len, scale, True))
     return out, lse
 
 
@@ -167,8 +164,8 @@ _STATE = ("page_table", "seq_lens", "ref_counts")
                          mutates_args=(*_STATE, "k_pages", "v_pages"))
 def _reserve_op(page_table: Tensor, seq_lens: Tensor, ref_counts: Tensor, slots: Tensor,
                 counts: Tensor, k_pages: Tensor, v_pages: Tensor) -> Tensor:
-    return N.torch_ext().paged_cache_reserve(page_table, seq_lens, ref_counts, slots, counts,
-                                             k_pages, v_pages)
+    return N.done(N.torch_ext().paged_cache_reserve(page_table, seq_lens, ref_counts, slots,
+                                                    counts, k_pages, v_pages))
 
 
 @_reserve_op.register_fake
@@ -179,7 +176,7 @@ def _(page_table, seq_lens, ref_counts, slots, counts, k_pages, v_pages):
 @torch.library.custom_op("nanochat_amd::paged_cache_fork", mutates_args=_STATE)
 def _fork_op(page_table: Tensor, seq_lens: Tensor, ref_counts: Tensor, src: Tensor,
              dst: Tensor) -> None:
-    N.torch_ext().paged_cache_fork(page_table, seq_lens, ref_counts, src, dst)
+    N.done(N.torch_ext().paged_cache_fork(page_table, seq_lens, ref_counts, src, dst))
 
 
 @_fork_op.register_fake
@@ -189,7 +186,7 @@ def _(page_table, seq_lens, ref_counts, src, dst):
 
 @torch.library.custom_op("nanochat_amd::paged_cache_free", mutates_args=_STATE)
 def _free_op(page_table: Tensor, seq_lens: Tensor, ref_counts: Tensor, slots: Tensor) -> None:
-    N.torch_ext().paged_cache_free(page_table, seq_lens, ref_counts, slots)
+    N.done(N.torch_ext().paged_cache_free(page_table, seq_lens, ref_counts, slots))
 
 
 @_free_op.register_fake
@@ -199,7 +196,7 @@ def _(page_table, seq_lens, ref_counts, slots):
 
 @torch.library.custom_op("nanochat_amd::paged_cache_copy", mutates_args=("k_pages", "v_pages"))
 def _copy_op(k_pages: Tensor, v_pages: Tensor, src: Tensor, dst: Tensor) -> None:
-    N.torch_ext().paged_cache_copy(k_pages, v_pages, src, dst)
+    N.done(N.torch_ext().paged_cache_copy(k_pages, v_pages, src, dst))
 
 
 @_copy_op.register_fake
@@ -211,7 +208,7 @@ def _(k_pages, v_pages, src, dst):
                          mutates_args=("page_table", "ref_counts", "k_pages", "v_pages"))
 def _compact_op(page_table: Tensor, ref_counts: Tensor, k_pages: Tensor,
                 v_pages: Tensor) -> Tensor:
-    return N.torch_ext().paged_cache_compact(page_table, ref_counts, k_pages, v_pages)
+    return N.done(N.torch_ext().paged_cache_compact(page_table, ref_counts, k_pages, v_pages))
 
 
 @_compact_op.register_fake

@@ -37,22 +37,23 @@ def token_logprobs(logits: Tensor, targets: Tensor, *, top_k: int = 0,
     cap = 0.0 if softcap is None else float(softcap)
     if softcap is not None and not cap > 0.0:
         raise ValueError(f"softcap must be positive and finite, got {softcap}")
-    if torch.compiler.is_compiling():
-        lp, ent, top, ids, _ = _logprobs_op(logits, targets, top_k, cap)
-    else:
-        lp, ent, top, ids = N.torch_ext().token_logprobs(logits, targets, top_k, cap)
+    got = None if torch.compiler.is_compiling() else N.torch_ext().token_logprobs(
+        logits, targets, top_k, cap)
+    if got is None:  # (as the cache's functions)
+        got = _logprobs_op(logits, targets, top_k, cap)[:4]
+    lp, ent, top, ids = got
     if top_k == 0:
         return TokenLogprobs(lp, ent, None, None)
     return TokenLogprobs(lp, ent, top, ids)
 
 
 # ---------------------------------------------------------------------------
-# library ops (torch.compile)
+# library ops (torch.compile, tracing, modes, transforms)
 # ---------------------------------------------------------------------------
 @torch.library.custom_op("nanochat_amd::token_logprobs", mutates_args=())
 def _logprobs_op(logits: Tensor, targets: Tensor, top_k: int,
                  softcap: float) -> Tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
-    return N.torch_ext().token_logprobs_forward(logits, targets, top_k, softcap)
+    return N.done(N.torch_ext().token_logprobs_forward(logits, targets, top_k, softcap))
 
 
 @_logprobs_op.register_fake
@@ -68,8 +69,8 @@ def _logprobs_backward_op(logits: Tensor, targets: Tensor, lse: Tensor, entropy:
                           top_ids: Tensor, g_logprobs: Optional[Tensor],
                           g_entropy: Optional[Tensor], g_top: Optional[Tensor],
                           softcap: float) -> Tensor:
-    return N.torch_ext().token_logprobs_backward(logits, targets, lse, entropy, top_ids,
-                                                 g_logprobs, g_entropy, g_top, softcap)
+    return N.done(N.torch_ext().token_logprobs_backward(logits, targets, lse, entropy, top_ids,
+                                                        g_logprobs, g_entropy, g_top, softcap))
 
 
 @_logprobs_backward_op.register_fake
