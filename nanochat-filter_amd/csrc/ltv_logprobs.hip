@@ -677,19 +677,33 @@ extern "C" int ltv_token_logprobs_forward(int dtype, const void* logits, int64_t
   uint64_t* keys = reinterpret_cast<uint64_t*>(workspace);
   // (a multiple of 64 elements: pieces of an aligned row are aligned)
   const int piece = ((V + pieces - 1) / pieces + 63) / 64 * 64;
-  const LogpArgs a{logits, row_stride, targets, logprobs, entropy, lse, top_logprobs, top_ids,
+  LogpArgs a{logits, row_stride, targets, logprobs, entropy, lse, top_logprobs, top_ids,
                    V, top_k, softcap, piece, (V + piece - 1) / piece,
                    reinterpret_cast<float*>(keys + N * pieces * top_k), keys};
   const hipStream_t st = (hipStream_t)stream;
-  const dim3 grid((unsigned)N, a.pieces);
+  // (a launch has less than 2^32 threads along an axis; so many rows are not cut)
+  constexpr int64_t kMostRows = int64_t(1) << 23;
   auto launch = [&](auto type, auto cap) -> int {
     using T = decltype(type);
     constexpr Cap C = decltype(cap)::value;
-    if (top_k > 0)
-      hipLaunchKernelGGL((logprobs_forward_kernel<T, C, true>), grid, dim3(kThreads), 0, st, a);
-    else
-      hipLaunchKernelGGL((logprobs_forward_kernel<T, C, false>), grid, dim3(kThreads), 0, st, a);
-    LTV_LAUNCH_CHECK();
+    for (int64_t n0 = 0; n0 < N; n0 += kMostRows) {
+      const int64_t m = std::min(kMostRows, N - n0);
+      const dim3 grid((unsigned)m, a.pieces);
+      if (top_k > 0)
+        hipLaunchKernelGGL((logprobs_forward_kernel<T, C, true>), grid, dim3(kThreads), 0, st, a);
+      else
+        hipLaunchKernelGGL((logprobs_forward_kernel<T, C, false>), grid, dim3(kThreads), 0, st,
+                           a);
+      LTV_LAUNCH_CHECK();
+      if (n0 + m == N) break;
+      a.x = (const T*)a.x + m * row_stride;
+      a.targets += m;
+      a.logprobs += m;
+      a.entropy = a.entropy ? a.entropy + m : nullptr;
+      a.lse = a.lse ? a.lse + m : nullptr;
+      a.top_lp = a.top_lp ? a.top_lp + m * top_k : nullptr;
+      a.top_ids = a.top_ids ? a.top_ids + m * top_k : nullptr;
+    }
     if (a.pieces > 1) {
       hipLaunchKernelGGL((logprobs_join_kernel<T, C>), dim3((unsigned)N), dim3(kJoinThreads),
                          0, st, a);
