@@ -273,7 +273,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_forward_kernel(const LogpAr
 #pragma unroll
       for (int i = 0; i < N; ++i) f(x[i], v * N + i);
     }
-    if (whole * N + tid < V) f(io_traits<T>::load(row + whole * N + tid), whole * N + tid);
+    if (tid < V - whole * N) f(io_traits<T>::load(row + whole * N + tid), whole * N + tid);
   };
 
   // collects anew, what is not below `low`
@@ -345,7 +345,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_forward_kernel(const LogpAr
     for (int j = 0; j < kAhead; ++j)
       if (v + j * kThreads < whole) take(q[j], v + j * kThreads);
   }
-  if (whole * N + tid < V) {
+  if (tid < V - whole * N) {
     const float x[1] = {io_traits<T>::load(row + whole * N + tid)};
     sums.add(x, p.cap);
     if (TOP && !(x[0] <= bound)) collect(x[0], whole * N + tid);
@@ -616,7 +616,7 @@ __global__ void __launch_bounds__(kGradThreads) logprobs_backward_kernel(const L
         __builtin_memcpy(gx + begin + (int64_t)(v + j * kGradThreads) * N, &o, 16);
       }
   }
-  if (begin + whole * N + tid < end) {
+  if (tid < end - begin - whole * N) {
     const int j = begin + whole * N + tid;
     io_traits<T>::store(gx + j, grad(io_traits<T>::load(x + j), 0.0f));
   }
@@ -676,9 +676,10 @@ extern "C" int ltv_token_logprobs_forward(int dtype, const void* logits, int64_t
               LTV_ERR_WORKSPACE, "workspace too small");
   uint64_t* keys = reinterpret_cast<uint64_t*>(workspace);
   // (a multiple of 64 elements: pieces of an aligned row are aligned)
-  const int piece = ((V + pieces - 1) / pieces + 63) / 64 * 64;
+  const int piece =
+      (int)std::min<int64_t>((((int64_t)V + pieces - 1) / pieces + 63) / 64 * 64, V);
   LogpArgs a{logits, row_stride, targets, logprobs, entropy, lse, top_logprobs, top_ids,
-                   V, top_k, softcap, piece, (V + piece - 1) / piece,
+                   V, top_k, softcap, piece, (int)(((int64_t)V + piece - 1) / piece),
                    reinterpret_cast<float*>(keys + N * pieces * top_k), keys};
   const hipStream_t st = (hipStream_t)stream;
   // (a launch has less than 2^32 threads along an axis; so many rows are not cut)
@@ -732,13 +733,14 @@ extern "C" int ltv_token_logprobs_backward(int dtype, const void* logits, int64_
               LTV_ERR_INVALID_ARG, "null pointer");
   // rows are cut into pieces, of 4,096 elements at least, until there are 4,096 of them
   const int64_t want = std::max<int64_t>(1, (4096 + N - 1) / N);
-  const int piece = (int)std::max<int64_t>(4096, ((V + want - 1) / want + 4095) / 4096 * 4096);
+  const int piece = (int)std::min<int64_t>(
+      std::max<int64_t>(4096, ((V + want - 1) / want + 4095) / 4096 * 4096), 1 << 30);
   LogpGradArgs a{logits, row_stride, targets, lse, entropy, top_ids, g_logprobs, g_entropy,
                  g_top, grad_logits, grad_row_stride, V, top_k, softcap, piece};
   const hipStream_t st = (hipStream_t)stream;
   // (the grid's second axis ends at 65,535)
   for (int64_t n0 = 0; n0 < N; n0 += 65535) {
-    const dim3 grid((unsigned)((V + piece - 1) / piece), (unsigned)std::min<int64_t>(65535, N - n0));
+    const dim3 grid((unsigned)(((int64_t)V + piece - 1) / piece), (unsigned)std::min<int64_t>(65535, N - n0));
     auto launch = [&](auto type, auto cap) {
       using T = decltype(type);
       constexpr Cap C = decltype(cap)::value;

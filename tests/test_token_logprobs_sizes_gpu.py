@@ -1,6 +1,8 @@
-"""Log probabilities of very many rows."""
+"""Log probabilities of very many rows, and of the widest one."""
 
 from __future__ import annotations
+
+import math
 
 import pytest
 import torch
@@ -56,3 +58,25 @@ def test_gradient_of_more_rows_than_a_launch_takes(N, V, k):
     # a rounding of the result, and float32's of each of its terms
     bound = 2.0 ** -8 * want.abs() + 1e-5 * size
     assert bool(((got.double() - want).abs() <= bound).all())
+
+
+def test_the_widest_row():
+    """2^31 - 1 logits: indices end where 32 bits do."""
+    V = 2 ** 31 - 1
+    at = torch.tensor([5, 2 ** 30 + 1, V - 1], device=DEV)
+    x = torch.full((1, V), -60.0, dtype=BF, device=DEV)
+    x[0, at] = torch.tensor([20.0, 19.0, 21.0], dtype=BF, device=DEV)
+    x.requires_grad_(True)
+    out = _ops().token_logprobs(x, torch.tensor([V - 1], device=DEV), top_k=4)
+    want = torch.log_softmax(torch.tensor([20.0, 19.0, 21.0], dtype=torch.float64, device=DEV), 0)
+    assert out.top_ids[0].tolist() == [V - 1, 5, 2 ** 30 + 1, 0]
+    # (the others' part is 2^31 e^-81)
+    assert abs(float(out.logprobs.detach()) - float(want[2])) <= 1e-5
+    assert float((out.top_logprobs[0, :3].double() - want[[2, 0, 1]]).abs().max()) <= 1e-5
+    (g,) = torch.autograd.grad(out.logprobs.sum(), [x])
+    exact = torch.tensor([0.0, 0.0, 1.0], device=DEV).double() - want.exp()
+    assert float((g[0, at].double() - exact).abs().max()) <= 2.0 ** -8
+    # everywhere else -e^(-60 - lse), which bfloat16 holds
+    other = math.exp(-60.0 - 21.0 + float(want[2]))
+    off = sum(int(((c.float() / -other - 1).abs() > 2.0 ** -7).sum()) for c in g[0].split(2 ** 28))
+    assert off == 3
