@@ -134,8 +134,11 @@ void check_pages(const Tensor& k, const Tensor& v, const Tensor& like) {
 
 struct Batch {
   ltv_paged_batch b{};
-  Tensor slots, starts;  // (kept until the call has been made)
+  Tensor table, slots, starts;  // (kept until the call has been made)
 };
+
+// A table whose rows lie one after the other, not in each other (an expanded row).
+bool rows_apart(const Tensor& t) { return t.size(0) <= 1 || t.stride(0) >= t.size(1); }
 
 // tok: the token tensor, (B, T, heads, D) or, with starts, (N, heads, D)
 Batch make_batch(const Tensor& tok, const char* name, const Tensor& k_pages, const Tensor& table,
@@ -146,9 +149,10 @@ Batch make_batch(const Tensor& tok, const char* name, const Tensor& k_pages, con
   int_table(lens, "seq_lens", 1, tok);
   TORCH_CHECK_VALUE(lens.size(0) == table.size(0), "page_table has ", table.size(0),
                     " rows, seq_lens ", lens.size(0));
-  r.b.page_table = table.numel() ? table.data_ptr<int32_t>() : nullptr;
+  r.table = rows_apart(table) ? table : table.contiguous();
+  r.b.page_table = table.numel() ? r.table.data_ptr<int32_t>() : nullptr;
   r.b.seq_lens = lens.numel() ? lens.data_ptr<int32_t>() : nullptr;
-  r.b.table_stride = std::max(table.stride(0), table.size(1));
+  r.b.table_stride = std::max(r.table.stride(0), table.size(1));
   r.b.num_slots = to_int(table.size(0), "the number of slots");
   r.b.table_width = to_int(table.size(1), "the page table's width");
   r.b.num_pages = to_int(k_pages.size(0), "the number of pages");
@@ -243,6 +247,7 @@ ltv_page_state make_state(const Tensor& table, const OptTensor& lens, const Tens
   TORCH_CHECK(table.is_cuda(), "LTV HIP kernels need GPU tensors, got page_table on ",
               table.device());
   int_table(table, "page_table", 2, table);
+  TORCH_CHECK_VALUE(rows_apart(table), "page_table's rows overlap, and are to be written");
   int_table(refs, "ref_counts", 1, table);
   ltv_page_state s{};
   if (lens.has_value()) {
