@@ -45,7 +45,7 @@ int ltv_serving_abi_version(void);
  * is an empty sequence.
  *
  * Limits (LTV_ERR_UNSUPPORTED past them): page_size <= 2^20, table_width * page_size
- * and total < 2^31.
+ * <= 2^31 - 1024, total < 2^31.
  * ---------------------------------------------------------------------- */
 typedef struct ltv_paged_batch {
   const int32_t* page_table;

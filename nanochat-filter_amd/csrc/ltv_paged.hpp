@@ -73,6 +73,9 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedBatch& p, int b) {
   return s;
 }
 
+// Of a sequence: the kernels' positions run past its end by some tiles of keys, in 31 bits.
+constexpr int64_t kMostTokens = (int64_t(1) << 31) - 1024;
+
 // Checks shared by the entry points that take a batch.
 inline int check_batch(const ltv_paged_batch* b) {
   LTV_REQUIRE(b != nullptr, LTV_ERR_INVALID_ARG, "null batch");
@@ -84,7 +87,7 @@ inline int check_batch(const ltv_paged_batch* b) {
               b->T, b->num_slots, b->num_pages, b->table_width, (long long)b->table_stride,
               b->page_size);
   LTV_REQUIRE(b->page_size <= (1 << 20) &&
-                  (int64_t)b->table_width * b->page_size < (int64_t(1) << 31) &&
+                  (int64_t)b->table_width * b->page_size <= kMostTokens &&
                   b->total < (int64_t(1) << 31),
               LTV_ERR_UNSUPPORTED, "a sequence's tokens and a call's new tokens must fit 31 bits");
   LTV_REQUIRE(b->starts != nullptr || b->total == (int64_t)b->B * b->T, LTV_ERR_INVALID_ARG,
