@@ -95,13 +95,16 @@ int to_int(int64_t v, const char* name) {
   return (int)v;
 }
 
-// An int32 vector on like's device, contiguous (int64 ones are converted).
+// An int32 vector on like's device, contiguous (int64 ones are converted; what 32 bits do
+// not hold becomes their end, which is out of every range, and not an id that is in one).
 Tensor int_vector(const Tensor& t, const char* name, const Tensor& like) {
   on_device(t, name, like);
   TORCH_CHECK_TYPE(t.scalar_type() == at::kInt || t.scalar_type() == at::kLong, name,
                    " must be int32 or int64, got ", t.scalar_type());
   TORCH_CHECK_VALUE(t.dim() == 1, name, " must be a vector, got ", t.sizes());
-  return (t.scalar_type() == at::kInt ? t : t.to(at::kInt)).contiguous();
+  if (t.scalar_type() == at::kInt) return t.contiguous();
+  using lim = std::numeric_limits<int32_t>;
+  return t.clamp(lim::min(), lim::max()).to(at::kInt).contiguous();
 }
 
 // The cache's own tables are read, or written, where they are.

@@ -43,3 +43,32 @@ def test_expanded_page_table():
     x = c.rand(1, 2, 4, 64, dtype=torch.bfloat16)
     assert torch.equal(_ops().paged_attention(x, c.k, c.v, wide[:1], lens[:1]),
                        _ops().paged_attention(x, c.k, c.v, c.table, lens[:1]))
+
+
+def test_ids_past_32_bits():
+    """int64 slots, pages, counts and starts that 32 bits do not hold are out of range, not
+    what is left of them."""
+    ops, far = _ops(), 2 ** 32
+    c = Cache([40, 20], 2, 64, 16, torch.bfloat16, 2, spare=4, width=6)
+    refs = torch.bincount(c.table[c.table >= 0], minlength=c.P).int()
+
+    def state():
+        return [x.clone() for x in (c.table, c.lens, refs, c.k, c.v)]
+
+    def same(a):
+        return all(torch.equal(x, y) for x, y in zip(a, state()))
+
+    before, l = state(), lambda *v: torch.tensor(v, device=DEV)
+    ops.paged_cache_free(c.table, c.lens, refs, l(far, -far, far + 1))
+    ops.paged_cache_fork(c.table, c.lens, refs, l(far, 1), l(1, far))
+    ops.paged_cache_copy(c.k, c.v, l(far, 0, -far), l(1, far + 2, 3))
+    assert same(before)
+    for slots, counts in ((l(far), l(1)), (l(0), l(far + 1)), (l(0), l(-far))):
+        assert int(ops.paged_cache_reserve(c.table, c.lens, refs, slots, counts, c.k, c.v)) == -1
+    assert same(before)
+    q = c.rand(3, 4, 64, dtype=torch.bfloat16)
+    out, lse = ops.paged_attention(q, c.k, c.v, c.table, c.lens, slots=l(far, 1),
+                                   starts=l(0, 2, far + 3), return_lse=True)
+    assert bool((out[:2] == 0).all()) and bool((lse[:2] == -float("inf")).all())
+    want = ops.paged_attention(q[2:], c.k, c.v, c.table, c.lens, slots=l(1), starts=l(0, 1))
+    assert torch.equal(out[2:], want)
