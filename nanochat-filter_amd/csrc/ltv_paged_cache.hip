@@ -141,6 +141,10 @@ inline State state_of(const ltv_page_state& s) {
 }
 
 __device__ __forceinline__ bool in(int i, int n) { return i >= 0 && i < n; }
+// Pages of `len` tokens (len + page - 1 may pass 31 bits, not 32).
+__device__ __forceinline__ int pages_of(int len, int page) {
+  return (int)(((unsigned)len + (unsigned)page - 1) / (unsigned)page);
+}
 
 constexpr int kScanThreads = 1024;
 constexpr int kScanWaves = kScanThreads / 64;
@@ -265,7 +269,7 @@ __global__ void __launch_bounds__(kScanThreads) reserve_kernel(const State s,
                                         __HIP_MEMORY_SCOPE_AGENT);
         copy = r > w || (r > 1 && l != i);
       }
-      need = copy + (len + s.page - 1) / s.page - (old + s.page - 1) / s.page;
+      need = copy + pages_of(len, s.page) - pages_of(old, s.page);
     }
     int total;
     const int before = block_scan(need, lds, total);
@@ -314,7 +318,7 @@ __global__ void __launch_bounds__(kScanThreads) reserve_kernel(const State s,
         ws.src[lo] = last;
         ws.dst[lo] = p;
       } else {
-        row[(old + s.page - 1) / s.page + j - copy] = p;
+        row[pages_of(old, s.page) + j - copy] = p;
       }
       s.refs[p] = 1;
     }

@@ -72,3 +72,22 @@ def test_ids_past_32_bits():
     assert bool((out[:2] == 0).all()) and bool((lse[:2] == -float("inf")).all())
     want = ops.paged_attention(q[2:], c.k, c.v, c.table, c.lens, slots=l(1), starts=l(0, 1))
     assert torch.equal(out[2:], want)
+
+
+@pytest.mark.parametrize("page,width,counts", [(1_500_000_000, 1, [1_400_000_000, 1, 1]),
+                                               (2 ** 20, 2047, [2047 * 2 ** 20, 2 ** 20, 1]),
+                                               (2 ** 31 - 1, 1, [2 ** 31 - 1, 0, 5])])
+def test_reserve_of_very_long_sequences(page, width, counts):
+    """Lengths whose rounding up to pages passes 31 bits (of a cache without layers: the
+    bookkeeping alone)."""
+    held = [-(-n // page) for n in counts]
+    P = sum(held) + 1
+    k = torch.empty(0, P, 1, page, 1, dtype=torch.uint8, device=DEV)
+    table = torch.full((3, width), -1, dtype=torch.int32, device=DEV)
+    lens, refs = _i([0, 0, 0]), torch.zeros(P, dtype=torch.int32, device=DEV)
+    assert int(_ops().paged_cache_reserve(table, lens, refs, _i([0, 1, 2]), _i(counts), k, k)) == 0
+    assert lens.tolist() == counts and refs.tolist() == [1] * (P - 1) + [0]
+    rows, at = table.tolist(), 0
+    for row, n in zip(rows, held):
+        assert row == list(range(at, at + n)) + [-1] * (width - n)
+        at += n
