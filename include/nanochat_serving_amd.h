@@ -126,10 +126,10 @@ typedef struct ltv_page_state {
  * another slot, the new tokens may not go there: the slot gets a copy of that page
  * (first of its new pages) and lets go of the shared one; among slots of one call
  * that all hold the page and no other does, the last keeps it.
- * *status: 0; or, with nothing changed at all, how many pages are missing; or -1 for
- * a slot or count out of range or a sequence that its table row cannot hold.  Where it is
- * not 0 the new tokens must not be appended: they would overwrite the last ones of
- * seq_lens (a batch whose slots are -1 then has no sequences).
+ * *status: 0; or, with nothing changed at all, how many pages are missing (at most
+ * 2^31 - 1); or -1 for a slot or count out of range or a sequence that its table row cannot
+ * hold.  Where it is not 0 the new tokens must not be appended: they would overwrite the last
+ * ones of seq_lens (a batch whose slots are -1 then has no sequences).
  * workspace: ltv_paged_cache_reserve_workspace_size bytes, 16-byte aligned. */
 size_t ltv_paged_cache_reserve_workspace_size(int n, int num_pages);
 int ltv_paged_cache_reserve(const ltv_page_state* state, const ltv_page_blocks* blocks,

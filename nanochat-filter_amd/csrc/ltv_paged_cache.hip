@@ -150,22 +150,23 @@ constexpr int kScanThreads = 1024;
 constexpr int kScanWaves = kScanThreads / 64;
 
 // Exclusive sum of v over the workgroup's threads, and the total.
-__device__ __forceinline__ int block_scan(int v, int* lds, int& total) {
+template <typename N>
+__device__ __forceinline__ N block_scan(N v, N* lds, N& total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int x = v;
+  N x = v;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
-    const int y = __shfl_up(x, d);
+    const N y = __shfl_up(x, d);
     if (lane >= d) x += y;
   }
   __syncthreads();  // (lds may still be read from the scan before)
   if (lane == 63) lds[wave] = x;
   __syncthreads();
-  int before = 0;
+  N before = 0;
   total = 0;
 #pragma unroll
   for (int w = 0; w < kScanWaves; ++w) {
-    const int t = lds[w];
+    const N t = lds[w];
     before += w < wave ? t : 0;
     total += t;
   }
@@ -254,7 +255,9 @@ __global__ void __launch_bounds__(kScanThreads) reserve_kernel(const State s,
   }
   __threadfence_block();
   __syncthreads();
-  int wanted = 0;  // (uniform)
+  // (what is wanted may pass 31 bits, as 3,000 times a million pages do)
+  __shared__ long long needs[kScanWaves];
+  long long wanted = 0;  // (uniform)
   for (int i0 = 0; i0 < n; i0 += kScanThreads) {
     const int i = i0 + tid;
     int need = 0, copy = 0;
@@ -271,10 +274,10 @@ __global__ void __launch_bounds__(kScanThreads) reserve_kernel(const State s,
       }
       need = copy + pages_of(len, s.page) - pages_of(old, s.page);
     }
-    int total;
-    const int before = block_scan(need, lds, total);
+    long long total;
+    const long long before = block_scan((long long)need, needs, total);
     if (i < n) {
-      ws.first[i] = wanted + before;
+      ws.first[i] = (int)(wanted + before);  // (read where there are enough)
       ws.plan[i] = copy;
     }
     wanted += total;
@@ -284,12 +287,12 @@ __global__ void __launch_bounds__(kScanThreads) reserve_kernel(const State s,
   for (int p0 = 0; p0 < s.P && free_pages < wanted; p0 += kScanThreads) {
     const int p = p0 + tid;
     int total;
-    block_scan(p < s.P && s.refs[p] == 0, lds, total);
+    block_scan((int)(p < s.P && s.refs[p] == 0), lds, total);
     free_pages += total;
   }
   if (free_pages < wanted) {
     if (tid == 0) {
-      *status = wanted - free_pages;
+      *status = (int)min(wanted - free_pages, 0x7fffffffll);
       *ws.count = 0;
     }
     return;
@@ -302,7 +305,7 @@ __global__ void __launch_bounds__(kScanThreads) reserve_kernel(const State s,
     const int p = p0 + tid;
     const bool is_free = p < s.P && s.refs[p] == 0;
     int total;
-    const int rank = rank0 + block_scan(is_free, lds, total);
+    const int rank = rank0 + block_scan((int)is_free, lds, total);
     if (is_free && rank < wanted) {
       int lo = 0, hi = n - 1;
       while (lo < hi) {

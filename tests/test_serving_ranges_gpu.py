@@ -91,3 +91,17 @@ def test_reserve_of_very_long_sequences(page, width, counts):
     for row, n in zip(rows, held):
         assert row == list(range(at, at + n)) + [-1] * (width - n)
         at += n
+
+
+def test_reserve_of_more_pages_than_31_bits_count():
+    """3,000 slots that want 2^20 pages each: missing, with nothing changed."""
+    n, width = 3000, 2 ** 20
+    k = torch.empty(0, 9, 1, 1, 8, dtype=torch.bfloat16, device=DEV)
+    table = torch.full((n, width), -1, dtype=torch.int32, device=DEV)
+    lens, refs = torch.zeros(n, dtype=torch.int32, device=DEV), _i([0] * 9)
+    slots = torch.arange(n, dtype=torch.int32, device=DEV)
+    for many, missing in ((n, 2 ** 31 - 1), (2000, 2000 * width - 9), (4, 4 * width - 9)):
+        counts = torch.full((many,), width, dtype=torch.int32, device=DEV)
+        status = _ops().paged_cache_reserve(table, lens, refs, slots[:many], counts, k, k)
+        assert int(status) == missing
+        assert int(lens.abs().sum()) == int(refs.sum()) == 0 and int(table.max()) == -1
