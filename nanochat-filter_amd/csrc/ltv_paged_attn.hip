@@ -1141,7 +1141,7 @@ extern "C" int ltv_paged_attention(int dtype, const void* q, const int64_t q_str
               LTV_ERR_INVALID_ARG, "bad heads (NH=%d NKVH=%d D=%d)", NH, NKVH, D);
   LTV_REQUIRE(D % 8 == 0 && D <= 128, LTV_ERR_UNSUPPORTED,
               "head_dim must be a multiple of 8, at most 128 (D=%d)", D);
-  LTV_REQUIRE(scale > 0.0f && scale < INFINITY, LTV_ERR_INVALID_ARG,
+  LTV_REQUIRE(scale > 0.0f && scale * kLog2e < INFINITY, LTV_ERR_INVALID_ARG,
               "scale must be positive and finite (%g)", scale);
   if (batch->B == 0 || batch->total == 0 || NH == 0) return LTV_OK;
   LTV_REQUIRE(batch->total * NH < (int64_t(1) << 30), LTV_ERR_UNSUPPORTED,

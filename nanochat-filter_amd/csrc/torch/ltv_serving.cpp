@@ -421,8 +421,10 @@ std::optional<std::tuple<Tensor, OptTensor>> attention(
                     " k/v heads do not divide q's ", NH);
   TORCH_CHECK_VALUE(D > 0 && D <= 128 && D % 8 == 0,
                     "head_dim must be a multiple of 8, at most 128, got ", D);
-  const double sc = scale.value_or(1.0 / std::sqrt((double)D));
-  TORCH_CHECK_VALUE(std::isfinite(sc) && sc > 0, "scale must be positive and finite, got ", sc);
+  // (as the kernels have it, which multiply it by log2(e))
+  const float sc = (float)scale.value_or(1.0 / std::sqrt((double)D));
+  TORCH_CHECK_VALUE(std::isfinite(sc * 1.4427f) && sc > 0,
+                    "scale must be positive and finite in float32, got ", scale.value_or(sc));
   const int most = to_int(std::min<int64_t>(max_len.value_or(table.size(1) * k_pages.size(2)),
                                             table.size(1) * k_pages.size(2)),
                           "max_len");
@@ -440,7 +442,7 @@ std::optional<std::tuple<Tensor, OptTensor>> attention(
                                v_pages.data_ptr(), vp.s, &b.b, out.data_ptr(), os.s,
                                lse.has_value() ? lse->data_ptr<float>() : nullptr,
                                ws.ptr(), ws.bytes, (int)NH, (int)NKVH,
-                               (int)D, most, (float)sc, stream_of(q)),
+                               (int)D, most, sc, stream_of(q)),
            "ltv_paged_attention");
   return std::make_tuple(out, lse);
 }
@@ -484,7 +486,8 @@ LogpOut logprobs_forward(const Tensor& logits, const Tensor& targets, int64_t to
   TORCH_CHECK_VALUE(top_k >= 0 && top_k <= 64 && top_k <= V,
                     "top_k must be 0 to 64 and no more than the vocabulary of ", V, ", got ",
                     top_k);
-  TORCH_CHECK_VALUE(std::isfinite(cap) && cap >= 0, "softcap must be positive and finite");
+  TORCH_CHECK_VALUE(std::isfinite((float)cap) && cap >= 0 && ((float)cap > 0 || cap == 0),
+                    "softcap must be positive and finite in float32, got ", cap);
   c10::OptionalDeviceGuard guard(r.x.device());
   const auto f32 = r.x.options().dtype(at::kFloat).requires_grad(false);
   const auto shape = targets.sizes().vec();

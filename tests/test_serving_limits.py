@@ -19,3 +19,8 @@ def test_a_sequence_ends_before_31_bits(lib):
     # (in range: as far as the workspace, and nothing to append without pages)
     for width, page in ((2 ** 31 - 1024, 1), (2 ** 27 - 64, 16), (2 ** 11 - 1, 2 ** 20)):
         assert both(width, page) == (4, 0), (width, page)
+
+
+def test_scale_times_log2_e_is_finite(lib):
+    assert _attention(lib, scale=3e38) == 1
+    assert _attention(lib, scale=2e38) == 4  # (as far as the workspace)

@@ -105,3 +105,15 @@ def test_reserve_of_more_pages_than_31_bits_count():
         status = _ops().paged_cache_reserve(table, lens, refs, slots[:many], counts, k, k)
         assert int(status) == missing
         assert int(lens.abs().sum()) == int(refs.sum()) == 0 and int(table.max()) == -1
+
+
+def test_numbers_that_float32_does_not_hold():
+    c = Cache([40], 2, 64, 16, torch.bfloat16, 3)
+    q = c.rand(1, 1, 4, 64, dtype=torch.bfloat16)
+    for scale in (1e-60, 1e39, 3e38, 1e300):
+        with pytest.raises(ValueError):
+            _ops().paged_attention(q, c.k, c.v, c.table, c.lens, scale=scale)
+    x, t = torch.randn(4, 50, device=DEV), torch.zeros(4, dtype=torch.int64, device=DEV)
+    for cap in (1e-60, 1e39, 1e300):
+        with pytest.raises(ValueError):
+            _ops().token_logprobs(x, t, softcap=cap)
