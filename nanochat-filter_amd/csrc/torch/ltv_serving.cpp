@@ -293,19 +293,20 @@ ltv_page_blocks make_blocks(const Tensor& k, const Tensor& v) {
     TORCH_CHECK_VALUE(t->numel() == 0 || want == t->size(d0) * t->size(d0 + 1) * t->size(d0 + 2),
                       "each page must be a dense block of memory");
   }
-  TORCH_CHECK_VALUE(k.numel() == 0 ||
-                        (k.stride(d0) == v.stride(d0) && k.stride(d0 + 1) == v.stride(d0 + 1) &&
-                         k.stride(d0 + 2) == v.stride(d0 + 2)),
-                    "k_pages and v_pages must be laid out alike");
+  // (an axis of one element has no stride to speak of)
+  for (int d = d0; d < d0 + 3; ++d)
+    TORCH_CHECK_VALUE(k.numel() == 0 || k.size(d) == 1 || k.stride(d) == v.stride(d),
+                      "k_pages and v_pages must be laid out alike");
   const int64_t es = k.element_size();
+  auto bytes = [es](const Tensor& t, int d) { return t.size(d) == 1 ? 0 : t.stride(d) * es; };
   ltv_page_blocks b{};
   b.k = k.data_ptr();
   b.v = v.data_ptr();
-  b.k_page_bytes = k.stride(d0 - 1) * es;
-  b.v_page_bytes = v.stride(d0 - 1) * es;
+  b.k_page_bytes = bytes(k, d0 - 1);
+  b.v_page_bytes = bytes(v, d0 - 1);
   b.layers = k.dim() == 5 ? to_int(k.size(0), "the number of layers") : 1;
-  b.k_layer_bytes = k.dim() == 5 ? k.stride(0) * es : 0;
-  b.v_layer_bytes = v.dim() == 5 ? v.stride(0) * es : 0;
+  b.k_layer_bytes = k.dim() == 5 ? bytes(k, 0) : 0;
+  b.v_layer_bytes = v.dim() == 5 ? bytes(v, 0) : 0;
   b.block_bytes = k.size(d0) * k.size(d0 + 1) * k.size(d0 + 2) * es;
   b.num_pages = to_int(k.size(d0 - 1), "the number of pages");
   return b;

@@ -117,3 +117,23 @@ def test_numbers_that_float32_does_not_hold():
     for cap in (1e-60, 1e39, 1e300):
         with pytest.raises(ValueError):
             _ops().token_logprobs(x, t, softcap=cap)
+
+
+def test_strides_of_axes_of_one_element():
+    """Pages that are laid out alike but for strides that say nothing."""
+    g = torch.Generator(DEV).manual_seed(4)
+    k = torch.randn(3, 10, 1, 16, 8, generator=g, device=DEV)
+    v = torch.randn(3, 10, 16, 1, 8, generator=g, device=DEV).transpose(2, 3)
+    assert k.stride(2) != v.stride(2)
+    for a, b in ((k, v), (k[0], v[0])):
+        wk, wv = a.clone(), b.clone()
+        wk[..., 7, :, :, :], wv[..., 7, :, :, :] = wk[..., 2, :, :, :], wv[..., 2, :, :, :]
+        _ops().paged_cache_copy(a, b, _i([2]), _i([7]))
+        assert torch.equal(a, wk) and torch.equal(b, wv)
+    # one page, one layer
+    odd = torch.randn(2 * 16 * 8 + 1, generator=g, device=DEV)
+    one = odd[:128].as_strided((1, 1, 1, 16, 8), (129, 129, 128, 8, 1))
+    table, lens, refs = _i([[-1]]), _i([0]), _i([0])
+    assert int(_ops().paged_cache_reserve(table, lens, refs, _i([0]), _i([3]), one, one)) == 0
+    assert table.tolist() == [[0]] and refs.tolist() == [1]
+    assert int(_ops().paged_cache_compact(table, refs, one, one)) == 1
