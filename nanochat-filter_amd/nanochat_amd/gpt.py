@@ -173,6 +173,9 @@ class GPT(nn.Module):
         """The final hidden states (B, T, C) of a step's new tokens idx (B, T)
         (``PagedKVCache.step``), given what the cache holds of their sequences."""
         T = idx.size(1)
+        longest = max(step.positions) + T
+        if longest > self.cos.size(1):  # (indexed on the device, where it would be a fault)
+            raise ValueError(f"{longest} tokens, but the model is made for {self.cos.size(1)}")
         at = torch.tensor(step.positions, device=idx.device)[:, None] + torch.arange(
             T, device=idx.device)
         cos_sin = self.cos[0][at], self.sin[0][at]

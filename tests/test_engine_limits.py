@@ -1,0 +1,23 @@
+"""CPU checks of what the GPT harness refuses before anything reaches the device."""
+
+from __future__ import annotations
+
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+
+@pytest.fixture(scope="module")
+def model():
+    from nanochat_amd.gpt import GPT, GPTConfig
+    return GPT(GPTConfig(sequence_len=64, vocab_size=50, n_layer=1, n_head=2, n_kv_head=1,
+                         n_embd=32, ltv_r=16))
+
+
+@pytest.mark.parametrize("positions,T", [([64], 1), ([0, 60], 5), ([0], 65)])
+def test_positions_past_the_rotary_table(model, positions, T):
+    """A cache may have room for more tokens than the model."""
+    step = SimpleNamespace(positions=positions)
+    with pytest.raises(ValueError, match="made for 64"):
+        model.cached_features(torch.zeros(len(positions), T, dtype=torch.int64), step)
