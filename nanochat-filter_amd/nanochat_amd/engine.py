@@ -35,6 +35,15 @@ def _autocast():
     return torch.autocast(device_type="cuda", dtype=torch.bfloat16)
 
 
+def _indices(model: GPT, tokens: Sequence[int], device) -> torch.Tensor:
+    """The tokens on the device, where one outside the vocabulary would be a fault."""
+    idx = torch.as_tensor(tokens, device="cpu")
+    if not 0 <= int(idx.min()) <= int(idx.max()) < model.config.vocab_size:
+        raise ValueError(f"tokens are 0 to {model.config.vocab_size - 1}, got {int(idx.min())} "
+                         f"to {int(idx.max())}")
+    return idx.to(device)
+
+
 @torch.no_grad()
 def prefill(model: GPT, cache: PagedKVCache, slot: int, tokens: Sequence[int],
             chunk: int = 2048) -> torch.Tensor:
@@ -42,7 +51,7 @@ def prefill(model: GPT, cache: PagedKVCache, slot: int, tokens: Sequence[int],
     its last token, (1, vocabulary), before the cap."""
     if not len(tokens):
         raise ValueError("an empty prompt")
-    idx = torch.tensor(tokens, device=cache.page_table.device)[None]
+    idx = _indices(model, tokens, cache.page_table.device)[None]
     with _autocast():
         for x in idx.split(chunk, dim=1):
             hidden = model.cached_features(x, cache.step([slot], x.size(1)))
@@ -111,7 +120,7 @@ def score(model: GPT, tokens: Sequence[int], *, top_k: int = 0,
         raise ValueError("at least two tokens")
     if cache is None:
         cache = make_cache(model, -(-len(tokens) // 64), slot + 1)
-    idx = torch.tensor(tokens, device=cache.page_table.device)
+    idx = _indices(model, tokens, cache.page_table.device)
     parts = []
     with _autocast():
         for x, y in zip(idx[:-1].split(chunk), idx[1:].split(chunk)):

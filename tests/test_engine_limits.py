@@ -21,3 +21,15 @@ def test_positions_past_the_rotary_table(model, positions, T):
     step = SimpleNamespace(positions=positions)
     with pytest.raises(ValueError, match="made for 64"):
         model.cached_features(torch.zeros(len(positions), T, dtype=torch.int64), step)
+
+
+@pytest.mark.parametrize("tokens", [[3, 50], [-1, 3], [2 ** 40, 1]])
+def test_tokens_outside_the_vocabulary(model, tokens):
+    from nanochat_amd import engine
+
+    cache = engine.make_cache(model, num_pages=4, max_seqs=2, page_size=16)
+    for call in (lambda: engine.prefill(model, cache, 0, tokens),
+                 lambda: engine.generate(model, tokens, 1, 3, cache=cache),
+                 lambda: engine.score(model, tokens, cache=cache)):
+        with pytest.raises(ValueError, match="tokens are 0 to 49"):
+            call()
