@@ -10,6 +10,7 @@ pass over the logits.
 
 from __future__ import annotations
 
+import contextlib
 from typing import NamedTuple, Optional, Sequence
 
 import torch
@@ -44,15 +45,36 @@ def _indices(model: GPT, tokens: Sequence[int], device) -> torch.Tensor:
     return idx.to(device)
 
 
+def _empty(cache: PagedKVCache, slots: Sequence[int]) -> None:
+    for s in slots:
+        if not 0 <= s < len(cache.lens):
+            raise ValueError(f"slots are 0 to {len(cache.lens) - 1}, got {s}")
+        if cache.lens[s]:
+            raise ValueError(f"slot {s} holds {cache.lens[s]} tokens of another sequence")
+
+
+@contextlib.contextmanager
+def _freed_on_error(cache: PagedKVCache, slots: Sequence[int]):
+    """Empties the slots, which were empty before, if what is done with them fails."""
+    try:
+        yield
+    except BaseException:
+        taken = [s for s in slots if cache.lens[s]]
+        if taken:
+            cache.free(taken)
+        raise
+
+
 @torch.no_grad()
 def prefill(model: GPT, cache: PagedKVCache, slot: int, tokens: Sequence[int],
             chunk: int = 2048) -> torch.Tensor:
     """Feeds the prompt into an empty slot, ``chunk`` tokens at a time; the logits after
-    its last token, (1, vocabulary), before the cap."""
+    its last token, (1, vocabulary), before the cap.  The slot is empty again if that fails."""
     if not len(tokens):
         raise ValueError("an empty prompt")
+    _empty(cache, [slot])
     idx = _indices(model, tokens, cache.page_table.device)[None]
-    with _autocast():
+    with _freed_on_error(cache, [slot]), _autocast():
         for x in idx.split(chunk, dim=1):
             hidden = model.cached_features(x, cache.step([slot], x.size(1)))
         return model.raw_logits(hidden[:, -1])
@@ -65,14 +87,31 @@ def generate(model: GPT, prompt: Sequence[int], num_samples: int, max_tokens: in
              chunk: int = 2048) -> list[Sample]:
     """``num_samples`` continuations of the prompt, sampled among the ``top_k`` most
     probable tokens (``temperature`` 0: the most probable).  The log probabilities are
-    the model's own, of the whole vocabulary."""
+    the model's own, of the whole vocabulary.  A given cache's slots 0 to
+    ``num_samples`` - 1 are used, which are empty before and after."""
     if num_samples <= 0 or max_tokens <= 0 or temperature < 0:
         raise ValueError("at least one sample of one token, and no negative temperature")
+    most = min(64, model.config.vocab_size)
+    if not 0 < top_k <= most:
+        raise ValueError(f"top_k must be 1 to {most}, got {top_k}")
+    longest = len(prompt) + max_tokens - 1  # (the last token is not fed)
+    if stop is None and longest > min(model.config.sequence_len, cache.max_len if cache else longest):
+        raise ValueError(f"{longest} tokens, more than the model or the cache is made for")
     n = num_samples
     if cache is None:
         page = 64
         shared, own = -(-len(prompt) // page), -(-max_tokens // page) + 1
         cache = make_cache(model, shared + n * own, n, page)
+    _empty(cache, range(n))
+    with _freed_on_error(cache, range(n)):
+        out = _sample(model, prompt, n, max_tokens, top_k, temperature, stop, seed, cache, chunk)
+    cache.compact()
+    return out
+
+
+def _sample(model: GPT, prompt: Sequence[int], n: int, max_tokens: int, top_k: int,
+            temperature: float, stop: Optional[int], seed: int, cache: PagedKVCache,
+            chunk: int) -> list[Sample]:
     device = cache.page_table.device
     g = torch.Generator(device=device).manual_seed(seed)
     logits = prefill(model, cache, 0, prompt, chunk).expand(n, -1)
@@ -106,7 +145,6 @@ def generate(model: GPT, prompt: Sequence[int], num_samples: int, max_tokens: in
             hidden = model.cached_features(tokens[torch.tensor(going, device=device)],
                                            cache.step(live, 1))
             logits = model.raw_logits(hidden[:, -1])
-    cache.compact()
     return out
 
 
@@ -120,9 +158,10 @@ def score(model: GPT, tokens: Sequence[int], *, top_k: int = 0,
         raise ValueError("at least two tokens")
     if cache is None:
         cache = make_cache(model, -(-len(tokens) // 64), slot + 1)
+    _empty(cache, [slot])
     idx = _indices(model, tokens, cache.page_table.device)
     parts = []
-    with _autocast():
+    with _freed_on_error(cache, [slot]), _autocast():
         for x, y in zip(idx[:-1].split(chunk), idx[1:].split(chunk)):
             hidden = model.cached_features(x[None], cache.step([slot], len(x)))
             parts.append(token_logprobs(model.raw_logits(hidden[0]), y, top_k=top_k,

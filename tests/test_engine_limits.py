@@ -33,3 +33,15 @@ def test_tokens_outside_the_vocabulary(model, tokens):
                  lambda: engine.score(model, tokens, cache=cache)):
         with pytest.raises(ValueError, match="tokens are 0 to 49"):
             call()
+
+
+@pytest.mark.parametrize("kw", [dict(top_k=0), dict(top_k=51), dict(top_k=-3),
+                                dict(max_tokens=63), dict(num_samples=3)])
+def test_generate_refuses_before_it_begins(model, kw):
+    """top_k outside the vocabulary, more tokens than there is room for, too few slots."""
+    from nanochat_amd import engine
+
+    cache = engine.make_cache(model, num_pages=4, max_seqs=2, page_size=16)
+    args = dict(num_samples=2, max_tokens=3, top_k=5, cache=cache) | kw
+    with pytest.raises(ValueError):
+        engine.generate(model, [1, 2, 3], **args)
