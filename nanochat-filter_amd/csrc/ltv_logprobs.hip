@@ -562,8 +562,8 @@ struct Grad {
       slope = fmaf(-t, t, 1.0f);
     }
     const float lp = z - lse, e = __builtin_amdgcn_exp2f(lp * kLog2e);
-    // (an entry without probability has none, however low its log)
-    const float d = -e * fmaf(ge, fmaxf(lp, -1e30f) + ent, total);
+    // (an entry without probability has none, however low its log and large the gradient)
+    const float d = -e * fmaf(ge, fmaxf(lp, -1000.0f) + ent, total);
     return (d + extra) * slope;
   }
 };

@@ -137,3 +137,18 @@ def test_strides_of_axes_of_one_element():
     assert int(_ops().paged_cache_reserve(table, lens, refs, _i([0]), _i([3]), one, one)) == 0
     assert table.tolist() == [[0]] and refs.tolist() == [1]
     assert int(_ops().paged_cache_compact(table, refs, one, one)) == 1
+
+
+@pytest.mark.parametrize("scale", [1.0, 2.0 ** 24, 1e12, 1e30])
+def test_gradient_of_a_scaled_entropy(scale):
+    """A loss scaled up: masked entries keep a gradient of 0."""
+    g = torch.Generator(DEV).manual_seed(5)
+    x = torch.randn(3, 300, generator=g, device=DEV)
+    x[0, ::2], x[1, ::3] = -float("inf"), torch.finfo(torch.float32).min
+    x.requires_grad_(True)
+    t = torch.ones(3, dtype=torch.int64, device=DEV)
+    (one,) = torch.autograd.grad(_ops().token_logprobs(x, t).entropy.sum(), [x])
+    (got,) = torch.autograd.grad((_ops().token_logprobs(x, t).entropy * scale).sum(), [x])
+    assert bool(got.isfinite().all())
+    assert bool((got[0, ::2] == 0).all()) and bool((got[1, ::3] == 0).all())
+    assert float((got / scale - one).abs().max()) <= 2.0 ** -20
