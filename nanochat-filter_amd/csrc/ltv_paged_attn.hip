@@ -66,6 +66,7 @@ struct AttnArgs {
   uint32_t kp, ks, vp, vs;    // 16-byte units from page to page and row to row
   int NH, NKVH, D, g;
   int q_aligned;
+  int all_rests;              // of probabilities
   int scalar_pages;           // load_full: pages are multiples of 16 rows
   float scale;                // with log2(e)
   int log_group, ranges;      // log2 of the workgroups side by side, and how many such groups
@@ -783,12 +784,16 @@ __global__ void __launch_bounds__((AttnShape<T, FEW>::kThreads), FEW ? 1 : 2)
               prob(e / 2, i + 1);
               return cvt_pk_bf16(sc[e / 2][i], sc[e / 2][i + 1]);
             };
-            // A probability is rounded to bfloat16 for the product, by 2^-8 of it at most.  Of
-            // 16 keys with one that weighs more than about a 32nd of its row so far, the rest
-            // is multiplied too; below that, the errors of a row's many terms average out far
-            // under the output's own rounding.
-            uint32_t fine = 0;
-            if (__any(__builtin_amdgcn_exp2f(top - base) * 16.0f > l)) {
+            // A probability is rounded to bfloat16 for the product, by 2^-8 of it at most, and
+            // what is left of it is multiplied too: the outputs then are off by their own
+            // rounding only.  Where the products bound a call (plan_shape) that is done for 16
+            // keys with one that weighs more than about a 32nd of its row so far; of the
+            // others' errors, each as large as the output's rounding beside its own term, part
+            // stays: 12,289 tokens over 32,289 have a relative error (of the whole output, of
+            // values around 0) of 0.00193 in place of 0.00166, and take 1,157 us in place of
+            // 1,427.
+            uint32_t fine = a.all_rests ? (1u << N) - 1 : 0;
+            if (!a.all_rests && __any(__builtin_amdgcn_exp2f(top - base) * 16.0f > l)) {
 #pragma unroll
               for (int e = 0; e < N; ++e)
                 if (__any(__builtin_amdgcn_exp2f(fmaf(part_top[e], a.scale, -base)) * 16.0f > l))
@@ -1042,7 +1047,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a, int ro
 struct AttnPlan {
   bool few;
   int log_rows, group, ranges, least, unit, group_tokens, slope, extra, part_tile;
-  bool joins;
+  bool joins, all_rests;
   int64_t part_rows;
   size_t bytes, cuts_at;
 };
@@ -1088,6 +1093,12 @@ AttnPlan plan_shape(const ltv_paged_batch& b, int NH, int NKVH, int D, int max_l
   // us, float32 chunks 50 and 48, a ragged decode step 282 and 261; a small one 17.6 and, with
   // one block, 18.4.  Two, four and eight for 256 sequences of up to 2,000 tokens 222, 219, 224.)
   p.extra = (FEW || rows > 32 || most > 8 * Shape::kGrid ? 4 : 0) >> p.unit;
+  // Up to 10^11 operations, by the hints, the products of all probabilities' rests cost next to
+  // nothing: 64 sequences of 8,000 tokens (4 heads) 183 us without most of them and 185 with all,
+  // 128 of up to 2,000 (8 heads) 108 and 111, 64 of 8,000 with 64 channels (8 heads) 213 and 222,
+  // 1,024 new tokens over 8,000 (6 heads) 68.6 and 67.5.  Beyond, 2,048 over 16,000 take 178 and
+  // 183, 4,096 over 32,000 518 and 618.
+  p.all_rests = 4.0 * D * NH * (double)b.total * std::max(max_len, 1) <= 1e11;
   const int64_t n = (int64_t)p.ranges * p.group;
   p.part_rows = n * 2 * p.part_tile;
   p.cuts_at = (size_t)p.part_rows * (D + 2) * sizeof(float);
@@ -1177,7 +1188,7 @@ extern "C" int ltv_paged_attention(int dtype, const void* q, const int64_t q_str
              (char*)out, lse, (float*)workspace, {}, {}, k_page_strides[1] * es,
              v_page_strides[1] * es, (uint32_t)(k_page_strides[0] / chunk),
              (uint32_t)(k_page_strides[2] / chunk), (uint32_t)(v_page_strides[0] / chunk),
-             (uint32_t)(v_page_strides[2] / chunk), NH, NKVH, D, NH / NKVH, q_aligned ? 1 : 0,
+             (uint32_t)(v_page_strides[2] / chunk), NH, NKVH, D, NH / NKVH, q_aligned ? 1 : 0, p.all_rests ? 1 : 0,
              rows_fit && batch->page_size % 16 == 0,
              scale * kLog2e, p.group == 4 ? 2 : p.group - 1, p.ranges, p.least, p.unit,
              p.group_tokens, p.slope, p.extra, p.log_rows, p.part_tile, PageDiv(NH / NKVH),
