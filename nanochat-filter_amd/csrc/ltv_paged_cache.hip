@@ -192,6 +192,10 @@ inline size_t reserve_ws_ints(int n, int P) { return 4 * (size_t)n + 2 * (size_t
 // reference counts hands the free pages out.  All latency: 8 entries and 70 pages 7.8 us, 192
 // entries and 900 pages 10.4.  (Entries kept in registers and LDS, the counts read ahead: 7.1
 // and 13.5.)
+//
+// N: what the pages wanted are counted in, 64 bits where n rows of W pages pass 31 (192 entries
+// 10.8 us with them, 10.2 without).
+template <typename N>
 __global__ void __launch_bounds__(kScanThreads) reserve_kernel(const State s,
                                                                const int32_t* slots,
                                                                const int32_t* counts, int n,
@@ -255,9 +259,8 @@ __global__ void __launch_bounds__(kScanThreads) reserve_kernel(const State s,
   }
   __threadfence_block();
   __syncthreads();
-  // (what is wanted may pass 31 bits, as 3,000 times a million pages do)
-  __shared__ long long needs[kScanWaves];
-  long long wanted = 0;  // (uniform)
+  __shared__ N needs[kScanWaves];
+  N wanted = 0;  // (uniform)
   for (int i0 = 0; i0 < n; i0 += kScanThreads) {
     const int i = i0 + tid;
     int need = 0, copy = 0;
@@ -274,8 +277,8 @@ __global__ void __launch_bounds__(kScanThreads) reserve_kernel(const State s,
       }
       need = copy + pages_of(len, s.page) - pages_of(old, s.page);
     }
-    long long total;
-    const long long before = block_scan((long long)need, needs, total);
+    N total;
+    const N before = block_scan((N)need, needs, total);
     if (i < n) {
       ws.first[i] = (int)(wanted + before);  // (read where there are enough)
       ws.plan[i] = copy;
@@ -292,7 +295,7 @@ __global__ void __launch_bounds__(kScanThreads) reserve_kernel(const State s,
   }
   if (free_pages < wanted) {
     if (tid == 0) {
-      *status = (int)min(wanted - free_pages, 0x7fffffffll);
+      *status = (int)min(wanted - (N)free_pages, (N)0x7fffffff);
       *ws.count = 0;
     }
     return;
@@ -583,8 +586,9 @@ extern "C" int ltv_paged_cache_reserve(const ltv_page_state* state, const ltv_pa
   ws.last = ws.writers + s.P;
   ws.count = ws.last + s.P;
   const hipStream_t st = (hipStream_t)stream;
-  hipLaunchKernelGGL(reserve_kernel, dim3(1), dim3(kScanThreads), 0, st, s, slots, counts, n, ws,
-                     status);
+  const bool wide = (int64_t)n * ((int64_t)s.W + 1) >= (int64_t(1) << 31);
+  hipLaunchKernelGGL(wide ? reserve_kernel<long long> : reserve_kernel<int>, dim3(1),
+                     dim3(kScanThreads), 0, st, s, slots, counts, n, ws, status);
   LTV_LAUNCH_CHECK();
   if (blocks->layers > 0 && blocks->block_bytes > 0 && state->num_pages > 0) {
     hipLaunchKernelGGL(copy_kernel, dim3(copy_grid(*blocks, n)), dim3(kCopyThreads), 0, st,
