@@ -80,8 +80,9 @@ int ltv_paged_cache_append(int dtype, const void* k, const int64_t k_strides[3],
  *
  * q: strides (sequence, token, head), last stride 1, any alignment.  out: strides
  * likewise, 16-byte aligned rows.  lse: one float per (row, head), contiguous.
- * scale > 0, log2(e) scale finite.  D a multiple of 8, at most 128.  max_len: the longest sequence expected (a hint:
- * it chooses how many workgroups there are, not which keys are read).  The pages of a layer
+ * scale > 0, log2(e) scale finite.  D a multiple of 8, at most 128.  max_len: the longest
+ * sequence expected (a hint: it chooses how many workgroups there are and, past 10^11
+ * operations, how bfloat16 probabilities are rounded, not which keys are read).  The pages of a layer
  * lie within 32 GiB, with strides that are not negative; total * NH < 2^30.
  * workspace: ltv_paged_attention_workspace_size bytes, 16-byte aligned.
  * ---------------------------------------------------------------------- */

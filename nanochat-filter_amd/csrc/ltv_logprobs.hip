@@ -22,11 +22,10 @@
 // many (a large vocabulary and k) is read again with the k-th of those collected as the bound.
 // If they are too many still (the row rises along its indices) the bound is found digit by
 // digit of the keys, counted in a reading each: eight at most, two or three as a rule, and one
-// that collects.  512 such rows of 131,072 float32 take 477 us, shuffled ones 74.
-// Bounded by the reads: 4,096 rows of
-// 65,536 bfloat16 logits with five alternatives 118 us, 4.6 TB/s; 16 rows of float32 in 256
-// pieces 7 us, half of it latency.  (Keys of value and index for each of the first elements,
-// not for the largest of a thread alone: 124.)
+// that collects.  512 such rows of 131,072 float32 take 477 us, shuffled ones 74.  Bounded by
+// the reads: 4,096 rows of 65,536 bfloat16 logits with five alternatives 116 us, 4.6 TB/s; 16
+// rows of float32 in 256 pieces 7 us, half of it latency.  (Keys of value and index for each of
+// the first elements, not for the largest of a thread alone: 6 us more.)
 //
 // Backward.  Elementwise given lse; a workgroup takes a piece of a row and sets the
 // elements of the target and the alternatives again, with their own terms.  4,096 rows of

@@ -28,10 +28,10 @@
 // step with one very long context, 144 and 98 for chunks among decoding sequences, 1,500 and
 // 1,195 for the last chunk of a long prompt.)
 //
-// What bounds it.  One new token of each sequence: memory, 64 sequences of 8,000 tokens at 5.8
-// TB/s (a copy reaches 5.0, half of it writes).  Long chunks: the matrix unit and the clock
-// that it leaves, 12,289 tokens over 32,289 at 803 to 826 TFLOP/s where a plain product of two 8,192
-// x 8,192 matrices reaches 1,121.  Little work: latency, 2 us until a workgroup has found its
+// What bounds it.  One new token of each sequence: memory, 64 sequences of 8,000 tokens at 5.7
+// TB/s (a copy reaches 5.0, half of it writes).  Long chunks: the matrix unit, busy 46 % of the
+// cycles, and the vector unit, issuing in 51 %, in turn: 12,289 tokens over 32,289 at 803 to 853
+// TFLOP/s where a plain product of two 8,192 x 8,192 matrices reaches 1,121.  Little work: latency, 2 us until a workgroup has found its
 // range, 4 until its first tile has landed, 2 to write, 3 to join.
 #include <algorithm>
 #include <type_traits>
