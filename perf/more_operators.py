@@ -576,6 +576,13 @@ def work(case):
 _STEPS = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
 
 
+def _power(e):
+    """2^e of whole numbers -200 to 200 (a device's pow may be a rounding off)."""
+    table = torch.tensor([math.ldexp(1.0, n) for n in range(-200, 201)], dtype=torch.float64,
+                         device=e.device)
+    return table[e.long() + 200]
+
+
 def _held4(x):
     """What 4-bit pages hold of x (..., D), float64."""
     shape = x.shape
@@ -583,16 +590,16 @@ def _held4(x):
     big = x.abs().max(1, keepdim=True).values
     e = torch.floor(torch.log2(torch.where(big > 0, big, 1.0)))
     # (log2 may be a rounding off)
-    e = e + (big >= 2.0 ** (e + 1)).double() - (big < 2.0 ** e).double()
+    e = e + (big >= _power(e + 1)).double() - (big < _power(e)).double()
     e = torch.where(big > 0, e - 2, -125.0)
-    e = torch.where(big > 7.0 * 2.0 ** e, e + 1, e).clamp(-125, 125)
-    a = x.abs() * 2.0 ** -e
+    e = torch.where(big > 7.0 * _power(e), e + 1, e).clamp(-125, 125)
+    a = x.abs() * _power(-e)
     steps = torch.tensor(_STEPS, dtype=torch.float64, device=x.device)
     far = (a[..., None] - steps).abs()
     # (a tie goes to the even place)
     odd = torch.tensor([0.0, 1e-12] * 4, dtype=torch.float64, device=x.device)
     at = (far + odd).argmin(-1)
-    return (steps[at] * x.sign() * 2.0 ** e).reshape(shape)
+    return (steps[at] * x.sign() * _power(e)).reshape(shape)
 
 
 def _cached4(pages, ids, n):
@@ -605,7 +612,7 @@ def _cached4(pages, ids, n):
     steps = torch.tensor(_STEPS, dtype=torch.float64, device=pages.device)
     value = steps[nibble % 8] * (1.0 - 2.0 * (nibble // 8))
     byte = raw[..., ps * D // 2:].reshape(len(ids), NKVH, D // 32, ps).transpose(2, 3)
-    value = value * (2.0 ** (byte.double() - 127.0)).repeat_interleave(32, -1)
+    value = value * _power(byte.long() - 127).repeat_interleave(32, -1)
     return value.transpose(0, 1).flatten(1, 2)[:, :n]
 
 
