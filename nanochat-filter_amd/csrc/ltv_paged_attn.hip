@@ -37,7 +37,7 @@
 #include <type_traits>
 
 #include "ltv_gemm_dma.hpp"
-#include "ltv_paged.hpp"
+#include "ltv_paged_line.hpp"
 
 namespace ltv {
 namespace {
@@ -50,38 +50,6 @@ struct AttnShape {
   static constexpr int kGrid = FEW ? 1024 : 512;  // workgroups that the card holds
   static constexpr int kKeys = FEW || sizeof(T) == 4 ? 32 : 64;  // of a tile
 };
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
-
-struct AttnArgs {
-  PagedBatch batch;
-  const char* q;
-  const char* k;
-  const char* v;
-  char* out;
-  float* lse;
-  float* part;                // partial o, then (m, l), of the tiles that are cut
-  int64_t qs[3], os[3];       // bytes
-  int64_t kh, vh;             // bytes from head to head of the pages
-  uint32_t kp, ks, vp, vs;    // 16-byte units from page to page and row to row
-  int NH, NKVH, D, g;
-  int q_aligned;
-  int all_rests;              // of probabilities
-  int scalar_pages;           // load_full: pages are multiples of 16 rows
-  float scale;                // with log2(e)
-  int log_group, ranges;      // log2 of the workgroups side by side, and how many such groups
-  int least;                  // shortest range
-  int unit;                   // log2 of the blocks of keys in a unit of length
-  int group_tokens, slope;    // tokens of a group's row tiles; units that each is longer by
-  int extra;                  // units that a group's begin counts for
-  int log_rows;               // of a row tile
-  int part_tile;              // rows of a partial tile, 0: none is cut
-  PageDiv by_g, by_ranges;    // divisions by g and by the number of ranges
-  int64_t part_rows;
-  int* head;                  // how many ranges the call came to
-  struct Cut* cuts;
-};
-
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
@@ -170,6 +138,12 @@ __device__ __forceinline__ void barrier() {
   asm volatile("" ::: "memory");
 }
 
+__device__ __forceinline__ float across_halves_max(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false,
+                                                  false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
 // Whether any of a chunk's elements is infinite or NaN (all exponent bits set).
 __device__ __forceinline__ bool any_nonfinite(uint4 x, bf16_t) {
   bool bad = false;
@@ -187,186 +161,22 @@ __device__ __forceinline__ bool any_nonfinite(uint4 x, float) {
   return bad;
 }
 
-__device__ __forceinline__ float across_halves_max(float x) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false,
-                                                  false);
-  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-
-// The sum of x over the lanes up to each: within rows of 16 by shifts, then the rows' last.
-__device__ __forceinline__ uint32_t wave_sum_up_to(uint32_t x) {
-  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8
-  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast 15, 31
-  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
-  return x;
-}
-
-// (row numbers stay below 2^30: divisions of 64 bits would take longer than small calls)
-__device__ __forceinline__ int over(int a, int b) { return (int)((unsigned)a / (unsigned)b); }
-
-// The line.  A sequence's row tiles are taken in groups of 2^a.log_group that workgroups of
-// one XCD work on side by side, so that its L2 holds what they read for all but the first:
-// tiles of one k/v head, which read the same keys, or where it has fewer, of several heads.
-// A group is as long as the blocks of keys (of one tile in LDS) of its longest row tile, in
-// units of 2^a.unit blocks, about: c0, and slope more for each group of the head.
-struct Line {
-  int tiles, heads;  // row tiles, heads of a group
-  int groups;        // of a head
-  int rounds;        // times that many heads, all together
-  uint32_t c0, head, all;
-
-  __device__ __forceinline__ uint32_t before(const AttnArgs& a, int j) const {
-    const uint32_t k = j;  // (the product's half modulo 2^32, whatever k is)
-    return k * c0 + a.slope * (k % 2 ? (k - 1) / 2 * k : k / 2 * (k - 1));
+// Keys and values of pages in the queries' type, for rows_one_by_one.
+template <typename T>
+struct ValuePages {
+  static __device__ __forceinline__ void load(const char* p, int c, float (&x)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = io_traits<T>::load(reinterpret_cast<const T*>(p) + c * 8 + e);
   }
-  template <int KT>
-  static __device__ __forceinline__ Line of(const AttnArgs& a, int n, int len) {
-    Line u{0, 1, 0, 0, 0, 0, 0};
-    if (n <= 0) return u;
-    u.tiles = (n * a.g + (1 << a.log_rows) - 1) >> a.log_rows;
-    const int several = u.tiles == 1 ? a.log_group : u.tiles == 2 && a.log_group == 2 ? 1 : 0;
-    u.heads = 1 << several;
-    u.groups = (u.tiles + (1 << a.log_group) - 1) >> a.log_group;
-    u.rounds = (a.NKVH + u.heads - 1) >> several;
-    const int past = max(len - n, 0);
-    u.c0 = max(1, (min(len, past + min(n, a.group_tokens)) + KT - 1) / KT >> a.unit) + a.extra;
-    u.head = u.before(a, u.groups);
-    u.all = u.rounds * u.head;
-    return u;
+  static __device__ __forceinline__ void keys(const AttnArgs& a, int kvh, int page, uint32_t in,
+                                              int c, float (&x)[8]) {
+    load(a.k + kvh * a.kh + (uint64_t)((uint32_t)page * a.kp + in * a.ks) * 16, c, x);
+  }
+  static __device__ __forceinline__ void values(const AttnArgs& a, int kvh, int page, uint32_t in,
+                                                int c, float (&x)[8]) {
+    load(a.v + kvh * a.vh + (uint64_t)((uint32_t)page * a.vp + in * a.vs) * 16, c, x);
   }
 };
-
-// Keys that the last row of a row tile sees, and the block of keys at which a cut at f of
-// the tile's c units is, the first `extra` of which stand for no keys.
-__device__ __forceinline__ int keys_of(const AttnArgs& a, const PagedSeq& s, int tile) {
-  const int last = a.by_g.quot(min((tile + 1) << a.log_rows, s.n * a.g) - 1);
-  return a.batch.P > 0 && a.batch.W > 0 ? max(s.len - s.n + last + 1, 0) : 0;
-}
-__device__ __forceinline__ int cut_at(uint32_t f, uint32_t c, int blocks, uint32_t extra) {
-  if (f >= c) return blocks;
-  if (f <= extra) return 0;
-  return min(blocks, (int)fmaf((float)(f - extra),
-                               (float)blocks * __builtin_amdgcn_rcpf((float)(c - extra)), 0.5f));
-}
-
-// Where the ranges begin: `length` apart, every other one by `lead` later.
-struct Ranges {
-  uint32_t length, lead;
-  int count;
-  __device__ __forceinline__ uint32_t begin(int i) const {
-    return i * length + (i & 1 ? lead : 0);
-  }
-  __device__ __forceinline__ int of(uint32_t x) const {  // .. which x is in
-    const int i = over(x, length);
-    return min(i - ((i & 1) && x < begin(i)), count - 1);
-  }
-};
-
-// A row tile whose first cut is a workgroup's begin, for the joining kernel.
-struct Cut {
-  int rows;           // 0: none
-  int b, kvh, token;  // token: of the sequence's first, in packed rows
-  int tile, last;     // last: range with a piece of it
-  int pad[2];
-};
-
-// Rows of partials (D values each; behind them all, each row's m and l): two row tiles for
-// each workgroup, of the piece that continues a tile and of the one that begins the last.
-__device__ __forceinline__ int64_t part_at(const AttnArgs& a, int range, int member, bool begins) {
-  return ((int64_t)((range << a.log_group) + member) * 2 + begins) * a.part_tile;
-}
-__device__ __forceinline__ float2* part_ml(const AttnArgs& a) {
-  return reinterpret_cast<float2*>(a.part + a.part_rows * a.D);
-}
-
-// Rows row0 .. row_end - 1 of a workgroup over keys begin .. end - 1, each key that a row
-// does not see left alone altogether: the way of tiles with infinite or NaN values among
-// those that some rows do not see.  Groups of sixteen lanes take a row's keys in turn, a lane
-// holding eight channels.  part0: the partials of row0, or -1.
-template <typename T, int THREADS>
-__device__ __forceinline__ void rows_one_by_one(const AttnArgs& a, const PagedSeq& s, int b,
-                                                int kvh, int row0, int row_end, int begin, int end,
-                                                int64_t part0, float* lds) {
-#pragma clang fp contract(off)  // (x - base below must not be a fused form of the product)
-  float* lds_m = lds;
-  constexpr int G = THREADS / 16;
-  float* lds_l = lds + G;
-  float* lds_o = lds + 2 * G;  // G x 128
-  const int c = threadIdx.x & 15, gi = threadIdx.x >> 4;
-  const bool on = c * 8 < a.D;
-  for (int row = row0; row < row_end; ++row) {
-    const int t = a.by_g.quot(row), h = kvh * a.g + row - t * a.g;
-    const int last = min(end - 1, s.len - s.n + t);
-    const int64_t trow = a.batch.starts != nullptr ? s.row0 + t : (int64_t)b * a.batch.T + t;
-    const char* q = a.q + (a.batch.starts != nullptr ? trow * a.qs[1]
-                                                     : b * a.qs[0] + t * a.qs[1]) + h * a.qs[2];
-    float qf[8], o[8], m = -INFINITY, l = 0.0f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      qf[e] = on ? io_traits<T>::load(reinterpret_cast<const T*>(q) + c * 8 + e) : 0.0f;
-      o[e] = 0.0f;
-    }
-    for (int j = begin + gi; j <= last; j += G) {
-      const int col = a.batch.div.quot(j), page = s.table[col];
-      if (page < 0 || page >= a.batch.P) continue;
-      const uint32_t in = (uint32_t)(j - col * a.batch.div.size);
-      const T* k = reinterpret_cast<const T*>(
-          a.k + kvh * a.kh + (uint64_t)((uint32_t)page * a.kp + in * a.ks) * 16) + c * 8;
-      const T* v = reinterpret_cast<const T*>(
-          a.v + kvh * a.vh + (uint64_t)((uint32_t)page * a.vp + in * a.vs) * 16) + c * 8;
-      float x = 0.0f;
-      if (on)
-        for (int e = 0; e < 8; ++e) x = fmaf(qf[e], io_traits<T>::load(k + e), x);
-      for (int d = 1; d < 16; d <<= 1) x += __shfl_xor(x, d);
-      x *= a.scale;
-      const float mn = fmaxf(m, x), base = mn == -INFINITY ? 0.0f : mn;
-      const float was = __builtin_amdgcn_exp2f(m - base), p = __builtin_amdgcn_exp2f(x - base);
-      l = fmaf(l, was, p);
-      m = mn;
-      if (on)
-        for (int e = 0; e < 8; ++e) o[e] = fmaf(p, io_traits<T>::load(v + e), o[e] * was);
-    }
-    __syncthreads();
-    if (c == 0) {
-      lds_m[gi] = m;
-      lds_l[gi] = l;
-    }
-    for (int e = 0; e < 8; ++e) lds_o[gi * 128 + c * 8 + e] = o[e];
-    __syncthreads();
-    float mx = -INFINITY;
-    for (int i = 0; i < G; ++i) mx = fmaxf(mx, lds_m[i]);
-    const float base = mx == -INFINITY ? 0.0f : mx;
-    float sum = 0.0f, acc[128 / THREADS + 1] = {};
-    const int d0 = threadIdx.x;
-    for (int i = 0; i < G; ++i) {
-      // (a group without keys has weight 0)
-      const float w = lds_m[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(lds_m[i] - base);
-      sum = fmaf(lds_l[i], w, sum);
-#pragma unroll
-      for (int e = 0, d = d0; d < 128; ++e, d += THREADS) acc[e] = fmaf(lds_o[i * 128 + d], w, acc[e]);
-    }
-    if (part0 >= 0) {
-      const int64_t at = part0 + row - row0;
-#pragma unroll
-      for (int e = 0, d = d0; d < 128; ++e, d += THREADS)
-        if (d < a.D) a.part[at * a.D + d] = acc[e];
-      if (d0 == 0) part_ml(a)[at] = make_float2(mx, sum);
-    } else {
-      char* out = a.out + (a.batch.starts != nullptr ? trow * a.os[1]
-                                                     : b * a.os[0] + t * a.os[1]) + h * a.os[2];
-#pragma unroll
-      for (int e = 0, d = d0; d < 128; ++e, d += THREADS)
-        if (d < a.D)
-          io_traits<T>::store(reinterpret_cast<T*>(out) + d, sum == 0.0f ? 0.0f : acc[e] / sum);
-      if (d0 == 0 && a.lse != nullptr)
-        a.lse[trow * a.NH + h] = sum == 0.0f ? -INFINITY
-                                             : (mx + __builtin_amdgcn_logf(sum)) * kLn2;
-    }
-  }
-}
 
 template <typename T, int DP, bool PAD, bool FEW>
 __global__ void __launch_bounds__((AttnShape<T, FEW>::kThreads), FEW ? 1 : 2)
@@ -858,7 +668,7 @@ __global__ void __launch_bounds__((AttnShape<T, FEW>::kThreads), FEW ? 1 : 2)
     }
 
     if (__syncthreads_or(again)) {
-      rows_one_by_one<T, kAttnThreads>(a, s, b, kvh, tile * kAttnRows, min(rows, (tile + 1) * kAttnRows), begin,
+      rows_one_by_one<T, kAttnThreads, ValuePages<T>>(a, s, b, kvh, tile * kAttnRows, min(rows, (tile + 1) * kAttnRows), begin,
                          end, part0, reinterpret_cast<float*>(lds));
       return;
     }
@@ -949,108 +759,6 @@ __global__ void __launch_bounds__((AttnShape<T, FEW>::kThreads), FEW ? 1 : 2)
     }
   }
 }
-
-// Joins the pieces of the row tiles that were cut, 32 lanes to a row and four channels to a
-// lane.  Of few pieces 32 lanes take all of a row, of many the eight groups of a workgroup
-// share a row's.  It is all latency: the record of the cut, then the partials of four pieces
-// at a time.
-template <typename T>
-__global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a, int rows_each) {
-  constexpr int G = 8;  // groups
-  __shared__ float lds_o[G][128];
-  __shared__ float2 lds_ml[G];
-  const int range = blockIdx.x >> a.log_group, member = blockIdx.x & ((1 << a.log_group) - 1);
-  const Cut cut = a.cuts[blockIdx.x];
-  if (range >= *a.head) return;
-  const int first = range - 1, pieces = cut.last - first + 1;
-  const int row0 = blockIdx.y * rows_each, row_end = min(cut.rows, row0 + rows_each);
-  if (row0 >= row_end) return;
-  const bool share = pieces > (rows_each == 1 ? 4 : 16);
-  const int lane = threadIdx.x & 31, gi = threadIdx.x >> 5;
-  const bool on = lane * 4 < a.D;
-  for (int row = row0 + (share ? 0 : gi); row < row_end; row += share ? 1 : G) {
-    float m = -INFINITY, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int p0 = first + (share ? gi : 0); p0 <= cut.last; p0 += 4 * (share ? G : 1)) {
-      float2 ml[4];
-      float4 v[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int p = p0 + i * (share ? G : 1), pp = min(p, cut.last);
-        const int64_t at = part_at(a, pp, member, pp == first) + row;
-        ml[i] = part_ml(a)[at];
-        v[i] = on ? *reinterpret_cast<const float4*>(a.part + at * a.D + lane * 4)
-                  : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        // (a piece without keys has no sums; a NaN is one)
-        if (p > cut.last || ml[i].y == 0.0f) {
-          ml[i] = make_float2(-INFINITY, 0.0f);
-          v[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        }
-      }
-      float mn = m;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) mn = fmaxf(mn, ml[i].x);
-      const float base = mn == -INFINITY ? 0.0f : mn;
-      const float was = __builtin_amdgcn_exp2f(m - base);
-      m = mn;
-      l *= was;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] *= was;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float w = __builtin_amdgcn_exp2f(ml[i].x - base);
-        l = fmaf(ml[i].y, w, l);
-        o[0] = fmaf(v[i].x, w, o[0]);
-        o[1] = fmaf(v[i].y, w, o[1]);
-        o[2] = fmaf(v[i].z, w, o[2]);
-        o[3] = fmaf(v[i].w, w, o[3]);
-      }
-    }
-    if (share) {
-      __syncthreads();  // (the row before is read)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) lds_o[gi][lane * 4 + e] = o[e];
-      if (lane == 0) lds_ml[gi] = make_float2(m, l);
-      __syncthreads();
-      if (gi != 0) continue;
-#pragma unroll
-      for (int i = 0; i < G; ++i) m = fmaxf(m, lds_ml[i].x);
-      const float base = m == -INFINITY ? 0.0f : m;
-      l = o[0] = o[1] = o[2] = o[3] = 0.0f;
-#pragma unroll
-      for (int i = 0; i < G; ++i) {
-        const float w = __builtin_amdgcn_exp2f(lds_ml[i].x - base);
-        l = fmaf(lds_ml[i].y, w, l);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = fmaf(lds_o[i][lane * 4 + e], w, o[e]);
-      }
-    }
-    const int r = (cut.tile << a.log_rows) + row, t = a.by_g.quot(r), h = cut.kvh * a.g + r - t * a.g;
-    const int64_t trow = (a.batch.starts != nullptr ? cut.token : (int64_t)cut.b * a.batch.T) + t;
-    char* out = a.out + (a.batch.starts != nullptr ? trow * a.os[1]
-                                                   : cut.b * a.os[0] + t * a.os[1]) + h * a.os[2];
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    if (on) {
-      if constexpr (sizeof(T) == 2)
-        reinterpret_cast<uint2*>(out)[lane] =
-            make_uint2(cvt_pk_bf16(o[0] * inv, o[1] * inv), cvt_pk_bf16(o[2] * inv, o[3] * inv));
-      else
-        reinterpret_cast<float4*>(out)[lane] =
-            make_float4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
-    }
-    if (lane == 0 && a.lse != nullptr)
-      a.lse[trow * a.NH + h] =
-          l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
-  }
-}
-
-// How a call is cut.
-struct AttnPlan {
-  bool few;
-  int log_rows, group, ranges, least, unit, group_tokens, slope, extra, part_tile;
-  bool joins, all_rests;
-  int64_t part_rows;
-  size_t bytes, cuts_at;
-};
 
 template <typename T, bool FEW>
 AttnPlan plan_shape(const ltv_paged_batch& b, int NH, int NKVH, int D, int max_len) {

@@ -7,6 +7,7 @@
 // copies are bounded by HBM: each byte read once, written once.
 #include <algorithm>
 
+#include "../../include/nanochat_decoding_amd.h"
 #include "ltv_paged.hpp"
 
 namespace ltv {
@@ -378,6 +379,35 @@ __global__ void __launch_bounds__(256) fork_kernel(const State s, const int32_t*
   if (blockIdx.x == 0 && threadIdx.x == 0) s.lens[to] = s.lens[from];
 }
 
+// Reordering: every row that is wanted is read, and the counts follow, before one is written.
+// All latency: two launches.
+__global__ void __launch_bounds__(256) reorder_read_kernel(const State s, const int32_t* slots,
+                                                           const int32_t* src, int32_t* rows,
+                                                           int32_t* lens) {
+  const int i = blockIdx.y, from = src[i], to = slots[i];
+  if (!in(from, s.S) || !in(to, s.S)) return;
+  for (int c = blockIdx.x * 256 + threadIdx.x; c < s.W; c += gridDim.x * 256) {
+    const int page = s.table[from * s.ts + c], old = s.table[to * s.ts + c];
+    if (page != old) {
+      if (in(page, s.P)) atomicAdd(&s.refs[page], 1);
+      if (in(old, s.P)) atomicSub(&s.refs[old], 1);
+    }
+    rows[(int64_t)i * s.W + c] = page;
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) lens[i] = s.lens[from];
+}
+
+__global__ void __launch_bounds__(256) reorder_write_kernel(const State s, const int32_t* slots,
+                                                            const int32_t* src,
+                                                            const int32_t* rows,
+                                                            const int32_t* lens) {
+  const int i = blockIdx.y, from = src[i], to = slots[i];
+  if (!in(from, s.S) || !in(to, s.S)) return;
+  for (int c = blockIdx.x * 256 + threadIdx.x; c < s.W; c += gridDim.x * 256)
+    s.table[to * s.ts + c] = rows[(int64_t)i * s.W + c];
+  if (blockIdx.x == 0 && threadIdx.x == 0) s.lens[to] = lens[i];
+}
+
 __global__ void __launch_bounds__(256) free_kernel(const State s, const int32_t* slots) {
   const int slot = slots[blockIdx.y];
   if (!in(slot, s.S)) return;
@@ -622,6 +652,35 @@ extern "C" int ltv_paged_cache_free(const ltv_page_state* state, const int32_t* 
   const int blocks = std::max(1, std::min((state->table_width + 255) / 256, 64));
   hipLaunchKernelGGL(free_kernel, dim3(blocks, n), dim3(256), 0, (hipStream_t)stream,
                      state_of(*state), slots);
+  LTV_LAUNCH_CHECK();
+  return LTV_OK;
+}
+
+extern "C" size_t ltv_paged_cache_reorder_workspace_size(int n, int table_width) {
+  if (n <= 0 || table_width < 0) return 0;
+  return (size_t)n * ((size_t)table_width + 1) * sizeof(int32_t);
+}
+
+extern "C" int ltv_paged_cache_reorder(const ltv_page_state* state, const int32_t* slots,
+                                       const int32_t* src, int n, void* workspace,
+                                       size_t workspace_bytes, void* stream) {
+  LTV_TRY(check_state(state));
+  LTV_REQUIRE(n >= 0, LTV_ERR_INVALID_ARG, "bad number of entries %d", n);
+  if (n == 0 || state->num_slots == 0) return LTV_OK;
+  LTV_REQUIRE(slots && src, LTV_ERR_INVALID_ARG, "null pointer");
+  LTV_REQUIRE(n <= 65535, LTV_ERR_UNSUPPORTED, "more than 65,535 entries");
+  LTV_REQUIRE(workspace && aligned16(workspace) &&
+                  workspace_bytes >= ltv_paged_cache_reorder_workspace_size(n, state->table_width),
+              LTV_ERR_WORKSPACE, "workspace too small");
+  int32_t* lens = reinterpret_cast<int32_t*>(workspace);
+  int32_t* rows = lens + n;
+  const dim3 grid(std::max(1, std::min((state->table_width + 255) / 256, 64)), n);
+  const hipStream_t st = (hipStream_t)stream;
+  hipLaunchKernelGGL(reorder_read_kernel, grid, dim3(256), 0, st, state_of(*state), slots, src,
+                     rows, lens);
+  LTV_LAUNCH_CHECK();
+  hipLaunchKernelGGL(reorder_write_kernel, grid, dim3(256), 0, st, state_of(*state), slots, src,
+                     (const int32_t*)rows, (const int32_t*)lens);
   LTV_LAUNCH_CHECK();
   return LTV_OK;
 }

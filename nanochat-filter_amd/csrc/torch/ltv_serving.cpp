@@ -23,6 +23,7 @@
 #include <limits>
 #include <optional>
 
+#include "../../../include/nanochat_decoding_amd.h"
 #include "../../../include/nanochat_serving_amd.h"
 #include "ltv_torch.hpp"
 
@@ -115,6 +116,33 @@ void int_table(const Tensor& t, const char* name, int dim, const Tensor& like) {
                     " must have ", dim, " dimensions, the last one contiguous");
 }
 
+// Whether pages are 4-bit ones, whose elements are bytes.
+bool is_fp4(const Tensor& pages) { return pages.scalar_type() == at::kByte; }
+
+// 4-bit pages of one layer, (P, NKVH, page, D / 2 + D / 32).
+void check_fp4_pages(const Tensor& k, const Tensor& v, const Tensor& like) {
+  on_device(k, "k_pages", like);
+  on_device(v, "v_pages", like);
+  TORCH_CHECK_VALUE(k.dim() == 4 && v.sizes() == k.sizes(),
+                    "k_pages and v_pages must be (pages, kv heads, page size, bytes of a token) and "
+                    "alike, got ", k.sizes(), " and ", v.sizes());
+  TORCH_CHECK_TYPE(is_fp4(k) && is_fp4(v), "k_pages are ", k.scalar_type(), ", v_pages ",
+                   v.scalar_type());
+  const int64_t row = k.size(3);
+  TORCH_CHECK_VALUE(row % 17 == 0 && row >= 17 && row <= 68,
+                    "a token's head takes 17 bytes for each 32 of a head_dim of 32 to 128 in 4 bits, "
+                    "got ", row);
+  TORCH_CHECK_VALUE(k.size(2) > 0 && k.size(2) % 16 == 0,
+                    "a 4-bit page must hold a multiple of 16 tokens, got ", k.size(2));
+  for (const Tensor* t : {&k, &v})
+    TORCH_CHECK_VALUE(
+        t->numel() == 0 ||
+            (t->stride(3) == 1 && t->stride(2) == row && (t->size(0) == 1 || t->stride(0) % 16 == 0) &&
+             (t->size(1) == 1 || t->stride(1) % 16 == 0) &&
+             reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0),
+        "4-bit pages must be dense blocks of a page and head, 16-byte aligned");
+}
+
 // Pages of one layer, (P, NKVH, page, D).
 void check_pages(const Tensor& k, const Tensor& v, const Tensor& like) {
   on_device(k, "k_pages", like);
@@ -200,10 +228,27 @@ struct Strides3 {
                         : Strides3{{0, t.stride(0), t.stride(1)}};
   }
   static Strides3 pages(const Tensor& t) { return {{t.stride(0), t.stride(1), t.stride(2)}}; }
+  // (an axis of one element has no stride to speak of)
+  static Strides3 fp4_pages(const Tensor& t) {
+    return {{t.size(0) == 1 ? 0 : t.stride(0), t.size(1) == 1 ? 0 : t.stride(1), t.size(3)}};
+  }
 };
 
 Tensor rows_contiguous(const Tensor& t) {
   return t.numel() == 0 || t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous();
+}
+
+int64_t head_dim_of(const Tensor& pages) {
+  return is_fp4(pages) ? pages.size(3) / 17 * 32 : pages.size(3);
+}
+
+void check_any_pages(const Tensor& k, const Tensor& v, const Tensor& like) {
+  if (is_fp4(k)) check_fp4_pages(k, v, like);
+  else check_pages(k, v, like);
+}
+
+Strides3 any_strides(const Tensor& pages) {
+  return is_fp4(pages) ? Strides3::fp4_pages(pages) : Strides3::pages(pages);
 }
 
 void no_grad_needed(const Tensor& t, const char* name) {
@@ -225,23 +270,135 @@ bool append(const Tensor& k_in, const Tensor& v_in, const Tensor& k_pages, const
   on_device(v_in, "v", k_in);
   no_grad_needed(k_in, "k");
   no_grad_needed(v_in, "v");
-  check_pages(k_pages, v_pages, k_in);
+  check_any_pages(k_pages, v_pages, k_in);
   const Batch b = make_batch(k_in, "k", k_pages, table, lens, slots, starts, max_new);
   TORCH_CHECK_VALUE(v_in.sizes() == k_in.sizes(), "k is ", k_in.sizes(), ", v ", v_in.sizes());
   TORCH_CHECK_TYPE(v_in.scalar_type() == k_in.scalar_type(), "k is ", k_in.scalar_type(), ", v ",
                    v_in.scalar_type());
-  const int64_t heads = k_pages.size(1), D = k_pages.size(3);
+  const int64_t heads = k_pages.size(1), D = head_dim_of(k_pages);
   TORCH_CHECK_VALUE(k_in.size(-2) == heads && k_in.size(-1) == D, "the pages hold ", heads,
                     " heads of ", D, ", k is ", k_in.sizes());
   const Tensor k = rows_contiguous(k_in), v = rows_contiguous(v_in);
   c10::OptionalDeviceGuard guard(k.device());
   const Strides3 ks = Strides3::tokens(k), vs = Strides3::tokens(v),
-                 kp = Strides3::pages(k_pages), vp = Strides3::pages(v_pages);
+                 kp = any_strides(k_pages), vp = any_strides(v_pages);
+  if (is_fp4(k_pages)) {
+    check_rc(ltv_paged_cache_append_fp4(dt, k.data_ptr(), ks.s, v.data_ptr(), vs.s,
+                                        k_pages.data_ptr(), kp.s, v_pages.data_ptr(), vp.s, &b.b,
+                                        (int)heads, (int)D, stream_of(k)),
+             "ltv_paged_cache_append_fp4");
+    return true;
+  }
   check_rc(ltv_paged_cache_append(dt, k.data_ptr(), ks.s, v.data_ptr(), vs.s, k_pages.data_ptr(),
                                   kp.s, v_pages.data_ptr(), vp.s, &b.b, (int)heads, (int)D,
                                   stream_of(k)),
            "ltv_paged_cache_append");
   return true;
+}
+
+// (the rotated queries)
+OptTensor rotary_append(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in,
+                        const Tensor& cos_in, const Tensor& sin_in, const Tensor& k_pages,
+                        const Tensor& v_pages, const Tensor& table, const Tensor& lens,
+                        const OptTensor& slots, const OptTensor& starts, const OptInt& max_new,
+                        std::optional<double> norm_eps) {
+  no_tangent(q_in, "q");
+  no_tangent(k_in, "k");
+  no_tangent(v_in, "v");
+  no_tangent(cos_in, "cos");
+  no_tangent(sin_in, "sin");
+  if (!ordinary_call(q_in, k_in, v_in, cos_in, sin_in, k_pages, v_pages, table, lens, slots, starts))
+    return {};
+  const int dt = dtype_of(q_in, "q");
+  TORCH_CHECK(q_in.is_cuda(), "LTV HIP kernels need GPU tensors, got q on ", q_in.device());
+  const std::pair<const Tensor*, const char*> others[] = {
+      {&k_in, "k"}, {&v_in, "v"}, {&cos_in, "cos"}, {&sin_in, "sin"}};
+  for (auto [t, name] : others) on_device(*t, name, q_in);
+  no_grad_needed(q_in, "q");
+  for (auto [t, name] : others) no_grad_needed(*t, name);
+  check_any_pages(k_pages, v_pages, q_in);
+  const Batch b = make_batch(q_in, "q", k_pages, table, lens, slots, starts, max_new);
+  TORCH_CHECK_VALUE(v_in.sizes() == k_in.sizes(), "k is ", k_in.sizes(), ", v ", v_in.sizes());
+  TORCH_CHECK_TYPE(k_in.scalar_type() == q_in.scalar_type() &&
+                       v_in.scalar_type() == q_in.scalar_type(),
+                   "q is ", q_in.scalar_type(), ", k ", k_in.scalar_type(), ", v ",
+                   v_in.scalar_type());
+  const int64_t NH = q_in.size(-2), NKVH = k_pages.size(1), D = head_dim_of(k_pages);
+  TORCH_CHECK_VALUE(k_in.dim() == q_in.dim() &&
+                        k_in.sizes().slice(0, k_in.dim() - 2) ==
+                            q_in.sizes().slice(0, q_in.dim() - 2),
+                    "q and k must have the same tokens, got ", q_in.sizes(), " and ", k_in.sizes());
+  TORCH_CHECK_VALUE(k_in.size(-2) == NKVH && k_in.size(-1) == D && q_in.size(-1) == D,
+                    "the pages hold ", NKVH, " heads of ", D, ", k is ", k_in.sizes(), ", q ",
+                    q_in.sizes());
+  TORCH_CHECK_VALUE(D > 0 && D <= 128 && D % 8 == 0,
+                    "head_dim must be a multiple of 8, at most 128, got ", D);
+  const int tdt = dtype_of(cos_in, "cos");
+  TORCH_CHECK_TYPE(sin_in.scalar_type() == cos_in.scalar_type(), "cos is ", cos_in.scalar_type(),
+                   ", sin ", sin_in.scalar_type());
+  TORCH_CHECK_VALUE(cos_in.dim() == 2 && cos_in.size(1) == D / 2 && sin_in.sizes() == cos_in.sizes(),
+                    "cos and sin must be (positions, ", D / 2, "), got ", cos_in.sizes(), " and ",
+                    sin_in.sizes());
+  TORCH_CHECK_VALUE(cos_in.size(0) >= (int64_t)b.b.table_width * b.b.page_size, "cos and sin have ",
+                    cos_in.size(0), " positions, but the page table has room for ",
+                    (int64_t)b.b.table_width * b.b.page_size);
+  TORCH_CHECK_VALUE(!norm_eps.has_value() ||
+                        (*norm_eps >= 0 && std::isfinite(*norm_eps)),
+                    "norm_eps must be finite and not negative, got ",
+                    norm_eps.value_or(0));
+  const Tensor q = rows_contiguous(q_in), k = rows_contiguous(k_in), v = rows_contiguous(v_in),
+               cos = rows_contiguous(cos_in), sin = rows_contiguous(sin_in);
+  c10::OptionalDeviceGuard guard(q.device());
+  Tensor out = at::empty(q.sizes(), q.options().requires_grad(false));
+  const Strides3 qs = Strides3::tokens(q), ks = Strides3::tokens(k), vs = Strides3::tokens(v),
+                 os = Strides3::tokens(out), kp = any_strides(k_pages), vp = any_strides(v_pages);
+  check_rc(ltv_paged_rotary_append(
+               dt, q.data_ptr(), qs.s, k.data_ptr(), ks.s, v.data_ptr(), vs.s, cos.data_ptr(),
+               cos.stride(0), sin.data_ptr(), sin.stride(0), tdt, cos.size(0),
+               norm_eps.value_or(-1.0), out.data_ptr(), os.s,
+               k_pages.data_ptr(), kp.s, v_pages.data_ptr(), vp.s,
+               is_fp4(k_pages) ? LTV_PAGES_FP4 : LTV_PAGES_VALUES, &b.b, (int)NH, (int)NKVH, (int)D,
+               stream_of(q)),
+           "ltv_paged_rotary_append");
+  return out;
+}
+
+// What the pages hold of the new tokens, in dtype.
+std::optional<std::tuple<Tensor, Tensor>> read_pages(
+    const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& lens,
+    int64_t tokens, const OptTensor& slots, const OptTensor& starts, const OptInt& max_new,
+    at::ScalarType dtype) {
+  no_tangent(k_pages, "k_pages");
+  no_tangent(v_pages, "v_pages");
+  if (!ordinary_call(k_pages, v_pages, table, lens, slots, starts)) return {};
+  TORCH_CHECK(k_pages.is_cuda(), "LTV HIP kernels need GPU tensors, got k_pages on ",
+              k_pages.device());
+  if (!is_fp4(k_pages)) dtype_of(k_pages, "k_pages");
+  check_any_pages(k_pages, v_pages, k_pages);
+  TORCH_CHECK_TYPE(dtype == at::kFloat || dtype == at::kBFloat16,
+                   "LTV kernels support float32 and bfloat16 tensors, got dtype ", dtype);
+  TORCH_CHECK_TYPE(is_fp4(k_pages) || dtype == k_pages.scalar_type(), "the pages are ",
+                   k_pages.scalar_type(), ", and are read as that, got dtype ", dtype);
+  TORCH_CHECK_VALUE(tokens >= 0, "a negative number of tokens: ", tokens);
+  const int64_t NKVH = k_pages.size(1), D = head_dim_of(k_pages);
+  TORCH_CHECK_VALUE(D > 0 && D <= 128 && D % 8 == 0,
+                    "head_dim must be a multiple of 8, at most 128, got ", D);
+  c10::OptionalDeviceGuard guard(k_pages.device());
+  const auto options = k_pages.options().dtype(dtype).requires_grad(false);
+  auto shape = [&]() -> std::vector<int64_t> {
+    if (starts.has_value()) return {tokens, NKVH, D};
+    return {slots.has_value() ? slots->numel() : table.dim() > 0 ? table.size(0) : 0, tokens, NKVH, D};
+  }();
+  Tensor k = at::empty(shape, options), v = at::empty(shape, options);
+  const Batch b = make_batch(k, "the result", k_pages, table, lens, slots, starts, max_new);
+  if (k.numel() == 0) return std::make_tuple(k, v);
+  const Strides3 kp = any_strides(k_pages), vp = any_strides(v_pages);
+  check_rc(ltv_paged_cache_read(dtype == at::kFloat ? LTV_DTYPE_F32 : LTV_DTYPE_BF16,
+                                is_fp4(k_pages) ? LTV_PAGES_FP4 : LTV_PAGES_VALUES,
+                                k_pages.data_ptr(), kp.s, v_pages.data_ptr(), vp.s, &b.b,
+                                k.data_ptr(), v.data_ptr(), (int)NKVH, (int)D, stream_of(k)),
+           "ltv_paged_cache_read");
+  return std::make_tuple(k, v);
 }
 
 // (compact needs no lengths)
@@ -354,6 +511,23 @@ bool fork_slots(const Tensor& table, const Tensor& lens, const Tensor& refs, con
   return true;
 }
 
+bool reorder_slots(const Tensor& table, const Tensor& lens, const Tensor& refs,
+                   const Tensor& slots_in, const Tensor& src_in) {
+  if (!ordinary_call(table, lens, refs, slots_in, src_in)) return false;
+  const ltv_page_state state = make_state(table, lens, refs, 1);
+  const Tensor slots = int_vector(slots_in, "slots", table), src = int_vector(src_in, "src", table);
+  TORCH_CHECK_VALUE(slots.numel() == src.numel(), slots.numel(), " slots, but ", src.numel(),
+                    " src slots");
+  c10::OptionalDeviceGuard guard(table.device());
+  if (slots.numel() == 0) return true;
+  const int n = to_int(slots.numel(), "the number of slots");
+  const Workspace ws(ltv_paged_cache_reorder_workspace_size(n, state.table_width));
+  check_rc(ltv_paged_cache_reorder(&state, slots.data_ptr<int32_t>(), src.data_ptr<int32_t>(), n,
+                                   ws.ptr(), ws.bytes, stream_of(table)),
+           "ltv_paged_cache_reorder");
+  return true;
+}
+
 bool free_slots(const Tensor& table, const Tensor& lens, const Tensor& refs,
                 const Tensor& slots_in) {
   if (!ordinary_call(table, lens, refs, slots_in)) return false;
@@ -414,10 +588,11 @@ std::optional<std::tuple<Tensor, OptTensor>> attention(
   const int dt = dtype_of(q_in, "q");
   TORCH_CHECK(q_in.is_cuda(), "LTV HIP kernels need GPU tensors, got q on ", q_in.device());
   no_grad_needed(q_in, "q");
-  check_pages(k_pages, v_pages, q_in);
+  check_any_pages(k_pages, v_pages, q_in);
   const Batch b = make_batch(q_in, "q", k_pages, table, lens, slots, starts, max_new);
   const int64_t NH = q_in.size(-2), D = q_in.size(-1), NKVH = k_pages.size(1);
-  TORCH_CHECK_VALUE(k_pages.size(3) == D, "q has head_dim ", D, ", the pages ", k_pages.size(3));
+  TORCH_CHECK_VALUE(head_dim_of(k_pages) == D, "q has head_dim ", D, ", the pages ",
+                    head_dim_of(k_pages));
   TORCH_CHECK_VALUE(NH == 0 || (NKVH > 0 && NH % NKVH == 0), NKVH,
                     " k/v heads do not divide q's ", NH);
   TORCH_CHECK_VALUE(D > 0 && D <= 128 && D % 8 == 0,
@@ -435,16 +610,17 @@ std::optional<std::tuple<Tensor, OptTensor>> attention(
   OptTensor lse;
   if (return_lse) lse = at::empty(q.sizes().slice(0, q.dim() - 1), out.options().dtype(at::kFloat));
   if (out.numel() == 0) return std::make_tuple(out, lse);
-  const Workspace ws(
-      ltv_paged_attention_workspace_size(dt, &b.b, (int)NH, (int)NKVH, (int)D, most));
+  const bool fp4 = is_fp4(k_pages);
+  const Workspace ws((fp4 ? ltv_paged_attention_fp4_workspace_size
+                          : ltv_paged_attention_workspace_size)(dt, &b.b, (int)NH, (int)NKVH,
+                                                                (int)D, most));
   const Strides3 qs = Strides3::tokens(q), os = Strides3::tokens(out),
-                 kp = Strides3::pages(k_pages), vp = Strides3::pages(v_pages);
-  check_rc(ltv_paged_attention(dt, q.data_ptr(), qs.s, k_pages.data_ptr(), kp.s,
-                               v_pages.data_ptr(), vp.s, &b.b, out.data_ptr(), os.s,
-                               lse.has_value() ? lse->data_ptr<float>() : nullptr,
-                               ws.ptr(), ws.bytes, (int)NH, (int)NKVH,
-                               (int)D, most, sc, stream_of(q)),
-           "ltv_paged_attention");
+                 kp = any_strides(k_pages), vp = any_strides(v_pages);
+  check_rc((fp4 ? ltv_paged_attention_fp4 : ltv_paged_attention)(
+               dt, q.data_ptr(), qs.s, k_pages.data_ptr(), kp.s, v_pages.data_ptr(), vp.s, &b.b,
+               out.data_ptr(), os.s, lse.has_value() ? lse->data_ptr<float>() : nullptr, ws.ptr(),
+               ws.bytes, (int)NH, (int)NKVH, (int)D, most, sc, stream_of(q)),
+           fp4 ? "ltv_paged_attention_fp4" : "ltv_paged_attention");
   return std::make_tuple(out, lse);
 }
 
@@ -599,6 +775,9 @@ OptTensor token_logprobs_backward(const Tensor& logits, const Tensor& targets, c
 void bind_serving(pybind11::module_& m) {
   using nogil = pybind11::call_guard<pybind11::gil_scoped_release>;
   m.def("paged_cache_append", &append, nogil());
+  m.def("paged_rotary_append", &rotary_append, nogil());
+  m.def("paged_cache_read", &read_pages, nogil());
+  m.def("paged_cache_reorder", &reorder_slots, nogil());
   m.def("paged_cache_reserve", &reserve, nogil());
   m.def("paged_cache_fork", &fork_slots, nogil());
   m.def("paged_cache_free", &free_slots, nogil());

@@ -8,6 +8,17 @@ One layer's cache is a pair of page arrays ``k_pages``, ``v_pages``
   seq_lens   (S)    int32 -- tokens of each slot, the ones being computed included
   ref_counts (P)    int32 -- how many slots hold a page; 0: free
 
+Pages may be held in 4 bits: uint8 arrays (P, kv heads, page size,
+``fp4_row_bytes(head_dim)``), head_dim 32, 64, 96 or 128 and the page size a multiple of
+16, each page and head a dense block.  Of a block the codes come first (page size,
+head_dim / 2), the even channel in the low half of a byte, then the scales (head_dim / 32,
+page size), one byte for 32 channels of a token.  They stand for code * 2^(scale - 127),
+the code's low three bits for 0, 0.5, 1, 1.5, 2, 3, 4, 6 and the fourth for the sign; the
+scale 255 for 32 times NaN.  ``paged_cache_append`` and ``paged_rotary_append`` round to
+the nearest such value (ties to the even code) with the smallest scale by which no channel
+is larger than 7 (6 is the largest code); ``paged_attention`` computes with the values and
+``paged_cache_read`` gives them back.  What moves pages moves these as any others.
+
 All of it lives on the GPU and is read and written there in stream order: no call
 waits for the device, and a step can be captured in a HIP graph.  A step of a
 serving loop is
@@ -56,6 +67,53 @@ def paged_cache_append(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, p
         _append_op(*args)
 
 
+def fp4_row_bytes(head_dim: int) -> int:
+    """Bytes that a token's head takes in 4-bit pages: the last size of their arrays."""
+    if head_dim not in (32, 64, 96, 128):
+        raise ValueError(f"4-bit pages have head_dim 32, 64, 96 or 128, got {head_dim}")
+    return head_dim // 2 + head_dim // 32
+
+
+def paged_rotary_append(q: Tensor, k: Tensor, v: Tensor, cos: Tensor, sin: Tensor,
+                        k_pages: Tensor, v_pages: Tensor, page_table: Tensor, seq_lens: Tensor,
+                        *, slots: Optional[Tensor] = None, starts: Optional[Tensor] = None,
+                        max_new: Optional[int] = None,
+                        norm_eps: Optional[float] = None) -> Tensor:
+    """Rotate the new tokens' queries and keys by their positions, with ``norm_eps`` divide
+    each head by sqrt(mean of squares + norm_eps), write keys and values into their pages
+    (as ``paged_cache_append``), and return the queries: q's shape, contiguous.
+
+    ``cos`` and ``sin`` (positions, head_dim / 2), float32 or bfloat16, have a row for every
+    position that the page table has room for.  The halves of a head are rotated as pairs:
+    (x1 cos + x2 sin, x2 cos - x1 sin) at the token's row.  Computed in float64, and only
+    then rounded, to q's dtype or to 4 bits.  A token at a negative position gives 0.
+    Inference only.
+
+    The reference rotates and normalises q and k in a dozen launches
+    (``nanochat/gpt.py:101-109, 231-236``) before its cache takes them."""
+    args = (q, k, v, cos, sin, k_pages, v_pages, page_table, seq_lens, slots, starts, max_new,
+            norm_eps)
+    got = None if torch.compiler.is_compiling() else N.torch_ext().paged_rotary_append(*args)
+    return _rotary_append_op(*args) if got is None else got
+
+
+def paged_cache_read(k_pages: Tensor, v_pages: Tensor, page_table: Tensor, seq_lens: Tensor,
+                     tokens: int, *, slots: Optional[Tensor] = None,
+                     starts: Optional[Tensor] = None, max_new: Optional[int] = None,
+                     dtype: Optional[torch.dtype] = None) -> Tuple[Tensor, Tensor]:
+    """What the pages hold of the last ``tokens`` tokens of each sequence, (B, tokens, kv
+    heads, head_dim), or, with ``starts``, of as many as it says, (tokens, kv heads,
+    head_dim) with ``tokens`` rows in all: what ``paged_cache_append`` was given, rounded if
+    the pages have 4 bits.  A token at a negative position or of no page, and a row of no
+    sequence, is 0.  ``dtype`` of 4-bit pages is bfloat16 or float32 (both hold the values
+    exactly; default bfloat16), else that of the pages."""
+    if dtype is None:
+        dtype = torch.bfloat16 if k_pages.dtype == torch.uint8 else k_pages.dtype
+    args = (k_pages, v_pages, page_table, seq_lens, tokens, slots, starts, max_new, dtype)
+    got = None if torch.compiler.is_compiling() else N.torch_ext().paged_cache_read(*args)
+    return _read_op(*args) if got is None else got
+
+
 def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tensor,
                     seq_lens: Tensor, *, slots: Optional[Tensor] = None,
                     starts: Optional[Tensor] = None, max_new: Optional[int] = None,
@@ -66,8 +124,8 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Ten
     ``scale`` > 0 defaults to 1 / sqrt(head_dim).  A token that has nothing to attend to
     gives 0.  With ``return_lse`` also the log of the softmax's denominators (fp32, q's
     shape without head_dim; -inf where there is nothing), which joins attention over
-    several caches.  float32 or bfloat16, head_dim a multiple of 8 up to 128; inference
-    only."""
+    several caches.  float32 or bfloat16, head_dim a multiple of 8 up to 128, pages of
+    that dtype or in 4 bits; inference only."""
     args = (q, k_pages, v_pages, page_table, seq_lens, slots, starts, max_new, max_len, scale)
     got = None if torch.compiler.is_compiling() else N.torch_ext().paged_attention(*args,
                                                                                    return_lse)
@@ -99,6 +157,19 @@ def paged_cache_fork(page_table: Tensor, seq_lens: Tensor, ref_counts: Tensor, s
     args = (page_table, seq_lens, ref_counts, src, dst)
     if torch.compiler.is_compiling() or not N.torch_ext().paged_cache_fork(*args):
         _fork_op(*args)
+
+
+def paged_cache_reorder(page_table: Tensor, seq_lens: Tensor, ref_counts: Tensor, slots: Tensor,
+                        src: Tensor) -> None:
+    """Slot slots[i] becomes what slot src[i] holds before the call, all at once: a search's
+    beams follow its selection, in whatever exchange.  A slot may be a src several times, and
+    both; pages are shared as by fork, and what no slot holds any more is free.  ``slots`` are
+    distinct.
+
+    The reference copies a contiguous cache row by row."""
+    args = (page_table, seq_lens, ref_counts, slots, src)
+    if torch.compiler.is_compiling() or not N.torch_ext().paged_cache_reorder(*args):
+        _reorder_op(*args)
 
 
 def paged_cache_free(page_table: Tensor, seq_lens: Tensor, ref_counts: Tensor,
@@ -143,6 +214,37 @@ def _(k, v, k_pages, v_pages, page_table, seq_lens, slots, starts, max_new):
     return None
 
 
+@torch.library.custom_op("nanochat_amd::paged_rotary_append", mutates_args=("k_pages", "v_pages"))
+def _rotary_append_op(q: Tensor, k: Tensor, v: Tensor, cos: Tensor, sin: Tensor, k_pages: Tensor,
+                      v_pages: Tensor, page_table: Tensor, seq_lens: Tensor,
+                      slots: Optional[Tensor], starts: Optional[Tensor], max_new: Optional[int],
+                      norm_eps: Optional[float]) -> Tensor:
+    return N.done(N.torch_ext().paged_rotary_append(q, k, v, cos, sin, k_pages, v_pages,
+                                                    page_table, seq_lens, slots, starts, max_new,
+                                                    norm_eps))
+
+
+@_rotary_append_op.register_fake
+def _(q, k, v, cos, sin, k_pages, v_pages, page_table, seq_lens, slots, starts, max_new, norm_eps):
+    return q.new_empty(q.shape)
+
+
+@torch.library.custom_op("nanochat_amd::paged_cache_read", mutates_args=())
+def _read_op(k_pages: Tensor, v_pages: Tensor, page_table: Tensor, seq_lens: Tensor, tokens: int,
+             slots: Optional[Tensor], starts: Optional[Tensor], max_new: Optional[int],
+             dtype: torch.dtype) -> Tuple[Tensor, Tensor]:
+    return N.done(N.torch_ext().paged_cache_read(k_pages, v_pages, page_table, seq_lens, tokens,
+                                                 slots, starts, max_new, dtype))
+
+
+@_read_op.register_fake
+def _(k_pages, v_pages, page_table, seq_lens, tokens, slots, starts, max_new, dtype):
+    D = k_pages.shape[3] // 17 * 32 if k_pages.dtype == torch.uint8 else k_pages.shape[3]
+    rows = [] if starts is not None else [(page_table if slots is None else slots).shape[0]]
+    shape = (*rows, tokens, k_pages.shape[1], D)
+    return k_pages.new_empty(shape, dtype=dtype), k_pages.new_empty(shape, dtype=dtype)
+
+
 @torch.library.custom_op("nanochat_amd::paged_attention", mutates_args=())
 def _attention_op(q: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tensor,
                   seq_lens: Tensor, slots: Optional[Tensor], starts: Optional[Tensor],
@@ -182,6 +284,17 @@ def _fork_op(page_table: Tensor, seq_lens: Tensor, ref_counts: Tensor, src: Tens
 
 @_fork_op.register_fake
 def _(page_table, seq_lens, ref_counts, src, dst):
+    return None
+
+
+@torch.library.custom_op("nanochat_amd::paged_cache_reorder", mutates_args=_STATE)
+def _reorder_op(page_table: Tensor, seq_lens: Tensor, ref_counts: Tensor, slots: Tensor,
+                src: Tensor) -> None:
+    N.done(N.torch_ext().paged_cache_reorder(page_table, seq_lens, ref_counts, slots, src))
+
+
+@_reorder_op.register_fake
+def _(page_table, seq_lens, ref_counts, slots, src):
     return None
 
 
