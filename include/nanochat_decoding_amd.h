@@ -98,6 +98,27 @@ size_t ltv_paged_cache_reorder_workspace_size(int n, int table_width);
 int ltv_paged_cache_reorder(const ltv_page_state* state, const int32_t* slots, const int32_t* src,
                             int n, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------
+ * A search's selection: of each of `groups` prompts with `beams` beams, the k best
+ * continuations over all beams and tokens.  logits x (groups * beams, V), row stride
+ * row_stride, last stride 1; scores (groups, beams) float32, contiguous, the beams' own.
+ *   score(b, v) = scores[b] + z[b, v] - log sum_w exp z[b, w],  z = softcap tanh(x / softcap)
+ *                 (softcap 0: z = x);  -inf where scores[b] or z[b, v] is
+ * in descending order (NaN above all); equal ones by beam, then by logit as top_ids of
+ * ltv_token_logprobs_forward.  A beam with finished[b] != 0 (finished may be NULL) has one
+ * continuation, itself, with its score and the token -1, and then min(k, V) - 1 with the
+ * score -inf and the token -1; its logits are not read.
+ *   out_scores (groups, k) float32, parents and tokens (groups, k): beam and token
+ * k <= beams * V; min(k, V) <= 64 and beams * min(k, V) <= 1024; groups * beams <= 2^20.
+ * Scores are compared in float64.  workspace: ltv_beam_select_workspace_size bytes, 16-byte
+ * aligned.
+ * ---------------------------------------------------------------------- */
+size_t ltv_beam_select_workspace_size(int64_t groups, int beams, int V, int k);
+int ltv_beam_select(int dtype, const void* logits, int64_t row_stride, const float* scores,
+                    const uint8_t* finished, float* out_scores, int64_t* parents, int64_t* tokens,
+                    void* workspace, size_t workspace_bytes, int64_t groups, int beams, int V,
+                    int k, float softcap, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

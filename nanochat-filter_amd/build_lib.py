@@ -25,7 +25,7 @@ OUT = os.path.join(HERE, "nanochat_amd", "libnanochat_filter_amd.so")
 SOURCES = ["ltv_scan_fwd_bf16.hip", "ltv_scan_fwd_f32.hip", "ltv_scan_bwd_bf16.hip",
            "ltv_scan_bwd_f32.hip", "ltv_scan_abi.hip", "ltv_scan_lb.hip", "ltv_gemm.hip", "ltv_decode.hip",
            "ltv_paged_cache.hip", "ltv_paged_attn.hip", "ltv_paged_attn4.hip", "ltv_rotary_append.hip",
-           "ltv_logprobs.hip", "ltv_abi.cpp"]
+           "ltv_logprobs.hip", "ltv_beam.hip", "ltv_abi.cpp"]
 ARCH = "gfx950"
 # roofline microbenchmarks for bench.py --workload peaks: a library of their own
 PEAKS_SOURCES = ["bench/ltv_peaks.hip"]

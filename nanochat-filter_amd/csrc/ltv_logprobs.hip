@@ -33,15 +33,10 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "../../include/nanochat_serving_amd.h"
-#include "ltv_abi_internal.hpp"
-#include "ltv_device.hpp"
+#include "ltv_logprobs.hpp"
 
 namespace ltv {
 namespace {
-
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
 
 struct LogpArgs {
   const void* x;
@@ -55,21 +50,11 @@ struct LogpArgs {
   int V, top_k;
   float cap;
   int piece, pieces;         // elements of a workgroup, workgroups of a row
-  float* part_sums;          // (N, pieces, 3), pieces > 1
+  bool parts;                // a kernel joins the pieces: pieces > 1, or another's
+  const uint8_t* skip;       // rows to leave out, or null
+  float* part_sums;          // (N, pieces, 3), parts
   uint64_t* part_keys;       // (N, pieces, top_k)
 };
-
-// How z follows from x: none, by r, by tanh.
-enum Cap { kNoCap, kCap, kWideCap };
-constexpr float kMostCap = 64.0f;  // by r
-
-// r of the cap's tanh; cap_scale = 2 log2(e) / c (finite for the smallest c, too)
-__device__ __forceinline__ float cap_scale_of(float cap) {
-  return fminf(2.0f * kLog2e / cap, 3.0e38f);
-}
-__device__ __forceinline__ float cap_r(float x, float cap_scale) {
-  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * cap_scale));
-}
 
 // (below 2^-13 of the cap x (1 - (x / c)^2 / 3 + ..) rounds to x)
 __device__ __forceinline__ float wide_capped(float x, float cap) {
@@ -81,22 +66,6 @@ __device__ __forceinline__ float capped(float x, float cap) {
   if constexpr (CAP == kNoCap) return x;
   if constexpr (CAP == kWideCap) return wide_capped(x, cap);
   return fmaf(-2.0f * cap, cap_r(x, cap_scale_of(cap)), cap);
-}
-
-// A total order of the logits with their indices: larger value first (NaN above all,
-// -0 = +0), then lower index.  Never 0 for a real entry.
-__device__ __forceinline__ uint64_t order_key(float x, int i) {
-  const uint32_t u = __float_as_uint(x + 0.0f);
-  uint32_t k = (u & 0x80000000u) ? ~u : u | 0x80000000u;
-  if (x != x) k = 0xffffffffu;
-  return ((uint64_t)k << 32) | (uint32_t)(0x7fffffff - i);
-}
-__device__ __forceinline__ float key_value(uint64_t key) {
-  const uint32_t k = (uint32_t)(key >> 32);
-  return __uint_as_float((k & 0x80000000u) ? k & 0x7fffffffu : ~k);
-}
-__device__ __forceinline__ int key_index(uint64_t key) {
-  return 0x7fffffff - (int)(uint32_t)key;
 }
 
 // 16 bytes at any alignment of the element.
@@ -121,11 +90,11 @@ struct Sums {
   template <int N>
   __device__ __forceinline__ void add(const float (&logits)[N], float cap) {
     if constexpr (CAP == kCap) {
-      const float cap_scale = cap_scale_of(cap), at0 = cap * kLog2e, slope = -2.0f * at0;
+      const float cap_scale = cap_scale_of(cap);
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         const float r = cap_r(logits[i], cap_scale);
-        const float e = __builtin_amdgcn_exp2f(fmaf(r, slope, at0));
+        const float e = cap_exp(r, cap);
         s += e;
         a = fmaf(r, e, a);
       }
@@ -176,20 +145,6 @@ struct Sums {
 constexpr int kGroups = 64;    // of the first elements: as many as top_k may be
 constexpr int kCands = 1024;   // collected elements
 
-__device__ __forceinline__ uint64_t of_lane(uint64_t x, int i) {  // (i uniform)
-  return ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), i) << 32) |
-         (uint32_t)__builtin_amdgcn_readlane((int)x, i);
-}
-
-// The k-th largest of the 64 lanes' keys, 0 if fewer are not 0 (every lane gets it).
-__device__ __forceinline__ uint64_t kth_of_lanes(uint64_t mine, int k) {
-  int above = 0;
-#pragma unroll
-  for (int i = 0; i < 64; ++i) above += of_lane(mine, i) > mine;
-  const uint64_t at = __ballot(above == k - 1 && mine != 0);
-  return at == 0 ? 0 : of_lane(mine, __builtin_ctzll(at));
-}
-
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 
 // What a row's sums make: log(sum of exponentials) and entropy.
@@ -235,6 +190,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_forward_kernel(const LogpAr
   __shared__ unsigned long long bound_lds;
   __shared__ int count, above_lds;
   const int64_t n = blockIdx.x;
+  if (p.skip != nullptr && p.skip[n] != 0) return;
   const int begin = blockIdx.y * p.piece;
   const T* whole_row = reinterpret_cast<const T*>(p.x) + n * p.xs;
   const T* row = whole_row + begin;
@@ -243,7 +199,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_forward_kernel(const LogpAr
   Sums<CAP> sums;
   float bound = INFINITY;
   Target target;
-  if (tid == 0 && p.pieces == 1) target = target_of(p, n, whole_row);
+  if (tid == 0 && !p.parts) target = target_of(p, n, whole_row);
 
   auto collect = [&](float x, int i) {
     const int at = atomicAdd(&count, 1);
@@ -365,7 +321,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_forward_kernel(const LogpAr
   for (int w = 0; w < kWaves; ++w) sums.join(lds_sums[w][0], lds_sums[w][1], lds_sums[w][2]);
   const int64_t part = n * p.pieces + blockIdx.y;
   float lse = 0.0f, entropy;
-  if (p.pieces > 1) {
+  if (p.parts) {
     if (tid < 3) p.part_sums[part * 3 + tid] = tid == 0 ? sums.m : tid == 1 ? sums.s : sums.a;
   } else {
     row_results(sums, p.cap, lse, entropy);
@@ -445,7 +401,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_forward_kernel(const LogpAr
 #pragma unroll 8
       for (int j = 0; j < have; ++j) above += cands[j] > mine;
       if (above >= p.top_k) continue;
-      if (p.pieces > 1) {
+      if (p.parts) {
         p.part_keys[part * p.top_k + above] = mine;
       } else {
         p.top_ids[n * p.top_k + above] = key_index(mine);
@@ -453,7 +409,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_forward_kernel(const LogpAr
       }
     }
     // (a last piece of fewer elements than alternatives)
-    if (p.pieces > 1)
+    if (p.parts)
       for (int e = have + tid; e < p.top_k; e += kThreads) p.part_keys[part * p.top_k + e] = 0;
   }
 }
@@ -526,6 +482,11 @@ __global__ void __launch_bounds__(kJoinThreads) logprobs_join_kernel(const LogpA
 int row_pieces(int64_t N, int V) {
   if (N >= 512 || N <= 0) return 1;
   return (int)std::max<int64_t>(1, std::min<int64_t>({kPieces, (1024 + N - 1) / N, V / 4096}));
+}
+
+// (a multiple of 64 elements: pieces of an aligned row are aligned)
+int piece_size(int V, int pieces) {
+  return (int)std::min<int64_t>((((int64_t)V + pieces - 1) / pieces + 63) / 64 * 64, V);
 }
 
 struct LogpGradArgs {
@@ -650,6 +611,36 @@ int check_rows(int dtype, const void* x, int64_t row_stride, const int64_t* targ
 }
 
 }  // namespace
+
+int logprobs_pieces(int64_t N, int V) {
+  const int piece = piece_size(V, row_pieces(N, V));
+  return (int)(((int64_t)V + piece - 1) / piece);
+}
+
+int logprobs_parts(int dtype, const void* x, int64_t row_stride, const uint8_t* skip,
+                   float* part_sums, uint64_t* part_keys, int64_t N, int V, int top_k,
+                   float softcap, hipStream_t stream) {
+  LogpArgs a{x, row_stride, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, V, top_k,
+             softcap, piece_size(V, row_pieces(N, V)), logprobs_pieces(N, V), true, skip, part_sums,
+             part_keys};
+  const dim3 grid((unsigned)N, a.pieces);
+  auto launch = [&](auto type) {
+    using T = decltype(type);
+    auto by_cap = [&](auto cap) {
+      hipLaunchKernelGGL((logprobs_forward_kernel<T, decltype(cap)::value, true>), grid,
+                         dim3(kThreads), 0, stream, a);
+    };
+    switch (cap_of(softcap)) {
+      case kNoCap: return by_cap(cap_type<kNoCap>());
+      case kCap: return by_cap(cap_type<kCap>());
+      case kWideCap: return by_cap(cap_type<kWideCap>());
+    }
+  };
+  if (dtype == LTV_DTYPE_F32) launch(float()); else launch(bf16_t());
+  LTV_LAUNCH_CHECK();
+  return LTV_OK;
+}
+
 }  // namespace ltv
 
 using namespace ltv;
@@ -674,12 +665,10 @@ extern "C" int ltv_token_logprobs_forward(int dtype, const void* logits, int64_t
                   (pieces == 1 || (workspace && aligned16(workspace))),
               LTV_ERR_WORKSPACE, "workspace too small");
   uint64_t* keys = reinterpret_cast<uint64_t*>(workspace);
-  // (a multiple of 64 elements: pieces of an aligned row are aligned)
-  const int piece =
-      (int)std::min<int64_t>((((int64_t)V + pieces - 1) / pieces + 63) / 64 * 64, V);
+  const int piece = piece_size(V, pieces);
   LogpArgs a{logits, row_stride, targets, logprobs, entropy, lse, top_logprobs, top_ids,
-                   V, top_k, softcap, piece, (int)(((int64_t)V + piece - 1) / piece),
-                   reinterpret_cast<float*>(keys + N * pieces * top_k), keys};
+                   V, top_k, softcap, piece, (int)(((int64_t)V + piece - 1) / piece), pieces > 1,
+                   nullptr, reinterpret_cast<float*>(keys + N * pieces * top_k), keys};
   const hipStream_t st = (hipStream_t)stream;
   // (a launch has less than 2^32 threads along an axis; so many rows are not cut)
   constexpr int64_t kMostRows = int64_t(1) << 23;

@@ -770,6 +770,75 @@ OptTensor token_logprobs_backward(const Tensor& logits, const Tensor& targets, c
   return backward_of(logits, targets, lse, entropy, ids, g_lp, g_ent, g_top, cap);
 }
 
+// ---------------------------------------------------------------------------
+// a search's selection
+// ---------------------------------------------------------------------------
+// (scores, parents, tokens)
+std::optional<std::tuple<Tensor, Tensor, Tensor>> beam_select(const Tensor& logits,
+                                                              const Tensor& scores_in, int64_t k,
+                                                              double cap,
+                                                              const OptTensor& finished_in) {
+  no_tangent(logits, "logits");
+  no_tangent(scores_in, "scores");
+  if (!ordinary_call(logits, scores_in, finished_in)) return {};
+  const int dt = dtype_of(logits, "logits");
+  TORCH_CHECK(logits.is_cuda(), "LTV HIP kernels need GPU tensors, got logits on ",
+              logits.device());
+  on_device(scores_in, "scores", logits);
+  const auto no_grad = [](const Tensor& t, const char* name) {
+    TORCH_CHECK(!(at::GradMode::is_enabled() && t.requires_grad()), name,
+                " requires grad, but a selection has none: call under torch.no_grad()");
+  };
+  no_grad(logits, "logits");
+  no_grad(scores_in, "scores");
+  TORCH_CHECK_VALUE(logits.dim() >= 2 &&
+                        scores_in.sizes() == logits.sizes().slice(0, logits.dim() - 1),
+                    "logits must be (..., beams, vocabulary) and scores (..., beams), got ",
+                    logits.sizes(), " and ", scores_in.sizes());
+  TORCH_CHECK_TYPE(scores_in.scalar_type() == at::kFloat, "scores must be float32, got ",
+                   scores_in.scalar_type());
+  const int64_t B = logits.size(-2), V = logits.size(-1);
+  TORCH_CHECK_VALUE(B > 0 && V > 0, "no beams, or an empty vocabulary: ", logits.sizes());
+  TORCH_CHECK_VALUE(k > 0 && (k - 1) / B < V, "k must be 1 to the ", B, " beams' tokens, got ", k);
+  const int64_t n = std::min(k, V);
+  TORCH_CHECK_VALUE(n <= 64 && B * n <= 1024, "at most 64 continuations of a beam and 1,024 of all, "
+                    "got k ", k, " of ", B, " beams");
+  TORCH_CHECK_VALUE(std::isfinite((float)cap) && cap >= 0 && ((float)cap > 0 || cap == 0),
+                    "softcap must be positive and finite in float32, got ", cap);
+  Tensor finished;
+  if (finished_in.has_value()) {
+    on_device(*finished_in, "finished", logits);
+    TORCH_CHECK_TYPE(finished_in->scalar_type() == at::kBool, "finished must be bool, got ",
+                     finished_in->scalar_type());
+    TORCH_CHECK_VALUE(finished_in->sizes() == scores_in.sizes(), "scores is ", scores_in.sizes(),
+                      ", finished ", finished_in->sizes());
+    finished = finished_in->contiguous();
+  }
+  c10::OptionalDeviceGuard guard(logits.device());
+  const int64_t G = scores_in.numel() / B;
+  Tensor x = logits.reshape({G * B, V});
+  if (V > 1 && x.stride(1) != 1) x = x.contiguous();
+  const Tensor scores = scores_in.contiguous();
+  auto shape = scores_in.sizes().vec();
+  shape.back() = k;
+  const auto f32 = scores.options().requires_grad(false);
+  Tensor best = at::empty(shape, f32), parents = at::empty(shape, f32.dtype(at::kLong)),
+         tokens = at::empty(shape, f32.dtype(at::kLong));
+  if (G == 0) return std::make_tuple(best, parents, tokens);
+  const int b = to_int(B, "the number of beams"), v = to_int(V, "the vocabulary"),
+            kk = to_int(k, "k");
+  const Workspace ws(ltv_beam_select_workspace_size(G, b, v, kk));
+  check_rc(ltv_beam_select(dt, x.data_ptr(), x.stride(0), scores.data_ptr<float>(),
+                           finished.defined()
+                               ? reinterpret_cast<const uint8_t*>(finished.data_ptr<bool>())
+                               : nullptr,
+                           best.data_ptr<float>(), parents.data_ptr<int64_t>(),
+                           tokens.data_ptr<int64_t>(), ws.ptr(), ws.bytes, G, b, v, kk, (float)cap,
+                           stream_of(x)),
+           "ltv_beam_select");
+  return std::make_tuple(best, parents, tokens);
+}
+
 }  // namespace
 
 void bind_serving(pybind11::module_& m) {
@@ -784,6 +853,7 @@ void bind_serving(pybind11::module_& m) {
   m.def("paged_cache_copy", &copy_pages, nogil());
   m.def("paged_cache_compact", &compact, nogil());
   m.def("paged_attention", &attention, nogil());
+  m.def("beam_select", &beam_select, nogil());
   m.def("token_logprobs", &token_logprobs, nogil());
   m.def("token_logprobs_forward", &token_logprobs_forward, nogil());
   m.def("token_logprobs_backward", &token_logprobs_backward, nogil());

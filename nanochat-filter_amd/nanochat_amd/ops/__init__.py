@@ -7,6 +7,7 @@ the first call, so importing works on a machine without a GPU.
 
 from nanochat_amd.ops import ltv_cuda_ops  # noqa: F401
 from nanochat_amd.ops import ltv_hm_fast  # noqa: F401
+from nanochat_amd.ops.beam_select import BeamSelection, beam_select  # noqa: F401
 from nanochat_amd.ops.paged_cache import (  # noqa: F401
     fp4_row_bytes,
     paged_attention,
