@@ -50,14 +50,6 @@ struct AttnShape {
   static constexpr int kGrid = FEW ? 1024 : 512;  // workgroups that the card holds
   static constexpr int kKeys = FEW || sizeof(T) == 4 ? 32 : 64;  // of a tile
 };
-typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-
-// Nothing is moved across: the tile's loop is written in the order that it is to run in,
-// reads from LDS well ahead of the products that take them and exponentials between the
-// products.  (Left to itself the compiler puts each read right before its product.)
-__device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0); }
-
 // What differs by element type.  A chunk is 16 bytes of a row.
 template <typename T>
 struct AttnType;
@@ -108,14 +100,6 @@ struct AttnTile {
 
 __device__ const uint4 kZeros = {0, 0, 0, 0};
 
-__device__ __forceinline__ uint32_t lds_address(uint4* p) {
-  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint4*)p;
-}
-template <typename V>
-__device__ __forceinline__ V lds_read(uint32_t at) {
-  return *(__attribute__((address_space(3))) const V*)(uintptr_t)at;
-}
-
 // One wavefront's 16 bytes per lane from `from` into LDS at `to` + 16 lane (`to` uniform).
 // Inline assembly, as in the projection's kernels: the compiler would wait for a builtin's
 // load before the next read of either buffer.  It has no output register; the wait is
@@ -130,18 +114,6 @@ __device__ __forceinline__ void load_lds16(uint4* to, const char* from, uint32_t
   const uint32_t base = lds_address(to);
   asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(from),
                "{m0}"(base) : "memory");
-}
-
-__device__ __forceinline__ void barrier() {
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
-}
-
-__device__ __forceinline__ float across_halves_max(float x) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false,
-                                                  false);
-  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
 // Whether any of a chunk's elements is infinite or NaN (all exponent bits set).
@@ -173,7 +145,7 @@ struct ValuePages {
     load(a.k + kvh * a.kh + (uint64_t)((uint32_t)page * a.kp + in * a.ks) * 16, c, x);
   }
   static __device__ __forceinline__ void values(const AttnArgs& a, int kvh, int page, uint32_t in,
-                                                int c, float (&x)[8]) {
+                                                int c, float (&x)[8], int) {
     load(a.v + kvh * a.vh + (uint64_t)((uint32_t)page * a.vp + in * a.vs) * 16, c, x);
   }
 };
@@ -184,8 +156,7 @@ __global__ void __launch_bounds__((AttnShape<T, FEW>::kThreads), FEW ? 1 : 2)
   using Ty = AttnType<T>;
   using Ti = AttnTile<T, DP, FEW>;
   using Shape = AttnShape<T, FEW>;
-  constexpr int kAttnWaves = Shape::kWaves, kAttnThreads = Shape::kThreads,
-                kAttnRows = Shape::kRows;
+  constexpr int kAttnThreads = Shape::kThreads, kAttnRows = Shape::kRows;
   constexpr int KT = Ti::kKeys, KB = KT / 32;
   constexpr int kSteps = Ti::kChunks / 2;  // score products' steps: two chunks each
   constexpr int kDB = DP / 32;
@@ -193,120 +164,13 @@ __global__ void __launch_bounds__((AttnShape<T, FEW>::kThreads), FEW ? 1 : 2)
   constexpr int kRow = Ti::kChunks * 16, kTile = Ti::kUnits * 16;  // bytes
   __shared__ uint4 lds[4 * Ti::kUnits];                            // K, V, and again
 
-  // The lengths of all sequences, a run of them to each thread, and their sum.
-  __shared__ uint32_t sums[kAttnWaves];
-  __shared__ struct { PagedSeq s; int b; uint32_t at; } found;  // the sequence of a range's begin
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int per = (a.batch.B + kAttnThreads - 1) / kAttnThreads;
-  const int b0 = min((int)threadIdx.x * per, a.batch.B), b1 = min(b0 + per, a.batch.B);
-  uint32_t mine = 0;
-  PagedSeq q{a.batch.table, 0, 0, 0};
-  for (int i = b0; i < b1; ++i) {
-    q = paged_seq(a.batch, i);
-    mine += Line::of<KT>(a, q.n, q.len).all;
-  }
-  uint32_t upto = wave_sum_up_to(mine);
-  if ((threadIdx.x & 63) == 63) sums[wave] = upto;
-  if (threadIdx.x == 0) {
-    found.s = q;
-    found.b = 0;
-    found.at = 0;
-  }
-  __syncthreads();
-  uint32_t all = 0;
-#pragma unroll
-  for (int w = 0; w < kAttnWaves; ++w) {
-    if (w < wave) upto += sums[w];
-    all += sums[w];
-  }
-  all = __builtin_amdgcn_readfirstlane(all);
-  Ranges line;
-  line.length = max(a.least, a.by_ranges.quot(all + a.ranges - 1));
-  line.count = min(over(all + line.length - 1, line.length), a.ranges);
-  // Of the two workgroups of a compute unit the older is served first where the products
-  // bound them, and had ended with a fifth of the other's work left: it gets more of it
-  // (a long prompt 1,225 us with equal ranges, 1,187 with these).
-  const bool full = a.log_group > 0 && line.count << a.log_group == Shape::kGrid;
-  line.lead = full ? line.length / 8 : 0;
-  if (blockIdx.x == 0 && threadIdx.x == 0) *a.head = line.count;
-  // Workgroup w runs on XCD w % 8: consecutive ranges stay on one.
-  const int per_xcd = (line.count + 7) / 8, local = blockIdx.x >> 3 >> a.log_group;
-  const int range = (blockIdx.x & 7) * per_xcd +
-                    (!full ? local : local < per_xcd / 2 ? local * 2 : local * 2 - per_xcd + 1);
-  const int member = (blockIdx.x >> 3) & ((1 << a.log_group) - 1);
-  if (local >= per_xcd || range >= line.count) return;
-  if (threadIdx.x == 0) a.cuts[(range << a.log_group) + member].rows = 0;  // (until it has one)
-  const uint32_t x0 = line.begin(range), x1 = min(line.begin(range + 1), all);
-  if (x0 >= all) return;
-  if (x0 >= upto - mine && x0 < upto) {
-    uint32_t at = upto - mine;
-    int i = b0;
-    if (!FEW && per > 1)
-      for (;; ++i) {
-        q = paged_seq(a.batch, i);
-        const uint32_t here = Line::of<KT>(a, q.n, q.len).all;
-        if (x0 - at < here || i == b1 - 1) break;
-        at += here;
-      }
-    found.s = q;
-    found.b = i;
-    found.at = at;
-  }
-  __syncthreads();
-  auto uniform = [](auto x) {  // (from LDS, into scalar registers)
-    static_assert(sizeof(x) % 4 == 0, "whole words");
-    int w[sizeof(x) / 4];
-    __builtin_memcpy(w, &x, sizeof(x));
-#pragma unroll
-    for (int i = 0; i < (int)sizeof(x) / 4; ++i) w[i] = __builtin_amdgcn_readfirstlane(w[i]);
-    __builtin_memcpy(&x, w, sizeof(x));
-    return x;
-  };
-  int b = uniform(found.b);
-  uint32_t at = uniform(found.at);  // of the group on the line
-  if (FEW && per > 1) {
-    // Which of the thread's sequences, one to a lane.  (2,048 of them 184 us searched by the
-    // thread, 176 so; in the other shape, with a fourth of them to a thread, it only adds
-    // instructions to every start: chunks among decoding sequences 103 and 104.)
-    const int end = min(b + per, a.batch.B), lane = threadIdx.x;
-    __syncthreads();  // (found is read)
-    for (;; b += 64) {
-      PagedSeq mine{a.batch.table, 0, 0, 0};
-      if (b + lane < end) mine = paged_seq(a.batch, b + lane);
-      const uint32_t here = Line::of<KT>(a, mine.n, mine.len).all, to = wave_sum_up_to(here);
-      const uint64_t past = __ballot(x0 - at < to);
-      if (past == 0 && b + 64 < end) {
-        at += __builtin_amdgcn_readlane(to, 63);
-        continue;
-      }
-      const int l = past == 0 ? 0 : __builtin_ctzll(past);
-      if (lane == l) {
-        found.s = mine;
-        found.b = b + l;
-        found.at = at + to - here;
-      }
-      break;
-    }
-    __syncthreads();
-    b = uniform(found.b);
-    at = uniform(found.at);
-  }
-  PagedSeq s{uniform(found.s.table), uniform(found.s.len), uniform(found.s.n),
-             uniform(found.s.row0)};
-  Line u = Line::of<KT>(a, s.n, s.len);
-  if (u.all == 0) return;  // (starts that do not ascend)
-  int round = over(x0 - at, u.head), group = 0;
-  at += round * u.head;
-  for (int hi = u.groups - 1; group < hi;) {
-    const int mid = (group + hi + 1) >> 1;
-    if (u.before(a, mid) <= x0 - at) group = mid; else hi = mid - 1;
-  }
-  at += u.before(a, group);
   const int chunks = a.D / Ty::kChunk;
 
   // Keys begin .. end of a row tile, into its rows of the output or the partials from part0
   // on (-1: none).
-  auto piece = [&](int kvh, int tile, int begin, int end, int64_t part0) {
+  auto piece = [&](const PagedSeq& s, int b, int kvh, int tile, int begin, int end,
+                   int64_t part0) {
     const char* kbase = a.k + (int64_t)kvh * a.kh;
     const char* vbase = a.v + (int64_t)kvh * a.vh;
     // The page of the lane-th key of a tile, -1: none.
@@ -711,106 +575,33 @@ __global__ void __launch_bounds__((AttnShape<T, FEW>::kThreads), FEW ? 1 : 2)
     }
   };
 
-  for (uint32_t x = x0;;) {
-    // units from .. to of a group's c
-    const uint32_t c = u.c0 + a.slope * group;
-    const uint32_t from = x - at, to = min(x1 - at, c);
-    // (several heads: one or two tiles of each)
-    const int k = u.heads == 1 ? 0 : member >> (u.tiles - 1);
-    const int kvh = round * u.heads + k;
-    const int tile = u.heads == 1 ? (group << a.log_group) + member : member & (u.tiles - 1);
-    const bool on = k < u.heads && (unsigned)kvh < (unsigned)a.NKVH && tile < u.tiles;
-    // (a sequence of more rows than there is room for is not cut)
-    const int rows = s.n * a.g;
-    const bool cuts = min(rows, kAttnRows) <= a.part_tile;
-    if (on && (cuts || from == 0)) {
-      const bool whole = !cuts || (from == 0 && to == c);
-      const int keys = keys_of(a, s, tile), blocks = (keys + KT - 1) / KT;
-      const int begin = whole ? 0 : cut_at(from, c, blocks, a.extra) * KT;
-      const int end = whole || to == c ? keys : min(keys, cut_at(to, c, blocks, a.extra) * KT);
-      if (x == x0 && from > 0 && at >= line.begin(range - 1) && threadIdx.x == 0)
-        a.cuts[(range << a.log_group) + member] =
-            Cut{min(rows - tile * kAttnRows, kAttnRows), b, kvh, (int)s.row0, tile,
-                line.of(at + c - 1), {}};
-      if (!whole && begin >= end) {  // (a piece of no keys)
-        const int64_t part0 = part_at(a, range, member, from == 0);
-        if ((int)threadIdx.x < min(rows - tile * kAttnRows, kAttnRows))
-          part_ml(a)[part0 + threadIdx.x] = make_float2(-INFINITY, 0.0f);
-      } else {
-        piece(kvh, tile, begin, end, whole ? -1 : part_at(a, range, member, from == 0));
-      }
-    }
-    x = at + to;
-    if (x >= x1) return;
-    at += c;
-    ++group;
-    // (taken anew, so that it is not kept in registers through a piece)
-    s = paged_seq(a.batch, b);
-    u = Line::of<KT>(a, s.n, s.len);
-    if (group == u.groups) {
-      group = 0;
-      ++round;
-    }
-    while (round >= u.rounds) {
-      if (++b >= a.batch.B) return;
-      s = paged_seq(a.batch, b);
-      u = Line::of<KT>(a, s.n, s.len);
-      round = 0;
-    }
-  }
+  walk_line<KT, FEW, kAttnThreads, kAttnRows, Shape::kGrid>(a, piece);
 }
 
 template <typename T, bool FEW>
 AttnPlan plan_shape(const ltv_paged_batch& b, int NH, int NKVH, int D, int max_len) {
   using Shape = AttnShape<T, FEW>;
-  constexpr int KT = Shape::kKeys, kAttnRows = Shape::kRows;
-  AttnPlan p;
-  p.few = FEW;
-  p.log_rows = FEW ? 5 : 7;
   const int64_t g = NH / NKVH, rows = std::max(b.T, 1) * g;
-  const int64_t tiles = (rows + kAttnRows - 1) / kAttnRows;
+  const int64_t tiles = (rows + Shape::kRows - 1) / Shape::kRows;
+  LineShape shape{};
+  shape.keys = Shape::kKeys;
+  shape.log_rows = FEW ? 5 : 7;
+  shape.grid = Shape::kGrid;
   // Groups of four (one, two and four: 132, 126 and 112 us of chunks among decoding sequences,
   // 1,270, 1,246 and 1,239 of the long prompt); float32, whose products take eight times as
   // long as its reads, is better off with each tile by itself (one and four: 49.6 and 52.2).
-  p.group = FEW || sizeof(T) == 4 ? 1 : tiles >= 3 ? 4 : (int)tiles;
-  p.group_tokens = (int)((p.group * kAttnRows + g - 1) / g);
-  // (where no sequence can have more than a block of keys none is cut)
-  const int64_t keys = (int64_t)b.table_width * b.page_size;
-  p.joins = keys > KT;
-  p.part_tile = p.joins ? (int)std::min<int64_t>(rows, kAttnRows) : 0;
+  shape.group = FEW || sizeof(T) == 4 ? 1 : tiles >= 3 ? 4 : (int)tiles;
   // (of few rows all their latency is a tile's: there no range is too short, 18.5 us of a small
   // decode step and 20.9 with two)
-  p.least = (rows <= 32 ? 64 : 128) / KT;
-  // (fewer, if the call has no more tiles than that)
-  const int64_t groups =
-      NKVH * std::min((tiles + p.group - 1) / p.group * b.B,
-                      b.total * g / (p.group * kAttnRows) + b.B);
-  const int64_t most = groups * ((std::max(max_len, 1) + KT - 1) / KT);
-  p.ranges = (int)std::min<int64_t>(Shape::kGrid / p.group, (most + p.least - 1) / p.least);
-  p.ranges = std::max(8, (p.ranges + 7) / 8 * 8);
-  // Positions on the line have 32 bits: units of more blocks where it could be longer than
-  // 2^30, whatever the lengths are.
-  const double bound = (double)NKVH * ((double)b.total * g / (p.group * kAttnRows) + b.B) *
-                       ((double)(keys + b.total) / KT + 64);
-  p.unit = 0;
-  while (bound / (double)(int64_t(1) << p.unit) > (double)(1 << 30)) ++p.unit;
-  p.slope = (int)(p.group * kAttnRows / g / KT) >> p.unit;
-  // What a piece costs beside its keys -- its rows, the first tile's way, the remainders that
-  // the first tiles take, its partials -- counted in blocks: four, or none where few rows have
-  // a range for every few blocks.  (Without and with it: chunks mixed with decoding 110 and 98
-  // us, float32 chunks 50 and 48, a ragged decode step 282 and 261; a small one 17.6 and, with
-  // one block, 18.4.  Two, four and eight for 256 sequences of up to 2,000 tokens 222, 219, 224.)
-  p.extra = (FEW || rows > 32 || most > 8 * Shape::kGrid ? 4 : 0) >> p.unit;
+  shape.least = (rows <= 32 ? 64 : 128) / Shape::kKeys;
+  shape.few = FEW;
+  AttnPlan p = plan_line(b, NH, NKVH, D, max_len, shape);
   // Up to 10^11 operations, by the hints, the products of all probabilities' rests cost next to
   // nothing: 64 sequences of 8,000 tokens (4 heads) 183 us without most of them and 185 with all,
   // 128 of up to 2,000 (8 heads) 108 and 111, 64 of 8,000 with 64 channels (8 heads) 213 and 222,
   // 1,024 new tokens over 8,000 (6 heads) 68.6 and 67.5.  Beyond, 2,048 over 16,000 take 178 and
   // 183, 4,096 over 32,000 518 and 618.
   p.all_rests = 4.0 * D * NH * (double)b.total * std::max(max_len, 1) <= 1e11;
-  const int64_t n = (int64_t)p.ranges * p.group;
-  p.part_rows = n * 2 * p.part_tile;
-  p.cuts_at = (size_t)p.part_rows * (D + 2) * sizeof(float);
-  p.bytes = p.cuts_at + n * sizeof(Cut) + 16;
   return p;
 }
 

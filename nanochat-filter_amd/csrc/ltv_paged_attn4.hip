@@ -13,36 +13,380 @@ namespace {
 // Keys and values of 4-bit pages, for rows_one_by_one.
 struct Fp4Pages {
   static __device__ __forceinline__ void load(const char* block, const AttnArgs& a, uint32_t in,
-                                              int c, float (&x)[8]) {
+                                              int c, float (&x)[8], int shift) {
     const int size = a.batch.div.size;
     const uint32_t codes = *reinterpret_cast<const uint32_t*>(block + in * (a.D / 2) + c * 4);
-    const float s = fp4_scale((uint8_t)block[size * (a.D / 2) + (c >> 2) * size + in]);
+    const float s =
+        ldexpf(fp4_scale((uint8_t)block[size * (a.D / 2) + (c >> 2) * size + in]), -shift);
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = fp4_value(codes >> (4 * e) & 15) * s;
   }
   static __device__ __forceinline__ void keys(const AttnArgs& a, int kvh, int page, uint32_t in,
                                               int c, float (&x)[8]) {
-    load(a.k + kvh * a.kh + (uint64_t)((uint32_t)page * (uint64_t)a.kp) * 16, a, in, c, x);
+    load(a.k + kvh * a.kh + (uint64_t)((uint32_t)page * (uint64_t)a.kp) * 16, a, in, c, x, 0);
   }
   static __device__ __forceinline__ void values(const AttnArgs& a, int kvh, int page, uint32_t in,
-                                                int c, float (&x)[8]) {
-    load(a.v + kvh * a.vh + (uint64_t)((uint32_t)page * (uint64_t)a.vp) * 16, a, in, c, x);
+                                                int c, float (&x)[8], int shift) {
+    load(a.v + kvh * a.vh + (uint64_t)((uint32_t)page * (uint64_t)a.vp) * 16, a, in, c, x, shift);
   }
 };
 
-constexpr int kRowsEach = 16;  // of a workgroup
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
+// How many bfloat16 numbers stand for a query's element and for a probability.  Keys and values
+// are such numbers themselves, so products are exact: a bfloat16 query is one, a float32 one the
+// three of 8 bits each that its 24 are.  A probability rounded to one would be off by 2^-9; two
+// leave 2^-17, three its float32 rounding.
 template <typename T>
-__global__ void __launch_bounds__(256) attn4_rows_kernel(const AttnArgs a) {
-  __shared__ float lds[16 * 130];
-  const int b = blockIdx.z, kvh = blockIdx.y;
-  const PagedSeq s = paged_seq(a.batch, b);
-  const int rows = s.n * a.g;
-  for (int row0 = blockIdx.x * kRowsEach; row0 < rows; row0 += gridDim.x * kRowsEach) {
-    const int end = min(rows, row0 + kRowsEach);
-    const int keys = max(s.len - s.n + a.by_g.quot(end - 1) + 1, 0);
-    rows_one_by_one<T, 256, Fp4Pages>(a, s, b, kvh, row0, end, 0, keys, -1, lds);
+struct Split {
+  static constexpr int kQuery = sizeof(T) == 2 ? 1 : 3, kProb = sizeof(T) == 2 ? 2 : 3;
+};
+
+// Two codes' values in bfloat16, of byte `of` of a word.
+template <int OF>
+__device__ __forceinline__ uint32_t fp4_pair(uint32_t codes, float scale) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, OF));
+}
+// A scale's byte as a float (255 as infinity: the conversion makes a NaN of it).
+__device__ __forceinline__ float scale_bits(uint32_t byte) { return __uint_as_float(byte << 23); }
+
+__device__ __forceinline__ uint4 fp4_eight(uint32_t codes, float s) {
+  return make_uint4(fp4_pair<0>(codes, s), fp4_pair<1>(codes, s), fp4_pair<2>(codes, s),
+                    fp4_pair<3>(codes, s));
+}
+
+// Eight float32 numbers' parts: bits of bfloat16, cut off and not rounded, so that no part passes
+// the range and what is left is exact.
+__device__ __forceinline__ void split_eight(const float (&x)[8], uint4 (&out)[3]) {
+  float rest[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) rest[i] = x[i];
+#pragma unroll
+  for (int n = 0; n < 3; ++n) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t lo = __float_as_uint(rest[2 * i]), hi = __float_as_uint(rest[2 * i + 1]);
+      w[i] = __builtin_amdgcn_perm(hi, lo, 0x07060302);
+      rest[2 * i] -= __uint_as_float(lo & 0xffff0000u);
+      rest[2 * i + 1] -= __uint_as_float(hi & 0xffff0000u);
+    }
+    out[n] = make_uint4(w[0], w[1], w[2], w[3]);
   }
+}
+
+// Eight probabilities' parts: bfloat16, two rounded ones; float32, three as above.
+template <typename T>
+__device__ __forceinline__ void split_probs(const float (&p)[8], uint4 (&out)[Split<T>::kProb]) {
+  if constexpr (sizeof(T) == 4) {
+    split_eight(p, out);
+  } else {
+    uint32_t w[4], r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      w[i] = cvt_pk_bf16(p[2 * i], p[2 * i + 1]);
+      r[i] = cvt_pk_bf16(p[2 * i] - __uint_as_float(w[i] << 16),
+                         p[2 * i + 1] - __uint_as_float(w[i] & 0xffff0000u));
+    }
+    out[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    out[1] = make_uint4(r[0], r[1], r[2], r[3]);
+  }
+}
+
+// Eight elements of a query from element `at` on, in parts.
+template <typename T>
+__device__ __forceinline__ void load_query(const char* q, int at, uint4 (&out)[Split<T>::kQuery]) {
+  if constexpr (sizeof(T) == 2) {
+    __builtin_memcpy(&out[0], reinterpret_cast<const T*>(q) + at, 16);
+  } else {
+    float x[8];
+    __builtin_memcpy(x, reinterpret_cast<const T*>(q) + at, 32);
+    split_eight(x, out);
+  }
+}
+
+__device__ __forceinline__ f32x4 product16(uint4 a, uint4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                 __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// (the four lanes 16 apart)
+__device__ __forceinline__ float across_quarters_max(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false,
+                                                  false);
+  return across_halves_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+
+// Bits of those of four scale bytes that are 192 or more: of values from 2^64 on, whose sums over
+// many keys might pass the range, or of a NaN.  Rows of tiles with such are computed again one by
+// one, with sums that are held 2^-60 smaller and each key left alone by rows that do not see it.
+__device__ __forceinline__ uint32_t large_scales(uint32_t w) { return w & (w << 1) & 0x80808080u; }
+constexpr int kShift = 60;
+
+// ---------------------------------------------------------------------------
+// Few rows: 16 of a row tile
+// ---------------------------------------------------------------------------
+// Each wavefront takes 32 keys of a block of 128 by itself, from memory into registers, and keeps
+// its own maxima, sums and outputs; they are joined through LDS at the end of a piece.
+//
+// Products of 16 x 16 blocks.  S^T = K Q^T: a lane has 8 channels of a key in each step, and the
+// order of the channels is free as long as the queries have it too: a lane takes D / 4 channels
+// that follow each other, one load.  O^T = V^T P^T: the order of the keys is that in which the
+// scores come, and the lane's channels of V are D / 16 that follow each other: one load for each
+// of eight keys, whose values are put beside each other in pairs.
+template <typename T, int D>
+struct FewTile {
+  static constexpr int kSteps = D / 32;                 // of the scores' products
+  static constexpr int kScales = D == 96 ? 3 : 1;       // of a lane's channels of a key
+  static constexpr int kLanes = D == 96 ? 12 : 16;      // with channels of V
+  static constexpr int kCh = D / kLanes;                // of a lane
+  uint32_t k[2][kSteps], ks[2][kScales];
+  uint32_t v[8], vs[2];
+  int n[2];  // keys that are there, of each 16
+};
+
+constexpr int kFewRows = 16, kFewKeys = 128, kFewThreads = 256, kFewGrid = 1024;
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kFewThreads, sizeof(T) == 2 ? 4 : 3)
+    attn4_few_kernel(const AttnArgs a) {
+  using Tile = FewTile<T, D>;
+  constexpr int kSteps = Tile::kSteps, kCh = Tile::kCh, kQ = Split<T>::kQuery,
+                kP = Split<T>::kProb;
+  constexpr int kPitch = D + 4;
+  __shared__ __attribute__((aligned(16))) float lds_o[4 * kFewRows * kPitch];
+  __shared__ float2 lds_ml[4 * kFewRows];
+  static_assert(sizeof(lds_o) >= 16 * 130 * sizeof(float), "room for rows_one_by_one");
+
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  auto piece = [&](const PagedSeq& s, int b, int kvh, int tile, int begin, int end,
+                   int64_t part0) {
+    const int lane = threadIdx.x & 63, c = lane & 15, j = lane >> 4;
+    const char* kbase = a.k + (int64_t)kvh * a.kh;
+    const char* vbase = a.v + (int64_t)kvh * a.vh;
+    const int size = a.batch.div.size, vc = min(c, Tile::kLanes - 1) * kCh;
+    const int row0 = tile * kFewRows, rows = min(s.n * a.g - row0, kFewRows);
+    const bool row_ok = c < rows;
+    const int t = row_ok ? a.by_g.quot(row0 + c) : 0;
+    const int h = kvh * a.g + (row_ok ? row0 + c - t * a.g : 0);
+    const int pos = row_ok ? s.len - s.n + t : -1;
+    const int first_pos = s.len - s.n + a.by_g.quot(row0);  // of the tile's rows
+
+    auto load = [&](int kt, Tile& x) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int at = kt + 16 * half;
+        const int col = min(a.batch.div.quot(at), a.batch.W - 1);
+        const int page = __builtin_amdgcn_readfirstlane(s.table[col]);
+        const bool ok = page >= 0 && page < a.batch.P && at < end;
+        x.n[half] = ok ? min(16, end - at) : 0;
+        const int in = ok ? at - col * size : 0;
+        const uint32_t from = ok ? (uint32_t)page : 0u;
+        const char* kb = kbase + (uint64_t)from * a.kp * 16;
+        const char* vb = vbase + (uint64_t)from * a.vp * 16;
+        __builtin_memcpy(x.k[half], reinterpret_cast<const uint32_t*>(
+                                        kb + (in + c) * (D / 2) + j * (D / 8)), D / 8);
+#pragma unroll
+        for (int e = 0; e < Tile::kScales; ++e)
+          x.ks[half][e] = (uint8_t)kb[size * (D / 2) + (j * (D / 4) + 8 * e) / 32 * size + in + c];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const char* p = vb + (in + 4 * j + e) * (D / 2) + vc / 2;
+          if constexpr (kCh == 8) x.v[4 * half + e] = *reinterpret_cast<const uint32_t*>(p);
+          if constexpr (kCh == 4) x.v[4 * half + e] = *reinterpret_cast<const uint16_t*>(p);
+          if constexpr (kCh == 2) x.v[4 * half + e] = *reinterpret_cast<const uint8_t*>(p);
+        }
+        x.vs[half] = *reinterpret_cast<const uint32_t*>(vb + size * (D / 2) + vc / 32 * size +
+                                                        in + 4 * j);
+      }
+    };
+
+    Tile next;
+    int kt = begin + 32 * wave;
+    if (kt < end) load(kt, next);
+
+    uint4 q[kSteps][kQ];
+    {
+      const int64_t trow = a.batch.starts != nullptr ? s.row0 + t : (int64_t)b * a.batch.T + t;
+      const char* from = a.q + (a.batch.starts != nullptr ? trow * a.qs[1]
+                                                          : b * a.qs[0] + t * a.qs[1]) + h * a.qs[2];
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+#pragma unroll
+        for (int n = 0; n < kQ; ++n) q[i][n] = make_uint4(0, 0, 0, 0);
+        if (row_ok) load_query<T>(from, j * (D / 4) + 8 * i, q[i]);
+      }
+    }
+
+    f32x4 o[kCh];
+#pragma unroll
+    for (int d = 0; d < kCh; ++d) o[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    float m = -INFINITY, l = 0.0f;  // l: of this lane's keys
+    int again = 0;
+    uint32_t large = 0;
+    for (; kt < end; kt += kFewKeys) {
+      Tile x = next;
+      if (kt + kFewKeys < end) load(kt + kFewKeys, next);
+      f32x4 sc[2];
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        sc[half] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+          const uint4 k = fp4_eight(x.k[half][i], scale_bits(x.ks[half][Tile::kScales == 1 ? 0 : i]));
+#pragma unroll
+          for (int n = 0; n < kQ; ++n) sc[half] = product16(k, q[i][n], sc[half]);
+        }
+      }
+      // (a full tile that every row sees needs none of this)
+      if (x.n[0] + x.n[1] < 32 || kt + 31 > first_pos) {
+        // (keys that are not there have no values: whatever their bytes are must not come in as 0
+        // times NaN)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          uint32_t there = 0;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int key = 4 * j + i;
+            if (key < x.n[half]) there |= 255u << (8 * i);
+            if (key >= x.n[half] || kt + 16 * half + key > pos) sc[half][i] = -INFINITY;
+          }
+          x.vs[half] &= there;
+        }
+      }
+      large |= large_scales(x.vs[0]) | large_scales(x.vs[1]);
+      float top = sc[0][0];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) top = fmaxf(top, sc[i / 4][i % 4]);
+      top = across_quarters_max(top) * a.scale;
+      // the maximum in use stays until a score passes it by a factor of 2^8
+      if (__any(top > m + 8.0f)) {
+        const float mn = fmaxf(m, top);
+        // (from here on the argument of an exponential is off by 2^-6 and more)
+        if (__any(fabsf(mn) > 0x1p18f && mn != -INFINITY)) again = 1;
+        const float was = m == mn ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+        m = mn;
+        l *= was;
+#pragma unroll
+        for (int d = 0; d < kCh; ++d)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[d][i] *= was;
+      }
+      const float base = m == -INFINITY ? 0.0f : m;
+      float p[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        p[i] = __builtin_amdgcn_exp2f(fmaf(sc[i / 4][i % 4], a.scale, -base));
+        l += p[i];
+      }
+      uint4 pw[kP];
+      split_probs<T>(p, pw);
+      // V: two channels of eight keys, and of each channel the keys beside each other
+      float scale[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) scale[e] = scale_bits(x.vs[e / 4] >> (8 * (e % 4)) & 255u);
+      auto channels = [&](auto of) {
+        constexpr int kOf = decltype(of)::value;
+        uint32_t w[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = fp4_pair<kOf>(x.v[e], scale[e]);
+#pragma unroll
+        for (int odd = 0; odd < 2; ++odd) {
+          const uint32_t sel = odd ? 0x07060302u : 0x05040100u;
+          const uint4 v = make_uint4(
+              __builtin_amdgcn_perm(w[1], w[0], sel), __builtin_amdgcn_perm(w[3], w[2], sel),
+              __builtin_amdgcn_perm(w[5], w[4], sel), __builtin_amdgcn_perm(w[7], w[6], sel));
+#pragma unroll
+          for (int n = 0; n < kP; ++n) o[2 * kOf + odd] = product16(v, pw[n], o[2 * kOf + odd]);
+        }
+      };
+      channels(std::integral_constant<int, 0>());
+      if constexpr (kCh >= 4) channels(std::integral_constant<int, 1>());
+      if constexpr (kCh == 8) {
+        channels(std::integral_constant<int, 2>());
+        channels(std::integral_constant<int, 3>());
+      }
+    }
+
+    if (__syncthreads_or(again | (int)large)) {
+      const int shift = __syncthreads_or((int)large) ? kShift : 0;
+      rows_one_by_one<T, kFewThreads, Fp4Pages>(a, s, b, kvh, row0, row0 + rows, begin, end, part0,
+                                                lds_o, shift);
+      __syncthreads();
+      return;
+    }
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    if (j == 0) lds_ml[wave * kFewRows + c] = make_float2(m, l);
+    barrier();
+    {
+      float mx = m;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) mx = fmaxf(mx, lds_ml[w * kFewRows + c].x);
+      const float f = __builtin_amdgcn_exp2f(m - (mx == -INFINITY ? 0.0f : mx));
+      // (column c of a block is a row, its rows 4 j .. groups of kCh channels)
+      if (row_ok)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if ((4 * j + i) * kCh >= D) continue;
+          float* to = lds_o + (wave * kFewRows + c) * kPitch + (4 * j + i) * kCh;
+#pragma unroll
+          for (int d = 0; d < kCh; ++d) to[d] = o[d][i] * f;
+        }
+    }
+    barrier();
+    for (int i = threadIdx.x; i < rows * (D / 4); i += kFewThreads) {
+      const int r = i / (D / 4), ch = (i - r * (D / 4)) * 4;
+      float mx = -INFINITY, sum = 0.0f;
+      float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) mx = fmaxf(mx, lds_ml[w * kFewRows + r].x);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float2 ml = lds_ml[w * kFewRows + r];
+        sum = fmaf(ml.y, __builtin_amdgcn_exp2f(ml.x - (mx == -INFINITY ? 0.0f : mx)), sum);
+        const float4 x = *reinterpret_cast<const float4*>(lds_o + (w * kFewRows + r) * kPitch + ch);
+        acc.x += x.x;
+        acc.y += x.y;
+        acc.z += x.z;
+        acc.w += x.w;
+      }
+      const int tt = a.by_g.quot(row0 + r), hh = kvh * a.g + row0 + r - tt * a.g;
+      if (part0 >= 0) {
+        *reinterpret_cast<float4*>(a.part + (part0 + r) * D + ch) = acc;
+        if (ch == 0) part_ml(a)[part0 + r] = make_float2(mx, sum);
+      } else {
+        const int64_t trow = a.batch.starts != nullptr ? s.row0 + tt : (int64_t)b * a.batch.T + tt;
+        char* out = a.out + (a.batch.starts != nullptr ? trow * a.os[1]
+                                                       : b * a.os[0] + tt * a.os[1]) + hh * a.os[2];
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        if constexpr (sizeof(T) == 2)
+          *reinterpret_cast<uint2*>(out + ch * 2) =
+              make_uint2(cvt_pk_bf16(acc.x * inv, acc.y * inv), cvt_pk_bf16(acc.z * inv, acc.w * inv));
+        else
+          *reinterpret_cast<float4*>(out + ch * 4) =
+              make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+        if (ch == 0 && a.lse != nullptr)
+          a.lse[trow * a.NH + hh] =
+              sum == 0.0f ? -INFINITY : (mx + __builtin_amdgcn_logf(sum)) * kLn2;
+      }
+    }
+    barrier();  // (LDS is read)
+  };
+  walk_line<kFewKeys, false, kFewThreads, kFewRows, kFewGrid>(a, piece);
+}
+
+AttnPlan plan_attention4(const ltv_paged_batch& b, int dtype, int NH, int NKVH, int D,
+                         int max_len) {
+  LineShape shape{};
+  shape.keys = kFewKeys;
+  shape.log_rows = 4;
+  shape.grid = kFewGrid;
+  shape.group = 1;
+  shape.least = 1;
+  return plan_line(b, NH, NKVH, D, max_len, shape);
 }
 
 }  // namespace
@@ -52,7 +396,9 @@ using namespace ltv;
 
 extern "C" size_t ltv_paged_attention_fp4_workspace_size(int dtype, const ltv_paged_batch* batch,
                                                          int NH, int NKVH, int D, int max_len) {
-  return 0;
+  if (batch == nullptr || batch->B <= 0 || batch->T < 0 || NKVH <= 0 || NH < NKVH || D <= 0)
+    return 0;
+  return plan_attention4(*batch, dtype, NH, NKVH, D, max_len).bytes;
 }
 
 extern "C" int ltv_paged_attention_fp4(int dtype, const void* q, const int64_t q_strides[3],
@@ -77,7 +423,6 @@ extern "C" int ltv_paged_attention_fp4(int dtype, const void* q, const int64_t q
   if (batch->B == 0 || batch->total == 0 || NH == 0) return LTV_OK;
   LTV_REQUIRE(batch->total * NH < (int64_t(1) << 30), LTV_ERR_UNSUPPORTED,
               "too many new tokens in a call");
-  LTV_REQUIRE(batch->B <= 65535, LTV_ERR_UNSUPPORTED, "more than 65,535 sequences in a call");
   const bool pages = batch->num_pages > 0;
   LTV_REQUIRE(q && out && q_strides && out_strides &&
                   (!pages || (k_pages && v_pages && k_page_strides && v_page_strides)),
@@ -96,25 +441,50 @@ extern "C" int ltv_paged_attention_fp4(int dtype, const void* q, const int64_t q
                 "4-bit pages must be 16-byte aligned");
   }
   const int es = elem_size(dtype);
+  bool out_ok = aligned16(out);
+  for (int i = batch->starts != nullptr ? 1 : 0; i < 3; ++i)
+    out_ok = out_ok && out_strides[i] * es % 16 == 0;
+  LTV_REQUIRE(out_ok, LTV_ERR_UNSUPPORTED, "the output's rows must be 16-byte aligned");
+  const AttnPlan p = plan_attention4(*batch, dtype, NH, NKVH, D, max_len);
+  LTV_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= p.bytes, LTV_ERR_WORKSPACE,
+              "workspace too small");
   AttnArgs a{PagedBatch(*batch), (const char*)q, (const char*)k_pages, (const char*)v_pages,
              (char*)out, lse, (float*)workspace, {}, {},
              pages ? k_page_strides[1] : 0, pages ? v_page_strides[1] : 0,
              pages ? (uint32_t)(k_page_strides[0] / 16) : 0, 0,
-             pages ? (uint32_t)(v_page_strides[0] / 16) : 0, 0, NH, NKVH, D, NH / NKVH, 0, 1, 0,
-             scale * kLog2e, 0, 0, 0, 0, 0, 0, 0, 0, 0, PageDiv(NH / NKVH), PageDiv(1), 0,
-             nullptr, nullptr};
+             pages ? (uint32_t)(v_page_strides[0] / 16) : 0, 0, NH, NKVH, D, NH / NKVH, 0,
+             p.all_rests ? 1 : 0, 0, scale * kLog2e, p.group == 4 ? 2 : p.group - 1, p.ranges,
+             p.least, p.unit, p.group_tokens, p.slope, p.extra, p.log_rows, p.part_tile,
+             PageDiv(NH / NKVH), PageDiv(p.ranges), p.part_rows, nullptr, nullptr};
+  a.cuts = (Cut*)((char*)workspace + p.cuts_at);
+  a.head = (int*)(a.cuts + (size_t)p.ranges * p.group);
   for (int i = 0; i < 3; ++i) {
     a.qs[i] = q_strides[i] * es;
     a.os[i] = out_strides[i] * es;
   }
-  const int64_t rows = (int64_t)std::max(batch->T, 1) * (NH / NKVH);
-  const dim3 grid((unsigned)std::min<int64_t>((rows + kRowsEach - 1) / kRowsEach, 1024), NKVH,
-                  batch->B);
+  const unsigned grid = p.ranges * p.group;
   const hipStream_t st = (hipStream_t)stream;
-  if (dtype == LTV_DTYPE_F32)
-    hipLaunchKernelGGL(attn4_rows_kernel<float>, grid, dim3(256), 0, st, a);
-  else
-    hipLaunchKernelGGL(attn4_rows_kernel<bf16_t>, grid, dim3(256), 0, st, a);
+  auto launch = [&](auto type, auto width) {
+    using T = decltype(type);
+    constexpr int W = decltype(width)::value;
+    hipLaunchKernelGGL((attn4_few_kernel<T, W>), dim3(grid), dim3(kFewThreads), 0, st, a);
+  };
+  auto by_width = [&](auto type) {
+    if (D == 32) launch(type, std::integral_constant<int, 32>());
+    else if (D == 64) launch(type, std::integral_constant<int, 64>());
+    else if (D == 96) launch(type, std::integral_constant<int, 96>());
+    else launch(type, std::integral_constant<int, 128>());
+  };
+  if (dtype == LTV_DTYPE_F32) by_width(float()); else by_width(bf16_t());
   LTV_LAUNCH_CHECK();
+  if (p.joins) {
+    auto join = [&](auto type) {
+      const int each = p.part_tile <= 16 ? 1 : 8;
+      hipLaunchKernelGGL(attn_join_kernel<decltype(type)>,
+                         dim3(grid, (p.part_tile + each - 1) / each), dim3(256), 0, st, a, each);
+    };
+    if (dtype == LTV_DTYPE_F32) join(float()); else join(bf16_t());
+    LTV_LAUNCH_CHECK();
+  }
   return LTV_OK;
 }

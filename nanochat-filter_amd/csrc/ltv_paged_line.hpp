@@ -43,6 +43,34 @@ struct AttnArgs {
   struct Cut* cuts;
 };
 
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+// Nothing is moved across: the tile's loop is written in the order that it is to run in,
+// reads from LDS well ahead of the products that take them and exponentials between the
+// products.  (Left to itself the compiler puts each read right before its product.)
+__device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0); }
+
+__device__ __forceinline__ uint32_t lds_address(uint4* p) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint4*)p;
+}
+template <typename V>
+__device__ __forceinline__ V lds_read(uint32_t at) {
+  return *(__attribute__((address_space(3))) const V*)(uintptr_t)at;
+}
+
+__device__ __forceinline__ void barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+__device__ __forceinline__ float across_halves_max(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false,
+                                                  false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
 // The sum of x over the lanes up to each: within rows of 16 by shifts, then the rows' last.
 __device__ __forceinline__ uint32_t wave_sum_up_to(uint32_t x) {
   x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8
@@ -136,11 +164,12 @@ __device__ __forceinline__ float2* part_ml(const AttnArgs& a) {
 // does not see left alone altogether: the way of tiles with infinite or NaN values among
 // those that some rows do not see.  Groups of sixteen lanes take a row's keys in turn, a lane
 // holding eight channels, which Pages reads (chunk c of a key in its page).  part0: the partials
-// of row0, or -1.
+// of row0, or -1.  shift: values come as 2^-shift of what they are, so that their sum stays in
+// range; (m, l, o) are left as the same (m + shift, l 2^-shift, o 2^-shift).
 template <typename T, int THREADS, typename Pages>
 __device__ __forceinline__ void rows_one_by_one(const AttnArgs& a, const PagedSeq& s, int b,
                                                 int kvh, int row0, int row_end, int begin, int end,
-                                                int64_t part0, float* lds) {
+                                                int64_t part0, float* lds, int shift = 0) {
 #pragma clang fp contract(off)  // (x - base below must not be a fused form of the product)
   float* lds_m = lds;
   constexpr int G = THREADS / 16;
@@ -177,7 +206,7 @@ __device__ __forceinline__ void rows_one_by_one(const AttnArgs& a, const PagedSe
       l = fmaf(l, was, p);
       m = mn;
       if (on) {
-        Pages::values(a, kvh, page, in, c, kv);
+        Pages::values(a, kvh, page, in, c, kv, shift);
         for (int e = 0; e < 8; ++e) o[e] = fmaf(p, kv[e], o[e] * was);
       }
     }
@@ -205,17 +234,183 @@ __device__ __forceinline__ void rows_one_by_one(const AttnArgs& a, const PagedSe
 #pragma unroll
       for (int e = 0, d = d0; d < 128; ++e, d += THREADS)
         if (d < a.D) a.part[at * a.D + d] = acc[e];
-      if (d0 == 0) part_ml(a)[at] = make_float2(mx, sum);
+      if (d0 == 0) part_ml(a)[at] = make_float2(mx + shift, ldexpf(sum, -shift));
     } else {
       char* out = a.out + (a.batch.starts != nullptr ? trow * a.os[1]
                                                      : b * a.os[0] + t * a.os[1]) + h * a.os[2];
 #pragma unroll
       for (int e = 0, d = d0; d < 128; ++e, d += THREADS)
         if (d < a.D)
-          io_traits<T>::store(reinterpret_cast<T*>(out) + d, sum == 0.0f ? 0.0f : acc[e] / sum);
+          io_traits<T>::store(reinterpret_cast<T*>(out) + d,
+                              sum == 0.0f ? 0.0f : ldexpf(acc[e] / sum, shift));
       if (d0 == 0 && a.lse != nullptr)
         a.lse[trow * a.NH + h] = sum == 0.0f ? -INFINITY
                                              : (mx + __builtin_amdgcn_logf(sum)) * kLn2;
+    }
+  }
+}
+
+// A workgroup's range of the line: piece(s, b, kvh, tile, begin, end, part0) computes keys begin ..
+// end of a row tile, into its rows of the output or the partials from part0 on (-1: none).  KT:
+// keys of a block, ROWS: of a row tile, GRID: workgroups that the card holds; FEW: one wavefront,
+// and many sequences to a thread.
+template <int KT, bool FEW, int THREADS, int ROWS, int GRID, typename Piece>
+__device__ __forceinline__ void walk_line(const AttnArgs& a, Piece piece) {
+  constexpr int WAVES = THREADS / 64;
+  // The lengths of all sequences, a run of them to each thread, and their sum.
+  __shared__ uint32_t sums[WAVES];
+  __shared__ struct { PagedSeq s; int b; uint32_t at; } found;  // the sequence of a range's begin
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int per = (a.batch.B + THREADS - 1) / THREADS;
+  const int b0 = min((int)threadIdx.x * per, a.batch.B), b1 = min(b0 + per, a.batch.B);
+  uint32_t mine = 0;
+  PagedSeq q{a.batch.table, 0, 0, 0};
+  for (int i = b0; i < b1; ++i) {
+    q = paged_seq(a.batch, i);
+    mine += Line::of<KT>(a, q.n, q.len).all;
+  }
+  uint32_t upto = wave_sum_up_to(mine);
+  if ((threadIdx.x & 63) == 63) sums[wave] = upto;
+  if (threadIdx.x == 0) {
+    found.s = q;
+    found.b = 0;
+    found.at = 0;
+  }
+  __syncthreads();
+  uint32_t all = 0;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) {
+    if (w < wave) upto += sums[w];
+    all += sums[w];
+  }
+  all = __builtin_amdgcn_readfirstlane(all);
+  Ranges line;
+  line.length = max(a.least, a.by_ranges.quot(all + a.ranges - 1));
+  line.count = min(over(all + line.length - 1, line.length), a.ranges);
+  // Of the two workgroups of a compute unit the older is served first where the products
+  // bound them, and had ended with a fifth of the other's work left: it gets more of it
+  // (a long prompt 1,225 us with equal ranges, 1,187 with these).
+  const bool full = a.log_group > 0 && line.count << a.log_group == GRID;
+  line.lead = full ? line.length / 8 : 0;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *a.head = line.count;
+  // Workgroup w runs on XCD w % 8: consecutive ranges stay on one.
+  const int per_xcd = (line.count + 7) / 8, local = blockIdx.x >> 3 >> a.log_group;
+  const int range = (blockIdx.x & 7) * per_xcd +
+                    (!full ? local : local < per_xcd / 2 ? local * 2 : local * 2 - per_xcd + 1);
+  const int member = (blockIdx.x >> 3) & ((1 << a.log_group) - 1);
+  if (local >= per_xcd || range >= line.count) return;
+  if (threadIdx.x == 0) a.cuts[(range << a.log_group) + member].rows = 0;  // (until it has one)
+  const uint32_t x0 = line.begin(range), x1 = min(line.begin(range + 1), all);
+  if (x0 >= all) return;
+  if (x0 >= upto - mine && x0 < upto) {
+    uint32_t at = upto - mine;
+    int i = b0;
+    if (!FEW && per > 1)
+      for (;; ++i) {
+        q = paged_seq(a.batch, i);
+        const uint32_t here = Line::of<KT>(a, q.n, q.len).all;
+        if (x0 - at < here || i == b1 - 1) break;
+        at += here;
+      }
+    found.s = q;
+    found.b = i;
+    found.at = at;
+  }
+  __syncthreads();
+  auto uniform = [](auto x) {  // (from LDS, into scalar registers)
+    static_assert(sizeof(x) % 4 == 0, "whole words");
+    int w[sizeof(x) / 4];
+    __builtin_memcpy(w, &x, sizeof(x));
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(x) / 4; ++i) w[i] = __builtin_amdgcn_readfirstlane(w[i]);
+    __builtin_memcpy(&x, w, sizeof(x));
+    return x;
+  };
+  int b = uniform(found.b);
+  uint32_t at = uniform(found.at);  // of the group on the line
+  if (FEW && per > 1) {
+    // Which of the thread's sequences, one to a lane.  (2,048 of them 184 us searched by the
+    // thread, 176 so; in the other shape, with a fourth of them to a thread, it only adds
+    // instructions to every start: chunks among decoding sequences 103 and 104.)
+    const int end = min(b + per, a.batch.B), lane = threadIdx.x;
+    __syncthreads();  // (found is read)
+    for (;; b += 64) {
+      PagedSeq mine{a.batch.table, 0, 0, 0};
+      if (b + lane < end) mine = paged_seq(a.batch, b + lane);
+      const uint32_t here = Line::of<KT>(a, mine.n, mine.len).all, to = wave_sum_up_to(here);
+      const uint64_t past = __ballot(x0 - at < to);
+      if (past == 0 && b + 64 < end) {
+        at += __builtin_amdgcn_readlane(to, 63);
+        continue;
+      }
+      const int l = past == 0 ? 0 : __builtin_ctzll(past);
+      if (lane == l) {
+        found.s = mine;
+        found.b = b + l;
+        found.at = at + to - here;
+      }
+      break;
+    }
+    __syncthreads();
+    b = uniform(found.b);
+    at = uniform(found.at);
+  }
+  PagedSeq s{uniform(found.s.table), uniform(found.s.len), uniform(found.s.n),
+             uniform(found.s.row0)};
+  Line u = Line::of<KT>(a, s.n, s.len);
+  if (u.all == 0) return;  // (starts that do not ascend)
+  int round = over(x0 - at, u.head), group = 0;
+  at += round * u.head;
+  for (int hi = u.groups - 1; group < hi;) {
+    const int mid = (group + hi + 1) >> 1;
+    if (u.before(a, mid) <= x0 - at) group = mid; else hi = mid - 1;
+  }
+  at += u.before(a, group);
+  for (uint32_t x = x0;;) {
+    // units from .. to of a group's c
+    const uint32_t c = u.c0 + a.slope * group;
+    const uint32_t from = x - at, to = min(x1 - at, c);
+    // (several heads: one or two tiles of each)
+    const int k = u.heads == 1 ? 0 : member >> (u.tiles - 1);
+    const int kvh = round * u.heads + k;
+    const int tile = u.heads == 1 ? (group << a.log_group) + member : member & (u.tiles - 1);
+    const bool on = k < u.heads && (unsigned)kvh < (unsigned)a.NKVH && tile < u.tiles;
+    // (a sequence of more rows than there is room for is not cut)
+    const int rows = s.n * a.g;
+    const bool cuts = min(rows, ROWS) <= a.part_tile;
+    if (on && (cuts || from == 0)) {
+      const bool whole = !cuts || (from == 0 && to == c);
+      const int keys = keys_of(a, s, tile), blocks = (keys + KT - 1) / KT;
+      const int begin = whole ? 0 : cut_at(from, c, blocks, a.extra) * KT;
+      const int end = whole || to == c ? keys : min(keys, cut_at(to, c, blocks, a.extra) * KT);
+      if (x == x0 && from > 0 && at >= line.begin(range - 1) && threadIdx.x == 0)
+        a.cuts[(range << a.log_group) + member] =
+            Cut{min(rows - tile * ROWS, ROWS), b, kvh, (int)s.row0, tile,
+                line.of(at + c - 1), {}};
+      if (!whole && begin >= end) {  // (a piece of no keys)
+        const int64_t part0 = part_at(a, range, member, from == 0);
+        if ((int)threadIdx.x < min(rows - tile * ROWS, ROWS))
+          part_ml(a)[part0 + threadIdx.x] = make_float2(-INFINITY, 0.0f);
+      } else {
+        piece(s, b, kvh, tile, begin, end, whole ? -1 : part_at(a, range, member, from == 0));
+      }
+    }
+    x = at + to;
+    if (x >= x1) return;
+    at += c;
+    ++group;
+    // (taken anew, so that it is not kept in registers through a piece)
+    s = paged_seq(a.batch, b);
+    u = Line::of<KT>(a, s.n, s.len);
+    if (group == u.groups) {
+      group = 0;
+      ++round;
+    }
+    while (round >= u.rounds) {
+      if (++b >= a.batch.B) return;
+      s = paged_seq(a.batch, b);
+      u = Line::of<KT>(a, s.n, s.len);
+      round = 0;
     }
   }
 }
@@ -321,6 +516,56 @@ struct AttnPlan {
   int64_t part_rows;
   size_t bytes, cuts_at;
 };
+
+// What a kernel is made for, and what was found best for it.
+struct LineShape {
+  int keys, log_rows;  // of a block, of a row tile
+  int grid;            // workgroups that the card holds
+  int group;           // row tiles side by side
+  int least;           // blocks of the shortest range
+  bool few;
+};
+
+AttnPlan plan_line(const ltv_paged_batch& b, int NH, int NKVH, int D, int max_len,
+                   const LineShape& shape) {
+  AttnPlan p{};
+  p.few = shape.few;
+  p.log_rows = shape.log_rows;
+  p.group = shape.group;
+  p.least = shape.least;
+  const int KT = shape.keys;
+  const int64_t tile = int64_t(1) << shape.log_rows, group_rows = p.group * tile;
+  const int64_t g = NH / NKVH, rows = std::max(b.T, 1) * g, tiles = (rows + tile - 1) / tile;
+  p.group_tokens = (int)((group_rows + g - 1) / g);
+  // (where no sequence can have more than a block of keys none is cut)
+  const int64_t keys = (int64_t)b.table_width * b.page_size;
+  p.joins = keys > KT;
+  p.part_tile = p.joins ? (int)std::min<int64_t>(rows, tile) : 0;
+  // (fewer, if the call has no more tiles than that)
+  const int64_t groups =
+      NKVH * std::min((tiles + p.group - 1) / p.group * b.B, b.total * g / group_rows + b.B);
+  const int64_t most = groups * ((std::max(max_len, 1) + KT - 1) / KT);
+  p.ranges = (int)std::min<int64_t>(shape.grid / p.group, (most + p.least - 1) / p.least);
+  p.ranges = std::max(8, (p.ranges + 7) / 8 * 8);
+  // Positions on the line have 32 bits: units of more blocks where it could be longer than
+  // 2^30, whatever the lengths are.
+  const double bound = (double)NKVH * ((double)b.total * g / group_rows + b.B) *
+                       ((double)(keys + b.total) / KT + 64);
+  p.unit = 0;
+  while (bound / (double)(int64_t(1) << p.unit) > (double)(1 << 30)) ++p.unit;
+  p.slope = (int)(group_rows / g / KT) >> p.unit;
+  // What a piece costs beside its keys -- its rows, the first tile's way, the remainders that
+  // the first tiles take, its partials -- counted in blocks: four, or none where few rows have
+  // a range for every few blocks.  (Without and with it: chunks mixed with decoding 110 and 98
+  // us, float32 chunks 50 and 48, a ragged decode step 282 and 261; a small one 17.6 and, with
+  // one block, 18.4.  Two, four and eight for 256 sequences of up to 2,000 tokens 222, 219, 224.)
+  p.extra = (p.few || rows > 32 || most > 8 * shape.grid ? 4 : 0) >> p.unit;
+  const int64_t n = (int64_t)p.ranges * p.group;
+  p.part_rows = n * 2 * p.part_tile;
+  p.cuts_at = (size_t)p.part_rows * (D + 2) * sizeof(float);
+  p.bytes = p.cuts_at + n * sizeof(Cut) + 16;
+  return p;
+}
 
 }  // namespace
 }  // namespace ltv
