@@ -144,13 +144,22 @@ struct FewTile {
   static constexpr int kCh = D / kLanes;                // of a lane
   uint32_t k[2][kSteps], ks[2][kScales];
   uint32_t v[8], vs[2];
-  int n[2];  // keys that are there, of each 16
 };
 
-constexpr int kFewRows = 16, kFewKeys = 128, kFewThreads = 256, kFewGrid = 1024;
+#ifndef LB
+#define LB 3
+#endif
+#ifndef LBF
+#define LBF 2
+#endif
+constexpr int kFewRows = 16, kFewKeys = 128, kFewThreads = 256;
+// Workgroups of a compute unit, as their registers allow.
+template <typename T>
+constexpr int kFewEach = sizeof(T) == 2 ? LB : LBF;
+
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kFewThreads, sizeof(T) == 2 ? 4 : 3)
+__global__ void __launch_bounds__(kFewThreads, kFewEach<T>)
     attn4_few_kernel(const AttnArgs a) {
   using Tile = FewTile<T, D>;
   constexpr int kSteps = Tile::kSteps, kCh = Tile::kCh, kQ = Split<T>::kQuery,
@@ -174,38 +183,68 @@ __global__ void __launch_bounds__(kFewThreads, sizeof(T) == 2 ? 4 : 3)
     const int pos = row_ok ? s.len - s.n + t : -1;
     const int first_pos = s.len - s.n + a.by_g.quot(row0);  // of the tile's rows
 
-    auto load = [&](int kt, Tile& x) {
+    // (offsets of the lane from what is the same for all: bases in scalar registers)
+    const uint32_t koff = c * (D / 2) + j * (D / 8), voff = 4 * j * (D / 2) + vc / 2;
+    const uint32_t vsoff = vc / 32 * size + 4 * j;
+    uint32_t ksoff[Tile::kScales];
+#pragma unroll
+    for (int e = 0; e < Tile::kScales; ++e) ksoff[e] = (j * (D / 4) + 8 * e) / 32 * size + c;
+    // The pages of the 32 keys from kt on, looked up a tile ahead of their use.
+    auto look_up = [&](int kt, int (&page)[2]) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+        page[half] = page_at(s.table, min(a.batch.div.quot(kt + 16 * half), a.batch.W - 1));
+    };
+    // Where the 16 keys from `at` on are, and how many there are.
+    struct Place {
+      const char *k, *v;  // their page's block
+      uint32_t in;
+      int n;
+    };
+    auto place = [&](int at, int page) {
+      const bool ok = page >= 0 && page < a.batch.P && at < end;
+      const uint32_t from = ok ? (uint32_t)page : 0u;
+      return Place{kbase + (uint64_t)from * a.kp * 16, vbase + (uint64_t)from * a.vp * 16,
+                   ok ? (uint32_t)(at - a.batch.div.quot(at) * size) : 0u, ok ? min(16, end - at) : 0};
+    };
+    Tile x;
+    auto load_keys = [&](const Place (&p)[2]) {
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const int at = kt + 16 * half;
-        const int col = min(a.batch.div.quot(at), a.batch.W - 1);
-        const int page = __builtin_amdgcn_readfirstlane(s.table[col]);
-        const bool ok = page >= 0 && page < a.batch.P && at < end;
-        x.n[half] = ok ? min(16, end - at) : 0;
-        const int in = ok ? at - col * size : 0;
-        const uint32_t from = ok ? (uint32_t)page : 0u;
-        const char* kb = kbase + (uint64_t)from * a.kp * 16;
-        const char* vb = vbase + (uint64_t)from * a.vp * 16;
-        __builtin_memcpy(x.k[half], reinterpret_cast<const uint32_t*>(
-                                        kb + (in + c) * (D / 2) + j * (D / 8)), D / 8);
+        const char* codes = p[half].k + p[half].in * (D / 2);
+        const char* scales = p[half].k + size * (D / 2) + p[half].in;
+        __builtin_memcpy(x.k[half], reinterpret_cast<const uint32_t*>(codes + koff), D / 8);
 #pragma unroll
-        for (int e = 0; e < Tile::kScales; ++e)
-          x.ks[half][e] = (uint8_t)kb[size * (D / 2) + (j * (D / 4) + 8 * e) / 32 * size + in + c];
+        for (int e = 0; e < Tile::kScales; ++e) x.ks[half][e] = (uint8_t)scales[ksoff[e]];
+      }
+    };
+    auto load_values = [&](const Place (&p)[2]) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const char* codes = p[half].v + p[half].in * (D / 2);
+        const char* scales = p[half].v + size * (D / 2) + p[half].in;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const char* p = vb + (in + 4 * j + e) * (D / 2) + vc / 2;
-          if constexpr (kCh == 8) x.v[4 * half + e] = *reinterpret_cast<const uint32_t*>(p);
-          if constexpr (kCh == 4) x.v[4 * half + e] = *reinterpret_cast<const uint16_t*>(p);
-          if constexpr (kCh == 2) x.v[4 * half + e] = *reinterpret_cast<const uint8_t*>(p);
+          const char* from = codes + voff + e * (D / 2);
+          if constexpr (kCh == 8) x.v[4 * half + e] = *reinterpret_cast<const uint32_t*>(from);
+          if constexpr (kCh == 4) x.v[4 * half + e] = *reinterpret_cast<const uint16_t*>(from);
+          if constexpr (kCh == 2) x.v[4 * half + e] = *reinterpret_cast<const uint8_t*>(from);
         }
-        x.vs[half] = *reinterpret_cast<const uint32_t*>(vb + size * (D / 2) + vc / 32 * size +
-                                                        in + 4 * j);
+        x.vs[half] = *reinterpret_cast<const uint32_t*>(scales + vsoff);
       }
     };
 
-    Tile next;
+    int pages[2] = {0, 0}, n[2] = {0, 0};
     int kt = begin + 32 * wave;
-    if (kt < end) load(kt, next);
+    if (kt < end) {
+      look_up(kt, pages);
+      const Place at[2] = {place(kt, pages[0]), place(kt + 16, pages[1])};
+      load_keys(at);
+      load_values(at);
+      n[0] = at[0].n;
+      n[1] = at[1].n;
+      look_up(kt + kFewKeys, pages);
+    }
 
     uint4 q[kSteps][kQ];
     {
@@ -226,9 +265,8 @@ __global__ void __launch_bounds__(kFewThreads, sizeof(T) == 2 ? 4 : 3)
     float m = -INFINITY, l = 0.0f;  // l: of this lane's keys
     int again = 0;
     uint32_t large = 0;
+    // The next tile's keys and values take the place of this one's as soon as those are used.
     for (; kt < end; kt += kFewKeys) {
-      Tile x = next;
-      if (kt + kFewKeys < end) load(kt + kFewKeys, next);
       f32x4 sc[2];
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
@@ -240,8 +278,12 @@ __global__ void __launch_bounds__(kFewThreads, sizeof(T) == 2 ? 4 : 3)
           for (int n = 0; n < kQ; ++n) sc[half] = product16(k, q[i][n], sc[half]);
         }
       }
+      in_order();
+      const Place next[2] = {place(kt + kFewKeys, pages[0]), place(kt + kFewKeys + 16, pages[1])};
+      const bool more = kt + kFewKeys < end;
+      if (more) load_keys(next);
       // (a full tile that every row sees needs none of this)
-      if (x.n[0] + x.n[1] < 32 || kt + 31 > first_pos) {
+      if (n[0] + n[1] < 32 || kt + 31 > first_pos) {
         // (keys that are not there have no values: whatever their bytes are must not come in as 0
         // times NaN)
 #pragma unroll
@@ -250,8 +292,8 @@ __global__ void __launch_bounds__(kFewThreads, sizeof(T) == 2 ? 4 : 3)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int key = 4 * j + i;
-            if (key < x.n[half]) there |= 255u << (8 * i);
-            if (key >= x.n[half] || kt + 16 * half + key > pos) sc[half][i] = -INFINITY;
+            if (key < n[half]) there |= 255u << (8 * i);
+            if (key >= n[half] || kt + 16 * half + key > pos) sc[half][i] = -INFINITY;
           }
           x.vs[half] &= there;
         }
@@ -307,6 +349,13 @@ __global__ void __launch_bounds__(kFewThreads, sizeof(T) == 2 ? 4 : 3)
       if constexpr (kCh == 8) {
         channels(std::integral_constant<int, 2>());
         channels(std::integral_constant<int, 3>());
+      }
+      in_order();
+      if (more) {
+        load_values(next);
+        n[0] = next[0].n;
+        n[1] = next[1].n;
+        look_up(kt + 2 * kFewKeys, pages);
       }
     }
 
@@ -375,7 +424,7 @@ __global__ void __launch_bounds__(kFewThreads, sizeof(T) == 2 ? 4 : 3)
     }
     barrier();  // (LDS is read)
   };
-  walk_line<kFewKeys, false, kFewThreads, kFewRows, kFewGrid>(a, piece);
+  walk_line<kFewKeys, false, kFewThreads, kFewRows, 256 * kFewEach<T>>(a, piece);
 }
 
 AttnPlan plan_attention4(const ltv_paged_batch& b, int dtype, int NH, int NKVH, int D,
@@ -383,7 +432,7 @@ AttnPlan plan_attention4(const ltv_paged_batch& b, int dtype, int NH, int NKVH, 
   LineShape shape{};
   shape.keys = kFewKeys;
   shape.log_rows = 4;
-  shape.grid = kFewGrid;
+  shape.grid = 256 * (dtype == LTV_DTYPE_F32 ? kFewEach<float> : kFewEach<bf16_t>);
   shape.group = 1;
   shape.least = 1;
   return plan_line(b, NH, NKVH, D, max_len, shape);

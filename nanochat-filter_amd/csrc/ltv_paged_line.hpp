@@ -82,6 +82,11 @@ __device__ __forceinline__ uint32_t wave_sum_up_to(uint32_t x) {
   return x;
 }
 
+// An entry of a page table, through the scalar cache (col and table are the same for all lanes).
+__device__ __forceinline__ int page_at(const int32_t* table, int col) {
+  return *(const __attribute__((address_space(4))) int32_t*)(uintptr_t)(table + col);
+}
+
 // (row numbers stay below 2^30: divisions of 64 bits would take longer than small calls)
 __device__ __forceinline__ int over(int a, int b) { return (int)((unsigned)a / (unsigned)b); }
 
