@@ -31,6 +31,7 @@ struct Fp4Pages {
   }
 };
 
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -427,15 +428,406 @@ __global__ void __launch_bounds__(kFewThreads, kFewEach<T>)
   walk_line<kFewKeys, false, kFewThreads, kFewRows, 256 * kFewEach<T>>(a, piece);
 }
 
+// ---------------------------------------------------------------------------
+// Many rows: 128 of a row tile
+// ---------------------------------------------------------------------------
+// 32 rows to each of four wavefronts, and tiles of 64 keys that they share: each thread turns a
+// sixteenth of a token's channels of K and of V into bfloat16 and puts them into LDS, a tile ahead
+// of the products.  Those are in 32 x 32 blocks, S^T = K Q^T and O^T = V^T P^T as over 16-bit
+// pages: a lane holds 16 keys of one row, and its probabilities are, without any exchange, the
+// right-hand operand of the second product (ds_read_b64_tr_b16 transposes four keys of a column).
+constexpr int kManyRows = 128, kManyKeys = 64, kManyThreads = 256;
+template <typename T>
+constexpr int kManyEach = sizeof(T) == 2 ? 2 : 1;  // workgroups of a compute unit
+
+// Rows of DP channels (D padded with zeros) in LDS; chunk c (8 channels) of row r sits in a slot
+// chosen so that the lanes of one read fall on different banks: of K 16 consecutive rows, one
+// chunk each, of V four rows, 64 bytes each.
+template <int DP>
+struct ManyTile {
+  static constexpr int kChunks = DP / 8, kPhase = kChunks < 16 ? 2 : 1;
+  static constexpr int kUnits = kManyKeys * kChunks, kRow = kChunks * 16, kBytes = kUnits * 16;
+  static __device__ __forceinline__ int k_slot(int r, int c) {
+    return r * kChunks + (c ^ ((r / kPhase) & (kChunks - 1)));
+  }
+  static __device__ __forceinline__ int v_swizzle(int r) {
+    return ((r / kPhase) & (4 / kPhase - 1)) * 4;
+  }
+  static __device__ __forceinline__ int v_slot(int r, int c) {
+    return r * kChunks + (c ^ v_swizzle(r));
+  }
+};
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ f32x16 product32(uint4 a, uint4 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
+                                                 __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kManyThreads, kManyEach<T>) attn4_many_kernel(const AttnArgs a) {
+  constexpr int DP = D <= 64 ? 64 : 128;
+  using Ti = ManyTile<DP>;
+  constexpr int KT = kManyKeys, KB = KT / 32, kSteps = DP / 16, kDB = DP / 32;
+  constexpr int kQ = Split<T>::kQuery, kP = Split<T>::kProb;
+  constexpr int NC = D / 32, NS = D == 96 ? 3 : 1;  // chunks and scales of a thread's channels
+  __shared__ uint4 lds[4 * Ti::kUnits];             // K, V, and again
+  static_assert(sizeof(lds) >= 16 * 130 * sizeof(float), "room for rows_one_by_one");
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+
+  auto zero_padding = [&]() {
+    if constexpr (D != DP) {
+      constexpr int kPad = Ti::kChunks - D / 8;
+      for (int i = threadIdx.x; i < 2 * KT * kPad; i += kManyThreads) {
+        const int buf = i / (KT * kPad), r = i / kPad % KT, c = D / 8 + i % kPad;
+        lds[buf * 2 * Ti::kUnits + Ti::k_slot(r, c)] = make_uint4(0, 0, 0, 0);
+        lds[(buf * 2 + 1) * Ti::kUnits + Ti::v_slot(r, c)] = make_uint4(0, 0, 0, 0);
+      }
+    }
+  };
+  zero_padding();
+
+  auto piece = [&](const PagedSeq& s, int b, int kvh, int tile, int begin, int end,
+                   int64_t part0) {
+    const char* kbase = a.k + (int64_t)kvh * a.kh;
+    const char* vbase = a.v + (int64_t)kvh * a.vh;
+    const int size = a.batch.div.size;
+    // (opaque: what follows from the lane is not kept in registers around the pieces)
+    int thread = threadIdx.x;
+    asm volatile("" : "+v"(thread));
+    const int lane = thread & 63, ln = lane & 31, hf = lane >> 5;
+    // The page of the lane-th key of a tile, -1: none or past the end.
+    auto page_of = [&](int kt) {
+      const int at = kt + lane;
+      const int page = s.table[min(a.batch.div.quot(at), a.batch.W - 1)];
+      return at < end && page < a.batch.P ? page : -1;
+    };
+    // A thread's part of a tile: a quarter of the channels of key thread / 4.
+    const int key = thread >> 2, quarter = thread & 3;
+    uint32_t kc[NC], vc[NC], ks[NS], vs[NS];
+    auto load = [&](int kt, int pages) {
+      const int page = __shfl(pages, key), at = kt + key;
+      const bool ok = page >= 0;
+      const uint32_t in = ok ? (uint32_t)(at - a.batch.div.quot(at) * size) : 0u;
+      const uint32_t from = ok ? (uint32_t)page : 0u;
+      const char* kb = kbase + (uint64_t)(from * a.kp) * 16;
+      const char* vb = vbase + (uint64_t)(from * a.vp) * 16;
+      const uint32_t codes = in * (D / 2) + quarter * (D / 8);
+      __builtin_memcpy(kc, reinterpret_cast<const uint32_t*>(kb + codes), D / 8);
+      __builtin_memcpy(vc, reinterpret_cast<const uint32_t*>(vb + codes), D / 8);
+#pragma unroll
+      for (int e = 0; e < NS; ++e) {
+        const uint32_t scale = size * (D / 2) + (quarter * NC + e) / 4 * size + in;
+        ks[e] = (uint8_t)kb[scale];
+        vs[e] = (uint8_t)vb[scale];
+      }
+    };
+    uint32_t large = 0;
+    // (a key that is not there is 0: whatever its bytes are must not come in as 0 times NaN)
+    auto store = [&](uint64_t there, int buf) {
+      const bool ok = there >> key & 1;
+      uint4* to = lds + buf * 2 * Ti::kUnits;
+#pragma unroll
+      for (int e = 0; e < NC; ++e) {
+        const int n = NS == 1 ? 0 : e, c = quarter * NC + e;
+        if (e < NS) large |= ok ? large_scales(vs[e]) : 0u;
+        to[Ti::k_slot(key, c)] = fp4_eight(ok ? kc[e] : 0u, ok ? scale_bits(ks[n]) : 1.0f);
+        to[Ti::kUnits + Ti::v_slot(key, c)] =
+            fp4_eight(ok ? vc[e] : 0u, ok ? scale_bits(vs[n]) : 1.0f);
+      }
+    };
+
+    // the first tile into LDS, the second on its way, the pages of the third
+    uint64_t there = 0, next = 0;
+    int page = -1;
+    if (begin < end) {
+      page = page_of(begin);
+      load(begin, page);
+      next = __ballot(page >= 0);
+      page = page_of(begin + KT);
+    }
+
+    // (Of few rows one wavefront has all products: not on the same SIMD in both workgroups.)
+    const int wrow = tile * kManyRows +
+                     ((wave + (int)(blockIdx.x / (128 * kManyEach<T>)) * 2) & 3) * 32;
+    const int rows = s.n * a.g, row = wrow + ln;
+    const bool row_ok = row < rows;
+    const int t = row_ok ? a.by_g.quot(row) : 0;
+    const int h = kvh * a.g + (row_ok ? row - t * a.g : 0);
+    const int pos = row_ok ? s.len - s.n + t : -1;
+    const int64_t trow = a.batch.starts != nullptr ? s.row0 + t : (int64_t)b * a.batch.T + t;
+    // the last position that any row of the wavefront sees, and the first one's
+    const bool wave_on = wrow < rows;
+    const int wave_end = wave_on ? s.len - s.n + a.by_g.quot(min(wrow + 31, rows - 1)) + 1 : 0;
+    const int wave_min = wave_on ? s.len - s.n + a.by_g.quot(wrow) : 0;
+
+    uint4 q[kQ][kSteps];
+    {
+      const char* from = a.q + (a.batch.starts != nullptr ? trow * a.qs[1]
+                                                          : b * a.qs[0] + t * a.qs[1]) + h * a.qs[2];
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+        uint4 parts[kQ];
+#pragma unroll
+        for (int n = 0; n < kQ; ++n) parts[n] = make_uint4(0, 0, 0, 0);
+        if (row_ok && (2 * i + hf) * 8 < D) load_query<T>(from, (2 * i + hf) * 8, parts);
+#pragma unroll
+        for (int n = 0; n < kQ; ++n) q[n][i] = parts[n];
+      }
+    }
+
+    // Where the lane reads K's row ln, and V's four rows from 4 hf, in the first buffer.  The
+    // swizzles exclusive-or a slot, so a later step's chunk is an exclusive or away; rows further
+    // on a constant.
+    const uint32_t lds0 = lds_address(lds);
+    const uint32_t kat = lds0 + Ti::k_slot(ln, hf) * 16;
+    const int vr = 4 * hf + (lane & 15) / 4;
+    const uint32_t vat = lds0 + Ti::kBytes +
+                         Ti::v_slot(vr, ((lane >> 4) & 1) * 2 + (lane & 3) / 2) * 16 + (lane & 1) * 8;
+
+    f32x16 o[kDB];
+#pragma unroll
+    for (int d = 0; d < kDB; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
+    float m = -INFINITY, l = 0.0f;  // l: of this lane's keys
+    int again = 0;
+
+    if (begin < end) {
+      barrier();  // (the piece before is read to its end)
+      store(next, 0);
+      if (begin + KT < end) load(begin + KT, page);
+    }
+    int buf = 0;
+    for (int kt = begin; kt < end; kt += KT, buf ^= 1) {
+      there = next;
+      barrier();  // this tile is there, and the other buffer is read
+      if (kt + KT < end) {
+        next = __ballot(page >= 0);
+        store(next, buf ^ 1);
+        page = page_of(kt + 2 * KT);
+        if (kt + 2 * KT < end) load(kt + 2 * KT, page);
+      }
+      if (kt >= wave_end) continue;
+      const uint32_t ka = kat + buf * 2 * Ti::kBytes, va = vat + buf * 2 * Ti::kBytes;
+      f32x16 sc[KB];
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sc[kb][i] = 0.0f;
+      {
+        constexpr int N = kSteps * KB, AHEAD = 6;
+        uint4 kf[AHEAD];
+        auto keys = [&](int n) {
+          return __builtin_bit_cast(
+              uint4, lds_read<u32x4>((ka ^ (32 * (n / KB))) + n % KB * 32 * Ti::kRow));
+        };
+#pragma unroll
+        for (int n = 0; n < AHEAD; ++n) kf[n] = keys(n);
+        in_order();
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+#pragma unroll
+          for (int e = 0; e < kQ; ++e) sc[n % KB] = product32(kf[n % AHEAD], q[e][n / KB], sc[n % KB]);
+          if (n + AHEAD < N) kf[n % AHEAD] = keys(n + AHEAD);
+          in_order();
+        }
+      }
+      // keys that the lane's row sees, as bits from the lane half's first
+      if (there != ~0ull || kt + KT - 1 > wave_min) {
+        const int n = pos - kt + 1;  // keys up to the row's own
+        const uint64_t seen = n <= 0 ? 0 : there & (n >= 64 ? ~0ull : (1ull << n) - 1);
+        const uint64_t mine = seen >> (4 * hf);
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (!((mine >> (kb * 32 + 8 * (i / 4) + i % 4)) & 1)) sc[kb][i] = -INFINITY;
+      }
+      float part_top[KB * 2], top = -INFINITY;  // of the lane's keys of each 16
+#pragma unroll
+      for (int e = 0; e < KB * 2; ++e) {
+        part_top[e] = sc[e / 2][8 * (e % 2)];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) part_top[e] = fmaxf(part_top[e], sc[e / 2][8 * (e % 2) + i]);
+        top = fmaxf(top, part_top[e]);
+      }
+      top = across_halves_max(top) * a.scale;
+      // the maximum in use stays until a score passes it by a factor of 2^8
+      if (__any(top > m + 8.0f)) {
+        const float mn = fmaxf(m, top);
+        // (from here on the argument of an exponential is off by 2^-6 and more)
+        if (__any(fabsf(mn) > 0x1p18f && mn != -INFINITY)) again = 1;
+        const float was = m == mn ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+        m = mn;
+        l *= was;
+#pragma unroll
+        for (int d = 0; d < kDB; ++d)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[d][i] *= was;
+      }
+      const float base = m == -INFINITY ? 0.0f : m;
+      constexpr int N = KB * 2;  // steps of 16 keys
+      uint4 vf[2][kDB];
+      auto values = [&](int e, int d) {
+        typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+        union {
+          s16x4 half[2];
+          uint4 v;
+        } f;
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          f.half[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (lds_s16x4*)(uintptr_t)((va ^ (64 * d)) + (16 * e + 8 * x) * Ti::kRow));
+        return f.v;
+      };
+      // Probabilities 2 x, 2 x + 1 of step e
+      auto pair = [&](int e, int x) {
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          const int i = 8 * (e % 2) + 2 * x + y;
+          const float v = __builtin_amdgcn_exp2f(fmaf(sc[e / 2][i], a.scale, -base));
+          sc[e / 2][i] = v;
+          l += v;
+        }
+      };
+      // .. and their next part in bfloat16; what is left of them takes their place
+      auto next_part = [&](int e, int x) {
+        const int i = 8 * (e % 2) + 2 * x;
+        const float p0 = sc[e / 2][i], p1 = sc[e / 2][i + 1];
+        const uint32_t w = sizeof(T) == 2
+                               ? cvt_pk_bf16(p0, p1)
+                               : __builtin_amdgcn_perm(__float_as_uint(p1), __float_as_uint(p0),
+                                                       0x07060302);
+        sc[e / 2][i] = p0 - __uint_as_float(w << 16);
+        sc[e / 2][i + 1] = p1 - __uint_as_float(w & 0xffff0000u);
+        return w;
+      };
+      // Where the products bound a call the rests of bfloat16 probabilities are multiplied for 16
+      // keys with one that weighs more than about a 32nd of its row so far, as over 16-bit pages.
+      uint32_t fine = sizeof(T) == 4 || a.all_rests ? (1u << N) - 1 : 0;
+      if (sizeof(T) == 2 && !a.all_rests && __any(__builtin_amdgcn_exp2f(top - base) * 16.0f > l)) {
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+          if (__any(__builtin_amdgcn_exp2f(fmaf(part_top[e], a.scale, -base)) * 16.0f > l))
+            fine |= 1u << e;
+      }
+      uint32_t w[4], ahead[4];
+#pragma unroll
+      for (int d = 0; d < kDB; ++d) vf[0][d] = values(0, d);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        pair(0, x);
+        w[x] = next_part(0, x);
+      }
+      in_order();
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+#pragma unroll
+        for (int d = 0; d < kDB; ++d) {
+          o[d] = product32(vf[e & 1][d], make_uint4(w[0], w[1], w[2], w[3]), o[d]);
+          if (e + 1 < N) {
+            vf[(e + 1) & 1][d] = values(e + 1, d);
+#pragma unroll
+            for (int x = d * 4 / kDB; x < (d + 1) * 4 / kDB; ++x) {
+              pair(e + 1, x);
+              ahead[x] = next_part(e + 1, x);
+            }
+          }
+          in_order();
+        }
+        if (fine & (1u << e)) {
+#pragma unroll
+          for (int n = 1; n < kP; ++n) {
+            uint32_t rest[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) rest[x] = next_part(e, x);
+#pragma unroll
+            for (int d = 0; d < kDB; ++d)
+              o[d] = product32(vf[e & 1][d], make_uint4(rest[0], rest[1], rest[2], rest[3]), o[d]);
+          }
+        }
+#pragma unroll
+        for (int x = 0; x < 4; ++x) w[x] = ahead[x];
+      }
+    }
+
+    if (__syncthreads_or(again | (int)large)) {
+      const int shift = __syncthreads_or((int)large) ? kShift : 0;
+      rows_one_by_one<T, kManyThreads, Fp4Pages>(a, s, b, kvh, tile * kManyRows,
+                                                 min(rows, (tile + 1) * kManyRows), begin, end,
+                                                 part0, reinterpret_cast<float*>(lds), shift);
+      __syncthreads();
+      zero_padding();
+      return;
+    }
+    l += __shfl_xor(l, 32);
+    if (!row_ok) return;
+    if (part0 >= 0) {
+      const int64_t at = part0 + row - tile * kManyRows;
+      float* po = a.part + at * D;
+#pragma unroll
+      for (int d = 0; d < kDB; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+          const int ch = d * 32 + 2 * i + 4 * hf;
+          if (ch < D)
+            *reinterpret_cast<float4*>(po + ch) =
+                make_float4(o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]);
+        }
+      if (hf == 0) part_ml(a)[at] = make_float2(m, l);
+      return;
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    char* out = a.out + (a.batch.starts != nullptr ? trow * a.os[1]
+                                                   : b * a.os[0] + t * a.os[1]) + h * a.os[2];
+#pragma unroll
+    for (int d = 0; d < kDB; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) {
+        const int ch = d * 32 + 2 * i + 4 * hf;
+        if (ch >= D) continue;
+        const float x[4] = {o[d][i] * inv, o[d][i + 1] * inv, o[d][i + 2] * inv, o[d][i + 3] * inv};
+        if constexpr (sizeof(T) == 2)
+          *reinterpret_cast<uint2*>(out + ch * 2) =
+              make_uint2(cvt_pk_bf16(x[0], x[1]), cvt_pk_bf16(x[2], x[3]));
+        else
+          *reinterpret_cast<float4*>(out + ch * 4) = make_float4(x[0], x[1], x[2], x[3]);
+      }
+    if (hf == 0 && a.lse != nullptr)
+      a.lse[trow * a.NH + h] = l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
+  };
+  walk_line<KT, false, kManyThreads, kManyRows, 256 * kManyEach<T>>(a, piece);
+}
+
+#ifndef FEWMOST
+#define FEWMOST 48
+#endif
 AttnPlan plan_attention4(const ltv_paged_batch& b, int dtype, int NH, int NKVH, int D,
                          int max_len) {
+  const bool f32 = dtype == LTV_DTYPE_F32;
+  const int64_t rows = (int64_t)std::max(b.T, 1) * (NH / NKVH);
   LineShape shape{};
-  shape.keys = kFewKeys;
-  shape.log_rows = 4;
-  shape.grid = 256 * (dtype == LTV_DTYPE_F32 ? kFewEach<float> : kFewEach<bf16_t>);
-  shape.group = 1;
-  shape.least = 1;
-  return plan_line(b, NH, NKVH, D, max_len, shape);
+  const bool few = rows <= FEWMOST;
+  if (few) {
+    shape.keys = kFewKeys;
+    shape.log_rows = 4;
+    shape.grid = 256 * (f32 ? kFewEach<float> : kFewEach<bf16_t>);
+    shape.group = 1;
+    shape.least = 1;
+  } else {
+    const int64_t tiles = (rows + kManyRows - 1) / kManyRows;
+    shape.keys = kManyKeys;
+    shape.log_rows = 7;
+    shape.grid = 256 * (f32 ? kManyEach<float> : kManyEach<bf16_t>);
+    shape.group = f32 ? 1 : tiles >= 3 ? 4 : (int)tiles;
+    shape.least = 2;
+  }
+  AttnPlan p = plan_line(b, NH, NKVH, D, max_len, shape);
+  p.few = few;
+  p.all_rests = 4.0 * D * NH * (double)b.total * std::max(max_len, 1) <= 1e11;
+  return p;
 }
 
 }  // namespace
@@ -516,7 +908,10 @@ extern "C" int ltv_paged_attention_fp4(int dtype, const void* q, const int64_t q
   auto launch = [&](auto type, auto width) {
     using T = decltype(type);
     constexpr int W = decltype(width)::value;
-    hipLaunchKernelGGL((attn4_few_kernel<T, W>), dim3(grid), dim3(kFewThreads), 0, st, a);
+    if (p.few)
+      hipLaunchKernelGGL((attn4_few_kernel<T, W>), dim3(grid), dim3(kFewThreads), 0, st, a);
+    else
+      hipLaunchKernelGGL((attn4_many_kernel<T, W>), dim3(grid), dim3(kManyThreads), 0, st, a);
   };
   auto by_width = [&](auto type) {
     if (D == 32) launch(type, std::integral_constant<int, 32>());
