@@ -505,6 +505,11 @@ __global__ void __launch_bounds__(kManyThreads, kManyEach<T>) attn4_many_kernel(
     };
     // A thread's part of a tile: a quarter of the channels of key thread / 4.
     const int key = thread >> 2, quarter = thread & 3;
+    // The chunks in an order that has the writes of eight lanes (two keys) on different banks, which
+    // the swizzles that the reads need do not.  (In order the conflicts cost 14 % of the cycles of a
+    // long prompt.)
+    const int kturn = NC == 4 ? quarter & 2 : NC == 2 ? key & 1 : 0;
+    const int vturn = NC == 4 ? (quarter & 2) | (key & 1) : kturn;
     uint32_t kc[NC], vc[NC], ks[NS], vs[NS];
     auto load = [&](int kt, int pages) {
       const int page = __shfl(pages, key), at = kt + key;
@@ -514,8 +519,11 @@ __global__ void __launch_bounds__(kManyThreads, kManyEach<T>) attn4_many_kernel(
       const char* kb = kbase + (uint64_t)(from * a.kp) * 16;
       const char* vb = vbase + (uint64_t)(from * a.vp) * 16;
       const uint32_t codes = in * (D / 2) + quarter * (D / 8);
-      __builtin_memcpy(kc, reinterpret_cast<const uint32_t*>(kb + codes), D / 8);
-      __builtin_memcpy(vc, reinterpret_cast<const uint32_t*>(vb + codes), D / 8);
+#pragma unroll
+      for (int e = 0; e < NC; ++e) {
+        kc[e] = *reinterpret_cast<const uint32_t*>(kb + codes + (e ^ kturn) * 4);
+        vc[e] = *reinterpret_cast<const uint32_t*>(vb + codes + (e ^ vturn) * 4);
+      }
 #pragma unroll
       for (int e = 0; e < NS; ++e) {
         const uint32_t scale = size * (D / 2) + (quarter * NC + e) / 4 * size + in;
@@ -530,10 +538,10 @@ __global__ void __launch_bounds__(kManyThreads, kManyEach<T>) attn4_many_kernel(
       uint4* to = lds + buf * 2 * Ti::kUnits;
 #pragma unroll
       for (int e = 0; e < NC; ++e) {
-        const int n = NS == 1 ? 0 : e, c = quarter * NC + e;
+        const int n = NS == 1 ? 0 : e, c = quarter * NC;
         if (e < NS) large |= ok ? large_scales(vs[e]) : 0u;
-        to[Ti::k_slot(key, c)] = fp4_eight(ok ? kc[e] : 0u, ok ? scale_bits(ks[n]) : 1.0f);
-        to[Ti::kUnits + Ti::v_slot(key, c)] =
+        to[Ti::k_slot(key, c + (e ^ kturn))] = fp4_eight(ok ? kc[e] : 0u, ok ? scale_bits(ks[n]) : 1.0f);
+        to[Ti::kUnits + Ti::v_slot(key, c + (e ^ vturn))] =
             fp4_eight(ok ? vc[e] : 0u, ok ? scale_bits(vs[n]) : 1.0f);
       }
     };
@@ -692,17 +700,21 @@ __global__ void __launch_bounds__(kManyThreads, kManyEach<T>) attn4_many_kernel(
           l += v;
         }
       };
-      // .. and their next part in bfloat16; what is left of them takes their place
-      auto next_part = [&](int e, int x) {
+      // .. and their first part in bfloat16, and what comes after part w (float32: in their place)
+      auto first_part = [&](int e, int x) {
         const int i = 8 * (e % 2) + 2 * x;
-        const float p0 = sc[e / 2][i], p1 = sc[e / 2][i + 1];
-        const uint32_t w = sizeof(T) == 2
-                               ? cvt_pk_bf16(p0, p1)
-                               : __builtin_amdgcn_perm(__float_as_uint(p1), __float_as_uint(p0),
-                                                       0x07060302);
-        sc[e / 2][i] = p0 - __uint_as_float(w << 16);
-        sc[e / 2][i + 1] = p1 - __uint_as_float(w & 0xffff0000u);
-        return w;
+        if constexpr (sizeof(T) == 2) return cvt_pk_bf16(sc[e / 2][i], sc[e / 2][i + 1]);
+        return __builtin_amdgcn_perm(__float_as_uint(sc[e / 2][i + 1]),
+                                     __float_as_uint(sc[e / 2][i]), 0x07060302);
+      };
+      auto part_after = [&](int e, int x, uint32_t w) {
+        const int i = 8 * (e % 2) + 2 * x;
+        const float p0 = sc[e / 2][i] - __uint_as_float(w << 16);
+        const float p1 = sc[e / 2][i + 1] - __uint_as_float(w & 0xffff0000u);
+        if constexpr (sizeof(T) == 2) return cvt_pk_bf16(p0, p1);
+        sc[e / 2][i] = p0;
+        sc[e / 2][i + 1] = p1;
+        return __builtin_amdgcn_perm(__float_as_uint(p1), __float_as_uint(p0), 0x07060302);
       };
       // Where the products bound a call the rests of bfloat16 probabilities are multiplied for 16
       // keys with one that weighs more than about a 32nd of its row so far, as over 16-bit pages.
@@ -719,7 +731,7 @@ __global__ void __launch_bounds__(kManyThreads, kManyEach<T>) attn4_many_kernel(
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
         pair(0, x);
-        w[x] = next_part(0, x);
+        w[x] = first_part(0, x);
       }
       in_order();
 #pragma unroll
@@ -732,7 +744,7 @@ __global__ void __launch_bounds__(kManyThreads, kManyEach<T>) attn4_many_kernel(
 #pragma unroll
             for (int x = d * 4 / kDB; x < (d + 1) * 4 / kDB; ++x) {
               pair(e + 1, x);
-              ahead[x] = next_part(e + 1, x);
+              ahead[x] = first_part(e + 1, x);
             }
           }
           in_order();
@@ -740,12 +752,11 @@ __global__ void __launch_bounds__(kManyThreads, kManyEach<T>) attn4_many_kernel(
         if (fine & (1u << e)) {
 #pragma unroll
           for (int n = 1; n < kP; ++n) {
-            uint32_t rest[4];
 #pragma unroll
-            for (int x = 0; x < 4; ++x) rest[x] = next_part(e, x);
+            for (int x = 0; x < 4; ++x) w[x] = part_after(e, x, w[x]);
 #pragma unroll
             for (int d = 0; d < kDB; ++d)
-              o[d] = product32(vf[e & 1][d], make_uint4(rest[0], rest[1], rest[2], rest[3]), o[d]);
+              o[d] = product32(vf[e & 1][d], make_uint4(w[0], w[1], w[2], w[3]), o[d]);
           }
         }
 #pragma unroll
@@ -802,7 +813,7 @@ __global__ void __launch_bounds__(kManyThreads, kManyEach<T>) attn4_many_kernel(
 }
 
 #ifndef FEWMOST
-#define FEWMOST 48
+#define FEWMOST 64
 #endif
 AttnPlan plan_attention4(const ltv_paged_batch& b, int dtype, int NH, int NKVH, int D,
                          int max_len) {
