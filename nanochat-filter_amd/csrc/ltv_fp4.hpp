@@ -26,45 +26,39 @@ __device__ __forceinline__ int fp4_byte(uint32_t abs_bits) {
   const int byte = e - 2 + ((abs_bits & 0x7fffffu) > 0x600000u);
   return e == 255 ? kFp4NaN : min(max(byte, kFp4Low), kFp4High);
 }
-__device__ __forceinline__ int fp4_byte(uint64_t abs_bits) {
-  const int e = (int)(abs_bits >> 52);
-  const int byte = e - 1023 + 127 - 2 + ((abs_bits & 0xfffffffffffffull) > 0xc000000000000ull);
-  return e == 2047 ? kFp4NaN : min(max(byte, kFp4Low), kFp4High);
-}
-
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
-__device__ __forceinline__ uint64_t abs_bits(double x) {
-  return (uint64_t)__double_as_longlong(x) & 0x7fffffffffffffffull;
+
+// The codes of eight values over s, of a byte that is not a NaN's: the conversion unit rounds to the
+// nearest, ties to the even code, and takes 6 for what is beyond.
+__device__ __forceinline__ uint32_t fp4_codes(const float (&x)[8], int byte) {
+  const float s = __uint_as_float((uint32_t)byte << 23);
+  uint32_t w = 0;
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[0], x[1], s, 0);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[2], x[3], s, 1);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[4], x[5], s, 2);
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[6], x[7], s, 3);
 }
 
-// 1 / s of a byte
-__device__ __forceinline__ float fp4_inverse(int byte, float) {
-  return __uint_as_float((uint32_t)(254 - byte) << 23);
+// A float32 number that is on the same side as x of all numbers of few bits, the borders of codes
+// among them: the nearest, or where x is not that its neighbour on x's side.
+__device__ __forceinline__ float beside(double x) {
+  const float f = (float)x;
+  const double d = x - (double)f;
+  // (signs by their bits: f may be -0)
+  const int bits = __float_as_int(f);
+  const int step = d == 0.0 || !(fabsf(f) < INFINITY) ? 0 : (d < 0.0) == (bits < 0) ? 1 : -1;
+  return __int_as_float(bits + step);
 }
-__device__ __forceinline__ double fp4_inverse(int byte, double) {
-  return __longlong_as_double((long long)(1023 + 127 - byte) << 52);
+// Two codes' values, of byte OF of a word, in bfloat16 (scale 2^(byte - 127), which all values
+// are exact with; infinity, the scale byte of a NaN, makes NaNs).
+template <int OF>
+__device__ __forceinline__ uint32_t fp4_pair(uint32_t codes, float scale) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, OF));
 }
-
-// The code of x / s: the nearest, ties to the even one.
-template <typename F>
-__device__ __forceinline__ uint32_t fp4_code(F x, F inverse) {
-  const F a = (x < 0 ? -x : x) * inverse;
-  const uint32_t c = (a > (F)0.25) + (a >= (F)0.75) + (a > (F)1.25) + (a >= (F)1.75) +
-                     (a > (F)2.5) + (a >= (F)3.5) + (a > (F)5.0);
-  return c | (x < 0 ? 8u : 0u);
-}
-
-// s; a NaN for the byte of one.
-__device__ __forceinline__ float fp4_scale(uint32_t byte) {
-  return byte == kFp4NaN ? __uint_as_float(0x7fc00000u) : __uint_as_float(byte << 23);
-}
-
-// The value of a code, without its scale.
-__device__ __forceinline__ float fp4_value(uint32_t code) {
-  const uint32_t m = code & 7;
-  // 0.5 is the only one below 1; 1, 1.5, 2, 3, 4, 6 are 2^(m / 2 - 1) (1 + m % 2 / 2)
-  const float f = m < 2 ? 0.5f * m : __uint_as_float((126 + (m >> 1)) << 23 | (m & 1) << 22);
-  return code & 8 ? -f : f;
+__device__ __forceinline__ float scale_bits(uint32_t byte) { return __uint_as_float(byte << 23); }
+__device__ __forceinline__ uint4 fp4_eight(uint32_t codes, float s) {
+  return make_uint4(fp4_pair<0>(codes, s), fp4_pair<1>(codes, s), fp4_pair<2>(codes, s),
+                    fp4_pair<3>(codes, s));
 }
 
 }  // namespace ltv

@@ -16,10 +16,11 @@ struct Fp4Pages {
                                               int c, float (&x)[8], int shift) {
     const int size = a.batch.div.size;
     const uint32_t codes = *reinterpret_cast<const uint32_t*>(block + in * (a.D / 2) + c * 4);
-    const float s =
-        ldexpf(fp4_scale((uint8_t)block[size * (a.D / 2) + (c >> 2) * size + in]), -shift);
+    const float s = scale_bits((uint8_t)block[size * (a.D / 2) + (c >> 2) * size + in]);
+    unpack16(fp4_eight(codes, s), x, bf16_t());
+    if (shift != 0)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = fp4_value(codes >> (4 * e) & 15) * s;
+      for (int e = 0; e < 8; ++e) x[e] = ldexpf(x[e], -shift);
   }
   static __device__ __forceinline__ void keys(const AttnArgs& a, int kvh, int page, uint32_t in,
                                               int c, float (&x)[8]) {
@@ -44,19 +45,6 @@ template <typename T>
 struct Split {
   static constexpr int kQuery = sizeof(T) == 2 ? 1 : 3, kProb = sizeof(T) == 2 ? 2 : 3;
 };
-
-// Two codes' values in bfloat16, of byte `of` of a word.
-template <int OF>
-__device__ __forceinline__ uint32_t fp4_pair(uint32_t codes, float scale) {
-  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, OF));
-}
-// A scale's byte as a float (255 as infinity: the conversion makes a NaN of it).
-__device__ __forceinline__ float scale_bits(uint32_t byte) { return __uint_as_float(byte << 23); }
-
-__device__ __forceinline__ uint4 fp4_eight(uint32_t codes, float s) {
-  return make_uint4(fp4_pair<0>(codes, s), fp4_pair<1>(codes, s), fp4_pair<2>(codes, s),
-                    fp4_pair<3>(codes, s));
-}
 
 // Eight float32 numbers' parts: bits of bfloat16, cut off and not rounded, so that no part passes
 // the range and what is left is exact.

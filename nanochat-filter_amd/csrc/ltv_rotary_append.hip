@@ -16,6 +16,9 @@
 #include "ltv_fp4.hpp"
 #include "ltv_paged.hpp"
 
+#ifndef AVG
+#define AVG 2
+#endif
 namespace ltv {
 namespace {
 
@@ -33,6 +36,7 @@ struct RotaryArgs {
   int first;      // section of blockIdx.z == 0: 0, or 1 without queries
   int D, log_lanes;
   double eps;  // of the norm, negative: none
+  double per_channel;  // 1 / D
   PageDiv by_heads[3];
 };
 
@@ -56,39 +60,53 @@ __device__ __forceinline__ void store_floats(char* p, const float (&x)[VEC]) {
   }
 }
 
-// Two chunks of eight channels, `lanes` chunks apart, of a token's head into its 4-bit page.
-// A lane of the row's has chunk c and chunk c + chunks.
-template <typename F>
-__device__ __forceinline__ void store_fp4(const F (&y)[2][8], char* block, int in, int page_size,
-                                          int D, int c, int chunks, int lanes) {
-  int own = 0;
+template <int CTRL>
+__device__ __forceinline__ int quad_perm(int x) {
+  return __builtin_amdgcn_update_dpp(0, x, CTRL, 0xf, 0xf, true);
+}
+
+// Two chunks of eight channels of a token's head, half a head apart, into its 4-bit page: a lane of
+// the row's `lanes` has chunks c and c + chunks.
+__device__ __forceinline__ void store_fp4(const float (&y)[2][8], char* block, int in,
+                                          int page_size, int D, int c, int chunks, int lanes) {
+  int byte[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    auto top = abs_bits(y[h][0]);
+    float top = fabsf(y[h][0]);  // (a NaN stays)
 #pragma unroll
-    for (int i = 1; i < 8; ++i) top = max(top, abs_bits(y[h][i]));
-    own |= fp4_byte(top) << (8 * h);
+    for (int i = 1; i < 8; ++i) top = __builtin_elementwise_maximum(top, fabsf(y[h][i]));
+    byte[h] = fp4_byte(abs_bits(top));
   }
-  // (a scale's 32 channels are four chunks: of one half, or of both)
-  const int lane0 = (threadIdx.x & 63) & ~(lanes - 1);
+  // a scale's 32 channels are four chunks
+  if ((chunks & 3) == 0) {  // .. of four lanes beside each other
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      byte[h] = max(byte[h], quad_perm<0xb1>(byte[h]));  // lanes 1, 0, 3, 2
+      byte[h] = max(byte[h], quad_perm<0x4e>(byte[h]));  // lanes 2, 3, 0, 1
+    }
+  } else {  // .. of one half, or of both
+    const int own = byte[0] | byte[1] << 8, lane0 = (threadIdx.x & 63) & ~(lanes - 1);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int j = c + h * chunks;
+      byte[h] = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int other = (j & ~3) + i;
+        const bool second = other >= chunks;
+        const int theirs = __shfl(own, lane0 + (second ? other - chunks : other));
+        byte[h] = max(byte[h], theirs >> (second ? 8 : 0) & 255);
+      }
+    }
+  }
+  if (c >= chunks) return;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int j = c + h * chunks;
-    int byte = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int other = (j & ~3) + i;
-      const bool second = other >= chunks;
-      const int theirs = __shfl(own, lane0 + (second ? other - chunks : other));
-      byte = max(byte, theirs >> (second ? 8 : 0) & 255);
-    }
-    if (c >= chunks) continue;
-    const F inverse = fp4_inverse(byte == kFp4NaN ? kFp4Low : byte, F());
-    uint32_t codes = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) codes |= fp4_code(y[h][i], inverse) << (4 * i);
-    *reinterpret_cast<uint32_t*>(block + in * (D / 2) + j * 4) = byte == kFp4NaN ? 0 : codes;
-    if ((j & 3) == 0) block[page_size * (D / 2) + (j >> 2) * page_size + in] = (char)byte;
+    const bool nan = byte[h] == kFp4NaN;
+    const uint32_t codes = fp4_codes(y[h], nan ? kFp4Low : byte[h]);
+    *reinterpret_cast<uint32_t*>(block + in * (D / 2) + j * 4) = nan ? 0 : codes;
+    if ((j & 3) == 0) block[page_size * (D / 2) + (j >> 2) * page_size + in] = (char)byte[h];
   }
 }
 
@@ -153,7 +171,7 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
           for (int e = 0; e < VEC; ++e) sum = fma(y[0][e], y[0][e], fma(y[1][e], y[1][e], sum));
           for (int d = 1; d < lanes; d <<= 1) sum += __shfl_xor(sum, d);
           // (a token at a negative position stays 0, also with eps 0)
-          const double r = pos < 0 ? 0.0 : 1.0 / sqrt(sum / a.D + a.eps);
+          const double r = pos < 0 ? 0.0 : rsqrt(fma(sum, a.per_channel, a.eps));
 #pragma unroll
           for (int e = 0; e < VEC; ++e) {
             y[0][e] *= r;
@@ -161,10 +179,9 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
           }
         }
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          x[0][e] = (float)y[0][e];
-          x[1][e] = (float)y[1][e];
-        }
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) x[h][e] = FP4 && w == 1 ? beside(y[h][e]) : (float)y[h][e];
       }
     }
     if (FP4 && w > 0) {
@@ -173,10 +190,7 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
         const int at = ok ? page : 0;
         char* block = a.pages[w - 1] + at * a.ps[w - 1][0] + h * a.ps[w - 1][1];
         const int cc = ok ? c : chunks;  // (nothing is written)
-        if (ROTATE && w == 1)
-          store_fp4(y, block, in, a.batch.div.size, a.D, cc, chunks, lanes);
-        else
-          store_fp4(x, block, in, a.batch.div.size, a.D, cc, chunks, lanes);
+        store_fp4(x, block, in, a.batch.div.size, a.D, cc, chunks, lanes);
       }
     } else if (ok && on) {
       char* to = w == 0 ? a.q_out + (a.batch.starts != nullptr ? (s.row0 + t) * a.qo[1]
@@ -247,11 +261,15 @@ __global__ void __launch_bounds__(256) read_kernel(const ReadArgs a) {
     if constexpr (FP4) {
       const int size = a.batch.div.size;
       const uint32_t codes = *reinterpret_cast<const uint32_t*>(block + in * (a.D / 2) + u * 4);
-      const float sc = fp4_scale((uint8_t)block[size * (a.D / 2) + (u >> 2) * size + in]);
-      float x[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = fp4_value(codes >> (4 * e) & 15) * sc;
-      store_floats<T, 8>(to, x);
+      const uint4 x =
+          fp4_eight(codes, scale_bits((uint8_t)block[size * (a.D / 2) + (u >> 2) * size + in]));
+      if constexpr (sizeof(T) == 2) {
+        *reinterpret_cast<uint4*>(to) = x;
+      } else {
+        float f[8];
+        unpack16(x, f, bf16_t());
+        store_floats<T, 8>(to, f);
+      }
     } else {
       *reinterpret_cast<U*>(to) = reinterpret_cast<const U*>(block + in * a.ps[w][2])[u];
     }
@@ -295,10 +313,14 @@ void launch_rotary(const RotaryArgs& a, dim3 grid, hipStream_t st) {
 }
 
 // Blocks over the new tokens of a sequence (T is a hint with starts: they stride over whatever
-// there is).
+// there is).  More than AVG times what the sequences need on average are mostly blocks that look
+// and leave: they cost a microsecond for each thousand or so.  And no more than turn round a few times: each block's
+// first round waits for the sequence's numbers, its page and its rows in turn (12,289 tokens, 1,024
+// blocks 31 us, four times as many 45).
 int blocks_for(const ltv_paged_batch& b, int64_t threads_per_token) {
-  const int64_t n = std::max(b.T, 1) * threads_per_token;
-  return (int)std::max<int64_t>(1, std::min<int64_t>((n + 255) / 256, 1024));
+  const int64_t longest = (std::max(b.T, 1) * threads_per_token + 255) / 256;
+  const int64_t mean = (b.total * threads_per_token / std::max(b.B, 1) + 255) / 256;
+  return (int)std::max<int64_t>(1, std::min({longest, AVG * mean, int64_t(1024)}));
 }
 
 }  // namespace
@@ -347,7 +369,7 @@ extern "C" int ltv_paged_rotary_append(
   RotaryArgs a{PagedBatch(*batch), {(const char*)q, (const char*)k, (const char*)v}, {},
                (char*)q_out, {}, {(char*)k_pages, (char*)v_pages}, {},
                {(const char*)cos, (const char*)sin}, {cos_stride * ts, sin_stride * ts},
-               {NH, NKVH, NKVH}, NH > 0 ? 0 : 1, D, log_lanes, norm_eps,
+               {NH, NKVH, NKVH}, NH > 0 ? 0 : 1, D, log_lanes, norm_eps, 1.0 / D,
                {PageDiv(std::max(NH, 1)), PageDiv(std::max(NKVH, 1)), PageDiv(std::max(NKVH, 1))}};
   for (int i = 0; i < 3; ++i) {
     if (NH > 0) {
@@ -408,7 +430,7 @@ extern "C" int ltv_paged_cache_append_fp4(int dtype, const void* k, const int64_
   while ((1 << log_lanes) < D / 16) ++log_lanes;
   RotaryArgs a{PagedBatch(*batch), {nullptr, (const char*)k, (const char*)v}, {}, nullptr, {},
                {(char*)k_pages, (char*)v_pages}, {}, {nullptr, nullptr}, {0, 0},
-               {0, NKVH, NKVH}, 1, D, log_lanes, -1.0,
+               {0, NKVH, NKVH}, 1, D, log_lanes, -1.0, 1.0 / D,
                {PageDiv(1), PageDiv(NKVH), PageDiv(NKVH)}};
   for (int i = 0; i < 3; ++i) {
     a.ss[1][i] = k_strides[i] * es;

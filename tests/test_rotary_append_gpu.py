@@ -231,6 +231,24 @@ def test_sizes_of_values(dtype, bits):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+def test_results_below_float32(dtype):
+    """Rotated keys that float32 does not hold are 0 in 4 bits, of both signs, beside others."""
+    cache = Cache4([16], 1, 64, 16, 1)
+    x = cache.rand(16, 1, 64)
+    x[:, :, ::3] *= 2.0 ** -126
+    x[::2] *= 2.0 ** -100
+    x = x.to(dtype)
+    c = torch.full((16, 32), 2.0 ** -40, device=DEV)
+    s = torch.full((16, 32), 2.0 ** -60, device=DEV)
+    _ops().paged_rotary_append(x[None], x[None], x[None], c, s, cache.k_pages, cache.v_pages,
+                               cache.table, cache.lens)
+    page = int(cache.table[0, 0])
+    want = held4(rotated64(x, c, s, torch.arange(16, device=DEV), None))[0][:, 0]
+    assert torch.equal(values4(cache.k_pages)[page, 0, :16], want)
+    assert torch.equal(values4(cache.v_pages)[page, 0, :16], held4(x)[0][:, 0])
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
 def test_borders_of_codes(dtype):
     """Every tie, the ends of the scales and what is beyond them, by ``paged_cache_append``."""
     base = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0, 7.0, 0.0], device=DEV)
