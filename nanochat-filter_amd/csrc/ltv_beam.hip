@@ -23,6 +23,7 @@ namespace ltv {
 namespace {
 
 constexpr int kMostBeams = 1024;  // times candidates of each
+constexpr int kMostPieces = 16;   // of a row
 
 struct BeamArgs {
   const float* sums;     // (G * B, pieces, 3)
@@ -53,21 +54,42 @@ __device__ __forceinline__ double wave_sum(double x) {
   return x;
 }
 
+// c tanh(x / c) for the candidates.  Of caps up to 64 by 1 - tanh y = 2 / (e^{2 y} + 1), off by
+// roundings of the cap; of larger ones, beside which z may be small, to its own last bits.
+template <Cap CAP>
+__device__ __forceinline__ double capped64(float x, double cap) {
+  if constexpr (CAP == kNoCap) return x;
+  const double y = (double)x / cap;
+  return CAP == kCap ? cap - 2.0 * cap / (exp(2.0 * y) + 1.0) : cap * tanh(y);
+}
+
 template <Cap CAP>
 __global__ void beam_kernel(const BeamArgs a) {
   extern __shared__ uint64_t lds[];
-  uint64_t* order = lds;                                            // (B, n) scores' keys
-  double* score = reinterpret_cast<double*>(lds + a.B * a.n);       // (B, n)
-  int* token = reinterpret_cast<int*>(lds + 2 * a.B * a.n);         // (B, n)
-  uint64_t* mine = lds + 2 * a.B * a.n + (a.B * a.n + 1) / 2;       // (waves, pieces * n)
+  const int entries = a.B * a.n, all = a.pieces * a.n;
+  uint64_t* order = lds;                                  // (B, n) scores' keys
+  double* score = reinterpret_cast<double*>(lds + entries);  // (B, n)
+  int* token = reinterpret_cast<int*>(lds + 2 * entries);    // (B, n)
+  int* before = token + entries;                          // (B, n)
+  uint64_t* mine = lds + 3 * entries;                     // (waves, pieces * n), pieces > 1
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, waves = blockDim.x >> 6;
-  mine += wave * a.pieces * a.n;
+  mine += wave * all;
   const int64_t g = blockIdx.x;
-  const int all = a.pieces * a.n;
   for (int b = wave; b < a.B; b += waves) {
     const int64_t row = g * a.B + b;
+    // (all on their way at once, also what a finished beam has no use for)
+    const uint64_t* keys = a.keys + row * all;
+    const float* part = a.sums + (row * a.pieces + lane) * 3;
+    const uint64_t first = lane < all ? keys[lane] : 0;
+    double m = 0.0, sum = 0.0;
+    if (lane < a.pieces) {
+      m = part[0];
+      sum = part[1];
+    }
     const double s = a.scores[row];
-    if (a.finished != nullptr && a.finished[row] != 0) {
+    const bool finished = a.finished != nullptr && a.finished[row] != 0;
+    for (int r = lane; r < a.n; r += 64) before[b * a.n + r] = 0;
+    if (finished) {
       for (int r = lane; r < a.n; r += 64) {
         const double x = r == 0 ? s : -INFINITY;
         order[b * a.n + r] = score_key(x);
@@ -77,17 +99,20 @@ __global__ void beam_kernel(const BeamArgs a) {
       continue;
     }
     // the n largest of the pieces' keys, in order, into this beam's part of `order`
-    const uint64_t* keys = a.keys + row * all;
     if (a.pieces == 1) {
-      for (int r = lane; r < a.n; r += 64) order[b * a.n + r] = keys[r];
+      if (lane < a.n) order[b * a.n + lane] = first;
+    } else if (all <= 64) {
+      int rank = 0;
+      for (int j = 0; j < all; ++j) rank += of_lane(first, j) > first;
+      if (first != 0 && rank < a.n) order[b * a.n + rank] = first;
     } else {
       // (the n-th of the first few of every piece is a bound)
       const int each = min(64 / a.pieces, a.n), piece = lane / each;
-      const uint64_t first = piece < a.pieces ? keys[piece * a.n + lane - piece * each] : 0;
-      const uint64_t bound = kth_of_lanes(first, a.n);
+      const uint64_t head = piece < a.pieces ? keys[piece * a.n + lane - piece * each] : 0;
+      const uint64_t bound = kth_of_lanes(head, a.n);
       int have = 0;
       for (int i0 = 0; i0 < all; i0 += 64) {
-        const uint64_t key = i0 + lane < all ? keys[i0 + lane] : 0;
+        const uint64_t key = i0 == 0 ? first : i0 + lane < all ? keys[i0 + lane] : 0;
         const bool in = key != 0 && key >= bound;
         const uint64_t who = __ballot(in);
         if (in) mine[have + __builtin_popcountll(who & ((1ull << lane) - 1))] = key;
@@ -97,54 +122,57 @@ __global__ void beam_kernel(const BeamArgs a) {
       for (int i = lane; i < have; i += 64) {
         const uint64_t key = mine[i];
         int rank = 0;
+#pragma unroll 8
         for (int j = 0; j < have; ++j) rank += mine[j] > key;
         if (rank < a.n) order[b * a.n + rank] = key;
       }
     }
     wave_sync();
     // the row's sums
-    const float* part = a.sums + (row * a.pieces + lane) * 3;
-    double m = 0.0, sum = 0.0;
-    if (lane < a.pieces) {
-      m = part[0];
-      sum = part[1];
-    }
     if constexpr (CAP != kCap) {
       double top = lane < a.pieces ? m : -INFINITY;
-      for (int d = 1; d < 64; d <<= 1) top = fmax(top, __shfl_xor(top, d));
+      for (int d = 1; d < kMostPieces; d <<= 1) top = fmax(top, __shfl_xor(top, d));
       // (a piece of -inf alone has the sum 0; a NaN in a sum stays)
       if (lane < a.pieces && m != -INFINITY) sum *= exp(m - top);
-      m = top;
+      m = __shfl(top, 0);
     } else {
       m = 0.0;
     }
-    // the candidates' z, and the exact terms in place of the pass's
-    double more = 0.0;
-    for (int r = lane; r < a.n; r += 64) {
-      const uint64_t key = order[b * a.n + r];
+    // the candidates' z, and the exact terms in place of the pass's (n is at most 64)
+    double z = 0.0;
+    if (lane < a.n) {
+      const uint64_t key = order[b * a.n + lane];
       const float x = key_value(key);
-      double z = x;
-      if constexpr (CAP != kNoCap) z = (double)a.cap * tanh((double)x / (double)a.cap);
+      z = capped64<CAP>(x, a.cap);
       if constexpr (CAP == kCap)
-        more += exp(z) - (double)cap_exp(cap_r(x, cap_scale_of(a.cap)), a.cap);
-      score[b * a.n + r] = z;
-      token[b * a.n + r] = key_index(key);
+        sum += exp(z) - (double)cap_exp(cap_r(x, cap_scale_of(a.cap)), a.cap);
+      token[b * a.n + lane] = key_index(key);
     }
-    sum = wave_sum(sum + more);
-    const double lse = m + log(sum);
-    for (int r = lane; r < a.n; r += 64) {
-      const double z = score[b * a.n + r];
+    sum = wave_sum(sum);
+    if (lane < a.n) {
+      const double lse = m + log(sum);
       const double x = s == -INFINITY || z == -INFINITY ? -INFINITY : s + (z - lse);
-      score[b * a.n + r] = x;
-      order[b * a.n + r] = score_key(x);
+      score[b * a.n + lane] = x;
+      order[b * a.n + lane] = score_key(x);
     }
   }
   __syncthreads();
-  // by score, beam and place in the beam
-  for (int i = threadIdx.x; i < a.B * a.n; i += blockDim.x) {
+  // By score, beam and place in the beam: how many are before each, counted by all threads.
+  const int shares = max(1, (int)blockDim.x / entries);
+  for (int u = threadIdx.x; u < entries * shares; u += blockDim.x) {
+    const int share = u / entries, i = u - share * entries;
     const uint64_t key = order[i];
     int rank = 0;
-    for (int j = 0; j < a.B * a.n; ++j) rank += order[j] > key || (order[j] == key && j < i);
+#pragma unroll 4
+    for (int j = share; j < entries; j += shares) {
+      const uint64_t other = order[j];
+      rank += other > key || (other == key && j < i);
+    }
+    if (shares > 1) atomicAdd(&before[i], rank); else before[i] = rank;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < entries; i += blockDim.x) {
+    const int rank = before[i];
     if (rank >= a.k) continue;
     const int64_t at = g * a.k + rank;
     a.out_scores[at] = (float)score[i];
@@ -154,8 +182,7 @@ __global__ void beam_kernel(const BeamArgs a) {
 }
 
 size_t beam_lds(int B, int n, int pieces, int waves) {
-  return ((size_t)2 * B * n + (B * n + 1) / 2 + (pieces > 1 ? (size_t)waves * pieces * n : 0)) *
-         sizeof(uint64_t);
+  return ((size_t)3 * B * n + (pieces > 1 ? (size_t)waves * pieces * n : 0)) * sizeof(uint64_t);
 }
 
 }  // namespace

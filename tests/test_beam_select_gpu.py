@@ -108,6 +108,22 @@ def test_selections(G, B, V, k, dtype, cap):
     _check(x, s, k, cap, fin)
 
 
+@pytest.mark.parametrize("G,B,V,k", [(2, 3, 900, 5), (1, 4, 70000, 8)])
+def test_caps_of_any_size(G, B, V, k):
+    """A cap far above the logits changes nothing; one far below leaves all tokens alike."""
+    x, s, fin = _rand(G, B, V, F32)
+    plain = _select(x, s, k, finished=fin)
+    for cap in (1e6, 1e30, 3e38):
+        got = _select(x, s, k, softcap=cap, finished=fin)
+        # (1 - (x / c)^2 / 3 of x is left, and the sums of two passes)
+        assert bool(((got.scores - plain.scores).abs() <= 1e-5).all())
+        assert torch.equal(got.parents, plain.parents) and torch.equal(got.tokens, plain.tokens)
+    for cap in (1e-3, 63.9, 64.1):
+        _check(x, s, k, cap, fin)
+    got = _select(x, s, k, softcap=1e-30)
+    assert bool(torch.isfinite(got.scores).all())
+
+
 @pytest.mark.parametrize("dtype", [BF, F32])
 def test_padding_and_strides(dtype):
     x, s, fin = _rand(3, 4, 1000, dtype, pad=24)
