@@ -1,21 +1,23 @@
 """Generation and scoring with the GPT harness over the paged cache: a prompt in
-chunks, several samples from it (``generate``), and the log probabilities of given
-texts (``score``).
+chunks, several samples from it (``generate``), its most probable continuations
+(``beam_search``), and the log probabilities of given texts (``score``).
 
 The reference's ``nanochat/engine.py`` prefills a prompt once and copies the cache to
 every sample; here the samples share the prompt's pages, a finished sample's pages are
 free for the others, and log probabilities, entropy and alternatives come from one
-pass over the logits.
+pass over the logits.  The cache may hold 4 bits (``make_cache``).
 """
 
 from __future__ import annotations
 
 import contextlib
+import math
 from typing import NamedTuple, Optional, Sequence
 
 import torch
 
 from nanochat_amd.gpt import GPT
+from nanochat_amd.ops.beam_select import beam_select
 from nanochat_amd.ops.token_logprobs import TokenLogprobs, token_logprobs
 from nanochat_amd.paged_kv_cache import PagedKVCache
 
@@ -25,11 +27,29 @@ class Sample(NamedTuple):
     logprobs: list    # of each of its tokens
 
 
-def make_cache(model: GPT, num_pages: int, max_seqs: int, page_size: int = 64) -> PagedKVCache:
+class Beam(NamedTuple):
+    tokens: list      # the continuation, a stop token included
+    logprob: float    # of all of them
+    score: float      # logprob / len(tokens) ** length_penalty
+
+
+# of the model's norm (torch's default for the float32 that it computes in)
+_NORM_EPS = 2.0 ** -23
+
+
+def make_cache(model: GPT, num_pages: int, max_seqs: int, page_size: int = 64, *,
+               bits: Optional[int] = None, rotate: Optional[bool] = None) -> PagedKVCache:
+    """A cache for the model, ``bits=4`` with keys and values in 4 bits.  With ``rotate``
+    (the default of 4 bits) it rotates and normalises queries and keys on their way, in one
+    launch and with one rounding; without, the model does, in its dtype."""
     c = model.config
+    rotary = None
+    if rotate or (rotate is None and bits == 4):
+        rotary = (model.cos[0, :, 0], model.sin[0, :, 0])
     return PagedKVCache(c.n_layer, c.n_head, c.n_kv_head, c.n_embd // c.n_head,
                         num_pages=num_pages, max_seqs=max_seqs, max_len=c.sequence_len,
-                        page_size=page_size, device=model.wte.weight.device)
+                        page_size=page_size, device=model.wte.weight.device, bits=bits,
+                        rotary=rotary, norm_eps=None if rotary is None else _NORM_EPS)
 
 
 def _autocast():
@@ -146,6 +166,69 @@ def _sample(model: GPT, prompt: Sequence[int], n: int, max_tokens: int, top_k: i
                                            cache.step(live, 1))
             logits = model.raw_logits(hidden[:, -1])
     return out
+
+
+@torch.no_grad()
+def beam_search(model: GPT, prompt: Sequence[int], beams: int, max_tokens: int, *,
+                stop: Optional[int] = None, length_penalty: float = 1.0,
+                cache: Optional[PagedKVCache] = None, chunk: int = 2048) -> list[Beam]:
+    """The ``beams`` continuations of the prompt that a search of that width finds the most
+    probable, best first: of up to ``max_tokens`` tokens, or to a ``stop`` token.  At each step
+    the best by log probability go on (an ended one stays as it is); in the end they are in the
+    order of logprob / length ** length_penalty.  A given cache's slots 0 to ``beams`` - 1 are
+    used, which are empty before and after."""
+    n = beams
+    if not 0 < n <= min(32, model.config.vocab_size):
+        raise ValueError(f"beams are 1 to {min(32, model.config.vocab_size)}, got {n}")
+    if max_tokens <= 0:
+        raise ValueError("at least one token")
+    if not math.isfinite(length_penalty):
+        raise ValueError(f"length_penalty must be finite, got {length_penalty}")
+    longest = len(prompt) + max_tokens - 1  # (the last token is not fed)
+    if longest > min(model.config.sequence_len, cache.max_len if cache else longest):
+        raise ValueError(f"{longest} tokens, more than the model or the cache is made for")
+    if cache is None:
+        page = 64
+        shared, own = -(-len(prompt) // page), -(-max_tokens // page) + 1
+        cache = make_cache(model, shared + n * own, n, page)
+    _empty(cache, range(n))
+    with _freed_on_error(cache, range(n)):
+        out = _search(model, prompt, n, max_tokens, stop, cache, chunk)
+    cache.free(range(n))
+    cache.compact()
+    out = [Beam(t, p, p / len(t) ** length_penalty) for t, p in out]
+    return sorted(out, key=lambda b: -b.score)
+
+
+def _search(model: GPT, prompt: Sequence[int], n: int, max_tokens: int, stop: Optional[int],
+            cache: PagedKVCache, chunk: int) -> list[tuple]:
+    """(tokens, log probability) of each beam."""
+    device = cache.page_table.device
+    logits = prefill(model, cache, 0, prompt, chunk).expand(n, -1)
+    if n > 1:
+        cache.fork([0] * (n - 1), list(range(1, n)))
+    # (of beams that are alike only the first counts)
+    scores = torch.full((n,), -math.inf, device=device)
+    scores[0] = 0.0
+    finished = torch.zeros(n, dtype=torch.bool, device=device)
+    tokens = [[] for _ in range(n)]
+    for step in range(max_tokens):
+        best = beam_select(logits, scores, n, softcap=GPT.SOFTCAP, finished=finished)
+        parents, new = best.parents.tolist(), best.tokens.tolist()
+        # (-1: an ended beam)
+        tokens = [tokens[p] + [t] * (t >= 0) for p, t in zip(parents, new)]
+        ended = [t < 0 or t == stop for t in new]
+        scores = best.scores
+        if all(ended) or step + 1 == max_tokens:
+            break
+        finished = torch.tensor(ended, device=device)
+        cache.reorder(list(range(n)), parents)
+        with _autocast():
+            # (an ended beam keeps its place, whatever token it is fed)
+            hidden = model.cached_features(best.tokens.clamp(min=0)[:, None],
+                                           cache.step(list(range(n)), 1))
+            logits = model.raw_logits(hidden[:, -1])
+    return list(zip(tokens, scores.tolist()))
 
 
 @torch.no_grad()

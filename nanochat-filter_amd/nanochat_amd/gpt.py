@@ -99,11 +99,12 @@ class CausalSelfAttention(nn.Module):
 
     def forward_cached(self, x, cos_sin, step):
         """The new tokens x (B, T, C) of a step of the paged cache; cos_sin at their
-        positions, (B, T, 1, head_dim / 2)."""
+        positions, (B, T, 1, head_dim / 2), or None where the cache rotates and normalises."""
         B, T, C = x.size()
         q, k, v = self.qkv_computer(x, step)
-        cos, sin = cos_sin
-        q, k = norm(apply_rotary_emb(q, cos, sin)), norm(apply_rotary_emb(k, cos, sin))
+        if cos_sin is not None:
+            cos, sin = cos_sin
+            q, k = norm(apply_rotary_emb(q, cos, sin)), norm(apply_rotary_emb(k, cos, sin))
         y = step.attend(self.layer_idx, q, k, v, scale=self.scale)
         return self.c_proj(y.reshape(B, T, C))
 
@@ -176,9 +177,11 @@ class GPT(nn.Module):
         longest = max(step.positions) + T
         if longest > self.cos.size(1):  # (indexed on the device, where it would be a fault)
             raise ValueError(f"{longest} tokens, but the model is made for {self.cos.size(1)}")
-        at = torch.tensor(step.positions, device=idx.device)[:, None] + torch.arange(
-            T, device=idx.device)
-        cos_sin = self.cos[0][at], self.sin[0][at]
+        cos_sin = None
+        if not step.rotates:
+            at = torch.tensor(step.positions, device=idx.device)[:, None] + torch.arange(
+                T, device=idx.device)
+            cos_sin = self.cos[0][at], self.sin[0][at]
         x = norm(self.wte(idx))
         for blk in self.h:
             x = blk.forward_cached(x, cos_sin, step)
