@@ -379,8 +379,40 @@ __global__ void __launch_bounds__(256) fork_kernel(const State s, const int32_t*
   if (blockIdx.x == 0 && threadIdx.x == 0) s.lens[to] = s.lens[from];
 }
 
-// Reordering: every row that is wanted is read, and the counts follow, before one is written.
-// All latency: two launches.
+// Reordering: what is wanted of a column is read, and the counts follow, before any of it is
+// written.  The columns do not meet: a workgroup takes some of them, for all entries at once, in
+// LDS.  All latency: 4 entries of 10 pages 1.8 us.
+constexpr int kReorderInts = 8192, kReorderThreads = 1024;
+
+__global__ void __launch_bounds__(kReorderThreads) reorder_kernel(const State s,
+                                                                  const int32_t* slots,
+                                                                  const int32_t* src, int n,
+                                                                  int log_cols) {
+  __shared__ int rows[kReorderInts];
+  __shared__ int lens[kReorderInts >> 2];  // (four columns at least)
+  const int c0 = blockIdx.x << log_cols, mask = (1 << log_cols) - 1;
+  for (int u = threadIdx.x; u < n << log_cols; u += kReorderThreads) {
+    const int i = u >> log_cols, c = c0 + (u & mask), from = src[i], to = slots[i];
+    if (!in(from, s.S) || !in(to, s.S)) continue;
+    if (blockIdx.x == 0 && (u & mask) == 0) lens[i] = s.lens[from];
+    if (c >= s.W) continue;
+    const int page = s.table[from * s.ts + c], old = s.table[to * s.ts + c];
+    if (page != old) {
+      if (in(page, s.P)) atomicAdd(&s.refs[page], 1);
+      if (in(old, s.P)) atomicSub(&s.refs[old], 1);
+    }
+    rows[u] = page;
+  }
+  __syncthreads();
+  for (int u = threadIdx.x; u < n << log_cols; u += kReorderThreads) {
+    const int i = u >> log_cols, c = c0 + (u & mask), from = src[i], to = slots[i];
+    if (!in(from, s.S) || !in(to, s.S)) continue;
+    if (blockIdx.x == 0 && (u & mask) == 0) s.lens[to] = lens[i];
+    if (c < s.W) s.table[to * s.ts + c] = rows[u];
+  }
+}
+
+// Of more entries than that, by way of memory.
 __global__ void __launch_bounds__(256) reorder_read_kernel(const State s, const int32_t* slots,
                                                            const int32_t* src, int32_t* rows,
                                                            int32_t* lens) {
@@ -672,10 +704,21 @@ extern "C" int ltv_paged_cache_reorder(const ltv_page_state* state, const int32_
   LTV_REQUIRE(workspace && aligned16(workspace) &&
                   workspace_bytes >= ltv_paged_cache_reorder_workspace_size(n, state->table_width),
               LTV_ERR_WORKSPACE, "workspace too small");
+  const hipStream_t st = (hipStream_t)stream;
+  if (n <= kReorderInts >> 2) {
+    // (two entries of a thread, so that many workgroups share a call; 384 rows of 502 pages 9.4 us
+    // with 16 columns to each)
+    int log_cols = 6;
+    while (log_cols > 2 && n << log_cols > 2 * kReorderThreads) --log_cols;
+    const int groups = (int)(((int64_t)state->table_width + (1 << log_cols) - 1) >> log_cols);
+    hipLaunchKernelGGL(reorder_kernel, dim3(std::max(1, groups)), dim3(kReorderThreads), 0, st,
+                       state_of(*state), slots, src, n, log_cols);
+    LTV_LAUNCH_CHECK();
+    return LTV_OK;
+  }
   int32_t* lens = reinterpret_cast<int32_t*>(workspace);
   int32_t* rows = lens + n;
   const dim3 grid(std::max(1, std::min((state->table_width + 255) / 256, 64)), n);
-  const hipStream_t st = (hipStream_t)stream;
   hipLaunchKernelGGL(reorder_read_kernel, grid, dim3(256), 0, st, state_of(*state), slots, src,
                      rows, lens);
   LTV_LAUNCH_CHECK();

@@ -127,6 +127,17 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
     const int i = i0 + round * step;
     const int t = a.by_heads[w].quot(min(i, all - 1)), h = min(i, all - 1) - t * a.heads[w];
     const int pos = s.len - s.n + t;
+    const char* from = a.src[w] + (a.batch.starts != nullptr ? (s.row0 + t) * a.ss[w][1]
+                                                             : b * a.ss[w][0] + t * a.ss[w][1]) +
+                       h * a.ss[w][2];
+    // (the row on its way before its page is looked up)
+    float x[2][VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) x[0][e] = x[1][e] = 0.0f;
+    if (i < all && on) {
+      load_floats<T, VEC>(from + c * VEC * sizeof(T), x[0]);
+      load_floats<T, VEC>(from + (half + c * VEC) * sizeof(T), x[1]);
+    }
     bool ok = i < all;
     int page = -1, in = 0;
     if (w > 0) {
@@ -137,16 +148,6 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
         in = pos - col * a.batch.div.size;
         ok = page >= 0 && page < a.batch.P;
       }
-    }
-    const char* from = a.src[w] + (a.batch.starts != nullptr ? (s.row0 + t) * a.ss[w][1]
-                                                             : b * a.ss[w][0] + t * a.ss[w][1]) +
-                       h * a.ss[w][2];
-    float x[2][VEC];
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) x[0][e] = x[1][e] = 0.0f;
-    if (ok && on) {
-      load_floats<T, VEC>(from + c * VEC * sizeof(T), x[0]);
-      load_floats<T, VEC>(from + (half + c * VEC) * sizeof(T), x[1]);
     }
     [[maybe_unused]] double y[2][VEC];
     if constexpr (ROTATE) {

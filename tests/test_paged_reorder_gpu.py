@@ -60,7 +60,9 @@ def _check(m, slots, src, stride=None):
     assert all(r >= 0 for r in m.refs)
 
 
-@pytest.mark.parametrize("S,W,page", [(1, 1, 16), (2, 3, 1), (5, 7, 16), (64, 20, 16), (7, 700, 4)])
+# (more than 2,048 entries go by way of memory; 4 to 64 columns to a workgroup)
+@pytest.mark.parametrize("S,W,page", [(1, 1, 16), (2, 3, 1), (5, 7, 16), (64, 20, 16), (7, 700, 4),
+                                      (300, 67, 16), (512, 33, 16), (513, 5, 16), (900, 18, 1), (2048, 5, 16), (2049, 5, 16), (2600, 9, 4)])
 def test_selections(S, W, page):
     r = random.Random(S)
     for seed in range(4):
