@@ -135,17 +135,11 @@ struct FewTile {
   uint32_t v[8], vs[2];
 };
 
-#ifndef LB
-#define LB 3
-#endif
-#ifndef LBF
-#define LBF 2
-#endif
 constexpr int kFewRows = 16, kFewKeys = 128, kFewThreads = 256;
-// Workgroups of a compute unit, as their registers allow.
+// Workgroups of a compute unit, as their registers allow.  (bfloat16, 64 sequences of 8,000 tokens
+// and 4 heads: two 54 us, three 51, four, which spill, 61.)
 template <typename T>
-constexpr int kFewEach = sizeof(T) == 2 ? LB : LBF;
-
+constexpr int kFewEach = sizeof(T) == 2 ? 3 : 2;
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kFewThreads, kFewEach<T>)
@@ -520,15 +514,17 @@ __global__ void __launch_bounds__(kManyThreads, kManyEach<T>) attn4_many_kernel(
       }
     };
     uint32_t large = 0;
-    // (a key that is not there is 0: whatever its bytes are must not come in as 0 times NaN)
-    auto store = [&](uint64_t there, int buf) {
-      const bool ok = there >> key & 1;
+    // Part x of a tile into LDS: chunk x / 2 of K or V.  (A key that is not there is 0: whatever its
+    // bytes are must not come in as 0 times NaN.)
+    constexpr int kParts = 2 * NC;
+    auto store = [&](int x, bool ok, int buf) {
+      const int e = x / 2, n = NS == 1 ? 0 : e, c = quarter * NC;
       uint4* to = lds + buf * 2 * Ti::kUnits;
-#pragma unroll
-      for (int e = 0; e < NC; ++e) {
-        const int n = NS == 1 ? 0 : e, c = quarter * NC;
+      if (x % 2 == 0) {
+        to[Ti::k_slot(key, c + (e ^ kturn))] =
+            fp4_eight(ok ? kc[e] : 0u, ok ? scale_bits(ks[n]) : 1.0f);
+      } else {
         if (e < NS) large |= ok ? large_scales(vs[e]) : 0u;
-        to[Ti::k_slot(key, c + (e ^ kturn))] = fp4_eight(ok ? kc[e] : 0u, ok ? scale_bits(ks[n]) : 1.0f);
         to[Ti::kUnits + Ti::v_slot(key, c + (e ^ vturn))] =
             fp4_eight(ok ? vc[e] : 0u, ok ? scale_bits(vs[n]) : 1.0f);
       }
@@ -592,27 +588,36 @@ __global__ void __launch_bounds__(kManyThreads, kManyEach<T>) attn4_many_kernel(
 
     if (begin < end) {
       barrier();  // (the piece before is read to its end)
-      store(next, 0);
+#pragma unroll
+      for (int x = 0; x < kParts; ++x) store(x, next >> key & 1, 0);
       if (begin + KT < end) load(begin + KT, page);
     }
     int buf = 0;
     for (int kt = begin; kt < end; kt += KT, buf ^= 1) {
       there = next;
       barrier();  // this tile is there, and the other buffer is read
-      if (kt + KT < end) {
+      // The next tile is put into LDS between the first products (all at once before them, its
+      // conversions and writes cost a long prompt 28 % of its time), the one after it loaded then.
+      const bool more = kt + KT < end, after = kt + 2 * KT < end;
+      if (more) {
         next = __ballot(page >= 0);
-        store(next, buf ^ 1);
         page = page_of(kt + 2 * KT);
-        if (kt + 2 * KT < end) load(kt + 2 * KT, page);
       }
-      if (kt >= wave_end) continue;
+      const bool ok = next >> key & 1;
+      if (kt >= wave_end) {
+        if (more)
+#pragma unroll
+          for (int x = 0; x < kParts; ++x) store(x, ok, buf ^ 1);
+        if (after) load(kt + 2 * KT, page);
+        continue;
+      }
       const uint32_t ka = kat + buf * 2 * Ti::kBytes, va = vat + buf * 2 * Ti::kBytes;
       f32x16 sc[KB];
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
         for (int i = 0; i < 16; ++i) sc[kb][i] = 0.0f;
-      {
+      auto scores = [&](auto with_store) {
         constexpr int N = kSteps * KB, AHEAD = 6;
         uint4 kf[AHEAD];
         auto keys = [&](int n) {
@@ -627,9 +632,14 @@ __global__ void __launch_bounds__(kManyThreads, kManyEach<T>) attn4_many_kernel(
 #pragma unroll
           for (int e = 0; e < kQ; ++e) sc[n % KB] = product32(kf[n % AHEAD], q[e][n / KB], sc[n % KB]);
           if (n + AHEAD < N) kf[n % AHEAD] = keys(n + AHEAD);
+          if constexpr (decltype(with_store)::value)
+#pragma unroll
+            for (int x = n * kParts / N; x < (n + 1) * kParts / N; ++x) store(x, ok, buf ^ 1);
           in_order();
         }
-      }
+      };
+      if (more) scores(std::true_type()); else scores(std::false_type());
+      if (after) load(kt + 2 * KT, page);
       // keys that the lane's row sees, as bits from the lane half's first
       if (there != ~0ull || kt + KT - 1 > wave_min) {
         const int n = pos - kt + 1;  // keys up to the row's own
@@ -800,15 +810,17 @@ __global__ void __launch_bounds__(kManyThreads, kManyEach<T>) attn4_many_kernel(
   walk_line<KT, false, kManyThreads, kManyRows, 256 * kManyEach<T>>(a, piece);
 }
 
-#ifndef FEWMOST
-#define FEWMOST 64
-#endif
+// Up to how many rows of a k/v head tiles of 16 read every key for themselves: 16 sequences of
+// 4,000 tokens, 4 heads with 32 rows 39 us in tiles of 16 and 45 in one of 128, with 64 rows 49 and
+// 55, with 128 rows 71 and 63.
+constexpr int kMostFewRows = 64;
+
 AttnPlan plan_attention4(const ltv_paged_batch& b, int dtype, int NH, int NKVH, int D,
                          int max_len) {
   const bool f32 = dtype == LTV_DTYPE_F32;
   const int64_t rows = (int64_t)std::max(b.T, 1) * (NH / NKVH);
   LineShape shape{};
-  const bool few = rows <= FEWMOST;
+  const bool few = rows <= kMostFewRows;
   if (few) {
     shape.keys = kFewKeys;
     shape.log_rows = 4;
