@@ -40,9 +40,11 @@ __device__ __forceinline__ uint32_t fp4_codes(const float (&x)[8], int byte) {
 }
 
 // A float32 number that is on the same side as x of all numbers of few bits, the borders of codes
-// among them: the nearest, or where x is not that its neighbour on x's side.
+// among them: the nearest, or where x is not that its neighbour on x's side; the largest for what
+// is finite beyond it.
 __device__ __forceinline__ float beside(double x) {
-  const float f = (float)x;
+  float f = (float)x;
+  if (fabsf(f) == INFINITY && fabs(x) < (double)INFINITY) return copysignf(3.4028234664e38f, f);
   const double d = x - (double)f;
   // (signs by their bits: f may be -0)
   const int bits = __float_as_int(f);

@@ -86,8 +86,8 @@ def paged_rotary_append(q: Tensor, k: Tensor, v: Tensor, cos: Tensor, sin: Tenso
     ``cos`` and ``sin`` (positions, head_dim / 2), float32 or bfloat16, have a row for every
     position that the page table has room for.  The halves of a head are rotated as pairs:
     (x1 cos + x2 sin, x2 cos - x1 sin) at the token's row.  Computed in float64, and only
-    then rounded, to q's dtype or to 4 bits.  A token at a negative position gives 0.
-    Inference only.
+    then rounded, to q's dtype or to 4 bits.  A token at a negative position gives 0; with
+    ``starts``, rows of no sequence are not written.  Inference only.
 
     The reference rotates and normalises q and k in a dozen launches
     (``nanochat/gpt.py:101-109, 231-236``) before its cache takes them."""

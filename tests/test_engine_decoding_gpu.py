@@ -88,6 +88,21 @@ def test_four_bits_score_alike_in_any_chunks(model):
     assert float((a.logprobs - whole.logprobs).abs().mean()) <= 0.3
 
 
+def test_sampling_from_four_bits(model):
+    """Samples share a prompt's pages and part ways in them."""
+    from nanochat_amd import engine
+    prompt = _tokens(70, seed=9)
+    cache = engine.make_cache(model, num_pages=40, max_seqs=4, page_size=16, bits=4)
+    samples = engine.generate(model, prompt, 4, 20, top_k=20, seed=4, cache=cache, chunk=50)
+    assert len({tuple(s.tokens) for s in samples}) > 1
+    assert int(cache.ref_counts.sum()) == 0 and cache.lens == [0] * 4
+    for s in samples[:2]:
+        got = engine.score(model, prompt + s.tokens, cache=cache, slot=3)
+        lp = got.logprobs[len(prompt) - 1:].tolist()
+        # (the chunks differ, and with them the keys' roundings to 4 bits here and there)
+        assert sum(abs(a - b) for a, b in zip(lp, s.logprobs)) <= 0.1 * len(lp)
+
+
 def _search64(model, prompt, n, steps, stop, make):
     """The same search with whole scorings: each continuation's log probabilities from a
     prefill of prompt and tokens; the widest difference between kept and dropped."""

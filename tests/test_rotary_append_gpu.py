@@ -249,6 +249,24 @@ def test_results_below_float32(dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+def test_results_beyond_float32(dtype):
+    """Rotated keys that are finite but past float32 are held as the largest there is."""
+    cache = Cache4([16], 1, 64, 16, 1)
+    x = (cache.rand(16, 1, 64).sign() * 3e38).to(dtype)
+    x[4:, :, 32:] = 0.0
+    x[8, 0, 3] = math.inf
+    c = torch.full((16, 32), 0.75, device=DEV)
+    s = torch.full((16, 32), 0.75, device=DEV)
+    _ops().paged_rotary_append(x[None], x[None], x[None], c, s, cache.k_pages, cache.v_pages,
+                               cache.table, cache.lens)
+    page = int(cache.table[0, 0])
+    want = held4(rotated64(x, c, s, torch.arange(16, device=DEV), None))[0][:, 0]
+    got = values4(cache.k_pages)[page, 0, :16]
+    assert torch.equal(got.isnan(), want.isnan()) and bool(got[8].isnan().all())
+    assert torch.equal(got.nan_to_num(), want.nan_to_num())
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
 def test_borders_of_codes(dtype):
     """Every tie, the ends of the scales and what is beyond them, by ``paged_cache_append``."""
     base = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0, 7.0, 0.0], device=DEV)
