@@ -374,6 +374,8 @@ std::optional<std::tuple<Tensor, Tensor>> read_pages(
   TORCH_CHECK(k_pages.is_cuda(), "LTV HIP kernels need GPU tensors, got k_pages on ",
               k_pages.device());
   if (!is_fp4(k_pages)) dtype_of(k_pages, "k_pages");
+  no_grad_needed(k_pages, "k_pages");
+  no_grad_needed(v_pages, "v_pages");
   check_any_pages(k_pages, v_pages, k_pages);
   TORCH_CHECK_TYPE(dtype == at::kFloat || dtype == at::kBFloat16,
                    "LTV kernels support float32 and bfloat16 tensors, got dtype ", dtype);

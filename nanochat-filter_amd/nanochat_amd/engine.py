@@ -182,8 +182,8 @@ def beam_search(model: GPT, prompt: Sequence[int], beams: int, max_tokens: int, 
         raise ValueError(f"beams are 1 to {min(32, model.config.vocab_size)}, got {n}")
     if max_tokens <= 0:
         raise ValueError("at least one token")
-    if not math.isfinite(length_penalty):
-        raise ValueError(f"length_penalty must be finite, got {length_penalty}")
+    if not abs(length_penalty) <= 32:  # (a length to that power is a float)
+        raise ValueError(f"length_penalty must be -32 to 32, got {length_penalty}")
     longest = len(prompt) + max_tokens - 1  # (the last token is not fed)
     if longest > min(model.config.sequence_len, cache.max_len if cache else longest):
         raise ValueError(f"{longest} tokens, more than the model or the cache is made for")

@@ -243,6 +243,8 @@ def test_refusals(model):
                  lambda: engine.beam_search(model, [1], 2, 0),
                  lambda: engine.beam_search(model, [1], 2, 600),
                  lambda: engine.beam_search(model, [1], 2, 5, length_penalty=math.inf),
+                 lambda: engine.beam_search(model, [1], 2, 5, length_penalty=math.nan),
+                 lambda: engine.beam_search(model, [1], 2, 5, length_penalty=-1e6),
                  lambda: engine.beam_search(model, [1], 3, 5, cache=cache),
                  lambda: engine.beam_search(model, [1], 2, 5, cache=cache),  # slot 0 is in use
                  lambda: PagedKVCache(1, 2, 2, 40, num_pages=2, max_seqs=1, max_len=32, bits=4),

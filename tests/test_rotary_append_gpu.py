@@ -485,6 +485,9 @@ def test_refusals():
     with pytest.raises(TypeError):
         ops.paged_cache_read(cache.k_pages, cache.v_pages, cache.table, cache.lens, 4,
                              dtype=torch.float16)
+    with pytest.raises(RuntimeError, match="v_pages"):
+        v = torch.zeros(4, 2, 16, 64, dtype=BF, device=DEV)
+        ops.paged_cache_read(v, v.clone().requires_grad_(), cache.table, cache.lens, 4)
     with pytest.raises(TypeError):
         v = torch.zeros(4, 2, 16, 64, dtype=BF, device=DEV)
         ops.paged_cache_read(v, v, cache.table, cache.lens, 4, dtype=F32)
