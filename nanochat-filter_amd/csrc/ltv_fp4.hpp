@@ -39,17 +39,17 @@ __device__ __forceinline__ uint32_t fp4_codes(const float (&x)[8], int byte) {
   return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[6], x[7], s, 3);
 }
 
-// A float32 number that is on the same side as x of all numbers of few bits, the borders of codes
-// among them: the nearest, or where x is not that its neighbour on x's side; the largest for what
-// is finite beyond it.
+// x in float32, on the same side of all numbers of fewer bits, the borders of codes among them: what
+// is between two float32 numbers becomes the one whose last bit is set, what is finite beyond them
+// the largest (whose is).
 __device__ __forceinline__ float beside(double x) {
-  float f = (float)x;
+  const float f = (float)x;
   if (fabsf(f) == INFINITY && fabs(x) < (double)INFINITY) return copysignf(3.4028234664e38f, f);
   const double d = x - (double)f;
   // (signs by their bits: f may be -0)
   const int bits = __float_as_int(f);
-  const int step = d == 0.0 || !(fabsf(f) < INFINITY) ? 0 : (d < 0.0) == (bits < 0) ? 1 : -1;
-  return __int_as_float(bits + step);
+  const bool stay = d == 0.0 || (bits & 1) != 0 || !(fabsf(f) < INFINITY);
+  return __int_as_float(bits + (stay ? 0 : (d < 0.0) == (bits < 0) ? 1 : -1));
 }
 // Two codes' values, of byte OF of a word, in bfloat16 (scale 2^(byte - 127), which all values
 // are exact with; infinity, the scale byte of a NaN, makes NaNs).

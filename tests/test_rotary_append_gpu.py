@@ -249,6 +249,26 @@ def test_results_below_float32(dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+def test_results_near_borders(dtype):
+    """Rotated keys a fraction of a float32 step, or some, from where a code or a scale ends."""
+    borders = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 7.0], device=DEV)
+    cache = Cache4([64], 1, 64, 16, 1)
+    x = torch.cat([borders, -borders]).repeat(64, 4)
+    x[32:, 7::8] = 6.0  # (the scale is theirs, or that of those beside 7)
+    powers = torch.tensor([1.0, 2.0 ** -9, 2.0 ** 40], device=DEV).repeat(22)[:64]
+    x = (x * powers[:, None])[:, None].to(dtype)
+    near = torch.arange(64, device=DEV, dtype=torch.float64) % 32 - 15.5
+    near = torch.where(near.abs() > 12, near * 16, near) * 2.0 ** -26
+    c, s = torch.ones(64, 32, device=DEV), near.float()[:, None].expand(64, 32).contiguous()
+    _ops().paged_rotary_append(x[None], x[None], x[None], c, s, cache.k_pages, cache.v_pages,
+                               cache.table, cache.lens)
+    pos = torch.arange(64, device=DEV)
+    want = held4(rotated64(x, c, s, pos, None))[0][:, 0]
+    got = values4(cache.k_pages)[cache.table[0, (pos // 16).long()].long(), 0, pos % 16]
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
 def test_results_beyond_float32(dtype):
     """Rotated keys that are finite but past float32 are held as the largest there is."""
     cache = Cache4([16], 1, 64, 16, 1)
