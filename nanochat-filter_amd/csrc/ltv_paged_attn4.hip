@@ -2,7 +2,16 @@
 //
 //   out[row] = sum_j p_j v_j,  p = softmax_{j <= pos(row)}(scale q[row] . k_j)
 //
-// k and v are the values that the codes and scales stand for.
+// k and v are the values that the codes and scales stand for, which bfloat16 holds exactly: the
+// products are bfloat16 ones, and only queries and probabilities have parts (Split).
+//
+// Two kernels, by the rows that share a k/v head.  Of few the reads are the bound, 17 bytes for 32
+// channels: 16 sequences, one of 131,072 tokens, 6 k/v heads (500 MB) 97 us, 5.1 TB/s, the vector
+// units issuing in half of the cycles.  Of many the products are, and the conversions and
+// exponentials beside them: 8,193 tokens over 16,000 (0.51 TFLOP) 697 us, 726 TFLOP/s; matrix
+// units busy in 35 % of the cycles, vector units in 45 %, seldom both.  Scores, maxima, sums and
+// outputs are float32.  The values are converted anew for each row tile: kept in 16 bits in memory
+// for all of them they would be read back at four times the bytes.
 #include "../../include/nanochat_decoding_amd.h"
 #include "ltv_fp4.hpp"
 #include "ltv_paged_line.hpp"
@@ -119,6 +128,15 @@ constexpr int kShift = 60;
 // ---------------------------------------------------------------------------
 // Each wavefront takes 32 keys of a block of 128 by itself, from memory into registers, and keeps
 // its own maxima, sums and outputs; they are joined through LDS at the end of a piece.
+//
+// A wavefront has one tile of keys in registers, refilled as it is used: with three workgroups
+// to a unit the others' reads are under way meanwhile.  (16 sequences as above, a call: 270 us
+// with a second set of registers, which spills, 108 so.  Two or three tiles ahead in LDS 113,
+// and 64 keys a step 125, for the registers and barriers they take; the rests of probabilities
+// only where one weighs much, a branch that spills, 123.  The same reads without any conversions
+// or products took 104 where all of it took 113.)  Beside the bytes a call pays for its start,
+// the joining of wavefronts and the second kernel: 96 sequences of up to 6,000 tokens, 4 k/v
+// heads of 64 with 8 rows each (62 MB), 27 + 6 us, four of up to 600 tokens 8 + 4.
 //
 // Products of 16 x 16 blocks.  S^T = K Q^T: a lane has 8 channels of a key in each step, and the
 // order of the channels is free as long as the queries have it too: a lane takes D / 4 channels
@@ -418,6 +436,9 @@ __global__ void __launch_bounds__(kFewThreads, kFewEach<T>)
 // of the products.  Those are in 32 x 32 blocks, S^T = K Q^T and O^T = V^T P^T as over 16-bit
 // pages: a lane holds 16 keys of one row, and its probabilities are, without any exchange, the
 // right-hand operand of the second product (ds_read_b64_tr_b16 transposes four keys of a column).
+// float32 has three products for each (of the queries' parts and of the probabilities'), and one
+// workgroup to a unit for the registers: a prompt of 4,096 tokens 125 us, 257 TFLOP/s counted once,
+// where a float32 product of two large matrices reaches 154.
 constexpr int kManyRows = 128, kManyKeys = 64, kManyThreads = 256;
 template <typename T>
 constexpr int kManyEach = sizeof(T) == 2 ? 2 : 1;  // workgroups of a compute unit

@@ -381,7 +381,7 @@ __global__ void __launch_bounds__(256) fork_kernel(const State s, const int32_t*
 
 // Reordering: what is wanted of a column is read, and the counts follow, before any of it is
 // written.  The columns do not meet: a workgroup takes some of them, for all entries at once, in
-// LDS.  All latency: 4 entries of 10 pages 1.8 us.
+// LDS.  All latency: 4 entries of 10 pages 1.8 us, 384 of 502 pages (1.5 MB of table) 5.6.
 constexpr int kReorderInts = 8192, kReorderThreads = 1024;
 
 __global__ void __launch_bounds__(kReorderThreads) reorder_kernel(const State s,

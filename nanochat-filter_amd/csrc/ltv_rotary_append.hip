@@ -9,6 +9,13 @@
 // 2^15 of them to the other side of a tie).  A code of 4 bits changes by up to half its size
 // where a value crosses a border, so which side it is on is worth deciding right, and squares
 // of large float32 values do not pass the range.
+//
+// Everything is read once and written once, in one launch for queries, keys and values.  Long
+// prompts are bounded by the reads and by the float64 arithmetic about alike: 12,289 tokens of 12
+// query and 4 k/v heads of 128, bfloat16 into 4-bit pages, 28 to 30 us (110 MB, 3.8 TB/s), and 9 us
+// to read its keys and values back.  Small calls are latency, of the sequence's numbers, its page
+// and its rows one after the other: 64 sequences of one token each 4.3 us, nine with chunks of up
+// to 700 float32 tokens 7.2.
 #include <algorithm>
 #include <type_traits>
 
@@ -107,8 +114,11 @@ __device__ __forceinline__ void store_fp4(const float (&y)[2][8], char* block, i
   }
 }
 
-// A group of lanes takes a token's head, a lane VEC channels of each half.  Grid: (blocks over
-// a sequence's tokens, B, q, k or v).
+// A group of lanes takes a token's head, a lane VEC channels of each half, so that a pair is in one
+// lane and 16 bytes of bfloat16 (or four float32) one load; sums and scales go from lane to lane.
+// Grid: (blocks over a sequence's tokens, B, q, k or v).  (Loading the next round's rows ahead, or
+// four heads to a group of lanes that read the tables once, takes registers that the float64 values
+// need: 12,289 tokens 39 to 52 us.)
 template <typename T, typename TAB, int VEC, bool ROTATE, bool FP4>
 __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
   const int b = blockIdx.y, w = blockIdx.z + a.first;
