@@ -155,12 +155,14 @@ struct FewTile {
 
 constexpr int kFewRows = 16, kFewKeys = 128, kFewThreads = 256;
 // Workgroups of a compute unit, as their registers allow.  (bfloat16, 64 sequences of 8,000 tokens
-// and 4 heads: two 54 us, three 51, four, which spill, 61.)
-template <typename T>
-constexpr int kFewEach = sizeof(T) == 2 ? 3 : 2;
+// and 4 heads of 128: two 54 us, three 51, four, which spill, 61; 16 heads of 32: three 105, four 98.
+// float32, 8 heads of 64: two 77, three 66.)
+constexpr int few_each(bool f32, int D) { return f32 ? (D <= 64 ? 3 : 2) : D <= 32 ? 4 : 3; }
+template <typename T, int D>
+constexpr int kFewEach = few_each(sizeof(T) == 4, D);
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kFewThreads, kFewEach<T>)
+__global__ void __launch_bounds__(kFewThreads, (kFewEach<T, D>))
     attn4_few_kernel(const AttnArgs a) {
   using Tile = FewTile<T, D>;
   constexpr int kSteps = Tile::kSteps, kCh = Tile::kCh, kQ = Split<T>::kQuery,
@@ -425,7 +427,7 @@ __global__ void __launch_bounds__(kFewThreads, kFewEach<T>)
     }
     barrier();  // (LDS is read)
   };
-  walk_line<kFewKeys, false, kFewThreads, kFewRows, 256 * kFewEach<T>>(a, piece);
+  walk_line<kFewKeys, false, kFewThreads, kFewRows, 256 * kFewEach<T, D>>(a, piece);
 }
 
 // ---------------------------------------------------------------------------
@@ -845,7 +847,7 @@ AttnPlan plan_attention4(const ltv_paged_batch& b, int dtype, int NH, int NKVH, 
   if (few) {
     shape.keys = kFewKeys;
     shape.log_rows = 4;
-    shape.grid = 256 * (f32 ? kFewEach<float> : kFewEach<bf16_t>);
+    shape.grid = 256 * few_each(f32, D);
     shape.group = 1;
     shape.least = 1;
   } else {
