@@ -5,7 +5,7 @@
 // k and v are the values that the codes and scales stand for, which bfloat16 holds exactly: the
 // products are bfloat16 ones, and only queries and probabilities have parts (Split).
 //
-// Two kernels, by the rows that share a k/v head.  Of few the reads are the bound, 17 bytes for 32
+// Two kernels, by the rows that share a k/v head (few_rows).  Of few the reads are the bound, 17 bytes for 32
 // channels: 16 sequences, one of 131,072 tokens, 6 k/v heads (500 MB) 97 us, 5.1 TB/s, the vector
 // units issuing in half of the cycles.  Of many the products are, and the conversions and
 // exponentials beside them: 8,193 tokens over 16,000 (0.51 TFLOP) 697 us, 726 TFLOP/s; matrix
@@ -838,12 +838,23 @@ __global__ void __launch_bounds__(kManyThreads, kManyEach<T>) attn4_many_kernel(
 // 55, with 128 rows 71 and 63.
 constexpr int kMostFewRows = 64;
 
+// Of more rows, calls so small that tiles of 128 would be cut into pieces of a few keys, for the
+// whole card to have some: by rows of all heads times the longest sequence, and in float32, whose
+// tiles of 128 have one workgroup to a unit, also by rows alone.  (In tiles of 128 and of 16 us,
+// 6 heads of 128: bfloat16, 512 tokens over 2,000 42 and 35, 2,048 alone 48 and 42, 1,024 over 8,000
+// 77 and 90, 16 chunks of 128 over up to 2,000 with 8 heads of 64 42 and 45; float32, 512 over 2,000 47
+// and 38, 1,024 over 8,000 121 and 114, 2,048 alone 61 and 69.)
+bool few_rows(bool f32, int64_t rows, double all_rows, double max_len) {
+  return rows <= kMostFewRows || all_rows * max_len <= (f32 ? 0x1p24 : 0x1p25) ||
+         (f32 && all_rows <= 8192);
+}
+
 AttnPlan plan_attention4(const ltv_paged_batch& b, int dtype, int NH, int NKVH, int D,
                          int max_len) {
   const bool f32 = dtype == LTV_DTYPE_F32;
   const int64_t rows = (int64_t)std::max(b.T, 1) * (NH / NKVH);
   LineShape shape{};
-  const bool few = rows <= kMostFewRows;
+  const bool few = few_rows(f32, rows, (double)b.total * NH, max_len);
   if (few) {
     shape.keys = kFewKeys;
     shape.log_rows = 4;
@@ -860,6 +871,8 @@ AttnPlan plan_attention4(const ltv_paged_batch& b, int dtype, int NH, int NKVH, 
   }
   AttnPlan p = plan_line(b, NH, NKVH, D, max_len, shape);
   p.few = few;
+  // (row tiles of 16 count alike on the line, as those in the middle of the longest chunk)
+  if (few) p.group_tokens = std::max(p.group_tokens, b.T / 2);
   p.all_rests = 4.0 * D * NH * (double)b.total * std::max(max_len, 1) <= 1e11;
   return p;
 }

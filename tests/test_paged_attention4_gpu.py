@@ -64,14 +64,25 @@ def _check(got, want, dtype, D, lens):
         assert bool(ok.all()), (i, float(e.abs().max()))
 
 
+# Pages that a table has room for where tiles of 128 rows are to be taken: the calls that are small by
+# their rows and by the longest sequence that there may be go in tiles of 16.
+ROOM = 1 << 14
+
+
+def _widen(cache, room):
+    if room:
+        cache.table = torch.nn.functional.pad(cache.table, (0, room), value=-1)
+
+
 def _case(dtype, NH, NKVH, D, page, new, cached, packed, seed=0, slots=None, layout="dense",
-          qscale=1.0, poison=None, **hints):
+          qscale=1.0, poison=None, room=0, **hints):
     lens = [a + b for a, b in zip(new, cached)]
     order = list(range(len(lens))) if slots is None else slots
     held = [0] * (max(order) + 1 if order else 0)
     for s, n in zip(order, lens):
         held[s] = n
     cache = Cache4(held, NKVH, D, page, seed, layout=layout)
+    _widen(cache, room)
     if poison is not None:
         poison(cache)
         cache.decode()
@@ -106,6 +117,23 @@ def test_chunks(NH, NKVH, D, page, dtype):
 @pytest.mark.parametrize("T,cached", [(1, 3000), (3, 2049), (17, 900), (40, 1500), (257, 100), (512, 0)])
 def test_longer(T, cached, D, dtype):
     _case(dtype, 4, 2, D, 32, [T] * 2, [cached, cached // 3], packed=False, seed=2, qscale=3.0)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("NH,NKVH,D,page", HEADS)
+def test_chunks_of_many_rows(NH, NKVH, D, page, dtype):
+    """.. in tiles of 128 rows."""
+    n = 8192 // NH
+    _case(dtype, NH, NKVH, D, page, [1, 5, 0, 33, n, 2, 130], [0, 7, 20, 0, 65, 300, 131],
+          packed=True, seed=1, room=ROOM)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("D", [32, 64, 96, 128])
+@pytest.mark.parametrize("T,cached", [(257, 100), (512, 0), (300, 1700)])
+def test_longer_of_many_rows(T, cached, D, dtype):
+    _case(dtype, 20, 2, D, 32, [T] * 2, [cached, cached // 3], packed=False, seed=2, qscale=3.0,
+          room=ROOM)
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
@@ -147,7 +175,7 @@ def _nan_scale(cache, which, slot, pos, block=0):
 
 @pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("which", ["k_pages", "v_pages"])
-@pytest.mark.parametrize("NH,new", [(2, 1), (2, 5), (16, 1), (4, 40), (2, 300)])
+@pytest.mark.parametrize("NH,new", [(2, 1), (2, 5), (16, 1), (4, 40), (2, 300), (32, 100)])
 def test_nan_in_sight(NH, new, which, dtype):
     """32 channels that are NaN: of a key every row that sees it is NaN, of a value those channels."""
 
@@ -155,11 +183,12 @@ def test_nan_in_sight(NH, new, which, dtype):
         _nan_scale(cache, which, 0, 30, 1)
         _nan_scale(cache, which, 1, 100 + new // 2, 0)
 
-    _case(dtype, NH, 2, 64, 16, [new] * 3, [80, 100, 50], packed=False, seed=6, poison=poison)
+    _case(dtype, NH, 2, 64, 16, [new] * 3, [80, 100, 50], packed=False, seed=6, poison=poison,
+          room=ROOM if NH == 32 else 0)
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
-@pytest.mark.parametrize("new", [1, 3, 40, 300])
+@pytest.mark.parametrize("new", [1, 3, 40, 300, 1100])
 def test_nan_out_of_sight(new, dtype):
     """What no row sees -- past the end, in pages of no sequence, behind the causal mask -- does not
     reach one, whatever its bytes are."""
@@ -177,11 +206,12 @@ def test_nan_out_of_sight(new, dtype):
                     s[p] = 255
             _nan_scale(cache, which, 1, int(cache.lens[1]) - 1)
 
-    _case(dtype, 4, 2, 128, 16, [new] * 2, [83, 100], packed=False, seed=7, poison=poison)
+    _case(dtype, 4, 2, 128, 16, [new] * 2, [83, 100], packed=False, seed=7, poison=poison,
+          room=ROOM if new == 1100 else 0)
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
-@pytest.mark.parametrize("new", [1, 20, 200])
+@pytest.mark.parametrize("new", [1, 20, 200, 1100])
 def test_missing_pages(new, dtype):
     """Ids outside the pages hold no keys; a sequence of none gives 0 and -inf."""
 
@@ -190,14 +220,16 @@ def test_missing_pages(new, dtype):
         cache.table[0, 4] = cache.P + 3
         cache.table[1, :] = -5
 
-    _case(dtype, 4, 2, 64, 16, [new] * 2, [150, 30], packed=False, seed=8, poison=poison)
+    _case(dtype, 4, 2, 64, 16, [new] * 2, [150, 30], packed=False, seed=8, poison=poison,
+          room=ROOM if new == 1100 else 0)
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
-@pytest.mark.parametrize("new", [5, 90])
+@pytest.mark.parametrize("new", [5, 90, 1100])
 def test_more_new_than_tokens(new, dtype):
     """Tokens at negative positions see nothing."""
     cache = Cache4([3, 40], 2, 64, 16, 9)
+    _widen(cache, ROOM if new == 1100 else 0)
     q = [cache.rand(new, 4, 64, dtype=dtype) for _ in range(2)]
     got = _run(cache, q, [new] * 2, False)
     want = attention64(q, cache, [0, 1], [new] * 2, 64 ** -0.5)
@@ -205,13 +237,14 @@ def test_more_new_than_tokens(new, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
-@pytest.mark.parametrize("new", [1, 70])
+@pytest.mark.parametrize("new", [1, 70, 1100])
 def test_large_scores(new, dtype):
     """Scores of thousands: one key takes all, exponents far from 0."""
-    _case(dtype, 4, 2, 64, 16, [new] * 2, [300, 20], packed=False, seed=10, qscale=3000.0)
+    _case(dtype, 4, 2, 64, 16, [new] * 2, [300, 20], packed=False, seed=10, qscale=3000.0,
+          room=ROOM if new == 1100 else 0)
 
 
-@pytest.mark.parametrize("new", [1, 60])
+@pytest.mark.parametrize("new", [1, 60, 1100])
 def test_extreme_scales(new):
     """Scales at both ends of their range."""
 
@@ -221,13 +254,15 @@ def test_extreme_scales(new):
             s.copy_(torch.randint(low, low + 3, s.shape, device=DEV))
             s[:, :, 0] = 120
 
-    _case(F32, 4, 2, 64, 16, [new] * 2, [100, 20], packed=False, seed=11, poison=poison)
+    _case(F32, 4, 2, 64, 16, [new] * 2, [100, 20], packed=False, seed=11, poison=poison,
+          room=ROOM if new == 1100 else 0)
 
     def large(cache):
         s = parts4(cache.v_pages)[1]
         s.fill_(249)
 
-    _case(BF, 4, 2, 64, 16, [new] * 2, [100, 20], packed=False, seed=12, poison=large)
+    _case(BF, 4, 2, 64, 16, [new] * 2, [100, 20], packed=False, seed=12, poison=large,
+          room=ROOM if new == 1100 else 0)
 
 
 def test_query_strides():
@@ -239,10 +274,11 @@ def test_query_strides():
     assert torch.equal(f(q), f(q.transpose(2, 3).contiguous().transpose(2, 3)))
 
 
-@pytest.mark.parametrize("new", [1, 50])
+@pytest.mark.parametrize("new", [1, 50, 1100])
 def test_rows_of_no_sequence_and_again(new):
     """A call does not depend on the one before, nor write rows of no sequence."""
     cache = Cache4([400, 33], 2, 64, 16, 14)
+    _widen(cache, ROOM if new == 1100 else 0)
     q = cache.rand(2, new, 4, 64, dtype=BF)
     a = _ops().paged_attention(q, cache.k_pages, cache.v_pages, cache.table, cache.lens)
     other = Cache4([900] * 5, 2, 64, 16, 15)
@@ -253,10 +289,11 @@ def test_rows_of_no_sequence_and_again(new):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
-@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("new", [1, 40, 1100])
 def test_captured(new, dtype):
     """Lengths, tables and pages change between replays; two graphs side by side."""
     cache = Cache4([2000, 600], 2, 64, 16, 16)
+    _widen(cache, ROOM if new == 1100 else 0)
     q = cache.rand(2, new, 4, 64, dtype=dtype)
     f = lambda: _ops().paged_attention(q, cache.k_pages, cache.v_pages, cache.table, cache.lens,  # noqa: E731
                                        return_lse=True)
