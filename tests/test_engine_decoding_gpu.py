@@ -180,6 +180,33 @@ def test_stopped_beams_stay(model):
         assert abs(own - b.logprob) <= 0.1 * len(b.tokens)
 
 
+def test_smallest_searches(model):
+    """One token; one that ends it; a prompt of one; more beams than differ at first."""
+    from nanochat_amd import engine
+    one = engine.beam_search(model, _tokens(5), 4, 1)
+    lp = engine.score(model, _tokens(5) + one[0].tokens, top_k=4)
+    assert [b.tokens for b in one] == [[t] for t in lp.top_ids[-1].tolist()]
+    for b in engine.beam_search(model, _tokens(5), 1, 6, stop=one[0].tokens[0]):
+        assert b.tokens == one[0].tokens
+    out = engine.beam_search(model, [7], 32, 3)
+    assert len({tuple(b.tokens) for b in out}) == 32 and all(len(b.tokens) == 3 for b in out)
+    assert [b.score for b in out] == sorted((b.score for b in out), reverse=True)
+
+
+def test_reorder_of_nothing(model):
+    from nanochat_amd import engine
+    cache = engine.make_cache(model, num_pages=8, max_seqs=2, page_size=16, bits=4)
+    engine.prefill(model, cache, 0, _tokens(20))
+    was = [t.clone() for t in (cache.page_table, cache.seq_lens, cache.ref_counts)]
+    cache.reorder([], [])
+    cache.reorder([0], [0])
+    assert all(torch.equal(a, b) for a, b in
+               zip(was, (cache.page_table, cache.seq_lens, cache.ref_counts)))
+    assert cache.lens == [20, 0]
+    cache.reorder([0], [1])  # (an empty slot: the other is let go)
+    assert cache.lens == [0, 0] and not cache.ref_counts.any() and not cache.seq_lens.any()
+
+
 def test_failure_leaves_the_slots_empty(model):
     from nanochat_amd import engine
     cache = engine.make_cache(model, 4, 3, 16, bits=4)
