@@ -265,6 +265,37 @@ def test_extreme_scales(new):
           room=ROOM if new == 1100 else 0)
 
 
+def test_pages_past_32_bits():
+    """Pages of 5 GiB: appended to, attended to and read as those of a small array are."""
+    ops, D, ps, NKVH = _ops(), 128, 64, 8
+    row = ops.fp4_row_bytes(D)
+    P = 5 * 2 ** 30 // (NKVH * ps * row)
+    small = Cache4([300, 90], NKVH, D, ps, 20)
+    far = torch.cat([torch.arange(P - 4, P), torch.arange(4)]).flip(0).to(DEV, torch.int32)
+    table = torch.full_like(small.table, -1)
+    k, v = (torch.empty(P, NKVH, ps, row, dtype=torch.uint8, device=DEV) for _ in range(2))
+    place = {}
+    for i, page in enumerate(p for p in small.table.flatten().tolist() if 0 <= p < small.P):
+        place[page] = int(far[i])
+        k[far[i].long()] = small.k_pages[page]
+        v[far[i].long()] = small.v_pages[page]
+    for old, new in place.items():
+        table[small.table == old] = new
+    assert max(place.values()) * NKVH * ps * row > 2 ** 32
+    new = [small.rand(2, 5, NKVH, D, dtype=BF) for _ in range(2)]
+    for kp, vp, t in ((small.k_pages, small.v_pages, small.table), (k, v, table)):
+        ops.paged_cache_append(*new, kp, vp, t, small.lens)
+    for T, NH in ((1, 8), (30, 64), (2, 64)):
+        q = small.rand(2, T, NH, D, dtype=BF)
+        f = lambda *c: ops.paged_attention(q, *c, small.lens)  # noqa: E731
+        assert torch.equal(f(small.k_pages, small.v_pages, small.table), f(k, v, table))
+        wide = [torch.nn.functional.pad(t, (0, ROOM), value=-1) for t in (small.table, table)]
+        assert torch.equal(f(small.k_pages, small.v_pages, wide[0]), f(k, v, wide[1]))
+    for a, b in zip(ops.paged_cache_read(small.k_pages, small.v_pages, small.table, small.lens, 90),
+                    ops.paged_cache_read(k, v, table, small.lens, 90)):
+        assert torch.equal(a, b)
+
+
 def test_query_strides():
     cache = Cache4([90, 33], 2, 64, 16, 13)
     big = cache.rand(2, 4, 9, 70, dtype=BF)
