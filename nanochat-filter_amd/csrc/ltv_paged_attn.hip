@@ -575,7 +575,7 @@ __global__ void __launch_bounds__((AttnShape<T, FEW>::kThreads), FEW ? 1 : 2)
     }
   };
 
-  walk_line<KT, FEW, kAttnThreads, kAttnRows, Shape::kGrid>(a, piece);
+  walk_line<KT, FEW, kAttnThreads, kAttnRows, Shape::kGrid, const AttnArgs>(a, piece);
 }
 
 template <typename T, bool FEW>

@@ -5,8 +5,8 @@
 // k and v are the values that the codes and scales stand for, which bfloat16 holds exactly: the
 // products are bfloat16 ones, and only queries and probabilities have parts (Split).
 //
-// Two kernels, by the rows that share a k/v head (few_rows).  Of few the reads are the bound, 17 bytes for 32
-// channels: 16 sequences, one of 131,072 tokens, 6 k/v heads (500 MB) 97 us, 5.1 TB/s, the vector
+// Two kernels, by the rows that share a k/v head (few_rows).  Of few the reads are the bound, 17
+// bytes for 32 channels: 16 sequences, one of 131,072 tokens, 6 k/v heads (500 MB) 97 us, 5.1 TB/s, the vector
 // units issuing in half of the cycles.  Of many the products are, and the conversions and
 // exponentials beside them: 8,193 tokens over 16,000 (0.51 TFLOP) 697 us, 726 TFLOP/s; matrix
 // units busy in 35 % of the cycles, vector units in 45 %, seldom both.  Scores, maxima, sums and
@@ -427,7 +427,7 @@ __global__ void __launch_bounds__(kFewThreads, (kFewEach<T, D>))
     }
     barrier();  // (LDS is read)
   };
-  walk_line<kFewKeys, false, kFewThreads, kFewRows, 256 * kFewEach<T, D>>(a, piece);
+  walk_line<kFewKeys, false, kFewThreads, kFewRows, 256 * kFewEach<T, D>, const AttnArgs&>(a, piece);
 }
 
 // ---------------------------------------------------------------------------
@@ -830,7 +830,7 @@ __global__ void __launch_bounds__(kManyThreads, kManyEach<T>) attn4_many_kernel(
     if (hf == 0 && a.lse != nullptr)
       a.lse[trow * a.NH + h] = l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
   };
-  walk_line<KT, false, kManyThreads, kManyRows, 256 * kManyEach<T>>(a, piece);
+  walk_line<KT, false, kManyThreads, kManyRows, 256 * kManyEach<T>, const AttnArgs&>(a, piece);
 }
 
 // Up to how many rows of a k/v head tiles of 16 read every key for themselves: 16 sequences of

@@ -258,9 +258,11 @@ __device__ __forceinline__ void rows_one_by_one(const AttnArgs& a, const PagedSe
 // A workgroup's range of the line: piece(s, b, kvh, tile, begin, end, part0) computes keys begin ..
 // end of a row tile, into its rows of the output or the partials from part0 on (-1: none).  KT:
 // keys of a block, ROWS: of a row tile, GRID: workgroups that the card holds; FEW: one wavefront,
-// and many sequences to a thread.
-template <int KT, bool FEW, int THREADS, int ROWS, int GRID, typename Piece>
-__device__ __forceinline__ void walk_line(const AttnArgs& a, Piece piece) {
+// and many sequences to a thread.  Args: AttnArgs, or a reference, as leaves the kernel's loop over
+// tiles with fewer numbers put aside for scalar registers (a long prompt over 16-bit pages 1,254 us
+// with a reference and 1,155 with a copy, over 4-bit pages 743 and 760).
+template <int KT, bool FEW, int THREADS, int ROWS, int GRID, typename Args, typename Piece>
+__device__ __forceinline__ void walk_line(Args a, Piece piece) {
   constexpr int WAVES = THREADS / 64;
   // The lengths of all sequences, a run of them to each thread, and their sum.
   __shared__ uint32_t sums[WAVES];
