@@ -110,7 +110,8 @@ int ltv_paged_cache_reorder(const ltv_page_state* state, const int32_t* slots, c
  * score -inf and the token -1; its logits are not read.
  *   out_scores (groups, k) float32, parents and tokens (groups, k): beam and token
  * k <= beams * V; min(k, V) <= 64 and beams * min(k, V) <= 1024; groups * beams <= 2^20.
- * Scores are compared in float64.  workspace: ltv_beam_select_workspace_size bytes, 16-byte
+ * Scores are compared in float64; the rows' sums are float32, off by some 2^-24 of them and, of
+ * caps up to 64, by some 2^-23 of the cap.  workspace: ltv_beam_select_workspace_size bytes, 16-byte
  * aligned.
  * ---------------------------------------------------------------------- */
 size_t ltv_beam_select_workspace_size(int64_t groups, int beams, int V, int k);

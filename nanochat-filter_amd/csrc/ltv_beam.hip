@@ -8,10 +8,12 @@
 // pieces, and then the beams' candidates are ranked, each by counting those before it.
 //
 // A score decides which of two beams goes on, so scores are float64, and so is what they are made
-// of as far as it may matter: a candidate's z, the joined sums and their logarithm.  The
-// exponentials of the pass are off by some roundings of the cap, all alike in size; of a few
-// logits that have most of the sum they would show in lse, so the candidates' terms (the largest
-// there are) are taken out of the sum as they went in and put back exactly.
+// of as far as it may matter: a candidate's z, the joined sums and their logarithm, and of caps
+// past 64 every z of the pass (a float32 one is off by more than the log probability of a likely
+// token).  Of smaller caps the exponentials of the pass are off by some roundings of the cap, all
+// alike in size.  Of a few logits that have most of the sum that would show in lse, so with a cap
+// the candidates' terms (the largest there are) are taken out of the sum as they went in and put
+// back exactly.  What is left is the float32 sum's: terms and additions off by some 2^-24 each.
 //
 // Bounded by the pass over the logits: 384 beams' rows of 50,257 bfloat16 (39 MB) 21 us, 1.8 TB/s --
 // at that length it is the pass's start, its bound for the candidates and its join within a
@@ -55,15 +57,6 @@ __device__ __forceinline__ void wave_sync() {
 __device__ __forceinline__ double wave_sum(double x) {
   for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d);
   return x;
-}
-
-// c tanh(x / c) for the candidates.  Of caps up to 64 by 1 - tanh y = 2 / (e^{2 y} + 1), off by
-// roundings of the cap; of larger ones, beside which z may be small, to its own last bits.
-template <Cap CAP>
-__device__ __forceinline__ double capped64(float x, double cap) {
-  if constexpr (CAP == kNoCap) return x;
-  const double y = (double)x / cap;
-  return CAP == kCap ? cap - 2.0 * cap / (exp(2.0 * y) + 1.0) : cap * tanh(y);
 }
 
 template <Cap CAP>
@@ -141,7 +134,8 @@ __global__ void beam_kernel(const BeamArgs a) {
     } else {
       m = 0.0;
     }
-    // the candidates' z, and the exact terms in place of the pass's (n is at most 64)
+    // the candidates' z, and the exact terms in place of the pass's (n is at most 64; without a cap
+    // the largest is 1 in both)
     double z = 0.0;
     if (lane < a.n) {
       const uint64_t key = order[b * a.n + lane];
@@ -149,6 +143,8 @@ __global__ void beam_kernel(const BeamArgs a) {
       z = capped64<CAP>(x, a.cap);
       if constexpr (CAP == kCap)
         sum += exp(z) - (double)cap_exp(cap_r(x, cap_scale_of(a.cap)), a.cap);
+      if constexpr (CAP == kCap64 || CAP == kTanh64)
+        sum += exp(z - m) - (double)below_exp(z, (float)m);
       token[b * a.n + lane] = key_index(key);
     }
     sum = wave_sum(sum);
@@ -240,10 +236,11 @@ extern "C" int ltv_beam_select(int dtype, const void* logits, int64_t row_stride
     hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(64 * waves),
                        beam_lds(beams, n, pieces, waves), st, a);
   };
-  switch (cap_of(softcap)) {
+  switch (exact_cap_of(softcap)) {
     case kNoCap: launch(beam_kernel<kNoCap>); break;
     case kCap: launch(beam_kernel<kCap>); break;
-    case kWideCap: launch(beam_kernel<kWideCap>); break;
+    case kCap64: launch(beam_kernel<kCap64>); break;
+    default: launch(beam_kernel<kTanh64>); break;
   }
   LTV_LAUNCH_CHECK();
   return LTV_OK;

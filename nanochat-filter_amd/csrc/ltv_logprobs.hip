@@ -99,9 +99,15 @@ struct Sums {
         a = fmaf(r, e, a);
       }
     } else {
+      using Z = std::conditional_t<CAP == kCap64 || CAP == kTanh64, double, float>;
+      Z z[N];
       float x[N];
 #pragma unroll
-      for (int i = 0; i < N; ++i) x[i] = capped<CAP>(logits[i], cap);
+      for (int i = 0; i < N; ++i) {
+        if constexpr (std::is_same_v<Z, double>) z[i] = capped64<CAP>(logits[i], cap);
+        else z[i] = capped<CAP>(logits[i], cap);
+        x[i] = (float)z[i];
+      }
       float top = x[0];
 #pragma unroll
       for (int i = 1; i < N; ++i) top = fmaxf(top, x[i]);
@@ -116,7 +122,7 @@ struct Sums {
       const float base = m == -INFINITY ? 0.0f : m;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const float d = (x[i] - base) * kLog2e;
+        const float d = (float)(z[i] - (Z)base) * kLog2e;
         const float e = __builtin_amdgcn_exp2f(d);
         s += e;
         a = fmaf(fmaxf(d, -1000.0f), e, a);  // (-inf adds nothing; NaN comes by e)
@@ -630,10 +636,13 @@ int logprobs_parts(int dtype, const void* x, int64_t row_stride, const uint8_t* 
       hipLaunchKernelGGL((logprobs_forward_kernel<T, decltype(cap)::value, true>), grid,
                          dim3(kThreads), 0, stream, a);
     };
-    switch (cap_of(softcap)) {
+    // (float32 z of large caps are off by 2^-22 of themselves and more, each in its own way: of two
+    // beams with one likely continuation each that would decide)
+    switch (exact_cap_of(softcap)) {
       case kNoCap: return by_cap(cap_type<kNoCap>());
       case kCap: return by_cap(cap_type<kCap>());
-      case kWideCap: return by_cap(cap_type<kWideCap>());
+      case kCap64: return by_cap(cap_type<kCap64>());
+      default: return by_cap(cap_type<kTanh64>());
     }
   };
   if (dtype == LTV_DTYPE_F32) launch(float()); else launch(bf16_t());

@@ -11,12 +11,19 @@ namespace ltv {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
-// How z follows from x: none, by r, by tanh.
-enum Cap { kNoCap, kCap, kWideCap };
-constexpr float kMostCap = 64.0f;  // by r
+// How z follows from x: none, by r, by tanh, by r in float64, by tanh in float64.
+enum Cap { kNoCap, kCap, kWideCap, kCap64, kTanh64 };
+constexpr float kMostCap = 64.0f;      // by r
+constexpr float kMostCap64 = 0x1p20f;  // .. in float64
 
 inline Cap cap_of(float softcap) {
   return softcap > kMostCap ? kWideCap : softcap > 0.0f ? kCap : kNoCap;
+}
+
+// .. where a float32 z of a large cap is too far off.
+inline Cap exact_cap_of(float softcap) {
+  const Cap c = cap_of(softcap);
+  return c != kWideCap ? c : softcap <= kMostCap64 ? kCap64 : kTanh64;
 }
 
 // r of the cap's tanh; cap_scale = 2 log2(e) / c (finite for the smallest c, too)
@@ -26,10 +33,24 @@ __device__ __forceinline__ float cap_scale_of(float cap) {
 __device__ __forceinline__ float cap_r(float x, float cap_scale) {
   return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * cap_scale));
 }
+// c tanh(x / c) in float64: by 1 - tanh y = 2 / (e^{2 y} + 1), off by roundings of the cap (some
+// 2^-32 at 2^20); of larger caps, beside which z may be small, to its own last bits, which takes
+// twice as long (a pass over 384 rows of 50,257 bfloat16: 137 us, 62 so, and 22 with a cap of 15).
+template <Cap CAP>
+__device__ __forceinline__ double capped64(float x, double cap) {
+  if constexpr (CAP == kNoCap) return x;
+  const double y = (double)x / cap;
+  return CAP != kTanh64 ? cap - 2.0 * cap / (exp(2.0 * y) + 1.0) : cap * tanh(y);
+}
 // e^z by r
 __device__ __forceinline__ float cap_exp(float r, float cap) {
   const float at0 = cap * kLog2e, slope = -2.0f * at0;
   return __builtin_amdgcn_exp2f(fmaf(r, slope, at0));
+}
+
+// e^(z - m) as the pass has it
+__device__ __forceinline__ float below_exp(double z, float m) {
+  return __builtin_amdgcn_exp2f((float)(z - (double)m) * kLog2e);
 }
 
 // A total order of the logits with their indices: larger value first (NaN above all,
@@ -66,8 +87,9 @@ __device__ __forceinline__ uint64_t kth_of_lanes(uint64_t mine, int k) {
 int logprobs_pieces(int64_t N, int V);
 
 // Of each piece of N <= 2^23 rows the sums (N, pieces, 3) -- m, S = sum e^(z - m) and one for
-// the entropy; by r there is no m: S = sum e^z -- and the keys of its top_k largest logits (N,
-// pieces, top_k), descending, 0 where it has fewer.  Rows n with skip[n] are left out.
+// the entropy; by r there is no m: S = sum e^z; of larger caps z is float64, and m its largest,
+// a float32 number -- and the keys of its top_k largest logits (N, pieces, top_k), descending, 0
+// where it has fewer.  Rows n with skip[n] are left out.
 int logprobs_parts(int dtype, const void* x, int64_t row_stride, const uint8_t* skip,
                    float* part_sums, uint64_t* part_keys, int64_t N, int V, int top_k,
                    float softcap, hipStream_t stream);

@@ -32,7 +32,11 @@ def beam_select(logits: Tensor, scores: Tensor, k: int, *, softcap: Optional[flo
     A beam that is ``finished`` ((..., beams) bool) has one continuation, itself: its score,
     and the token -1.  (Where there are fewer than k, others of score -inf follow; such of
     finished beams have the token -1.)  k is at most 64, or the vocabulary where that is less,
-    which times the beams is at most 1,024.  Scores are compared in float64.  No gradient."""
+    which times the beams is at most 1,024.  No gradient.
+
+    Scores are compared in float64, with rows' sums of exponentials that were added up in float32:
+    off by some 2^-24 of them, of caps up to 64 also by some 2^-23 of the cap.  Continuations
+    nearer to each other than that may change places."""
     cap = 0.0 if softcap is None else float(softcap)
     if softcap is not None and not cap > 0.0:
         raise ValueError(f"softcap must be positive and finite, got {softcap}")

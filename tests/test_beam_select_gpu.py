@@ -208,6 +208,45 @@ def test_one_token_has_most(cap):
     assert got.parents[0].tolist() == [e[1] for e in want[:2]] == [1, 0]
 
 
+@pytest.mark.parametrize("rows", ["one", "near", "spread"])
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("cap", [65.0, 100.0, 1000.0, 3e4, 2.0 ** 20, 3e6])
+def test_large_caps_are_as_exact_as_none(cap, dtype, rows):
+    """Logits as large as the cap, of which a float32 z is off by more than a likely token's log
+    probability: one token near the cap, many near each other, or ordinary ones.
+
+    What a row's sum may be off, in units of 2^-24 of it: a term's argument d by two roundings (2 |d| in
+    binary digits, over the terms by their weights at most 2 log2 V), its exponential by 4, a thread's
+    additions by one each (4 here) and the joins of 64 lanes, 4 wavefronts and two pieces' sums by 3 each,
+    the candidates that are taken out and put back by 8 more; the score by its own rounding."""
+    G, B, V, k = 32, 2, 300, 4
+    g = torch.Generator(device=DEV).manual_seed(int(cap))
+    x = torch.randn(G, B, V, generator=g, device=DEV)
+    u01 = torch.rand(G, B, 1, generator=g, device=DEV)
+    if rows == "one":
+        x = x * cap * 0.01
+        x[..., 7:8] = cap * (0.8 + u01)
+        # (the next one from some millionths to some hundredths as likely)
+        z = cap * torch.tanh(x[..., 7:8].double() / cap) - 3.0 - 10.0 * u01.flip(0)
+        x[..., 8:9] = cap * torch.atanh(z / cap)
+    elif rows == "near":
+        x = cap * (0.3 + 0.6 * u01) + 2.0 * x
+    else:
+        x = 3.0 * x
+    x = x.to(dtype)
+    s = torch.zeros(G, B, device=DEV)
+    got = _select(x, s, k, softcap=cap)
+    u = 2.0 ** -24
+    off = u * (2 * math.log2(V) + 4 + 4 + 3 * (6 + 4 + 1) + 8)
+    for i, c in enumerate(_all64(x, s, k, cap, None)):
+        place = {(b, v): t for t, b, _, v in c}
+        for j in range(k):
+            t, e = float(got.scores[i, j]), (int(got.parents[i, j]), int(got.tokens[i, j]))
+            assert abs(t - place[e]) <= off + u * abs(place[e]), (i, j, t, place[e])
+            # not after one that is better by more than the two may be off
+            assert place[e] >= c[j][0] - 2 * off, (i, j, place[e], c[j])
+
+
 def test_all_finished():
     x, s, _ = _rand(2, 3, 1000, BF)
     fin = torch.ones(2, 3, dtype=torch.bool, device=DEV)
