@@ -79,7 +79,8 @@ int ltv_paged_cache_read(int dtype, int page_format, const void* k_pages,
 
 /* ltv_paged_attention over 4-bit pages: the same sums over the values that the pages stand
  * for, q and out of dtype.  D 32, 64, 96 or 128; page strides in bytes, pages of a layer
- * within 32 GiB.  Keys and values that a token does not attend to never reach its output. */
+ * within 32 GiB.  max_len is a hint that chooses launch shapes and no roundings.  Keys and values
+ * that a token does not attend to never reach its output. */
 size_t ltv_paged_attention_fp4_workspace_size(int dtype, const ltv_paged_batch* batch, int NH,
                                               int NKVH, int D, int max_len);
 int ltv_paged_attention_fp4(int dtype, const void* q, const int64_t q_strides[3],

@@ -296,6 +296,41 @@ def test_pages_past_32_bits():
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("max_len", [None, 2048])
+@pytest.mark.parametrize("new", [1, 256])
+def test_probabilities_are_not_rounded_to_bfloat16(new, max_len):
+    """All keys of a row but one have the same probability, so that its roundings would add up: outputs
+    are within their own rounding (half a step of bfloat16), float32 sums, and the two bfloat16 parts of
+    a probability, whose second is off by 2^-8 of at most 2^-8, whatever room for keys there is."""
+    NH, NKVH, D, n = 8, 2, 64, 2000
+    cache = Cache4([n, n // 3], NKVH, D, 16, 30)
+    _widen(cache, ROOM)
+    for which in ("k_pages", "v_pages"):
+        codes, s = parts4(getattr(cache, which))
+        s.fill_(127)
+        if which == "k_pages":
+            codes.zero_()
+            for i in range(2):  # the first key: 1 in the first channel
+                codes[int(cache.table[i, 0]), :, 0, 0] = 2
+        else:
+            codes.copy_((torch.arange(D // 2, device=DEV) % 7 + 1) * 17)
+            for i in range(2):
+                codes[int(cache.table[i, 0]), :, 0] = 0
+    cache.decode()
+    lens = [n, n // 3]
+    q = [torch.zeros(new, NH, D, dtype=BF, device=DEV) for _ in lens]
+    for x in q:
+        x[..., 0] = (4.0 + 40.0 * torch.rand(new, NH, generator=cache.g, device=DEV)).to(BF)
+    got = _run(cache, q, [new] * 2, False, max_len=max_len)
+    for i, ((out, _), (o64, _, mag, big)) in enumerate(
+            zip(got, attention64(q, cache, [0, 1], [new] * 2, D ** -0.5))):
+        u = 2.0 ** -24
+        off = mag * (2.0 ** -16 + u * (4 * (D + 8) * (1 + big) + 2 * lens[i] + 64))
+        half = 2.0 ** ((o64.abs() + off).clamp(min=1e-30).log2().floor() - 8)
+        err = (out.double() - o64).abs()
+        assert bool((err <= half + off).all()), (i, float((err / (half + off)).max()))
+
+
 def test_query_strides():
     cache = Cache4([90, 33], 2, 64, 16, 13)
     big = cache.rand(2, 4, 9, 70, dtype=BF)
