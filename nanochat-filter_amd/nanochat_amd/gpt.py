@@ -177,6 +177,9 @@ class GPT(nn.Module):
         longest = max(step.positions) + T
         if longest > self.cos.size(1):  # (indexed on the device, where it would be a fault)
             raise ValueError(f"{longest} tokens, but the model is made for {self.cos.size(1)}")
+        if step.rotates and not step.normalises:  # (it is the rotated ones that are normalised)
+            raise ValueError("a cache that rotates queries and keys must normalise them for this "
+                             "model: norm_eps")
         cos_sin = None
         if not step.rotates:
             at = torch.tensor(step.positions, device=idx.device)[:, None] + torch.arange(

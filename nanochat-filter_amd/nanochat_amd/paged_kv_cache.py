@@ -233,8 +233,13 @@ class PagedStep:
 
     @property
     def rotates(self) -> bool:
-        """Whether ``attend`` rotates and normalises queries and keys."""
+        """Whether ``attend`` rotates queries and keys."""
         return self.cache.rotary is not None
+
+    @property
+    def normalises(self) -> bool:
+        """Whether it divides their heads by their size, too."""
+        return self.cache.norm_eps is not None
 
     @property
     def last_qkv(self) -> "PagedStep":
@@ -256,7 +261,7 @@ class PagedStep:
         """q (B, T, n_head, head_dim), k and v (B, T, n_kv_head, head_dim), B the step's
         slots and T its new tokens: writes k and v into the pages and returns the
         attention of q over each sequence up to itself, (B, T, n_head, head_dim); q and k
-        rotated and normalised first where the cache does that."""
+        rotated, and normalised, first where the cache does that."""
         c = self.cache
         dt = c.dtype
         kp, vp = c.k_pages[layer_idx], c.v_pages[layer_idx]

@@ -281,3 +281,21 @@ def test_refusals(model):
         with pytest.raises(ValueError):
             call()
     assert cache.lens == [20, 0]
+
+
+def test_cache_that_does_not_normalise(model):
+    """A cache that rotates and leaves the norm out, which this model has: refused, and the slot is as it
+    was."""
+    from nanochat_amd import engine
+    from nanochat_amd.paged_kv_cache import PagedKVCache
+    tables = model.cos[0, :, 0], model.sin[0, :, 0]
+    make = lambda **kw: PagedKVCache(3, 4, 2, 64, num_pages=8, max_seqs=1, max_len=128, page_size=16,  # noqa: E731
+                                     rotary=tables, **kw)
+    cache = make()
+    assert cache.step([0], 1).rotates
+    cache.free([0])
+    with pytest.raises(ValueError, match="norm"):
+        engine.prefill(model, cache, 0, _tokens(20))
+    assert cache.lens == [0] and not cache.seq_lens.any() and not cache.ref_counts.any()
+    want = engine.prefill(model, engine.make_cache(model, 8, 1, 16, rotate=True), 0, _tokens(20))
+    assert torch.equal(engine.prefill(model, make(norm_eps=2.0 ** -23), 0, _tokens(20)), want)
