@@ -299,3 +299,38 @@ def test_cache_that_does_not_normalise(model):
     assert cache.lens == [0] and not cache.seq_lens.any() and not cache.ref_counts.any()
     want = engine.prefill(model, engine.make_cache(model, 8, 1, 16, rotate=True), 0, _tokens(20))
     assert torch.equal(engine.prefill(model, make(norm_eps=2.0 ** -23), 0, _tokens(20)), want)
+
+
+@pytest.mark.parametrize("n", [2, 4])
+def test_beam_search_keeps_the_best(n, monkeypatch):
+    """In float32, where the dataflows differ by little: whenever the candidates that an independent
+    search keeps and drops are further apart than that, the beams are the same, all of them.
+
+    A log probability may be off by 2^-24 for each of 256 products' additions, some 20 such sums deep,
+    of logits up to 15: 0.005 a token."""
+    import contextlib
+
+    from nanochat_amd import engine
+    from nanochat_amd.gpt import GPT, GPTConfig
+    from nanochat_amd.paged_kv_cache import PagedKVCache
+    torch.manual_seed(2)
+    model = GPT(GPTConfig(sequence_len=200, vocab_size=VOCAB, n_layer=2, n_head=4, n_kv_head=2,
+                          n_embd=256, ltv_r=64)).to(DEV)
+    model.init_weights(randomise_output_projections=True)
+    model.lm_head.weight.data.normal_(0.0, 0.3, generator=torch.Generator(DEV).manual_seed(3))
+    monkeypatch.setattr(engine, "_autocast", contextlib.nullcontext)
+    make = lambda: PagedKVCache(2, 4, 2, 64, num_pages=8 * n, max_seqs=n, max_len=200, page_size=16,  # noqa: E731
+                                dtype=torch.float32)
+    steps, off, decided = 5, 0.005 * 5, 0
+    for seed in range(8):
+        prompt = _tokens(20 + seed, seed=40 + seed)
+        want, gap = _search64(model, prompt, n, steps, None, make)
+        got = engine.beam_search(model, prompt, n, steps, cache=make(), length_penalty=0.0)
+        if gap <= 2 * off:
+            continue
+        decided += 1
+        lp = {tuple(t): p for t, p in want}
+        assert {tuple(b.tokens) for b in got} == set(lp), (seed, gap)
+        for b in got:
+            assert abs(b.logprob - lp[tuple(b.tokens)]) <= off, seed
+    assert decided >= 2

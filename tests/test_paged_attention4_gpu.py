@@ -355,6 +355,62 @@ def test_rows_of_no_sequence_and_again(new):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("room", [0, ROOM])
+@pytest.mark.parametrize("new,cached", [([1, 1, 1], [5000, 3, 90]), ([40, 1, 200], [60, 3000, 700]),
+                                        ([1100, 0, 3], [200, 5, 0])])
+def test_rows_of_no_sequence_are_left(new, cached, room, dtype):
+    """Rows before the first sequence and behind the last one, and what is between the heads' rows,
+    stay as they were, in the output and in the log-sum-exps; cut tiles among them."""
+    import ctypes
+
+    from nanochat_amd import _native as N
+    from test_serving_abi import Batch, _s
+
+    _ops()
+    N.torch_ext()
+    lib = ctypes.CDLL(N.LIB_PATH)
+    vp, i32 = ctypes.c_void_p, ctypes.c_int
+    NH, NKVH, D, ps, before, behind = 8, 2, 64, 16, 3, 5
+    lens = [a + b for a, b in zip(new, cached)]
+    cache = Cache4(lens, NKVH, D, ps, 31)
+    _widen(cache, room)
+    starts = [before]
+    for n in new:
+        starts.append(starts[-1] + n)
+    total = starts[-1] + behind
+    q = cache.rand(total, NH, D, dtype=dtype)
+    out = torch.full((total, NH, D + 16), 77.0, dtype=dtype, device=DEV)
+    lse = torch.full((total, NH), 77.0, device=DEV)
+    st = torch.tensor(starts, dtype=torch.int32, device=DEV)
+    b = Batch(page_table=cache.table.data_ptr(), seq_lens=cache.lens.data_ptr(), slots=None,
+              starts=st.data_ptr(), table_stride=cache.table.stride(0), total=total, B=len(new),
+              T=max(new), num_slots=len(new), num_pages=cache.P, table_width=cache.table.shape[1],
+              page_size=ps)
+    max_len = cache.table.shape[1] * ps
+    code = 0 if dtype == F32 else 1
+    size = lib.ltv_paged_attention_fp4_workspace_size
+    size.restype, size.argtypes = ctypes.c_size_t, [i32, vp, i32, i32, i32, i32]
+    nws = size(code, ctypes.byref(b), NH, NKVH, D, max_len)
+    ws = torch.empty(nws, dtype=torch.uint8, device=DEV)
+    row = D // 2 + D // 32
+    pages = _s(NKVH * ps * row, ps * row, row)
+    f = lib.ltv_paged_attention_fp4
+    f.argtypes = [i32, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, ctypes.c_size_t, i32, i32, i32, i32,
+                  ctypes.c_float, vp]
+    rc = f(code, q.data_ptr(), _s(0, NH * D, D), cache.k_pages.data_ptr(), pages,
+           cache.v_pages.data_ptr(), pages, ctypes.byref(b), out.data_ptr(),
+           _s(0, NH * (D + 16), D + 16), lse.data_ptr(), ws.data_ptr(), nws, NH, NKVH, D, max_len,
+           D ** -0.5, torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    rows = slice(starts[0], starts[-1])
+    for x in (out[:before], out[starts[-1]:], out[..., D:], lse[:before], lse[starts[-1]:]):
+        assert bool((x == 77.0).all())
+    qs, outs, lses = (x[rows].split(new) for x in (q, out[..., :D], lse))
+    _check(list(zip(outs, lses)), attention64(list(qs), cache, [0, 1, 2], new, D ** -0.5), dtype, D,
+           lens)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("new", [1, 40, 1100])
 def test_captured(new, dtype):
     """Lengths, tables and pages change between replays; two graphs side by side."""
