@@ -15,7 +15,7 @@
 // the candidates' terms (the largest there are) are taken out of the sum as they went in and put
 // back exactly.  What is left is the float32 sum's: terms and additions off by some 2^-24 each.
 //
-// Bounded by the pass over the logits: 384 beams' rows of 50,257 bfloat16 (39 MB) 21 us, 1.8 TB/s --
+// Bounded by the pass over the logits: 384 beams' rows of 50,257 bfloat16 (39 MB) 22 us, 1.8 TB/s --
 // at that length it is the pass's start, its bound for the candidates and its join within a
 // workgroup, three pieces to a row (2, 3, 6 and 11 pieces: 20.5, 21, 24 and 29 us).  The joining
 // is latency: 7 us for 48 prompts of 8 beams each, 5 for one of 4.

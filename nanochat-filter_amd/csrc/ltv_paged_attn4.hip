@@ -6,12 +6,13 @@
 // products are bfloat16 ones, and only queries and probabilities have parts (Split).
 //
 // Two kernels, by the rows that share a k/v head (few_rows).  Of few the reads are the bound, 17
-// bytes for 32 channels: 16 sequences, one of 131,072 tokens, 6 k/v heads (500 MB) 97 us, 5.1 TB/s, the vector
-// units issuing in half of the cycles.  Of many the products are, and the conversions and
-// exponentials beside them: 8,193 tokens over 16,000 (0.51 TFLOP) 697 us, 726 TFLOP/s; matrix
-// units busy in 35 % of the cycles, vector units in 45 %, seldom both.  Scores, maxima, sums and
-// outputs are float32.  The values are converted anew for each row tile: kept in 16 bits in memory
-// for all of them they would be read back at four times the bytes.
+// bytes for 32 channels: 16 sequences, one of 131,072 tokens, 6 k/v heads (500 MB) 96 us, 5.2 TB/s, the
+// vector units issuing in half of the cycles.  Of many the products are, and the conversions and
+// exponentials beside them: 8,193 tokens over 16,000 (0.51 TFLOP) 770 us, 657 TFLOP/s, the second
+// parts of the probabilities, another 0.25, not counted; matrix units busy in 42 % of the cycles,
+// vector units in 47 %, seldom both.  Scores, maxima, sums and outputs are float32.  The values are
+// converted anew for each row tile; converted once, into a workspace of 16 bits that all of them
+// read, is not built.
 #include "../../include/nanochat_decoding_amd.h"
 #include "ltv_fp4.hpp"
 #include "ltv_paged_line.hpp"
@@ -439,8 +440,8 @@ __global__ void __launch_bounds__(kFewThreads, (kFewEach<T, D>))
 // pages: a lane holds 16 keys of one row, and its probabilities are, without any exchange, the
 // right-hand operand of the second product (ds_read_b64_tr_b16 transposes four keys of a column).
 // float32 has three products for each (of the queries' parts and of the probabilities'), and one
-// workgroup to a unit for the registers: a prompt of 4,096 tokens 125 us, 257 TFLOP/s counted once,
-// where a float32 product of two large matrices reaches 154.
+// workgroup to a unit for the registers: a prompt of 4,096 tokens 116 us with the joining, 222 TFLOP/s
+// counted once, where a float32 product of two large matrices reaches 154.
 constexpr int kManyRows = 128, kManyKeys = 64, kManyThreads = 256;
 template <typename T>
 constexpr int kManyEach = sizeof(T) == 2 ? 2 : 1;  // workgroups of a compute unit
@@ -821,16 +822,17 @@ __global__ void __launch_bounds__(kManyThreads, kManyEach<T>) attn4_many_kernel(
 }
 
 // Up to how many rows of a k/v head tiles of 16 read every key for themselves: 16 sequences of
-// 4,000 tokens, 4 heads with 32 rows 39 us in tiles of 16 and 45 in one of 128, with 64 rows 49 and
-// 55, with 128 rows 71 and 63.
+// 4,000 tokens, 4 heads with 32 rows 39 us in tiles of 16 and 45 in one of 128, with 64 rows 48 and
+// 54, with 128 rows 70 and 64.
 constexpr int kMostFewRows = 64;
 
 // Of more rows, calls so small that tiles of 128 would be cut into pieces of a few keys, for the
 // whole card to have some: by rows of all heads times the longest sequence, and in float32, whose
 // tiles of 128 have one workgroup to a unit, also by rows alone.  (In tiles of 128 and of 16 us,
-// 6 heads of 128: bfloat16, 512 tokens over 2,000 42 and 35, 2,048 alone 48 and 42, 1,024 over 8,000
-// 77 and 90, 16 chunks of 128 over up to 2,000 with 8 heads of 64 42 and 45; float32, 512 over 2,000 47
-// and 38, 1,024 over 8,000 121 and 114, 2,048 alone 61 and 69.)
+// 6 heads of 128: bfloat16, 512 tokens over 2,000 41 and 34, 2,048 alone 47 and 42, 1,024 over 8,000
+// 75 and 87, 16 chunks of 128 over up to 2,000 with 8 heads of 64 42 and 44; float32, 512 over 2,000 44
+// and 37, five chunks of up to 600 over up to 4,000 among three single tokens 67 and 61, 1,024 over
+// 8,000 110 and 113, 2,048 alone 58 and 68.)
 bool few_rows(bool f32, int64_t rows, double all_rows, double max_len) {
   return rows <= kMostFewRows || all_rows * max_len <= (f32 ? 0x1p24 : 0x1p25) ||
          (f32 && all_rows <= 8192);

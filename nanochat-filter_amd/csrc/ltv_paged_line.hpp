@@ -260,7 +260,7 @@ __device__ __forceinline__ void rows_one_by_one(const AttnArgs& a, const PagedSe
 // keys of a block, ROWS: of a row tile, GRID: workgroups that the card holds; FEW: one wavefront,
 // and many sequences to a thread.  Args: AttnArgs, or a reference, as leaves the kernel's loop over
 // tiles with fewer numbers put aside for scalar registers (a long prompt over 16-bit pages 1,254 us
-// with a reference and 1,155 with a copy, over 4-bit pages 743 and 760).
+// with a reference and 1,155 with a copy; over 4-bit pages they are alike).
 template <int KT, bool FEW, int THREADS, int ROWS, int GRID, typename Args, typename Piece>
 __device__ __forceinline__ void walk_line(Args a, Piece piece) {
   constexpr int WAVES = THREADS / 64;

@@ -15,7 +15,7 @@
 // query and 4 k/v heads of 128, bfloat16 into 4-bit pages, 28 to 30 us (110 MB, 3.8 TB/s), and 9 us
 // to read its keys and values back.  Small calls are latency, of the sequence's numbers, its page
 // and its rows one after the other: 64 sequences of one token each 4.3 us, nine with chunks of up
-// to 700 float32 tokens 7.2.
+// to 700 float32 tokens 7.1.
 #include <algorithm>
 #include <type_traits>
 
@@ -322,7 +322,7 @@ void launch_rotary(const RotaryArgs& a, dim3 grid, hipStream_t st) {
 
 // Blocks over the new tokens of a sequence (T is a hint with starts: they stride over whatever
 // there is).  Not more than twice what a sequence has on average, or most of them look and leave
-// (chunks of nine sequences of up to 700 tokens 7.2 us, and 11 with blocks for the longest each),
+// (chunks of nine sequences of up to 700 tokens 7.1 us, and 11 with blocks for the longest each),
 // nor than go round a few times: each block's first round waits for its sequence's numbers, its
 // page and its rows (12,289 tokens 28 us, with four times the blocks 45).
 int blocks_for(const ltv_paged_batch& b, int64_t threads_per_token) {

@@ -36,7 +36,7 @@ tokens in rows starts[i] .. starts[i + 1], so that one call takes a batch in whi
 some sequences decode and the prompts of others come in chunks.  Sequence i is slot
 ``slots[i]`` (default: slot i).  ``max_new`` and ``max_len`` are what the caller knows
 of the longest chunk and sequence; they choose launch shapes, and past 10^11 operations
-how probabilities are rounded, not which keys are read.
+how probabilities are rounded (not over 4-bit pages), not which keys are read.
 
 The reference's cache is contiguous (``nanochat/kv_cache.py`` ``insert_kv``) and is
 copied whole to start several samples from one prompt (``prefill``).
